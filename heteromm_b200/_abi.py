@@ -24,6 +24,31 @@ _I = C.c_int64
 _F = C.c_float
 _S = C.c_size_t
 
+HMM_DTYPE_BF16, HMM_DTYPE_F16, HMM_DTYPE_F32 = 0, 1, 2
+
+
+class PagedCache(C.Structure):     # hmm_paged_cache_t
+    _fields_ = [("k", _P), ("v", _P)] + [(n, _I) for n in (
+        "n_pages", "n_kv_heads", "page_tokens", "D", "k_page", "k_head", "k_token", "v_page",
+        "v_head", "v_token")] + [("dtype", C.c_int32)]
+
+
+class PagedBatch(C.Structure):     # hmm_paged_batch_t
+    _fields_ = [("page_table", _P), ("n_seq", _I), ("pages_per_seq", _I), ("cu_new", _P),
+                ("n_tokens", _I), ("kv_len", _P)]
+
+
+class PageStore(C.Structure):      # hmm_page_store_t
+    _fields_ = [("k", _P), ("v", _P)] + [(n, _I) for n in (
+        "n_pages", "page_bytes", "n_layers", "k_page", "k_layer", "v_page", "v_layer")]
+
+
+class PagedState(C.Structure):     # hmm_paged_state_t
+    _fields_ = [(n, _P) for n in ("table_in", "refs_in", "kv_len_in", "table_out", "refs_out",
+                                  "kv_len_out")] + \
+               [(n, _I) for n in ("n_seq", "pages_per_seq", "n_pages")]
+
+
 # name -> (restype, argtypes); mirrors include/heteromm_cuda.h
 SIGNATURES = {
     "hmm_last_error": (C.c_char_p, []),
@@ -57,6 +82,14 @@ SIGNATURES = {
     "hmm_status_read": (C.c_int, [_P, _P]),
     "hmm_block_sparse_decode_bf16": (C.c_int, [_P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I,
                                                _I, _P, _P, _P, _S, _P]),
+    "hmm_paged_kv_append": (C.c_int, [_P, _P, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P,
+                                      C.c_int, _F, _P, _I, _I, C.c_int, _P, _P, _I, _I, _P, _P]),
+    "hmm_paged_state_workspace_size": (_S, [_I, _I]),
+    "hmm_paged_copy_pages": (C.c_int, [_P, _P, _P, _I, _P, _P, _S, _P]),
+    "hmm_paged_free": (C.c_int, [_P, _P, _I, _P, _P, _S, _P]),
+    "hmm_paged_fork": (C.c_int, [_P, _P, _I, _P, _P, _I, _P, _P, _S, _P]),
+    "hmm_paged_grow": (C.c_int, [_P, _I, _P, _P, _P, _S, _P]),
+    "hmm_paged_compact": (C.c_int, [_P, _P, _P, _P, _P, _S, _P]),
     "hmm_bm25_stats_host": (C.c_int, [_P, _I, _P, _I, _P, _P]),
     "hmm_bm25_skips_count": (_S, [_I, _I]),
     "hmm_bm25_prepare": (C.c_int, [_P, _P, _P, _I, _P, _I, _P, C.c_double, _P, _P, _P, _S,

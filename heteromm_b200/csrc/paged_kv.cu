@@ -864,6 +864,11 @@ hmm_status_t read_status(const int* status, cudaStream_t st, const char* what) {
         return set_error(HMM_ERR_BOUNDS, "%s: a page-table entry is outside [0, n_pages)", what);
     if (h & HMM_STATUS_BLOCK_BOUNDS)
         return set_error(HMM_ERR_BOUNDS, "%s: a selected block id is negative", what);
+    if (h & HMM_STATUS_BATCH_BOUNDS)
+        return set_error(HMM_ERR_BOUNDS,
+                         "%s: a length, position, offset or sequence number is outside its extent",
+                         what);
+    if (h & HMM_STATUS_NO_PAGES) return set_error(HMM_ERR_OOM, "%s: too few free pages", what);
     if (h & HMM_STATUS_TIMEOUT)
         return set_error(HMM_ERR_TIMEOUT, "%s: a bounded pipeline wait gave up; outputs invalid",
                          what);

@@ -290,7 +290,8 @@ hmm_status_t hmm_block_sparse_decode_bf16(const uint16_t* q, const float* summar
  * HMM_ERR_BOUNDS; the kernels never follow them.  hmm_status_read waits for
  * `stream` and turns the bits of a device status word into a status:
  * HMM_ERR_BOUNDS for the two above, HMM_ERR_TIMEOUT for HMM_STATUS_TIMEOUT,
- * HMM_ERR_UNSUPPORTED for HMM_STATUS_POOL_OVERFLOW.  For loops that check
+ * HMM_ERR_UNSUPPORTED for HMM_STATUS_POOL_OVERFLOW (two more bits: "serving a
+ * paged cache" below).  For loops that check
  * once per many steps. */
 #define HMM_STATUS_PAGE_BOUNDS 1
 #define HMM_STATUS_BLOCK_BOUNDS 2
@@ -303,6 +304,139 @@ hmm_status_t hmm_block_sparse_decode_bf16_async(
     int32_t* out_blocks, float* out, int32_t* device_status, void* workspace,
     size_t workspace_bytes, void* stream);
 hmm_status_t hmm_status_read(const int32_t* device_status, void* stream);
+
+/* ------------------------------------------------- serving a paged cache
+ * No counterpart in the reference, whose cache holds one sequence's one head:
+ * filling, attending over and managing a paged cache of several KV heads that
+ * ragged sequences share.  Entry points below are asynchronous and take a
+ * device_status word (required, see above): HMM_STATUS_PAGE_BOUNDS for a
+ * page-table entry outside [0, n_pages) that a token needs,
+ * HMM_STATUS_BATCH_BOUNDS for a length, position, offset or sequence number
+ * outside its extent, HMM_STATUS_NO_PAGES for too few free pages;
+ * hmm_status_read turns them into HMM_ERR_BOUNDS and HMM_ERR_OOM.  No kernel
+ * follows such a value.
+ *
+ * hmm_paged_cache_t: the K and V page arrays [n_pages][n_kv_heads]
+ * [page_tokens][D] of 16-bit floats, both 16-byte aligned, with page, head
+ * and token strides in elements (multiples of 8; the last dimension is
+ * contiguous), so that token-major pages [page_tokens][n_kv_heads][D] and K
+ * and V interleaved in one array are views too.  With dense strides page
+ * `phys` of head h is page phys * n_kv_heads + h of the single-head cache
+ * above, whose summaries and block-sparse decode apply to it.
+ *
+ * hmm_paged_batch_t: n_seq sequences with the page table [n_seq]
+ * [pages_per_seq] (-1 or anything where no token lives) and kv_len [n_seq]
+ * cached tokens, the new ones among them.  The new tokens of sequence s are
+ * rows [cu_new[s], cu_new[s+1]) of the packed arrays of n_tokens rows; new
+ * token j has position kv_len[s] - n_new[s] + j.  Rows that no sequence owns
+ * (before cu_new[0], from cu_new[n_seq] on) are neither read nor written. */
+#define HMM_DTYPE_BF16 0
+#define HMM_DTYPE_F16 1
+#define HMM_DTYPE_F32 2
+#define HMM_STATUS_BATCH_BOUNDS 16
+#define HMM_STATUS_NO_PAGES 32
+typedef struct {
+    void* k;
+    void* v;
+    int64_t n_pages, n_kv_heads, page_tokens, D;
+    int64_t k_page, k_head, k_token;   /* strides in elements */
+    int64_t v_page, v_head, v_token;
+    int32_t dtype;                     /* HMM_DTYPE_BF16 or HMM_DTYPE_F16 */
+} hmm_paged_cache_t;
+typedef struct {
+    const int32_t* page_table;
+    int64_t n_seq, pages_per_seq;
+    const int32_t* cu_new;
+    int64_t n_tokens;
+    const int32_t* kv_len;
+} hmm_paged_batch_t;
+
+/* The step before attention, in one pass over the new tokens' heads: RMS norm
+ * of each query and key head (y = x / sqrt(mean(x^2) + eps) * weight, weights
+ * [D] fp32 or of the cache's type, NULL = no norm), position rotation of their
+ * first rotary_dim values, and the store of keys and values at the tokens'
+ * positions in the cache.  Computed in fp32, rounded once.
+ *   q [n_tokens][n_heads][D] -> q_out (q itself is allowed; n_heads = 0 for
+ *   none), k, v [n_tokens][n_kv_heads][D], all of the cache's type, 16-byte
+ *   aligned, with token and head strides in elements (multiples of 8)
+ *   rope [n_pos][rotary_dim / 2][2] fp32 (cos, sin), 8-byte aligned, or NULL:
+ *   no rotation; pair i is values (i, i + rotary_dim / 2), or with
+ *   `interleaved` (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin)
+ *   positions [n_tokens] rows of `rope`, or NULL: the tokens' own positions
+ * A token whose page or angle is out of bounds is flagged and skipped.  No
+ * two tokens of a call may share a slot.  D % 8 == 0, 8 <= D <= 512. */
+hmm_status_t hmm_paged_kv_append(
+    const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch, const void* q, int64_t q_token,
+    int64_t q_head, int64_t n_heads, const void* k, int64_t k_token, int64_t k_head, const void* v,
+    int64_t v_token, int64_t v_head, const void* q_weight, const void* k_weight, int weight_dtype,
+    float eps, const float* rope, int64_t n_pos, int64_t rotary_dim, int interleaved,
+    const int32_t* positions, void* q_out, int64_t out_token, int64_t out_head,
+    int32_t* device_status, void* stream);
+
+/* Page management.  The state is the page table [n_seq][pages_per_seq] (an
+ * entry below 0 holds no page), the references [n_pages] of each page (0 =
+ * free) and kv_len [n_seq].  Every call reads the state from *_in and writes
+ * the whole new state to *_out; the two may be the same arrays (in place).
+ * New pages are always the lowest free ones.  A request that cannot be met as
+ * a whole - a sequence number or length out of bounds, too few free pages -
+ * sets its status bit and leaves the state (and the pages) as they were.
+ * Page data: hmm_page_store_t, n_layers >= 1 pairs of K and V page arrays that
+ * share the state; a page is page_bytes contiguous bytes (a multiple of 16),
+ * strides in bytes (multiples of 16), 16-byte aligned.
+ * Workspace: hmm_paged_state_workspace_size bytes (hmm_paged_copy_pages: 4),
+ * 4-byte aligned. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t n_pages, page_bytes, n_layers;
+    int64_t k_page, k_layer, v_page, v_layer;   /* strides in bytes */
+} hmm_page_store_t;
+typedef struct {
+    const int32_t* table_in;
+    const int32_t* refs_in;
+    const int32_t* kv_len_in;
+    int32_t* table_out;
+    int32_t* refs_out;
+    int32_t* kv_len_out;
+    int64_t n_seq, pages_per_seq, n_pages;
+} hmm_paged_state_t;
+size_t hmm_paged_state_workspace_size(int64_t n_seq, int64_t n_pages);
+
+/* Page src[i] is copied to page dst[i] in every layer, K and V.  A pair with an
+ * entry below 0 is skipped.  A page outside [0, n_pages), a dst listed twice,
+ * or one that is another pair's src: HMM_STATUS_BATCH_BOUNDS, nothing copied. */
+hmm_status_t hmm_paged_copy_pages(const hmm_page_store_t* store, const int32_t* src,
+                                  const int32_t* dst, int64_t n, int32_t* device_status,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Frees sequences: every page that a listed row holds loses one reference, the
+ * row becomes -1 and its kv_len 0.  A sequence listed twice is freed once. */
+hmm_status_t hmm_paged_free(const hmm_paged_state_t* state, const int32_t* seqs, int64_t n,
+                            int32_t* device_status, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Forks sequence src[i] into the empty row dst[i] (no pages held, kv_len 0; no
+ * dst twice): the pages that its kv_len tokens fill are shared (one reference
+ * more), a partly filled last one is copied into a new page, so that neither
+ * sequence writes into the other's.  A src may be forked several times. */
+hmm_status_t hmm_paged_fork(const hmm_paged_state_t* state, const hmm_page_store_t* store,
+                            int64_t page_tokens, const int32_t* src, const int32_t* dst, int64_t n,
+                            int32_t* device_status, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Makes room for n_new[s] >= 0 more tokens of every sequence: the entries of
+ * the pages that they touch and that hold none get new pages (in row order),
+ * and kv_len_out = kv_len_in + n_new. */
+hmm_status_t hmm_paged_grow(const hmm_paged_state_t* state, int64_t page_tokens,
+                            const int32_t* n_new, int32_t* device_status, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Moves the live pages (references != 0) to the front: with L live pages, the
+ * k-th live page at or behind L goes to the k-th free one before it; table and
+ * references follow (kv_len is not used), out_live [1] = L. */
+hmm_status_t hmm_paged_compact(const hmm_paged_state_t* state, const hmm_page_store_t* store,
+                               int32_t* out_live, int32_t* device_status, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /* ----------------------------------------------------------------- BM25
  * FusedBM25Retrieval (reference steps/example_kernel/bm25_fpga_retrieval.cpp:
