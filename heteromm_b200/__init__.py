@@ -13,7 +13,7 @@ from .indexers import (dsa_indexer_fp8, dsa_indexer_fp8_host, lserve_topk_i16,  
 from .paged import (block_pages, block_sparse_attention_bf16, block_sparse_attention_f32,  # noqa: F401,E501
                     block_select_minmax, block_sparse_decode_bf16, paged_kv_minmax_bf16,
                     paged_kv_summary_bf16, paged_kv_summary_f32)
-from .serve import (paged_compact, paged_copy_pages, paged_fork, paged_free, paged_grow,  # noqa: F401,E501
-                    paged_kv_append, rope_table)
+from .serve import (paged_attention, paged_compact, paged_copy_pages, paged_fork, paged_free,  # noqa: F401,E501
+                    paged_grow, paged_kv_append, rope_table)
 
 __version__ = "0.1.0"

@@ -84,6 +84,9 @@ SIGNATURES = {
                                                _I, _P, _P, _P, _S, _P]),
     "hmm_paged_kv_append": (C.c_int, [_P, _P, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P,
                                       C.c_int, _F, _P, _I, _I, C.c_int, _P, _P, _I, _I, _P, _P]),
+    "hmm_paged_attention_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "hmm_paged_attention": (C.c_int, [_P, _P, _P, _I, _I, _I, _F, C.c_int, _I, _I, _I, _P, _P, _P,
+                                      _P, _S, _P]),
     "hmm_paged_state_workspace_size": (_S, [_I, _I]),
     "hmm_paged_copy_pages": (C.c_int, [_P, _P, _P, _I, _P, _P, _S, _P]),
     "hmm_paged_free": (C.c_int, [_P, _P, _I, _P, _P, _S, _P]),

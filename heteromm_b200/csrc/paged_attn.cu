@@ -1,0 +1,555 @@
+// paged_attn.cu — attention of ragged chunks of new tokens over a paged cache:
+// the entry point, and the kernel for few rows (decoding, drafted tokens).
+//
+// paged_rows_kernel.  A unit is (sequence, KV head, 16 rows): rows are (new
+// token, query head of the group), so grouped heads read their keys once.  With
+// few rows the cache has to be read for next to no arithmetic and HBM bounds it;
+// the design keeps reads in flight:
+//   - all units' key tiles form one list, cut into as many equal pieces as CTAs
+//     fit the GPU (ragged lengths balance by themselves); a CTA finds its piece
+//     from the lengths on the device, so no host value goes stale;
+//   - each warp owns 16 keys of a tile and its own ring of cp.async stages, with
+//     no barrier between warps: page lookup one stage ahead, 16-byte copies, zero
+//     fill for what no row of the tile sees;
+//   - scores and the product with V on mma.sync (m16n8k16, fp32 sums), the
+//     running maximum and sum in fp32 per warp, warps joined once per piece;
+//   - a unit that several CTAs share leaves (maximum, sum, unnormalised rows) per
+//     piece in the workspace, and paged_rows_join_kernel adds the pieces in order.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace hmm {
+namespace serve {
+namespace {
+
+constexpr int RW_WARPS = 4;
+constexpr int RW_THREADS = 32 * RW_WARPS;
+constexpr int RW_KEYS = 16;                   // keys of a warp's tile
+constexpr int RW_TILE = RW_WARPS * RW_KEYS;   // keys of a CTA's tile
+constexpr int RW_ROWS = 16;
+constexpr int RW_STAGES = 3;
+
+struct RowsWork {
+    int4* joint;      // [ctas] unit begun in the CTA and ended in another: sequence, head, row tile, pieces
+    float* part;      // [ctas][2][RW_ROWS * (DP + 2)]: rows, then maxima, then sums
+};
+
+struct RowsArgs {
+    AttnArgs a;
+    RowsWork w;
+    int max_rows;     // sequences of more rows are another kernel's
+};
+
+template <int DP>
+constexpr int rows_ctas_per_sm() { return DP == 64 ? 4 : DP == 128 ? 2 : 1; }
+
+template <int DP>
+constexpr size_t rows_smem() {
+    return (size_t)RW_WARPS * RW_STAGES * 2 * RW_KEYS * DP * 2;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldm4(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldm4t(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Units and key tiles of a sequence.  `tiles` is the same for each of its
+// units, an upper bound of what a unit's rows see.
+struct Load {
+    int units, tiles, row_tiles;
+};
+
+__device__ __forceinline__ Load seq_load(const RowsArgs& r, const Seq& q) {
+    const int64_t rows = (int64_t)q.n_new * r.a.group;
+    Load x{0, 0, 0};
+    if (rows == 0 || rows > r.max_rows) return x;
+    x.row_tiles = (int)((rows + RW_ROWS - 1) / RW_ROWS);
+    x.units = x.row_tiles * r.a.hk;
+    int64_t t = ((int64_t)q.kv + RW_TILE - 1) / RW_TILE;
+    if (r.a.window > 0) {
+        const int64_t near = ((int64_t)r.a.window + RW_ROWS + RW_TILE - 1) / RW_TILE + 1;
+        t = min(t, near + ((int64_t)r.a.sinks + RW_TILE - 1) / RW_TILE);
+    }
+    x.tiles = (int)max(t, (int64_t)1);   // a row that sees nothing is written too
+    return x;
+}
+
+// Inclusive scan over the block's threads.
+__device__ __forceinline__ int64_t scan_incl(int64_t v, int64_t* wt, int64_t* total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    if (lane == 31) wt[w] = v;
+    __syncthreads();
+    int64_t add = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < RW_WARPS; ++i) {
+        if (i < w) add += wt[i];
+        sum += wt[i];
+    }
+    __syncthreads();
+    *total = sum;
+    return v + add;
+}
+
+// Joins (maximum, sum, row) pieces of the unit's rows and writes them out; rows
+// that come out not finite are computed again by attn_row_exact.  piece(i, row,
+// -1 / -2 / d) reads the maximum, sum or value of piece i.  Whole block.
+template <typename T, typename Piece>
+__device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
+                                            int rows, int pieces, Piece piece, int* again) {
+    if (threadIdx.x == 0) *again = 0;
+    __syncthreads();
+    const int pairs = a.D / 2;
+    for (int i = threadIdx.x; i < rows * pairs; i += blockDim.x) {
+        const int r = i / pairs, d = 2 * (i - r * pairs);
+        float m = -INFINITY;
+        for (int p = 0; p < pieces; ++p) m = fmaxf(m, piece(p, r, -1));
+        const float ms = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, x = 0.0f, y = 0.0f;
+        for (int p = 0; p < pieces; ++p) {
+            const float wgt = ex2(piece(p, r, -1) - ms);
+            if (wgt == 0.0f) continue;   // a piece in which the row saw nothing
+            l = fmaf(wgt, piece(p, r, -2), l);
+            x = fmaf(wgt, piece(p, r, d), x);
+            y = fmaf(wgt, piece(p, r, d + 1), y);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        x = l == 0.0f ? 0.0f : x * inv;
+        y = l == 0.0f ? 0.0f : y * inv;
+        if (!isfinite(x) || !isfinite(y) || l != l) atomicOr(again, 1 << r);
+        const int tok = q.begin + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
+        const int64_t at = (int64_t)tok * a.hq + head;
+        *reinterpret_cast<uint32_t*>(a.out + 2 * (at * a.D + d)) = pack2<T>(x, y);
+        if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+    }
+    __syncthreads();
+    const int bits = *again;
+    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
+        if ((bits >> r) & 1) attn_row_exact<T>(a, s, q, kvh, row0 + r);
+    __syncthreads();
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP>())
+paged_rows_kernel(const __grid_constant__ RowsArgs r) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int64_t wt[RW_WARPS];
+    __shared__ int64_t sh_pre;
+    __shared__ int sh_seq, again;
+    constexpr int ROWB = DP * 2;                       // bytes of a staged row
+    constexpr int CH = DP / 8;                         // its 16-byte chunks
+    constexpr int STAGE = 2 * RW_KEYS * ROWB;          // K then V
+    constexpr int MR = DP + 4;                         // joining rows: 4 banks apart
+    const AttnArgs& a = r.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- this CTA's piece of the list of all units' tiles
+    int64_t total = 0;
+    for (int s0 = 0; s0 < a.b.n_seq; s0 += RW_THREADS) {
+        const int s = s0 + threadIdx.x;
+        int64_t v = 0, sum;
+        if (s < a.b.n_seq) {
+            const Load x = seq_load(r, load_seq(a.b, a.max_kv, s, a.status));
+            v = (int64_t)x.units * x.tiles;
+        }
+        scan_incl(v, wt, &sum);
+        total += sum;
+    }
+    const int64_t per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
+    int64_t cur = blockIdx.x * per;
+    const int64_t end = min(total, cur + per);
+    if (threadIdx.x == 0) r.w.joint[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (cur >= end) return;
+    {
+        int64_t run = 0;
+        for (int s0 = 0; s0 < a.b.n_seq; s0 += RW_THREADS) {
+            const int s = s0 + threadIdx.x;
+            int64_t v = 0, sum;
+            if (s < a.b.n_seq) {
+                const Load x = seq_load(r, load_seq(a.b, a.max_kv, s, a.status));
+                v = (int64_t)x.units * x.tiles;
+            }
+            const int64_t incl = scan_incl(v, wt, &sum) + run;
+            if (incl - v <= cur && cur < incl) {
+                sh_seq = s;
+                sh_pre = incl - v;
+            }
+            run += sum;
+            if (run > cur) break;
+        }
+        __syncthreads();
+    }
+    int s = sh_seq;
+    int64_t pre = sh_pre;                              // tiles before sequence s
+    Seq q = load_seq(a.b, a.max_kv, s, a.status);
+    Load ld = seq_load(r, q);
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * RW_STAGES * STAGE;
+    while (cur < end) {
+        while (cur >= pre + (int64_t)ld.units * ld.tiles) {
+            pre += (int64_t)ld.units * ld.tiles;
+            q = load_seq(a.b, a.max_kv, ++s, a.status);
+            ld = seq_load(r, q);
+        }
+        const int unit = (int)((cur - pre) / ld.tiles);
+        const int t0 = (int)(cur - pre - (int64_t)unit * ld.tiles);
+        const int t1 = (int)min((int64_t)ld.tiles, t0 + (end - cur));
+        const int kvh = unit / ld.row_tiles, rt = unit - kvh * ld.row_tiles;
+        const int row0 = rt * RW_ROWS;
+        const int rows = (int)min((int64_t)RW_ROWS, (int64_t)q.n_new * a.group - row0);
+        const Span sp = tile_span(a, q, row0, row0 + rows);
+        const int sink_tiles = (sp.sink + RW_TILE - 1) / RW_TILE;
+        const int first = max(sp.lo / RW_TILE, sink_tiles);
+        const int n_tiles = sink_tiles + max(0, (sp.hi + RW_TILE - 1) / RW_TILE - first);
+        const int n = min(t1, n_tiles) - t0;           // tiles of this piece, <= 0: none
+
+        auto key0_of = [&](int i) {                    // first key of this warp's part of tile t0 + i
+            const int t = t0 + i;
+            return (t < sink_tiles ? t : first + t - sink_tiles) * RW_TILE + warp * RW_KEYS;
+        };
+        // lanes 0-15: page and slot of key (key0 + lane), page -1 where no row sees it
+        int phys = -1, slot = 0;
+        auto lookup = [&](int i) {
+            phys = -1;
+            if (i < n && lane < RW_KEYS) {
+                const int key = key0_of(i) + lane;
+                if (span_has(sp, key)) {
+                    const int lp = key / a.page_tokens;
+                    phys = page_of(a, s, lp);
+                    slot = key - lp * a.page_tokens;
+                }
+            }
+        };
+        auto issue = [&](int i) {                      // copies of tile i, whose lookup is in phys / slot
+            if (i < n) {
+                const uint32_t st = ring + (i % RW_STAGES) * STAGE;
+#pragma unroll
+                for (int it = 0; it < RW_KEYS * CH / 32; ++it) {
+                    const int idx = it * 32 + lane, row = idx / CH, c = idx % CH;
+                    const int ph = __shfl_sync(0xffffffffu, phys, row);
+                    const int sl = __shfl_sync(0xffffffffu, slot, row);
+                    const bool real = ph >= 0 && c * 8 < a.D;
+                    const unsigned char* kp = a.k.base;
+                    const unsigned char* vp = a.v.base;
+                    if (real) {
+                        kp += ph * a.k.page + kvh * a.k.head + sl * a.k.token + c * 16;
+                        vp += ph * a.v.page + kvh * a.v.head + sl * a.v.token + c * 16;
+                    }
+                    const uint32_t d = st + row * ROWB + ((c ^ (row & 7)) * 16);
+                    cp16(d, kp, real);
+                    cp16(d + RW_KEYS * ROWB, vp, real);
+                }
+            }
+            cp_commit();
+        };
+
+        // q fragments: rows lane / 4 and lane / 4 + 8
+        uint32_t qf[DP / 16][4];
+        int pos[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = lane / 4 + 8 * h;
+            const bool real = row < rows;
+            const int at = row0 + (real ? row : 0);
+            pos[h] = real ? q.kv - q.n_new + at / a.group : -1;
+            const unsigned char* src = a.q + (int64_t)(q.begin + at / a.group) * a.q_token +
+                                       (int64_t)(kvh * a.group + at % a.group) * a.q_head;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int d = k * 16 + j * 8 + (lane & 3) * 2;
+                    qf[k][h + 2 * j] = real && d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(src + 2 * d)) : 0u;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < RW_STAGES - 1; ++i) {
+            lookup(i);
+            issue(i);
+        }
+        lookup(RW_STAGES - 1);
+
+        float o[DP / 8][4];
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+
+        for (int i = 0; i < n; ++i) {
+            cp_wait<RW_STAGES - 2>();
+            __syncwarp();
+            issue(i + RW_STAGES - 1);                  // into the stage that tile i - 1 left
+            lookup(i + RW_STAGES);
+            const uint32_t kt = ring + (i % RW_STAGES) * STAGE, vt = kt + RW_KEYS * ROWB;
+            float sc[2][4] = {};
+            const int mi = lane >> 3, ml = lane & 7;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t b[4];
+                const int row = ml + (mi >> 1) * 8, c = 2 * k + (mi & 1);
+                ldm4(b, kt + row * ROWB + ((c ^ (row & 7)) * 16));
+                mma16816<T>(sc[0], qf[k], b[0], b[1]);
+                mma16816<T>(sc[1], qf[k], b[2], b[3]);
+            }
+            const int key0 = key0_of(i);
+            const bool all = key0 + RW_KEYS <= q.kv && (!a.causal || key0 + RW_KEYS - 1 <= sp.p0) &&
+                             (a.window <= 0 || key0 > sp.p1 - a.window || key0 + RW_KEYS <= a.sinks);
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x = sc[nb][j] * a.scale_log2;
+                    if (!all && !sees(a, q.kv, pos[j >> 1], key0 + nb * 8 + (lane & 3) * 2 + (j & 1)))
+                        x = -INFINITY;
+                    sc[nb][j] = x;
+                    mx[j >> 1] = fmaxf(mx[j >> 1], x);
+                }
+            float al[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                const float ms = mx[h] == -INFINITY ? 0.0f : mx[h];
+                al[h] = ex2(m[h] - ms);
+                m[h] = mx[h];
+                mx[h] = ms;
+            }
+            if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < DP / 8; ++d) {
+                    o[d][0] *= al[0]; o[d][1] *= al[0]; o[d][2] *= al[1]; o[d][3] *= al[1];
+                }
+                l[0] *= al[0];
+                l[1] *= al[1];
+            }
+            uint32_t p[4];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float e0 = ex2(sc[nb][2 * h] - mx[h]), e1 = ex2(sc[nb][2 * h + 1] - mx[h]);
+                    l[h] += e0 + e1;
+                    // weights in the cache's type for the product: relative 2^-9 (bf16) or 2^-12,
+                    // the size of the output's own rounding; the sum keeps fp32
+                    p[2 * nb + h] = pack2<T>(e0, e1);
+                }
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                uint32_t b[4];
+                const int row = ml + (mi & 1) * 8, c = 2 * d + (mi >> 1);
+                ldm4t(b, vt + row * ROWB + ((c ^ (row & 7)) * 16));
+                mma16816<T>(o[2 * d], p, b[0], b[1]);
+                mma16816<T>(o[2 * d + 1], p, b[2], b[3]);
+            }
+            __syncwarp();                              // the stage may be overwritten
+        }
+        cp_wait<0>();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+
+        // ---- join the warps in the rings' memory
+        __syncthreads();
+        float* jm = reinterpret_cast<float*>(smem);    // [warp][16][MR], then [warp][16] maxima, sums
+        float* jst = jm + RW_WARPS * RW_ROWS * MR;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = lane / 4 + 8 * h;
+            float* dst = jm + (warp * RW_ROWS + row) * MR + (lane & 3) * 2;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) {
+                dst[8 * d] = o[d][2 * h];
+                dst[8 * d + 1] = o[d][2 * h + 1];
+            }
+            if ((lane & 3) == 0) {
+                jst[warp * RW_ROWS + row] = m[h];
+                jst[(RW_WARPS + warp) * RW_ROWS + row] = l[h];
+            }
+        }
+        __syncthreads();
+        auto piece = [&](int w, int row, int d) {
+            return d == -1   ? jst[w * RW_ROWS + row]
+                   : d == -2 ? jst[(RW_WARPS + w) * RW_ROWS + row]
+                             : jm[(w * RW_ROWS + row) * MR + d];
+        };
+        if (t0 == 0 && t1 == ld.tiles) {
+            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, piece, &again);
+        } else {
+            float* part = r.w.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * RW_ROWS * (DP + 2);
+            for (int i = threadIdx.x; i < rows * a.D; i += RW_THREADS) {
+                const int row = i / a.D, d = i - row * a.D;
+                float mm = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < RW_WARPS; ++w) mm = fmaxf(mm, piece(w, row, -1));
+                const float ms = mm == -INFINITY ? 0.0f : mm;
+                float x = 0.0f, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < RW_WARPS; ++w) {
+                    const float wgt = ex2(piece(w, row, -1) - ms);
+                    x = fmaf(wgt, piece(w, row, d), x);
+                    sum = fmaf(wgt, piece(w, row, -2), sum);
+                }
+                part[row * DP + d] = x;
+                if (d == 0) {
+                    part[RW_ROWS * DP + row] = mm;
+                    part[RW_ROWS * (DP + 1) + row] = sum;
+                }
+            }
+            if (t0 == 0 && threadIdx.x == 0)
+                r.w.joint[blockIdx.x] = make_int4(s, kvh, rt, 1 + (int)((ld.tiles - t1 + per - 1) / per));
+            __syncthreads();                           // the rings' memory is free again
+        }
+        cur += t1 - t0;
+    }
+}
+
+// Block c: the unit begun in CTA c and ended in a later one.
+template <typename T, int DP>
+__global__ void __launch_bounds__(RW_THREADS) paged_rows_join_kernel(const __grid_constant__ RowsArgs r) {
+    __shared__ int again;
+    const int4 u = r.w.joint[blockIdx.x];
+    if (u.w == 0) return;
+    const Seq q = load_seq(r.a.b, r.a.max_kv, u.x, r.a.status);
+    const int row0 = u.z * RW_ROWS;
+    const int rows = (int)min((int64_t)RW_ROWS, (int64_t)q.n_new * r.a.group - row0);
+    const float* part = r.w.part;
+    const int64_t c = blockIdx.x;
+    finish_rows<T>(r.a, u.x, q, u.y, row0, rows, u.w, [&](int i, int row, int d) {
+        const float* p = part + ((c + i) * 2 + (i == 0)) * RW_ROWS * (DP + 2);
+        return d == -1 ? p[RW_ROWS * DP + row] : d == -2 ? p[RW_ROWS * (DP + 1) + row] : p[row * DP + d];
+    }, &again);
+}
+
+int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+int64_t rows_ctas(int dp) {
+    return (int64_t)device_sm_count() * (dp == 64 ? rows_ctas_per_sm<64>() : dp == 128 ? rows_ctas_per_sm<128>() : 1);
+}
+
+size_t rows_workspace(int dp) {
+    const size_t g = (size_t)rows_ctas(dp);
+    return g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
+}
+
+template <typename T, int DP>
+hmm_status_t launch_rows(const RowsArgs& r, cudaStream_t st) {
+    const unsigned g = (unsigned)rows_ctas(DP);
+    HMM_CUDA_TRY(cudaFuncSetAttribute(paged_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)rows_smem<DP>()));
+    paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(r);
+    hmm_status_t s = check_launch("paged_rows_kernel");
+    if (s != HMM_OK) return s;
+    paged_rows_join_kernel<T, DP><<<g, RW_THREADS, 0, st>>>(r);
+    return check_launch("paged_rows_join_kernel");
+}
+
+template <typename T>
+hmm_status_t run_rows(const AttnArgs& a, int max_rows, unsigned char* ws, cudaStream_t st) {
+    const int dp = rows_dp(a.D);
+    RowsArgs r{a, {(int4*)ws, (float*)(ws + (size_t)rows_ctas(dp) * sizeof(int4))}, max_rows};
+    return dp == 64 ? launch_rows<T, 64>(r, st) : dp == 128 ? launch_rows<T, 128>(r, st)
+                                                            : launch_rows<T, 256>(r, st);
+}
+
+}  // namespace
+}  // namespace serve
+}  // namespace hmm
+
+using namespace hmm;
+using namespace hmm::serve;
+
+extern "C" size_t hmm_paged_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
+                                                     int64_t n_kv_heads, int64_t D) {
+    if (n_seq < 0 || n_tokens < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256) return 0;
+    return rows_workspace(rows_dp(D));
+}
+
+extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
+                                            const void* q, int64_t q_token, int64_t q_head,
+                                            int64_t n_heads, float scale, int causal, int64_t window,
+                                            int64_t sinks, int64_t max_new, void* out, float* lse,
+                                            int32_t* device_status, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+    AttnArgs a{};
+    hmm_status_t s = check_batch(cache, batch, &a.b, &a.k, &a.v);
+    if (s != HMM_OK) return s;
+    HMM_REQUIRE(cache->D <= 256, "D must be a multiple of 8 in [8, 256], got %lld", (long long)cache->D);
+    HMM_REQUIRE(n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
+                "n_heads must be a multiple of n_kv_heads in [1, 65535], got %lld", (long long)n_heads);
+    HMM_REQUIRE(device_status, "null device_status");
+    HMM_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must be >= 0");
+    HMM_REQUIRE(causal || (window == 0 && sinks == 0), "a window and sinks need causal attention");
+    HMM_REQUIRE(max_new >= 0, "max_new must be >= 0");
+    HMM_REQUIRE(q_token >= 0 && q_token % 8 == 0 && q_head >= 0 && q_head % 8 == 0,
+                "q strides must be multiples of 8 elements");
+    HMM_REQUIRE(batch->n_tokens * n_heads / cache->n_kv_heads < (int64_t(1) << 31),
+                "n_tokens * (n_heads / n_kv_heads) must be < 2^31");
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return HMM_OK;
+    HMM_REQUIRE(q && out, "null q or out");
+    HMM_REQUIRE(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
+    const size_t need = hmm_paged_attention_workspace_size(batch->n_seq, batch->n_tokens, n_heads,
+                                                           cache->n_kv_heads, cache->D);
+    if (!workspace || workspace_bytes < need)
+        return set_error(HMM_ERR_OOM, "workspace too small: %zu < %zu", workspace_bytes, need);
+    HMM_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+    a.q = (const unsigned char*)q;
+    a.q_token = 2 * q_token;
+    a.q_head = 2 * q_head;
+    a.out = (unsigned char*)out;
+    a.lse = lse;
+    a.scale = scale;
+    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.causal = causal != 0;
+    a.window = (int)std::min<int64_t>(window, INT32_MAX);
+    a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX);
+    a.hq = (int)n_heads;
+    a.hk = (int)cache->n_kv_heads;
+    a.group = a.hq / a.hk;
+    a.D = (int)cache->D;
+    a.page_tokens = (int)cache->page_tokens;
+    a.n_pages = (int)cache->n_pages;
+    a.max_kv = batch->pages_per_seq * cache->page_tokens;
+    a.status = device_status;
+    const cudaStream_t st = (cudaStream_t)stream;
+    (void)max_new;
+    if (cache->dtype == HMM_DTYPE_BF16) return run_rows<__nv_bfloat16>(a, INT32_MAX, (unsigned char*)workspace, st);
+    return run_rows<__half>(a, INT32_MAX, (unsigned char*)workspace, st);
+}

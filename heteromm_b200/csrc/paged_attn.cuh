@@ -1,0 +1,123 @@
+// paged_attn.cuh — what the two attention kernels over a paged cache share: the
+// arguments, which keys a row sees, and a row computed from the definition.
+//
+//   o = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale q.k_i - m),  m = the largest score
+//   key i is seen from position p iff i < kv_len, (not causal or i <= p) and
+//   (no window or i > p - window or i < sinks)
+#pragma once
+
+#include "paged_serve.cuh"
+
+namespace hmm {
+namespace serve {
+
+struct AttnArgs {
+    Batch b;
+    Pages k, v;
+    const unsigned char* q;      // token / head strides in bytes
+    int64_t q_token, q_head;
+    unsigned char* out;          // [n_tokens][hq][D], contiguous
+    float* lse;                  // [n_tokens][hq] or null
+    float scale, scale_log2;     // scale * log2(e)
+    int causal, window, sinks;
+    int hq, hk, group, D, page_tokens, n_pages;
+    int64_t max_kv;
+    int32_t* status;
+};
+
+// A row of a unit (sequence, KV head): row r is new token r / group, head r % group.
+struct Span {                    // keys [0, sink) and [lo, hi) hold all that some row of a tile sees
+    int p0, p1;                  // positions of the tile's first and last row
+    int lo, hi, sink;
+};
+
+__device__ __forceinline__ Span tile_span(const AttnArgs& a, const Seq& q, int row0, int row1) {
+    Span s;
+    s.p0 = q.kv - q.n_new + row0 / a.group;
+    s.p1 = q.kv - q.n_new + (row1 - 1) / a.group;
+    s.hi = a.causal ? max(0, min(q.kv, s.p1 + 1)) : q.kv;
+    s.lo = a.window > 0 ? min(s.hi, max(0, s.p0 - a.window + 1)) : 0;
+    s.sink = a.window > 0 ? min(a.sinks, s.lo) : 0;
+    return s;
+}
+
+__device__ __forceinline__ bool span_has(const Span& s, int key) {
+    return key < s.sink || (key >= s.lo && key < s.hi);
+}
+
+__device__ __forceinline__ bool sees(const AttnArgs& a, int kv, int pos, int key) {
+    return key < kv && (!a.causal || key <= pos) &&
+           (a.window <= 0 || key > pos - a.window || key < a.sinks);
+}
+
+// The physical page of a token, or -1 with HMM_STATUS_PAGE_BOUNDS set.
+__device__ __forceinline__ int page_of(const AttnArgs& a, int s, int logical) {
+    const int e = __ldg(a.b.table + (int64_t)s * a.b.pages_per_seq + logical);
+    if (e >= 0 && e < a.n_pages) return e;
+    atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
+    return -1;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr float LN2 = 0.693147180559945309417f;
+
+// One row from the definition, by one warp, key by key in fp32: the row's
+// result where the tiled product does not hold.  A tile multiplies weights of
+// zero with the values of keys that only other rows see, and a zero times an
+// infinity or NaN there is NaN; such a row comes here, so that what a row does
+// not see never reaches it.  (It also comes here, to the same NaN or infinity,
+// when what it sees is not finite.)
+template <typename T>
+__device__ __noinline__ void attn_row_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row) {
+    constexpr int NV = 8;   // 32 lanes x 8 = D <= 256
+    const int lane = threadIdx.x & 31;
+    const int tok = q.begin + row / a.group, head = kvh * a.group + row % a.group;
+    const int pos = q.kv - q.n_new + row / a.group;
+    const Span sp = tile_span(a, q, row, row + 1);
+    const T* qr = reinterpret_cast<const T*>(a.q + tok * a.q_token + head * a.q_head);
+    float qf[NV], acc[NV], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        qf[i] = lane + 32 * i < a.D ? to_f32<T>(qr[lane + 32 * i]) : 0.0f;
+        acc[i] = 0.0f;
+    }
+    for (int key = sp.sink > 0 ? 0 : sp.lo; key < sp.hi; ++key) {
+        if (key == sp.sink && key < sp.lo) key = sp.lo;
+        if (key >= sp.hi) break;
+        if (!sees(a, q.kv, pos, key)) continue;
+        const int phys = page_of(a, s, key / a.page_tokens);
+        if (phys < 0) continue;
+        const int in = key % a.page_tokens;
+        const T* kr = reinterpret_cast<const T*>(a.k.base + phys * a.k.page + kvh * a.k.head + in * a.k.token);
+        const T* vr = reinterpret_cast<const T*>(a.v.base + phys * a.v.page + kvh * a.v.head + in * a.v.token);
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < a.D) x = fmaf(qf[i], to_f32<T>(kr[lane + 32 * i]), x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        x *= a.scale_log2;
+        const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.0f : mn;
+        const float al = ex2(m - ms), p = ex2(x - ms);
+        l = l * al + p;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < a.D) acc[i] = acc[i] * al + p * to_f32<T>(vr[lane + 32 * i]);
+    }
+    T* o = reinterpret_cast<T*>(a.out) + ((int64_t)tok * a.hq + head) * a.D;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (lane + 32 * i < a.D) o[lane + 32 * i] = l == 0.0f ? T(0.0f) : T(acc[i] * inv);
+    if (a.lse && lane == 0)
+        a.lse[(int64_t)tok * a.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+}  // namespace serve
+}  // namespace hmm

@@ -174,6 +174,40 @@ def paged_kv_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     return out
 
 
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    page_table: torch.Tensor, cu_new: torch.Tensor, kv_len: torch.Tensor, *,
+                    causal: bool = True, window: int = 0, sinks: int = 0,
+                    scale: float | None = None, max_new: int = 0, return_lse: bool = False,
+                    out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Attention of the batch's new tokens over the cache, which holds them already
+    (paged_kv_append): out [n_tokens, n_heads, D] of q's dtype, and with return_lse the
+    log of each row's sum of exponentials [n_tokens, n_heads] fp32.
+
+    A token at position p sees keys i <= p (all with causal=False) of its sequence; with a
+    window only i > p - window, and i < sinks.  One that sees none gives zeros and -inf.
+    q [n_tokens, n_heads, D]; query head h reads KV head h // (n_heads // n_kv_heads).
+    scale defaults to D ** -0.5.  max_new, a bound on the new tokens of any sequence,
+    helps to choose the kernel (decoding: 1); results do not depend on it."""
+    device, dtype, hk, _, d, cache = _cache(k_pages, v_pages)
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be [n_tokens, n_heads, D]")
+    n_tokens, heads = q.shape[:2]
+    qp = _rows(q, "q", dtype, device, n_tokens, heads, d)
+    batch = _batch(page_table, cu_new, kv_len, n_tokens, device)
+    if out is None:
+        out = torch.empty((n_tokens, heads, d), dtype=dtype, device=device)
+    else:
+        _tensor(out, "out", dtype, device, (n_tokens, heads, d))
+    lse = torch.empty((n_tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    ws = torch.empty(load().hmm_paged_attention_workspace_size(
+        batch.n_seq, n_tokens, heads, hk, d), dtype=torch.uint8, device=device)
+    _run(device, status, lambda st, stream: call(
+        "hmm_paged_attention", C.byref(cache), C.byref(batch), *qp, heads,
+        d ** -0.5 if scale is None else scale, int(causal), window, sinks, max_new, out.data_ptr(),
+        None if lse is None else lse.data_ptr(), st, ws.data_ptr(), ws.numel(), stream))
+    return (out, lse) if return_lse else out
+
+
 # ------------------------------------------------------------------ pages
 
 

@@ -373,6 +373,33 @@ hmm_status_t hmm_paged_kv_append(
     const int32_t* positions, void* q_out, int64_t out_token, int64_t out_head,
     int32_t* device_status, void* stream);
 
+/* Attention of the batch's new tokens over the cache (which holds them already):
+ *   out = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale q.k_i - max),
+ *   lse = log sum_i exp(scale q.k_i)
+ * over the keys that a token at position p sees: i < kv_len; with `causal`
+ * i <= p; with a window > 0 (causal only) i > p - window or i < sinks (a few
+ * first tokens that stay visible).  A token that sees no key (kv_len 0, or
+ * fewer cached than new tokens) gives zeros and lse -inf, as does one whose
+ * every score is -inf.  Keys and values that a token does not see never reach
+ * its result, NaN and infinities included; page-table entries are read only
+ * for pages that hold a seen key, so pages behind a window may be gone.
+ * Query head h reads KV head h / (n_heads / n_kv_heads).  fp32 scores, softmax
+ * and sums; the weights are rounded to the cache's type for the product with V.
+ * Deterministic: the same call gives the same bits.
+ *   q [n_tokens][n_heads][D] of the cache's type, 16-byte aligned, token and
+ *   head strides in elements (multiples of 8); out [n_tokens][n_heads][D] of
+ *   the same type, contiguous, 16-byte aligned; lse [n_tokens][n_heads] fp32 or NULL
+ *   max_new: a bound on the new tokens of any sequence, or 0 for none known; it
+ *   chooses between kernels and never changes which rows are computed
+ * D % 8 == 0, 8 <= D <= 256; workspace 16-byte aligned. */
+size_t hmm_paged_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
+                                          int64_t n_kv_heads, int64_t D);
+hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
+                                 const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
+                                 float scale, int causal, int64_t window, int64_t sinks,
+                                 int64_t max_new, void* out, float* lse, int32_t* device_status,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 /* Page management.  The state is the page table [n_seq][pages_per_seq] (an
  * entry below 0 holds no page), the references [n_pages] of each page (0 =
  * free) and kv_len [n_seq].  Every call reads the state from *_in and writes
