@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace hmm {
 namespace serve {
@@ -285,7 +286,7 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
             const int row = lane / 4 + 8 * h;
             const bool real = row < rows;
             const int at = row0 + (real ? row : 0);
-            pos[h] = real ? q.kv - q.n_new + at / a.group : -1;
+            pos[h] = real ? row_pos(a, q, at) : -1;
             const unsigned char* src = a.q + (int64_t)(q.begin + at / a.group) * a.q_token +
                                        (int64_t)(kvh * a.group + at % a.group) * a.q_head;
 #pragma unroll
@@ -538,18 +539,29 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     a.scale = scale;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.causal = causal != 0;
-    a.window = (int)std::min<int64_t>(window, INT32_MAX);
-    a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX);
+    a.max_kv = batch->pages_per_seq * cache->page_tokens;
+    a.window = window < a.max_kv ? (int)window : 0;   // a window over everything is none
+    a.sinks = (int)std::min<int64_t>(sinks, a.max_kv);
     a.hq = (int)n_heads;
     a.hk = (int)cache->n_kv_heads;
     a.group = a.hq / a.hk;
     a.D = (int)cache->D;
     a.page_tokens = (int)cache->page_tokens;
     a.n_pages = (int)cache->n_pages;
-    a.max_kv = batch->pages_per_seq * cache->page_tokens;
     a.status = device_status;
     const cudaStream_t st = (cudaStream_t)stream;
-    (void)max_new;
-    if (cache->dtype == HMM_DTYPE_BF16) return run_rows<__nv_bfloat16>(a, INT32_MAX, (unsigned char*)workspace, st);
-    return run_rows<__half>(a, INT32_MAX, (unsigned char*)workspace, st);
+    // A unit of up to 16 rows (one MMA's) reads its keys once either way and the
+    // many small CTAs of the rows kernel keep more reads in flight; more rows
+    // would read them again there.
+    const bool chunk = chunk_applies(a);
+    const bool few = max_new > 0 && std::min(max_new, batch->n_tokens) * a.group <= RW_ROWS;
+    const bool rows_too = few || !chunk || batch->n_seq > 1;
+    const int split = !chunk || few ? INT32_MAX : batch->n_seq == 1 ? 0 : RW_ROWS;
+    const bool bf16 = cache->dtype == HMM_DTYPE_BF16;
+    if (rows_too) {
+        s = bf16 ? run_rows<__nv_bfloat16>(a, split, (unsigned char*)workspace, st)
+                 : run_rows<__half>(a, split, (unsigned char*)workspace, st);
+        if (s != HMM_OK) return s;
+    }
+    return chunk && !few ? run_chunk(a, bf16, split == 0 ? 1 : split + 1, st) : HMM_OK;
 }

@@ -31,10 +31,15 @@ struct Span {                    // keys [0, sink) and [lo, hi) hold all that so
     int lo, hi, sink;
 };
 
+// -1 for a row before the first cached token: it sees nothing.
+__device__ __forceinline__ int row_pos(const AttnArgs& a, const Seq& q, int row) {
+    return max(-1, q.kv - q.n_new + row / a.group);
+}
+
 __device__ __forceinline__ Span tile_span(const AttnArgs& a, const Seq& q, int row0, int row1) {
     Span s;
-    s.p0 = q.kv - q.n_new + row0 / a.group;
-    s.p1 = q.kv - q.n_new + (row1 - 1) / a.group;
+    s.p0 = row_pos(a, q, row0);
+    s.p1 = row_pos(a, q, row1 - 1);
     s.hi = a.causal ? max(0, min(q.kv, s.p1 + 1)) : q.kv;
     s.lo = a.window > 0 ? min(s.hi, max(0, s.p0 - a.window + 1)) : 0;
     s.sink = a.window > 0 ? min(a.sinks, s.lo) : 0;
@@ -77,7 +82,7 @@ __device__ __noinline__ void attn_row_exact(const AttnArgs& a, int s, const Seq 
     constexpr int NV = 8;   // 32 lanes x 8 = D <= 256
     const int lane = threadIdx.x & 31;
     const int tok = q.begin + row / a.group, head = kvh * a.group + row % a.group;
-    const int pos = q.kv - q.n_new + row / a.group;
+    const int pos = row_pos(a, q, row);
     const Span sp = tile_span(a, q, row, row + 1);
     const T* qr = reinterpret_cast<const T*>(a.q + tok * a.q_token + head * a.q_head);
     float qf[NV], acc[NV], m = -INFINITY, l = 0.0f;

@@ -1,0 +1,622 @@
+// paged_attn_tc.cu — attention of chunks of new tokens over a paged cache on
+// tcgen05 tensor cores.
+//
+// A CTA takes 256 rows of one (sequence, KV head) - row = (new token, query head
+// of the group) - as two tiles of 128, and the keys they see in tiles of 128:
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: scores from
+//                   TMEM, running maximum and sum in registers, weights back to
+//                   TMEM; at the end the rows' results
+//   warp 8          TMA: K and V tiles in turn into a ring of stages, page by
+//                   page (boxes of up to 128 rows of one page and head; a box
+//                   that no row sees is asked for out of range and arrives as zeros)
+//   warp 9          MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
+//                   P_w V with P_w from TMEM over S_w's columns
+// While one tile's rows are in the exponentials the tensor cores work on the
+// other.  S_w of the next key tile is issued after P_w V of this one, so one
+// barrier per tile and direction is enough: scores that are ready imply that
+// the sum with the previous weights is complete.
+//
+// The maximum that the weights refer to is only moved when a row's has grown by
+// more than 2^8: weights then stay below 256 (exact in the fp32 sums, a common
+// factor in the result), and the sums in TMEM are rescaled rarely.
+//
+// Bound: 4 D FLOP per (row, key) on the tensor cores, against one exponential
+// per (row, key) on the special-function units, 16 a clock and SM: at D = 128
+// both take 1,024 clocks a tile.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
+#include "sm100_ptx.cuh"
+
+namespace hmm {
+namespace serve {
+using namespace sm100;
+namespace {
+
+constexpr int TC_ROWS = 128;                 // rows of a tile (MMA M, TMEM lanes)
+constexpr int TC_TILES = 2;
+constexpr int TC_CTA_ROWS = TC_ROWS * TC_TILES;
+constexpr int TC_KEYS = 128;                 // keys of a tile
+constexpr int TC_WARPS = 10;
+constexpr int TC_THREADS = 32 * TC_WARPS;
+constexpr int TC_SOFTMAX = 256;              // threads of the softmax warps
+constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
+
+template <int DP>
+__host__ __device__ constexpr int tc_stages() { return DP == 64 ? 8 : 5; }
+template <int DP>
+__host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * DP * 2; }
+template <int DP>
+__host__ __device__ constexpr int tc_q_bytes() { return TC_CTA_ROWS * DP * 2; }
+
+struct TcCtrl {
+    uint64_t full[8], empty[8];
+    uint64_t s_full[TC_TILES], p_full[TC_TILES], o_full, drain;
+    int64_t scan[TC_WARPS];
+    int64_t pre;
+    int seq;
+    uint32_t tmem;
+    int abort;
+};
+template <int DP>
+__host__ __device__ constexpr size_t tc_smem() {
+    return 1024 + tc_q_bytes<DP>() + tc_stages<DP>() * tc_tile_bytes<DP>() + sizeof(TcCtrl);
+}
+
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t ns) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, ns));
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
+                                            int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+// D[tmem] (+)= A[tmem] x B[smem desc], one CTA, kind::f16.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory descriptor of an MN-major operand (V: keys are the MMA's K, the
+// values of a key are contiguous): 128-byte rows of 64 values with the 128-byte
+// swizzle, 8 rows 1,024 bytes apart (stride offset), blocks of 64 values
+// `block` bytes apart (leading offset), version 1.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t block) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// CTAs of a sequence: row blocks x heads.
+struct TcLoad {
+    int64_t blocks;
+    int row_blocks;
+};
+
+__device__ __forceinline__ TcLoad tc_load(const TcArgs& t, const Seq& q) {
+    const int64_t rows = (int64_t)q.n_new * t.a.group;
+    TcLoad x{0, 0};
+    if (rows < t.min_rows) return x;
+    x.row_blocks = (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
+    x.blocks = (int64_t)x.row_blocks * t.a.hk;
+    return x;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ TcArgs t) {
+    constexpr int ST = tc_stages<DP>();
+    constexpr int TILE = tc_tile_bytes<DP>();
+    constexpr int HALVES = DP / 64;                    // 128-byte column blocks
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* Qs = smem;                          // [tile][half][128 rows][128 B], swizzled
+    unsigned char* Rs = Qs + tc_q_bytes<DP>();         // ring: [stage][half][128 keys][128 B]
+    TcCtrl* ctl = reinterpret_cast<TcCtrl*>(Rs + ST * TILE);
+    const AttnArgs& a = t.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- this CTA's unit
+    {
+        int64_t run = 0;
+        bool found = false;
+        for (int s0 = 0; s0 < a.b.n_seq; s0 += TC_THREADS) {
+            const int s = s0 + threadIdx.x;
+            int64_t v = 0;
+            if (s < a.b.n_seq) v = tc_load(t, load_seq(a.b, a.max_kv, s, a.status)).blocks;
+            int64_t incl = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += u;
+            }
+            if (lane == 31) ctl->scan[warp] = incl;
+            __syncthreads();
+            int64_t sum = 0;
+#pragma unroll
+            for (int w = 0; w < TC_WARPS; ++w) {
+                if (w < warp) incl += ctl->scan[w];
+                sum += ctl->scan[w];
+            }
+            incl += run;
+            if (incl - v <= (int64_t)blockIdx.x && (int64_t)blockIdx.x < incl) {
+                ctl->seq = s;
+                ctl->pre = incl - v;
+            }
+            run += sum;
+            found = run > (int64_t)blockIdx.x;
+            __syncthreads();
+            if (found) break;
+        }
+        if (!found) return;
+    }
+    const int s = ctl->seq;
+    const Seq q = load_seq(a.b, a.max_kv, s, a.status);
+    const TcLoad ld = tc_load(t, q);
+    const int unit = (int)(blockIdx.x - ctl->pre);
+    // a sequence's last rows see the most keys: they go first, so that the
+    // short blocks fill the end
+    const int kvh = unit % a.hk, rb = ld.row_blocks - 1 - unit / a.hk;
+    const int row0 = rb * TC_CTA_ROWS;
+    const int rows = (int)min((int64_t)TC_CTA_ROWS, (int64_t)q.n_new * a.group - row0);
+    const Span sp = tile_span(a, q, row0, row0 + rows);
+    const int sink_tiles = (sp.sink + TC_KEYS - 1) / TC_KEYS;
+    const int first = max(sp.lo / TC_KEYS, sink_tiles);
+    auto tiles_to = [&](int hi) { return sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - first); };
+    auto key0_of = [&](int j) { return (j < sink_tiles ? j : first + j - sink_tiles) * TC_KEYS; };
+    // key tiles of each row tile: a prefix of the CTA's
+    int n_of[TC_TILES];
+#pragma unroll
+    for (int w = 0; w < TC_TILES; ++w) {
+        const int r0 = row0 + w * TC_ROWS, r1 = min(row0 + rows, r0 + TC_ROWS);
+        n_of[w] = r0 < r1 ? tiles_to(tile_span(a, q, r0, r1).hi) : 0;
+    }
+    const int n = max(n_of[0], n_of[1]);
+    volatile int* abort = &ctl->abort;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        for (int w = 0; w < TC_TILES; ++w) {
+            mbar_init(&ctl->s_full[w], 1);
+            mbar_init(&ctl->p_full[w], 4);
+        }
+        mbar_init(&ctl->o_full, 1);
+        mbar_init(&ctl->drain, 1);
+        ctl->abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(&ctl->tmem, 512);
+        tmem_relinquish();
+    }
+    if (warp < 8) {
+        // q rows, swizzled; a negative scale turns their signs, so that the
+        // largest score is the largest product
+        constexpr int CH = DP / 8;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < TC_CTA_ROWS * CH; i += TC_SOFTMAX) {
+            const int r = i / CH, c = i % CH;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (r < rows && c * 8 < a.D) {
+                const int at = row0 + r;
+                v = __ldg(reinterpret_cast<const uint4*>(
+                        a.q + (int64_t)(q.begin + at / a.group) * a.q_token +
+                        (int64_t)(kvh * a.group + at % a.group) * a.q_head) + c);
+                v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+            }
+            const int tile = r / TC_ROWS, rr = r % TC_ROWS;
+            *reinterpret_cast<uint4*>(Qs + tile * (TC_ROWS * DP * 2) + (c >> 3) * (TC_ROWS * 128) + rr * 128 +
+                                      (((c & 7) ^ (rr & 7)) * 16)) = v;
+        }
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem;   // S_w at 128 w, O_w at 256 + DP w
+
+    if (warp == 8) {
+        // -------------------------------------------------------- producer
+        const int br = t.box_rows, subs = TC_KEYS / br;
+        if (lane == 0) {
+            prefetch_tmap(&tmK);
+            prefetch_tmap(&tmV);
+        }
+        auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
+            *page = a.n_pages;                            // out of range: zeros
+            *row = 0;
+            if (j < n && lane < subs) {
+                const int k0 = key0_of(j) + lane * br;
+                if (k0 < sp.sink || (k0 + br > sp.lo && k0 < sp.hi)) {
+                    const int e = page_of(a, s, k0 / a.page_tokens);
+                    if (e >= 0) {
+                        *page = e;
+                        *row = k0 % a.page_tokens;
+                    }
+                }
+            }
+        };
+        int page, row, issued = 0;
+        bool ok = true;
+        lookup(0, &page, &row);
+        for (int j = 0; ok && j < n; ++j) {
+            int next_page, next_row;
+            lookup(j + 1, &next_page, &next_row);
+            for (int kv = 0; kv < 2; ++kv) {
+                const int i = 2 * j + kv, st = i % ST;
+                if (!wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
+                __syncwarp();
+                issued = i + 1;
+                if (lane < subs) {
+                    const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h)
+                        tma_load_4d(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
+                                    kvh, page);
+                }
+            }
+            page = next_page;
+            row = next_row;
+        }
+        if (!ok) {
+            if (lane == 0) {
+                atomicExch(&ctl->abort, 1);
+                atomicOr(a.status, HMM_STATUS_TIMEOUT);
+            }
+            for (int i = max(0, issued - ST); i < issued; ++i)   // copies in flight land first
+                mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------- MMA
+        constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        const uint32_t id_qk = idesc_f16(TC_ROWS, TC_KEYS, FMT);
+        const uint32_t id_pv = idesc_f16(TC_ROWS, DP, FMT) | (1u << 16);   // B is MN-major
+        const uint32_t q0 = smem_u32(Qs), ring = smem_u32(Rs);
+        auto qk = [&](int w, uint32_t kt) {
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const uint32_t off = (ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32;
+                mma_f16(tmem + 128 * w, desc_k_sw128(q0 + w * (TC_ROWS * DP * 2) + off),
+                        desc_k_sw128(kt + off), id_qk, ks != 0);
+            }
+            mma_commit(&ctl->s_full[w]);
+        };
+        bool ok = n > 0;
+        if (ok) ok = wait_warp(&ctl->full[0], 0, abort, t.wait_ns);
+        if (ok && lane == 0) {
+            tc_fence_after();
+            for (int w = 0; w < TC_TILES; ++w)
+                if (n_of[w] > 0) qk(w, ring);
+            mma_commit(&ctl->empty[0]);
+        }
+        __syncwarp();
+        for (int j = 0; ok && j < n; ++j) {
+            const int iv = 2 * j + 1, sv = iv % ST, ik = 2 * j + 2, sk = ik % ST;
+            if (!wait_warp(&ctl->full[sv], (iv / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
+            const uint32_t vt = ring + sv * TILE, kt = ring + sk * TILE;
+            // V rows that no row of the CTA sees, in boxes that were read, become zeros:
+            // a weight of zero times what a slot of nobody holds is only zero then
+            const int key0 = key0_of(j);
+            if (!(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink) {
+                for (int r = lane; r < TC_KEYS; r += 32) {
+                    const int key = key0 + r, k0 = key - r % t.box_rows;
+                    if (!span_has(sp, key) &&
+                        (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                *reinterpret_cast<uint4*>(Rs + sv * TILE + h * (TC_KEYS * 128) + r * 128 + c * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            bool k_ready = false;
+            for (int w = 0; w < TC_TILES; ++w) {
+                if (j >= n_of[w]) continue;
+                if (!wait_warp(&ctl->p_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int ks = 0; ks < TC_KEYS / 16; ++ks)
+                        mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + 8 * ks,
+                                   desc_mn_sw128(vt + ks * 2048, TC_KEYS * 128), id_pv, j > 0 || ks > 0);
+                }
+                __syncwarp();
+                if (j + 1 < n_of[w]) {
+                    if (!k_ready) {
+                        if (!wait_warp(&ctl->full[sk], (ik / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
+                        k_ready = true;
+                    }
+                    if (lane == 0) qk(w, kt);
+                    __syncwarp();
+                }
+            }
+            if (!ok) break;
+            if (lane == 0) {
+                mma_commit(&ctl->empty[sv]);
+                if (j + 1 < n) mma_commit(&ctl->empty[sk]);
+                else mma_commit(&ctl->o_full);
+            }
+            __syncwarp();
+        }
+        if (n > 0 && !ok) {
+            if (lane == 0) {
+                atomicExch(&ctl->abort, 1);
+                atomicOr(a.status, HMM_STATUS_TIMEOUT);
+                mma_commit(&ctl->drain);             // the MMAs issued end before TMEM is freed
+            }
+            __syncwarp();
+            mbar_wait_drain(&ctl->drain, 0);
+        }
+    } else {
+        // --------------------------------------------------------- softmax
+        const int w = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + lanes;
+        const int r = w * TC_ROWS + (warp & 3) * 32 + lane;   // row of the CTA
+        const int wr0 = r - lane;                              // the warp's rows: [wr0, wr1)
+        const int wr1 = min(rows, wr0 + 32);
+        const int pos = row_pos(a, q, row0 + min(r, rows - 1));
+        const int pos_first = row_pos(a, q, row0 + min(wr0, rows - 1));
+        const int pos_last = row_pos(a, q, row0 + max(wr1, 1) - 1);
+        const float sc = fabsf(a.scale_log2);
+        const uint64_t sc2 = pack_f2(sc, sc);
+        float m = -INFINITY;
+        uint64_t l2 = pack_f2(0.0f, 0.0f);
+        bool ok = true;
+        const int nw = n_of[w];
+        for (int j = 0; j < nw; ++j) {
+            if (!wait_warp(&ctl->s_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[TC_KEYS];
+#pragma unroll
+            for (int c = 0; c < TC_KEYS; c += 32) tmem_ld_x32(ts + c, v + c);
+            tmem_wait_ld();
+            const int key0 = key0_of(j);
+            if (!(key0 + TC_KEYS <= q.kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
+                  (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
+                const int hi = (a.causal ? min(q.kv, pos + 1) : q.kv) - key0;
+                const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : -1;
+                const int sink = a.window > 0 ? a.sinks - key0 : 0;
+#pragma unroll
+                for (int c = 0; c < TC_KEYS; ++c)
+                    if (c >= hi || (c < lo && c >= sink)) v[c] = 0xff800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool grow = (top - m) * sc > TC_GROWTH;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float al = grow ? ex2((m - top) * sc) : 1.0f;
+                if (grow) m = top;
+                const uint64_t al2 = pack_f2(al, al);
+                l2 = fma_f2(l2, al2, pack_f2(0.0f, 0.0f));
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_x32(to + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                        tmem_st_x32(to + c, o);
+                    }
+                }
+            }
+            const float neg = m == -INFINITY ? 0.0f : -m * sc;
+            const uint64_t neg2 = pack_f2(neg, neg);
+#pragma unroll
+            for (int c0 = 0; c0 < TC_KEYS; c0 += 64) {
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int c = c0 + 2 * i;
+                    float x, y;
+                    unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2, neg2), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    l2 = add_f2(l2, pack_f2(x, y));
+                    // weights in the cache's type for the product: relative 2^-9 (bf16) or
+                    // 2^-12, the size of the output's own rounding; the sum keeps fp32
+                    p[i] = pack2<T>(x, y);
+                }
+                tmem_st_x32(ts + c0 / 2, p);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[w]);
+        }
+        // ---- the rows' results
+        if (ok && n > 0) ok = wait_warp(&ctl->o_full, 0, abort, t.wait_ns);
+        if (!ok) {
+            if (lane == 0) {
+                atomicExch(&ctl->abort, 1);
+                atomicOr(a.status, HMM_STATUS_TIMEOUT);
+            }
+        } else {
+            tc_fence_after();
+            float l, lb;
+            unpack_f2(l2, l, lb);
+            l += lb;
+            const bool live = r < rows;
+            const int at = row0 + (live ? r : 0);
+            const int64_t orow = (int64_t)(q.begin + at / a.group) * a.hq + kvh * a.group + at % a.group;
+            T* dst = reinterpret_cast<T*>(a.out) + orow * a.D;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            bool fine = l == l;
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                if (nw > 0) {
+                    tmem_ld_x32(to + c, o);
+                    tmem_wait_ld();
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            f[e] = nw > 0 && l != 0.0f ? __uint_as_float(o[i + e]) * inv : 0.0f;
+                            if (c + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
+                        }
+                        if (c + i < a.D)
+                            *reinterpret_cast<uint4*>(dst + c + i) =
+                                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
+                                           pack2<T>(f[6], f[7]));
+                    }
+                }
+            }
+            if (live && a.lse)
+                a.lse[orow] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * sc) + log2f(l)) * LN2;
+            unsigned again = __ballot_sync(0xffffffffu, live && !fine);
+            while (again) {
+                const int i = __ffs(again) - 1;
+                again &= again - 1;
+                __syncwarp();
+                attn_row_exact<T>(a, s, q, kvh, row0 + wr0 + i);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess &&
+            r == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+// A page array as a tensor (D, page_tokens, heads, pages) of boxes {64, rows, 1, 1},
+// 128-byte swizzle; values behind D and pages behind the last read as zeros.
+hmm_status_t make_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_tokens, (cuuint64_t)a.hk, (cuuint64_t)a.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)p.token, (cuuint64_t)p.head, (cuuint64_t)p.page};
+    for (int i = 0; i < 3; ++i)
+        if (dims[i + 1] == 1) strides[i] = 16;   // never stepped over
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, p.base, dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return HMM_OK;
+}
+
+template <typename T, int DP>
+hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
+                          cudaStream_t st) {
+    HMM_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)tc_smem<DP>()));
+    paged_chunk_kernel<T, DP><<<grid, TC_THREADS, tc_smem<DP>(), st>>>(k, v, t);
+    return check_launch("paged_chunk_kernel");
+}
+
+int box_rows_of(int64_t page_tokens) {
+    int64_t r = page_tokens & -page_tokens;   // the largest power of two that divides it
+    return (int)std::min<int64_t>(r, TC_KEYS);
+}
+
+}  // namespace
+
+bool chunk_applies(const AttnArgs& a) {
+    auto steps = [&](const Pages& p) {
+        return (a.page_tokens == 1 || p.token > 0) && (a.hk == 1 || p.head > 0) && (a.n_pages == 1 || p.page > 0) &&
+               p.token < (int64_t(1) << 40) && p.head < (int64_t(1) << 40) && p.page < (int64_t(1) << 40);
+    };
+    return a.D <= 128 && box_rows_of(a.page_tokens) >= 8 && a.n_pages > 0 && steps(a.k) && steps(a.v);
+}
+
+hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, cudaStream_t st) {
+    TcArgs t{a, min_rows, box_rows_of(a.page_tokens), wait_limit_ns()};
+    CUtensorMap k, v;
+    hmm_status_t s = make_map(&k, a, a.k, t.box_rows);
+    if (s != HMM_OK) return s;
+    s = make_map(&v, a, a.v, t.box_rows);
+    if (s != HMM_OK) return s;
+    // every sequence's rows in blocks: one more than its share of the tokens at most
+    const int64_t most = ((int64_t)a.b.n_tokens * a.group / TC_CTA_ROWS + a.b.n_seq) * a.hk;
+    HMM_REQUIRE(most < (int64_t(1) << 31), "n_tokens * n_heads is too large for one call");
+    const unsigned grid = (unsigned)most;
+    if (a.D <= 64)
+        return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, grid, st) : launch_chunk<__half, 64>(t, k, v, grid, st);
+    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, grid, st) : launch_chunk<__half, 128>(t, k, v, grid, st);
+}
+
+}  // namespace serve
+}  // namespace hmm
