@@ -473,10 +473,11 @@ size_t rows_workspace(int dp) {
 template <typename T, int DP>
 hmm_status_t launch_rows(const RowsArgs& r, cudaStream_t st) {
     const unsigned g = (unsigned)rows_ctas(DP);
-    HMM_CUDA_TRY(cudaFuncSetAttribute(paged_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)rows_smem<DP>()));
+    static std::atomic<uint64_t> done{0};
+    hmm_status_t s = allow_smem(paged_rows_kernel<T, DP>, rows_smem<DP>(), &done);
+    if (s != HMM_OK) return s;
     paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(r);
-    hmm_status_t s = check_launch("paged_rows_kernel");
+    s = check_launch("paged_rows_kernel");
     if (s != HMM_OK) return s;
     paged_rows_join_kernel<T, DP><<<g, RW_THREADS, 0, st>>>(r);
     return check_launch("paged_rows_join_kernel");

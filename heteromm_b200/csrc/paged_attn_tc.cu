@@ -581,8 +581,9 @@ hmm_status_t make_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box
 template <typename T, int DP>
 hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
                           cudaStream_t st) {
-    HMM_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)tc_smem<DP>()));
+    static std::atomic<uint64_t> done{0};
+    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
+    if (s != HMM_OK) return s;
     paged_chunk_kernel<T, DP><<<grid, TC_THREADS, tc_smem<DP>(), st>>>(k, v, t);
     return check_launch("paged_chunk_kernel");
 }

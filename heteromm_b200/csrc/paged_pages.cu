@@ -601,8 +601,9 @@ extern "C" hmm_status_t hmm_paged_copy_pages(const hmm_page_store_t* store, cons
         return set_error(HMM_ERR_OOM, "workspace too small: %zu < 4", workspace_bytes);
     const cudaStream_t st = (cudaStream_t)stream;
     const int64_t words = std::min<int64_t>(PG_BITMAP_WORDS, std::max<int64_t>(1, (store->n_pages + 31) / 32));
-    HMM_CUDA_TRY(cudaFuncSetAttribute(check_pairs_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      PG_BITMAP_WORDS * 4));
+    static std::atomic<uint64_t> done{0};
+    s = allow_smem(check_pairs_kernel, PG_BITMAP_WORDS * 4, &done);
+    if (s != HMM_OK) return s;
     int32_t* refused = (int32_t*)workspace;
     check_pairs_kernel<<<1, 1024, words * 4, st>>>(src, dst, (int)n, (int)store->n_pages, (int)words,
                                                    refused, device_status);

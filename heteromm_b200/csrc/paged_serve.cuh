@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "heteromm_cuda.h"
 #include "hmm_common.cuh"
 
@@ -101,7 +103,20 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return
 template <>
 __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 
-// ------------------------------------------------------------ host checks
+// ------------------------------------------------------------ host helpers
+
+// Lets kernel `fn` use `bytes` of dynamic shared memory on the current device;
+// `done` (static, one per kernel) remembers the devices that have been asked.
+template <typename F>
+hmm_status_t allow_smem(F fn, size_t bytes, std::atomic<uint64_t>* done) {
+    int dev = 0;
+    HMM_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (bit && (done->load(std::memory_order_relaxed) & bit)) return HMM_OK;
+    HMM_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done->fetch_or(bit, std::memory_order_relaxed);
+    return HMM_OK;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

@@ -22,31 +22,54 @@ HmmError itself, so inside a stream capture a status is needed.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from ._abi import HMM_DTYPE_BF16, HMM_DTYPE_F16, HMM_DTYPE_F32, PageStore, PagedBatch, PagedCache, \
     PagedState, call, load
 
 _DTYPES = {torch.bfloat16: HMM_DTYPE_BF16, torch.int16: HMM_DTYPE_BF16,
            torch.float16: HMM_DTYPE_F16}
+_i32 = torch.int32
+
+# These calls are issued once per layer and token, so the checks of a valid call are one
+# expression; what is wrong is worked out only for the message.
 
 
-def _tensor(t, name: str, dtype, device, shape=None, contiguous: bool = True):
-    """Checks one argument; `device` None accepts any CUDA device."""
+def _refuse(t, name: str, dtype, dev: int, shape) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the others are on {device}")
-    if shape is not None and tuple(t.shape) != shape:
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the others are on cuda:{dev}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _four(pages: torch.Tensor, name: str) -> torch.Tensor:
+def _tensor(t, name: str, dtype, dev: int, shape=None) -> int:
+    """The pointer of a contiguous tensor of this dtype, device and shape."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and
+            (shape is None or t.shape == shape) and t.is_contiguous()):
+        _refuse(t, name, dtype, dev, shape)
+    return t.data_ptr()
+
+
+def _rows(t, name: str, dtype, dev: int, shape):
+    """(pointer, token stride, head stride) of packed rows [n_tokens, heads, D]."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and
+            t.shape == shape):
+        _refuse(t, name, dtype, dev, shape)
+    st = t.stride()
+    if st[2] != 1 and shape[2] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr(), st[0], st[1]
+
+
+def _four(pages, name: str) -> torch.Tensor:
     if not isinstance(pages, torch.Tensor) or not pages.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if pages.dim() == 3:
@@ -60,53 +83,66 @@ def _four(pages: torch.Tensor, name: str) -> torch.Tensor:
     return pages
 
 
-def _cache(k_pages: torch.Tensor, v_pages: torch.Tensor):
-    """(device, dtype, n_kv_heads, page_tokens, D, PagedCache)."""
+def _cache(k_pages, v_pages):
+    """(device index, dtype, n_kv_heads, D, PagedCache)."""
     k, v = _four(k_pages, "k_pages"), _four(v_pages, "v_pages")
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+    shape, dtype, dev = k.shape, k.dtype, k.get_device()
+    if v.shape != shape or v.dtype is not dtype or v.get_device() != dev:
         raise ValueError("k_pages and v_pages differ in shape, dtype or device")
-    n, h, pt, d = k.shape
+    n, h, pt, d = shape
     ks, vs = k.stride(), v.stride()
-    return k.device, k.dtype, h, pt, d, PagedCache(
-        k.data_ptr(), v.data_ptr(), n, h, pt, d, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        _DTYPES[k.dtype])
+    return dev, dtype, h, d, PagedCache(k.data_ptr(), v.data_ptr(), n, h, pt, d, ks[0], ks[1], ks[2],
+                                        vs[0], vs[1], vs[2], _DTYPES[dtype])
 
 
-def _batch(page_table, cu_new, kv_len, n_tokens: int, device) -> PagedBatch:
-    _tensor(page_table, "page_table", torch.int32, device)
+def _table(page_table, dev: int):
+    """(pointer, n_seq, pages_per_seq)."""
+    p = _tensor(page_table, "page_table", _i32, dev)
     if page_table.dim() != 2:
         raise ValueError("page_table must be [n_seq, pages_per_seq]")
-    n_seq, pps = page_table.shape
-    _tensor(cu_new, "cu_new", torch.int32, device, (n_seq + 1,))
-    _tensor(kv_len, "kv_len", torch.int32, device, (n_seq,))
-    return PagedBatch(page_table.data_ptr(), n_seq, pps, cu_new.data_ptr(), n_tokens,
-                      kv_len.data_ptr())
+    return p, *page_table.shape
 
 
-def _rows(t, name: str, dtype, device, n_tokens: int, heads: int, d: int):
-    """(pointer, token stride, head stride) of packed rows [n_tokens, heads, D]."""
-    _tensor(t, name, dtype, device, (n_tokens, heads, d), contiguous=False)
-    if t.stride(2) != 1 and d > 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+def _batch(page_table, cu_new, kv_len, n_tokens: int, dev: int) -> PagedBatch:
+    p, n_seq, pps = _table(page_table, dev)
+    return PagedBatch(p, n_seq, pps, _tensor(cu_new, "cu_new", _i32, dev, (n_seq + 1,)), n_tokens,
+                      _tensor(kv_len, "kv_len", _i32, dev, (n_seq,)))
 
 
-def _run(device, status, issue):
-    """issue(status pointer, stream) on the current stream of `device`; without a
-    status waits for it and raises."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _run(device, status, issue)
-    stream = torch.cuda.current_stream().cuda_stream
-    if status is not None:
-        _tensor(status, "status", torch.int32, device)
-        if status.numel() < 1:
-            raise ValueError("status must hold an int32")
-        issue(status.data_ptr(), stream)
-        return
-    own = torch.zeros(1, dtype=torch.int32, device=device)
-    issue(own.data_ptr(), stream)
+def _on_device(f):
+    """Runs the call with the device of its first tensor as the current one."""
+    @functools.wraps(f)
+    def g(*args, **kw):
+        for t in args:
+            if t is not None:
+                break
+        else:
+            t = None
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.get_device()):
+                return f(*args, **kw)
+        return f(*args, **kw)
+    return g
+
+
+def _status(status, dev: int):
+    """(the status tensor of the call, its pointer, whether the call waits for it)."""
+    if status is None:
+        status = torch.zeros(1, dtype=_i32, device=dev)
+        return status, status.data_ptr(), True
+    if not (isinstance(status, torch.Tensor) and status.dtype is _i32 and status.get_device() == dev and
+            status.numel() > 0):
+        _refuse(status, "status", _i32, dev, (1,))
+    return status, status.data_ptr(), False
+
+
+def _wait(own, stream: int) -> None:
     call("hmm_status_read", own.data_ptr(), stream)
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(dev: int, *sizes) -> int:
+    return load().hmm_paged_attention_workspace_size(*sizes)
 
 
 def rope_table(n_pos: int, rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -119,6 +155,7 @@ def rope_table(n_pos: int, rotary_dim: int, theta: float = 10000.0, device="cuda
     return torch.stack([a.cos(), a.sin()], -1).float().contiguous().to(device)
 
 
+@_on_device
 def paged_kv_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
                     v_pages: torch.Tensor, page_table: torch.Tensor, cu_new: torch.Tensor,
                     kv_len: torch.Tensor, rope: torch.Tensor | None = None, *, q_weight=None,
@@ -133,47 +170,49 @@ def paged_kv_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     [n_tokens, n_kv_heads, D], views of one projection included.  Pairs are halves
     (i, i + pairs), or neighbours with `interleaved`; the angle's row is the token's
     position, or positions [n_tokens] int32."""
-    device, dtype, hk, _, d, cache = _cache(k_pages, v_pages)
+    dev, dtype, hk, d, cache = _cache(k_pages, v_pages)
     n_tokens = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else -1
-    kp = _rows(k, "k", dtype, device, n_tokens, hk, d)
-    vp = _rows(v, "v", dtype, device, n_tokens, hk, d)
+    kp = _rows(k, "k", dtype, dev, (n_tokens, hk, d))
+    vp = _rows(v, "v", dtype, dev, (n_tokens, hk, d))
     heads, qp, op = 0, (None, 0, 0), (None, 0, 0)
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q must be [n_tokens, n_heads, D]")
         heads = q.shape[1]
-        qp = _rows(q, "q", dtype, device, n_tokens, heads, d)
+        qp = _rows(q, "q", dtype, dev, (n_tokens, heads, d))
         if out is None:
-            out = torch.empty((n_tokens, heads, d), dtype=dtype, device=device)
-        op = _rows(out, "out", dtype, device, n_tokens, heads, d)
-    batch = _batch(page_table, cu_new, kv_len, n_tokens, device)
-    wdt, wptr = -1, [None, None]
-    for i, (w, name) in enumerate(((q_weight, "q_weight"), (k_weight, "k_weight"))):
-        if w is None:
-            continue
-        if isinstance(w, torch.Tensor) and w.dtype != dtype and w.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32 or {dtype}, got {w.dtype}")
-        _tensor(w, name, w.dtype if isinstance(w, torch.Tensor) else dtype, device, (d,))
-        this = HMM_DTYPE_F32 if w.dtype == torch.float32 else _DTYPES[dtype]
-        if wdt not in (-1, this):
-            raise TypeError("q_weight and k_weight must have the same dtype")
-        wdt, wptr[i] = this, w.data_ptr()
-    rp, n_pos, rotary = None, 0, 0
+            out = torch.empty((n_tokens, heads, d), dtype=dtype, device=q.device)
+        op = _rows(out, "out", dtype, dev, (n_tokens, heads, d))
+    batch = _batch(page_table, cu_new, kv_len, n_tokens, dev)
+    wdt, wq, wk = -1, None, None
+    if q_weight is not None or k_weight is not None:
+        w = k_weight if q_weight is None else q_weight
+        if not isinstance(w, torch.Tensor) or w.dtype not in (dtype, torch.float32):
+            raise TypeError(f"norm weights must be float32 or {dtype}")
+        wdt = HMM_DTYPE_F32 if w.dtype is torch.float32 else _DTYPES[dtype]
+        if q_weight is not None:
+            wq = _tensor(q_weight, "q_weight", w.dtype, dev, (d,))
+        if k_weight is not None:
+            wk = _tensor(k_weight, "k_weight", w.dtype, dev, (d,))
+    rp, n_pos, rotary, pp = None, 0, 0, None
     if rope is not None:
-        _tensor(rope, "rope", torch.float32, device)
+        rp = _tensor(rope, "rope", torch.float32, dev)
         if rope.dim() != 3 or rope.shape[2] != 2:
             raise ValueError("rope must be [n_pos, pairs, 2]")
-        rp, n_pos, rotary = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
+        n_pos, rotary = rope.shape[0], 2 * rope.shape[1]
     if positions is not None:
-        _tensor(positions, "positions", torch.int32, device, (n_tokens,))
-
-    _run(device, status, lambda st, stream: call(
-        "hmm_paged_kv_append", C.byref(cache), C.byref(batch), qp[0], qp[1], qp[2], heads, *kp, *vp,
-        wptr[0], wptr[1], wdt, eps, rp, n_pos, rotary, int(interleaved),
-        None if positions is None else positions.data_ptr(), op[0], op[1], op[2], st, stream))
+        pp = _tensor(positions, "positions", _i32, dev, (n_tokens,))
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_kv_append", C.byref(cache), C.byref(batch), qp[0], qp[1], qp[2], heads, kp[0],
+         kp[1], kp[2], vp[0], vp[1], vp[2], wq, wk, wdt, eps, rp, n_pos, rotary, interleaved, pp, op[0],
+         op[1], op[2], sp, stream)
+    if waits:
+        _wait(status, stream)
     return out
 
 
+@_on_device
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     page_table: torch.Tensor, cu_new: torch.Tensor, kv_len: torch.Tensor, *,
                     causal: bool = True, window: int = 0, sinks: int = 0,
@@ -188,120 +227,142 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     q [n_tokens, n_heads, D]; query head h reads KV head h // (n_heads // n_kv_heads).
     scale defaults to D ** -0.5.  max_new, a bound on the new tokens of any sequence,
     helps to choose the kernel (decoding: 1); results do not depend on it."""
-    device, dtype, hk, _, d, cache = _cache(k_pages, v_pages)
+    dev, dtype, hk, d, cache = _cache(k_pages, v_pages)
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [n_tokens, n_heads, D]")
-    n_tokens, heads = q.shape[:2]
-    qp = _rows(q, "q", dtype, device, n_tokens, heads, d)
-    batch = _batch(page_table, cu_new, kv_len, n_tokens, device)
+    n_tokens, heads, _ = shape = q.shape
+    if shape[2] != d:
+        raise ValueError(f"q has heads of {shape[2]}, the cache of {d}")
+    qp, qt, qh = _rows(q, "q", dtype, dev, shape)
+    batch = _batch(page_table, cu_new, kv_len, n_tokens, dev)
     if out is None:
-        out = torch.empty((n_tokens, heads, d), dtype=dtype, device=device)
-    else:
-        _tensor(out, "out", dtype, device, (n_tokens, heads, d))
-    lse = torch.empty((n_tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    ws = torch.empty(load().hmm_paged_attention_workspace_size(
-        batch.n_seq, n_tokens, heads, hk, d), dtype=torch.uint8, device=device)
-    _run(device, status, lambda st, stream: call(
-        "hmm_paged_attention", C.byref(cache), C.byref(batch), *qp, heads,
-        d ** -0.5 if scale is None else scale, int(causal), window, sinks, max_new, out.data_ptr(),
-        None if lse is None else lse.data_ptr(), st, ws.data_ptr(), ws.numel(), stream))
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    op = _tensor(out, "out", dtype, dev, shape)
+    lse = torch.empty((n_tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    nws = _attention_workspace(dev, batch.n_seq, n_tokens, heads, hk, d)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_attention", C.byref(cache), C.byref(batch), qp, qt, qh, heads,
+         d ** -0.5 if scale is None else scale, causal, window, sinks, max_new, op,
+         lse.data_ptr() if return_lse else None, sp, ws.data_ptr(), nws, stream)
+    if waits:
+        _wait(status, stream)
     return (out, lse) if return_lse else out
 
 
 # ------------------------------------------------------------------ pages
 
 
-def _store(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple:
-    """(device, PageStore) of page arrays [(n_layers,) n_pages, ...]; a page (all but the
-    leading dimensions) must be one block of memory."""
-    views = []
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-        if t.dim() not in (3, 4, 5):
-            raise ValueError(f"{name} must be [n_pages, n_kv_heads, page_tokens, D], with a "
-                             "leading dimension of layers or not")
-        layers, rest = (t.shape[0], t.shape[2:]) if t.dim() == 5 else (1, t.shape[1:])
-        strides = t.stride()[2:] if t.dim() == 5 else t.stride()[1:]
-        need = 1
-        for n, s in sorted(zip(rest, strides), key=lambda x: (x[1], x[0])):
-            if n != 1 and s != need:
+def _pages(t, name: str):
+    """(pointer, n_layers, layer stride, n_pages, page stride, bytes of a page) in bytes, of
+    [(n_layers,) n_pages, ...]; a page (all but the leading dimensions) must be one block."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    shape, strides, b = t.shape, t.stride(), t.element_size()
+    lead = len(shape) == 5
+    if not 3 <= len(shape) <= 5:
+        raise ValueError(f"{name} must be [n_pages, n_kv_heads, page_tokens, D], with a leading "
+                         "dimension of layers or not")
+    need = 1
+    for st, n in sorted(zip(strides[1 + lead:], shape[1 + lead:])):
+        if n != 1:
+            if st != need:
                 raise ValueError(f"{name}: a page must be one block of memory")
             need *= n
-        b = t.element_size()
-        page = t.stride(1 if t.dim() == 5 else 0) * b
-        views.append((t.data_ptr(), page, t.stride(0) * b if t.dim() == 5 else 0, need * b, layers))
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or \
-            k_pages.device != v_pages.device:
+    return (t.data_ptr(), shape[0] if lead else 1, strides[0] * b if lead else 0, shape[lead],
+            strides[lead] * b, need * b)
+
+
+def _store(k_pages, v_pages):
+    """(device index, PageStore)."""
+    kp, layers, kl, n, ks, size = _pages(k_pages, "k_pages")
+    vp, _, vl, _, vs, _ = _pages(v_pages, "v_pages")
+    dev = k_pages.get_device()
+    if k_pages.shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or v_pages.get_device() != dev:
         raise ValueError("k_pages and v_pages differ in shape, dtype or device")
-    (kp, kps, kls, nbytes, layers), (vp, vps, vls, _, _) = views
-    n_pages = k_pages.shape[1 if k_pages.dim() == 5 else 0]
-    return k_pages.device, PageStore(kp, vp, n_pages, nbytes, layers, kps, kls, vps, vls)
+    return dev, PageStore(kp, vp, n, size, layers, ks, kl, vs, vl)
 
 
-def _state(page_table, refs, kv_len, out, device):
+def _state(page_table, refs, kv_len, out, dev):
     """(PagedState, [new page_table, refs, kv_len], workspace)."""
-    _tensor(page_table, "page_table", torch.int32, device)
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [n_seq, pages_per_seq]")
-    device = page_table.device
-    n_seq, pps = page_table.shape
-    _tensor(refs, "refs", torch.int32, device)
+    tp, n_seq, pps = _table(page_table, dev)
+    rp = _tensor(refs, "refs", _i32, dev)
     if refs.dim() != 1:
         raise ValueError("refs must be [n_pages]")
+    n = refs.shape[0]
     old = [page_table, refs]
+    lp = 0
     if kv_len is not None:
-        _tensor(kv_len, "kv_len", torch.int32, device, (n_seq,))
+        lp = _tensor(kv_len, "kv_len", _i32, dev, (n_seq,))
         old.append(kv_len)
     if out is None:
         new = [torch.empty_like(t) for t in old]
+        ptr = [t.data_ptr() for t in new]
     else:
         new = list(out)
         if len(new) != len(old):
             raise ValueError(f"out must hold {len(old)} tensors")
-        for t, o, name in zip(new, old, ("page_table", "refs", "kv_len")):
-            _tensor(t, f"out {name}", torch.int32, device, tuple(o.shape))
-    ptr = [t.data_ptr() for t in old] + ([0] if kv_len is None else [])
-    nptr = [t.data_ptr() for t in new] + ([0] if kv_len is None else [])
-    ws = torch.empty(load().hmm_paged_state_workspace_size(n_seq, refs.shape[0]), dtype=torch.uint8,
-                     device=device)
-    return PagedState(*ptr, *nptr, n_seq, pps, refs.shape[0]), new, ws
+        ptr = [_tensor(t, f"out {name}", _i32, dev, o.shape)
+               for t, o, name in zip(new, old, ("page_table", "refs", "kv_len"))]
+    ws = torch.empty(_state_workspace(n_seq, n), dtype=torch.uint8, device=page_table.device)
+    return PagedState(tp, rp, lp, ptr[0], ptr[1], ptr[2] if lp else 0, n_seq, pps, n), new, ws
 
 
-def _ids(t, name: str, device, n=None) -> int:
-    _tensor(t, name, torch.int32, device)
-    if t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be a vector" + ("" if n is None else f" of {n}"))
-    return t.shape[0]
+@functools.lru_cache(maxsize=256)
+def _state_workspace(n_seq: int, n_pages: int) -> int:
+    return load().hmm_paged_state_workspace_size(n_seq, n_pages)
 
 
+def _ids(t, name: str, dev: int, shape=None) -> int:
+    p = _tensor(t, name, _i32, dev, shape)
+    if t.dim() != 1:
+        raise ValueError(f"{name} must be a vector")
+    return p
+
+
+def _device_of(t, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+@_on_device
 def paged_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor,
                      dst: torch.Tensor, *, status: torch.Tensor | None = None) -> None:
     """Copies page src[i] to page dst[i] (int32) of K and V, in every layer of
     [n_layers, n_pages, n_kv_heads, page_tokens, D] arrays; a pair with a negative entry
     is skipped.  Nothing is copied, and BOUNDS raised, if a page is out of range, a dst is
     listed twice or is another pair's src."""
-    device, store = _store(k_pages, v_pages)
-    n = _ids(src, "src", device)
-    _ids(dst, "dst", device, n)
-    ws = torch.empty(1, dtype=torch.int32, device=device)
-    _run(device, status, lambda st, stream: call(
-        "hmm_paged_copy_pages", C.byref(store), src.data_ptr(), dst.data_ptr(), n, st,
-        ws.data_ptr(), 4, stream))
+    dev, store = _store(k_pages, v_pages)
+    a = _ids(src, "src", dev)
+    b = _ids(dst, "dst", dev, src.shape)
+    ws = torch.empty(1, dtype=_i32, device=k_pages.device)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_copy_pages", C.byref(store), a, b, src.shape[0], sp, ws.data_ptr(), 4, stream)
+    if waits:
+        _wait(status, stream)
 
 
+@_on_device
 def paged_free(page_table: torch.Tensor, refs: torch.Tensor, kv_len: torch.Tensor,
                seqs: torch.Tensor, *, out=None, status: torch.Tensor | None = None):
     """Frees the sequences of `seqs` (int32; one listed twice is freed once): their pages
     lose a reference each, their rows become -1 and their lengths 0.  Returns the new
     (page_table, refs, kv_len): new tensors, or `out`, which may be the old ones."""
-    state, new, ws = _state(page_table, refs, kv_len, out, None)
-    n = _ids(seqs, "seqs", page_table.device)
-    _run(page_table.device, status, lambda st, stream: call(
-        "hmm_paged_free", C.byref(state), seqs.data_ptr(), n, st, ws.data_ptr(), ws.numel(), stream))
+    dev = _device_of(page_table, "page_table")
+    state, new, ws = _state(page_table, refs, kv_len, out, dev)
+    a = _ids(seqs, "seqs", dev)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_free", C.byref(state), a, seqs.shape[0], sp, ws.data_ptr(), ws.numel(), stream)
+    if waits:
+        _wait(status, stream)
     return tuple(new)
 
 
+@_on_device
 def paged_fork(page_table: torch.Tensor, refs: torch.Tensor, kv_len: torch.Tensor,
                src: torch.Tensor, dst: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                *, out=None, status: torch.Tensor | None = None):
@@ -309,41 +370,51 @@ def paged_fork(page_table: torch.Tensor, refs: torch.Tensor, kv_len: torch.Tenso
     filled last page is copied into the lowest free one (in every layer of
     [n_layers, n_pages, ...] arrays).  Returns the new (page_table, refs, kv_len) as
     paged_free does.  A request that cannot be met as a whole changes nothing."""
-    device, store = _store(k_pages, v_pages)
-    state, new, ws = _state(page_table, refs, kv_len, out, device)
-    n = _ids(src, "src", device)
-    _ids(dst, "dst", device, n)
-    pt = k_pages.shape[-2]
-    _run(device, status, lambda st, stream: call(
-        "hmm_paged_fork", C.byref(state), C.byref(store), pt, src.data_ptr(), dst.data_ptr(), n, st,
-        ws.data_ptr(), ws.numel(), stream))
+    dev, store = _store(k_pages, v_pages)
+    state, new, ws = _state(page_table, refs, kv_len, out, dev)
+    a = _ids(src, "src", dev)
+    b = _ids(dst, "dst", dev, src.shape)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_fork", C.byref(state), C.byref(store), k_pages.shape[-2], a, b, src.shape[0], sp,
+         ws.data_ptr(), ws.numel(), stream)
+    if waits:
+        _wait(status, stream)
     return tuple(new)
 
 
+@_on_device
 def paged_grow(page_table: torch.Tensor, refs: torch.Tensor, kv_len: torch.Tensor,
                n_new: torch.Tensor, page_tokens: int, *, out=None,
                status: torch.Tensor | None = None):
     """Makes room for n_new[s] more tokens of every sequence: entries of the pages they
     touch that hold none get the lowest free pages, in row order.  Returns the new
     (page_table, refs, kv_len + n_new) as paged_free does."""
-    state, new, ws = _state(page_table, refs, kv_len, out, None)
-    _ids(n_new, "n_new", page_table.device, page_table.shape[0])
-    _run(page_table.device, status, lambda st, stream: call(
-        "hmm_paged_grow", C.byref(state), page_tokens, n_new.data_ptr(), st, ws.data_ptr(),
-        ws.numel(), stream))
+    dev = _device_of(page_table, "page_table")
+    state, new, ws = _state(page_table, refs, kv_len, out, dev)
+    a = _ids(n_new, "n_new", dev, kv_len.shape)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_grow", C.byref(state), page_tokens, a, sp, ws.data_ptr(), ws.numel(), stream)
+    if waits:
+        _wait(status, stream)
     return tuple(new)
 
 
+@_on_device
 def paged_compact(page_table: torch.Tensor, refs: torch.Tensor, k_pages: torch.Tensor,
                   v_pages: torch.Tensor, *, out=None, status: torch.Tensor | None = None):
     """Moves the live pages (refs != 0) to the front of the cache, each at most once: the
     k-th live page behind the front goes to the k-th free one in it.  Returns
     (page_table, refs, live [1] int32); `out` holds the first two.  Page numbers kept
     elsewhere than in page_table do not follow."""
-    device, store = _store(k_pages, v_pages)
-    state, new, ws = _state(page_table, refs, None, out, device)
-    live = torch.empty(1, dtype=torch.int32, device=device)
-    _run(device, status, lambda st, stream: call(
-        "hmm_paged_compact", C.byref(state), C.byref(store), live.data_ptr(), st, ws.data_ptr(),
-        ws.numel(), stream))
+    dev, store = _store(k_pages, v_pages)
+    state, new, ws = _state(page_table, refs, None, out, dev)
+    live = torch.empty(1, dtype=_i32, device=k_pages.device)
+    status, sp, waits = _status(status, dev)
+    stream = _raw_stream(dev)
+    call("hmm_paged_compact", C.byref(state), C.byref(store), live.data_ptr(), sp, ws.data_ptr(),
+         ws.numel(), stream)
+    if waits:
+        _wait(status, stream)
     return (*new, live)
