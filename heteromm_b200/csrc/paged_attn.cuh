@@ -78,7 +78,7 @@ constexpr float LN2 = 0.693147180559945309417f;
 // not see never reaches it.  (It also comes here, to the same NaN or infinity,
 // when what it sees is not finite.)
 template <typename T>
-__device__ __noinline__ void attn_row_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row) {
+__device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row) {
     constexpr int NV = 8;   // 32 lanes x 8 = D <= 256
     const int lane = threadIdx.x & 31;
     const int tok = q.begin + row / a.group, head = kvh * a.group + row % a.group;

@@ -42,9 +42,12 @@ constexpr int TC_ROWS = 128;                 // rows of a tile (MMA M, TMEM lane
 constexpr int TC_TILES = 2;
 constexpr int TC_CTA_ROWS = TC_ROWS * TC_TILES;
 constexpr int TC_KEYS = 128;                 // keys of a tile
-constexpr int TC_WARPS = 10;
+constexpr int TC_WARPS = 12;                 // three warpgroups, the last with two warps idle
 constexpr int TC_THREADS = 32 * TC_WARPS;
 constexpr int TC_SOFTMAX = 256;              // threads of the softmax warps
+// Registers: 12 warps are launched with 168 each (64,512 in all); the two softmax
+// warpgroups take 224 (a row's 128 scores stay in registers), the third gives up to 56.
+constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
 template <int DP>
@@ -61,11 +64,23 @@ struct TcCtrl {
     int64_t pre;
     int seq;
     uint32_t tmem;
+    uint32_t again[8];   // each softmax warp's rows that came out not finite
     int abort;
 };
 template <int DP>
 __host__ __device__ constexpr size_t tc_smem() {
     return 1024 + tc_q_bytes<DP>() + tc_stages<DP>() * tc_tile_bytes<DP>() + sizeof(TcCtrl);
+}
+
+template <int N>
+__device__ __forceinline__ void set_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void set_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// All warps, between the roles and what follows.  No warp may take registers
+// back before it: the softmax warps might still be waiting for them.
+__device__ __forceinline__ void roles_done() {
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(TC_THREADS) : "memory");
 }
 
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t ns) {
@@ -269,148 +284,157 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     tc_fence_after();
     const uint32_t tmem = ctl->tmem;   // S_w at 128 w, O_w at 256 + DP w
 
-    if (warp == 8) {
-        // -------------------------------------------------------- producer
-        const int br = t.box_rows, subs = TC_KEYS / br;
-        if (lane == 0) {
-            prefetch_tmap(&tmK);
-            prefetch_tmap(&tmV);
-        }
-        auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
-            *page = a.n_pages;                            // out of range: zeros
-            *row = 0;
-            if (j < n && lane < subs) {
-                const int k0 = key0_of(j) + lane * br;
-                if (k0 < sp.sink || (k0 + br > sp.lo && k0 < sp.hi)) {
-                    const int e = page_of(a, s, k0 / a.page_tokens);
-                    if (e >= 0) {
-                        *page = e;
-                        *row = k0 % a.page_tokens;
+    // The same setmaxnreg for all warps of a warpgroup; what is outside of the roles runs
+    // with the launch's registers again.
+    if (warp >= 8) {
+        set_regs_down<TC_REGS_OTHER>();
+        if (warp == 8) {
+            // -------------------------------------------------------- producer
+            const int br = t.box_rows, subs = TC_KEYS / br;
+            if (lane == 0) {
+                prefetch_tmap(&tmK);
+                prefetch_tmap(&tmV);
+            }
+            auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
+                *page = a.n_pages;                            // out of range: zeros
+                *row = 0;
+                if (j < n && lane < subs) {
+                    const int k0 = key0_of(j) + lane * br;
+                    if (k0 < sp.sink || (k0 + br > sp.lo && k0 < sp.hi)) {
+                        const int e = page_of(a, s, k0 / a.page_tokens);
+                        if (e >= 0) {
+                            *page = e;
+                            *row = k0 % a.page_tokens;
+                        }
                     }
                 }
-            }
-        };
-        int page, row, issued = 0;
-        bool ok = true;
-        lookup(0, &page, &row);
-        for (int j = 0; ok && j < n; ++j) {
-            int next_page, next_row;
-            lookup(j + 1, &next_page, &next_row);
-            for (int kv = 0; kv < 2; ++kv) {
-                const int i = 2 * j + kv, st = i % ST;
-                if (!wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
-                __syncwarp();
-                issued = i + 1;
-                if (lane < subs) {
-                    const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h)
-                        tma_load_4d(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
-                                    kvh, page);
-                }
-            }
-            page = next_page;
-            row = next_row;
-        }
-        if (!ok) {
-            if (lane == 0) {
-                atomicExch(&ctl->abort, 1);
-                atomicOr(a.status, HMM_STATUS_TIMEOUT);
-            }
-            for (int i = max(0, issued - ST); i < issued; ++i)   // copies in flight land first
-                mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
-        }
-    } else if (warp == 9) {
-        // ------------------------------------------------------------- MMA
-        constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-        const uint32_t id_qk = idesc_f16(TC_ROWS, TC_KEYS, FMT);
-        const uint32_t id_pv = idesc_f16(TC_ROWS, DP, FMT) | (1u << 16);   // B is MN-major
-        const uint32_t q0 = smem_u32(Qs), ring = smem_u32(Rs);
-        auto qk = [&](int w, uint32_t kt) {
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                const uint32_t off = (ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32;
-                mma_f16(tmem + 128 * w, desc_k_sw128(q0 + w * (TC_ROWS * DP * 2) + off),
-                        desc_k_sw128(kt + off), id_qk, ks != 0);
-            }
-            mma_commit(&ctl->s_full[w]);
-        };
-        bool ok = n > 0;
-        if (ok) ok = wait_warp(&ctl->full[0], 0, abort, t.wait_ns);
-        if (ok && lane == 0) {
-            tc_fence_after();
-            for (int w = 0; w < TC_TILES; ++w)
-                if (n_of[w] > 0) qk(w, ring);
-            mma_commit(&ctl->empty[0]);
-        }
-        __syncwarp();
-        for (int j = 0; ok && j < n; ++j) {
-            const int iv = 2 * j + 1, sv = iv % ST, ik = 2 * j + 2, sk = ik % ST;
-            if (!wait_warp(&ctl->full[sv], (iv / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
-            const uint32_t vt = ring + sv * TILE, kt = ring + sk * TILE;
-            // V rows that no row of the CTA sees, in boxes that were read, become zeros:
-            // a weight of zero times what a slot of nobody holds is only zero then
-            const int key0 = key0_of(j);
-            if (!(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink) {
-                for (int r = lane; r < TC_KEYS; r += 32) {
-                    const int key = key0 + r, k0 = key - r % t.box_rows;
-                    if (!span_has(sp, key) &&
-                        (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
+            };
+            int page, row, issued = 0;
+            bool ok = true;
+            lookup(0, &page, &row);
+            for (int j = 0; ok && j < n; ++j) {
+                int next_page, next_row;
+                lookup(j + 1, &next_page, &next_row);
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int i = 2 * j + kv, st = i % ST;
+                    if (!wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
+                    __syncwarp();
+                    issued = i + 1;
+                    if (lane < subs) {
+                        const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
 #pragma unroll
                         for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                            for (int c = 0; c < 8; ++c)
-                                *reinterpret_cast<uint4*>(Rs + sv * TILE + h * (TC_KEYS * 128) + r * 128 + c * 16) =
-                                    make_uint4(0u, 0u, 0u, 0u);
+                            tma_load_4d(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
+                                        kvh, page);
                     }
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
+                page = next_page;
+                row = next_row;
             }
-            bool k_ready = false;
-            for (int w = 0; w < TC_TILES; ++w) {
-                if (j >= n_of[w]) continue;
-                if (!wait_warp(&ctl->p_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
-                tc_fence_after();
+            if (!ok) {
                 if (lane == 0) {
-#pragma unroll
-                    for (int ks = 0; ks < TC_KEYS / 16; ++ks)
-                        mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + 8 * ks,
-                                   desc_mn_sw128(vt + ks * 2048, TC_KEYS * 128), id_pv, j > 0 || ks > 0);
+                    atomicExch(&ctl->abort, 1);
+                    atomicOr(a.status, HMM_STATUS_TIMEOUT);
                 }
-                __syncwarp();
-                if (j + 1 < n_of[w]) {
-                    if (!k_ready) {
-                        if (!wait_warp(&ctl->full[sk], (ik / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
-                        k_ready = true;
+                for (int i = max(0, issued - ST); i < issued; ++i)   // copies in flight land first
+                    mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------- MMA
+            constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+            const uint32_t id_qk = idesc_f16(TC_ROWS, TC_KEYS, FMT);
+            const uint32_t id_pv = idesc_f16(TC_ROWS, DP, FMT) | (1u << 16);   // B is MN-major
+            const uint32_t q0 = smem_u32(Qs), ring = smem_u32(Rs);
+            auto qk = [&](int w, uint32_t kt) {
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ++ks) {
+                    const uint32_t off = (ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32;
+                    mma_f16(tmem + 128 * w, desc_k_sw128(q0 + w * (TC_ROWS * DP * 2) + off),
+                            desc_k_sw128(kt + off), id_qk, ks != 0);
+                }
+                mma_commit(&ctl->s_full[w]);
+            };
+            bool ok = n > 0;
+            if (ok) ok = wait_warp(&ctl->full[0], 0, abort, t.wait_ns);
+            if (ok && lane == 0) {
+                tc_fence_after();
+                for (int w = 0; w < TC_TILES; ++w)
+                    if (n_of[w] > 0) qk(w, ring);
+                mma_commit(&ctl->empty[0]);
+            }
+            __syncwarp();
+            for (int j = 0; ok && j < n; ++j) {
+                const int iv = 2 * j + 1, sv = iv % ST, ik = 2 * j + 2, sk = ik % ST;
+                if (!wait_warp(&ctl->full[sv], (iv / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
+                const uint32_t vt = ring + sv * TILE, kt = ring + sk * TILE;
+                // V rows that no row of the CTA sees, in boxes that were read, become zeros:
+                // a weight of zero times what a slot of nobody holds is only zero then
+                const int key0 = key0_of(j);
+                if (!(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink) {
+                    for (int r = lane; r < TC_KEYS; r += 32) {
+                        const int key = key0 + r, k0 = key - r % t.box_rows;
+                        if (!span_has(sp, key) &&
+                            (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
+#pragma unroll
+                            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                                for (int c = 0; c < 8; ++c)
+                                    *reinterpret_cast<uint4*>(Rs + sv * TILE + h * (TC_KEYS * 128) + r * 128 + c * 16) =
+                                        make_uint4(0u, 0u, 0u, 0u);
+                        }
                     }
-                    if (lane == 0) qk(w, kt);
+                    fence_proxy_async_smem();
                     __syncwarp();
                 }
+                bool k_ready = false;
+                for (int w = 0; w < TC_TILES; ++w) {
+                    if (j >= n_of[w]) continue;
+                    if (!wait_warp(&ctl->p_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
+                    tc_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (int ks = 0; ks < TC_KEYS / 16; ++ks)
+                            mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + 8 * ks,
+                                       desc_mn_sw128(vt + ks * 2048, TC_KEYS * 128), id_pv, j > 0 || ks > 0);
+                    }
+                    __syncwarp();
+                    if (j + 1 < n_of[w]) {
+                        if (!k_ready) {
+                            if (!wait_warp(&ctl->full[sk], (ik / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
+                            k_ready = true;
+                        }
+                        if (lane == 0) qk(w, kt);
+                        __syncwarp();
+                    }
+                }
+                if (!ok) break;
+                if (lane == 0) {
+                    mma_commit(&ctl->empty[sv]);
+                    if (j + 1 < n) mma_commit(&ctl->empty[sk]);
+                    else mma_commit(&ctl->o_full);
+                }
+                __syncwarp();
             }
-            if (!ok) break;
-            if (lane == 0) {
-                mma_commit(&ctl->empty[sv]);
-                if (j + 1 < n) mma_commit(&ctl->empty[sk]);
-                else mma_commit(&ctl->o_full);
+            if (n > 0 && !ok) {
+                if (lane == 0) {
+                    atomicExch(&ctl->abort, 1);
+                    atomicOr(a.status, HMM_STATUS_TIMEOUT);
+                    mma_commit(&ctl->drain);             // the MMAs issued end before TMEM is freed
+                }
+                __syncwarp();
+                mbar_wait_drain(&ctl->drain, 0);
             }
-            __syncwarp();
         }
-        if (n > 0 && !ok) {
-            if (lane == 0) {
-                atomicExch(&ctl->abort, 1);
-                atomicOr(a.status, HMM_STATUS_TIMEOUT);
-                mma_commit(&ctl->drain);             // the MMAs issued end before TMEM is freed
-            }
-            __syncwarp();
-            mbar_wait_drain(&ctl->drain, 0);
-        }
+        tc_fence_before();
+        roles_done();
+        set_regs_up<TC_REGS_LAUNCH>();   // the softmax warps have given theirs back
     } else {
         // --------------------------------------------------------- softmax
+        set_regs_up<TC_REGS_SOFTMAX>();
         const int w = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + lanes;
@@ -532,19 +556,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
             if (live && a.lse)
                 a.lse[orow] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * sc) + log2f(l)) * LN2;
-            unsigned again = __ballot_sync(0xffffffffu, live && !fine);
-            while (again) {
-                const int i = __ffs(again) - 1;
-                again &= again - 1;
-                __syncwarp();
-                attn_row_exact<T>(a, s, q, kvh, row0 + wr0 + i);
-            }
+            const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
+            if (lane == 0) ctl->again[warp] = again;
         }
+        set_regs_down<TC_REGS_LAUNCH>();
+        tc_fence_before();
+        roles_done();
     }
-    tc_fence_before();
-    __syncthreads();
     tc_fence_after();
     if (warp == 9) tmem_dealloc(tmem, 512);
+    if (warp < 8) {
+        unsigned again = ctl->abort ? 0u : ctl->again[warp];
+        while (again) {
+            const int i = __ffs(again) - 1;
+            again &= again - 1;
+            attn_row_exact<T>(a, s, q, kvh, row0 + warp * 32 + i);
+        }
+    }
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
