@@ -9,6 +9,7 @@
 //   warp 8          TMA: K and V tiles in turn into a ring of stages, page by
 //                   page (boxes of up to 128 rows of one page and head; a box
 //                   that no row sees is asked for out of range and arrives as zeros)
+//   warp 10         zeros over V rows that no row of the CTA sees (a page's end)
 //   warp 9          MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
 //                   P_w V with P_w from TMEM over S_w's columns
 // While one tile's rows are in the exponentials the tensor cores work on the
@@ -50,6 +51,13 @@ constexpr int TC_SOFTMAX = 256;              // threads of the softmax warps
 constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
+// Of 8 pairs of exponentials, those that go to the FMA pipe.
+#ifndef TC_POLY
+#define TC_POLY 0
+#endif
+constexpr float EXP2_C1 = 0.6931470036506653f, EXP2_C2 = 0.24022242426872253f, EXP2_C3 = 0.05550733581185341f,
+                EXP2_C4 = 0.009671512991189957f, EXP2_C5 = 0.001326472731307149f;
+
 template <int DP>
 __host__ __device__ constexpr int tc_stages() { return DP == 64 ? 8 : 5; }
 template <int DP>
@@ -59,7 +67,7 @@ __host__ __device__ constexpr int tc_q_bytes() { return TC_CTA_ROWS * DP * 2; }
 
 struct TcCtrl {
     uint64_t full[8], empty[8];
-    uint64_t s_full[TC_TILES], p_full[TC_TILES], o_full, drain;
+    uint64_t s_full[TC_TILES], p_full[TC_TILES][2], v_mend, v_fixed, o_full, drain;
     int64_t scan[TC_WARPS];
     int64_t pre;
     int seq;
@@ -96,15 +104,45 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// D[tmem] (+)= A[tmem] x B[smem desc], one CTA, kind::f16.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// One CTA's kind::f16 MMAs with the descriptors' halves apart: the upper words are
+// constants and the lower ones differ by constants (addresses are below 2^18, so a
+// descriptor's address field never carries), which leaves the issuing thread one
+// addition per operand.  D[tmem] (+)= A[smem] x B[smem] and D (+)= A[tmem] x B[smem].
+// One lane of the warp issues (`one`); the warp's flow stays uniform, so that the
+// operands are computed once per warp.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint32_t alo, uint32_t ahi, uint32_t blo,
+                                       uint32_t bhi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "r"(one)
         : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint32_t blo, uint32_t bhi,
+                                       uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_u32(bar)),
+        "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(one));
+    return one;
 }
 
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
@@ -149,6 +187,36 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x of a pair on the FMA pipe, x <= 2^22: x = n + f with n the nearest whole number
+// (read off the low bits of x + 1.5 2^23), 2^f on [-1/2, 1/2] by the polynomial of
+// degree 5 with p(0) = 1 that is nearest in relative error (a weighted least-squares
+// fit: 2^-23.4), and n added to the exponent.  From -127 down it is 0 (p(0) = 1 makes
+// that exact).  A NaN is lost: the caller looks for it in the maximum.
+__device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
+    unpack_f2(e, x, y);
+    e = pack_f2(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
+    const uint64_t big = pack_f2(12582912.0f, 12582912.0f), nbig = pack_f2(-12582912.0f, -12582912.0f);
+    const uint64_t t = add_f2(e, big);
+    const uint64_t f = fma_f2(add_f2(t, nbig), pack_f2(-1.0f, -1.0f), e);
+    uint64_t p = fma_f2(f, pack_f2(EXP2_C5, EXP2_C5), pack_f2(EXP2_C4, EXP2_C4));
+    p = fma_f2(f, p, pack_f2(EXP2_C3, EXP2_C3));
+    p = fma_f2(f, p, pack_f2(EXP2_C2, EXP2_C2));
+    p = fma_f2(f, p, pack_f2(EXP2_C1, EXP2_C1));
+    p = fma_f2(f, p, pack_f2(1.0f, 1.0f));
+    float tx, ty;
+    unpack_f2(t, tx, ty);
+    unpack_f2(p, x, y);
+    x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
+    y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 
 // CTAs of a sequence: row blocks x heads.
@@ -229,6 +297,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const int first = max(sp.lo / TC_KEYS, sink_tiles);
     auto tiles_to = [&](int hi) { return sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - first); };
     auto key0_of = [&](int j) { return (j < sink_tiles ? j : first + j - sink_tiles) * TC_KEYS; };
+    // tiles with keys that no row sees beside some that are seen
+    auto mends = [&](int key0) {
+        return !(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink;
+    };
     // key tiles of each row tile: a prefix of the CTA's
     int n_of[TC_TILES];
 #pragma unroll
@@ -246,8 +318,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         for (int w = 0; w < TC_TILES; ++w) {
             mbar_init(&ctl->s_full[w], 1);
-            mbar_init(&ctl->p_full[w], 4);
+            mbar_init(&ctl->p_full[w][0], 4);
+            mbar_init(&ctl->p_full[w][1], 4);
         }
+        mbar_init(&ctl->v_mend, 1);
+        mbar_init(&ctl->v_fixed, 1);
         mbar_init(&ctl->o_full, 1);
         mbar_init(&ctl->drain, 1);
         ctl->abort = 0;
@@ -344,89 +419,107 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
             }
         } else if (warp == 9) {
-            // ------------------------------------------------------------- MMA
-            constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+            // --------------------------------------------------------- MMA
+            constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
             const uint32_t id_qk = idesc_f16(TC_ROWS, TC_KEYS, FMT);
             const uint32_t id_pv = idesc_f16(TC_ROWS, DP, FMT) | (1u << 16);   // B is MN-major
-            const uint32_t q0 = smem_u32(Qs), ring = smem_u32(Rs);
-            auto qk = [&](int w, uint32_t kt) {
+            const uint32_t one = elect_one();
+            const uint64_t dk = desc_k_sw128(smem_u32(Rs)), dv = desc_mn_sw128(smem_u32(Rs), TC_KEYS * 128);
+            const uint64_t dq = desc_k_sw128(smem_u32(Qs));
+            const uint32_t khi = (uint32_t)(dk >> 32), vhi = (uint32_t)(dv >> 32);
+            const uint32_t klo = (uint32_t)dk, vlo = (uint32_t)dv, qlo = (uint32_t)dq;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int nu = __shfl_sync(0xffffffffu, n, 0);
+            const int nu_of[2] = {__shfl_sync(0xffffffffu, n_of[0], 0), __shfl_sync(0xffffffffu, n_of[1], 0)};
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                return wait_warp(bar, parity, abort, t.wait_ns);
+            };
+            auto qk = [&](int w, uint32_t k) {
+                const uint32_t ql = qlo + w * (TC_ROWS * DP * 2 / 16), d = tm + 128 * w;
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
-                    const uint32_t off = (ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32;
-                    mma_f16(tmem + 128 * w, desc_k_sw128(q0 + w * (TC_ROWS * DP * 2) + off),
-                            desc_k_sw128(kt + off), id_qk, ks != 0);
+                    const uint32_t off = ((ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32) / 16;
+                    mma_ss(one, d, ql + off, khi, k + off, khi, id_qk, ks != 0);
                 }
-                mma_commit(&ctl->s_full[w]);
+                commit_one(one, &ctl->s_full[w]);
             };
-            bool ok = n > 0;
-            if (ok) ok = wait_warp(&ctl->full[0], 0, abort, t.wait_ns);
-            if (ok && lane == 0) {
-                tc_fence_after();
-                for (int w = 0; w < TC_TILES; ++w)
-                    if (n_of[w] > 0) qk(w, ring);
-                mma_commit(&ctl->empty[0]);
+            if (nu > 0) {
+                int fixed = 0, sv = 1, pv = 0, sk = 2 % ST, pk = 2 / ST;   // stages of V_j, K_j+1 and their phases
+                bool ok = wait(&ctl->full[0], 0);
+                if (ok) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int w = 0; w < TC_TILES; ++w)
+                        if (nu_of[w] > 0) qk(w, klo);
+                    commit_one(one, &ctl->empty[0]);
+                }
+                for (int j = 0; ok && j < nu; ++j) {
+                    const uint32_t v = vlo + sv * (TILE / 16), k = klo + sk * (TILE / 16);
+                    if (!(ok = wait(&ctl->full[sv], pv))) break;
+                    if (mends(key0_of(j))) {
+                        if (lane == 0) mbar_arrive(&ctl->v_mend);
+                        if (!(ok = wait(&ctl->v_fixed, fixed++ & 1))) break;
+                    }
+                    bool k_ready = false;
+#pragma unroll
+                    for (int w = 0; w < TC_TILES; ++w) {
+                        if (j >= nu_of[w]) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (!(ok = wait(&ctl->p_full[w][h], j & 1))) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+                                mma_ts(one, tm + 256 + DP * w, tm + 128 * w + 8 * ks, v + ks * 128, vhi, id_pv,
+                                       j > 0 || ks > 0);
+                        }
+                        if (!ok) break;
+                        if (j + 1 < nu_of[w]) {
+                            if (!k_ready && !(ok = wait(&ctl->full[sk], pk))) break;
+                            k_ready = true;
+                            qk(w, k);
+                        }
+                    }
+                    if (!ok) break;
+                    commit_one(one, &ctl->empty[sv]);
+                    if (j + 1 < nu) commit_one(one, &ctl->empty[sk]);
+                    else commit_one(one, &ctl->o_full);
+                    if ((sv += 2) >= ST) { sv -= ST; pv ^= 1; }
+                    if ((sk += 2) >= ST) { sk -= ST; pk ^= 1; }
+                }
+                if (!ok) {
+                    if (lane == 0) {
+                        atomicExch(&ctl->abort, 1);
+                        atomicOr(a.status, HMM_STATUS_TIMEOUT);
+                    }
+                    commit_one(one, &ctl->drain);    // the MMAs issued end before TMEM is freed
+                    mbar_wait_drain(&ctl->drain, 0);
+                }
             }
             __syncwarp();
-            for (int j = 0; ok && j < n; ++j) {
-                const int iv = 2 * j + 1, sv = iv % ST, ik = 2 * j + 2, sk = ik % ST;
-                if (!wait_warp(&ctl->full[sv], (iv / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
-                const uint32_t vt = ring + sv * TILE, kt = ring + sk * TILE;
-                // V rows that no row of the CTA sees, in boxes that were read, become zeros:
-                // a weight of zero times what a slot of nobody holds is only zero then
-                const int key0 = key0_of(j);
-                if (!(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink) {
-                    for (int r = lane; r < TC_KEYS; r += 32) {
-                        const int key = key0 + r, k0 = key - r % t.box_rows;
-                        if (!span_has(sp, key) &&
-                            (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
+        } else if (warp == 10) {
+            // ------------------------------------------------ V's unseen rows
+            // V rows that no row of the CTA sees, in boxes that were read, become zeros:
+            // a weight of zero times what a slot of nobody holds is only zero then.
+            // The MMA lane says when such a tile has arrived, and waits: this warp, which
+            // skips the others, could not tell a stage's phases apart.
+            int mended = 0;
+            for (int j = 0; j < n; ++j) {
+                const int key0 = key0_of(j), st = (2 * j + 1) % ST;
+                if (!mends(key0)) continue;
+                if (!wait_warp(&ctl->v_mend, mended++ & 1, abort, t.wait_ns)) break;
+                for (int r = lane; r < TC_KEYS; r += 32) {
+                    const int key = key0 + r, k0 = key - r % t.box_rows;
+                    if (!span_has(sp, key) && (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
 #pragma unroll
-                            for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                                for (int c = 0; c < 8; ++c)
-                                    *reinterpret_cast<uint4*>(Rs + sv * TILE + h * (TC_KEYS * 128) + r * 128 + c * 16) =
-                                        make_uint4(0u, 0u, 0u, 0u);
-                        }
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                bool k_ready = false;
-                for (int w = 0; w < TC_TILES; ++w) {
-                    if (j >= n_of[w]) continue;
-                    if (!wait_warp(&ctl->p_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
-                    tc_fence_after();
-                    if (lane == 0) {
-#pragma unroll
-                        for (int ks = 0; ks < TC_KEYS / 16; ++ks)
-                            mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + 8 * ks,
-                                       desc_mn_sw128(vt + ks * 2048, TC_KEYS * 128), id_pv, j > 0 || ks > 0);
-                    }
-                    __syncwarp();
-                    if (j + 1 < n_of[w]) {
-                        if (!k_ready) {
-                            if (!wait_warp(&ctl->full[sk], (ik / ST) & 1, abort, t.wait_ns)) { ok = false; break; }
-                            k_ready = true;
-                        }
-                        if (lane == 0) qk(w, kt);
-                        __syncwarp();
+                        for (int c = 0; c < HALVES * 8; ++c)
+                            *reinterpret_cast<uint4*>(Rs + st * TILE + (c >> 3) * (TC_KEYS * 128) + r * 128 +
+                                                      (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                 }
-                if (!ok) break;
-                if (lane == 0) {
-                    mma_commit(&ctl->empty[sv]);
-                    if (j + 1 < n) mma_commit(&ctl->empty[sk]);
-                    else mma_commit(&ctl->o_full);
-                }
+                fence_proxy_async_smem();
                 __syncwarp();
-            }
-            if (n > 0 && !ok) {
-                if (lane == 0) {
-                    atomicExch(&ctl->abort, 1);
-                    atomicOr(a.status, HMM_STATUS_TIMEOUT);
-                    mma_commit(&ctl->drain);             // the MMAs issued end before TMEM is freed
-                }
-                __syncwarp();
-                mbar_wait_drain(&ctl->drain, 0);
+                if (lane == 0) mbar_arrive(&ctl->v_fixed);
             }
         }
         tc_fence_before();
@@ -447,8 +540,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const float sc = fabsf(a.scale_log2);
         const uint64_t sc2 = pack_f2(sc, sc);
         float m = -INFINITY;
-        uint64_t l2 = pack_f2(0.0f, 0.0f);
-        bool ok = true;
+        uint64_t l2[2] = {pack_f2(0.0f, 0.0f), pack_f2(0.0f, 0.0f)};
+        bool ok = true, fine = true;
         const int nw = n_of[w];
         for (int j = 0; j < nw; ++j) {
             if (!wait_warp(&ctl->s_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
@@ -467,16 +560,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 for (int c = 0; c < TC_KEYS; ++c)
                     if (c >= hi || (c < lo && c >= sink)) v[c] = 0xff800000u;
             }
+            // NaN and +inf show in the maximum: such a row is computed again at the end
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int c = 0; c < TC_KEYS; c += 2)
+                mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            fine = fine && top < INFINITY;
             const bool grow = (top - m) * sc > TC_GROWTH;
             if (__any_sync(0xffffffffu, grow)) {
                 const float al = grow ? ex2((m - top) * sc) : 1.0f;
                 if (grow) m = top;
                 const uint64_t al2 = pack_f2(al, al);
-                l2 = fma_f2(l2, al2, pack_f2(0.0f, 0.0f));
+                l2[0] = fma_f2(l2[0], al2, pack_f2(0.0f, 0.0f));
+                l2[1] = fma_f2(l2[1], al2, pack_f2(0.0f, 0.0f));
                 if (j > 0) {
 #pragma unroll
                     for (int c = 0; c < DP; c += 32) {
@@ -492,26 +589,32 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const float neg = m == -INFINITY ? 0.0f : -m * sc;
             const uint64_t neg2 = pack_f2(neg, neg);
 #pragma unroll
-            for (int c0 = 0; c0 < TC_KEYS; c0 += 64) {
+            for (int h = 0; h < 2; ++h) {
                 uint32_t p[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const int c = c0 + 2 * i;
+                    const int c = 64 * h + 2 * i;
+                    uint64_t e = fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2, neg2);
                     float x, y;
-                    unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2, neg2), x, y);
-                    x = ex2(x);
-                    y = ex2(y);
-                    l2 = add_f2(l2, pack_f2(x, y));
+                    if (i % 8 < TC_POLY) {
+                        exp2_pair(e, x, y);
+                    } else {
+                        unpack_f2(e, x, y);
+                        x = ex2(x);
+                        y = ex2(y);
+                    }
+                    l2[i & 1] = add_f2(l2[i & 1], pack_f2(x, y));
                     // weights in the cache's type for the product: relative 2^-9 (bf16) or
                     // 2^-12, the size of the output's own rounding; the sum keeps fp32
                     p[i] = pack2<T>(x, y);
                 }
-                tmem_st_x32(ts + c0 / 2, p);
+                // the first half's product starts while the second half is in the exponentials
+                tmem_st_x32(ts + 32 * h, p);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_full[w][h]);
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->p_full[w]);
         }
         // ---- the rows' results
         if (ok && n > 0) ok = wait_warp(&ctl->o_full, 0, abort, t.wait_ns);
@@ -523,14 +626,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         } else {
             tc_fence_after();
             float l, lb;
-            unpack_f2(l2, l, lb);
+            unpack_f2(add_f2(l2[0], l2[1]), l, lb);
             l += lb;
             const bool live = r < rows;
             const int at = row0 + (live ? r : 0);
             const int64_t orow = (int64_t)(q.begin + at / a.group) * a.hq + kvh * a.group + at % a.group;
             T* dst = reinterpret_cast<T*>(a.out) + orow * a.D;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            bool fine = l == l;
+            fine = fine && l == l;
 #pragma unroll
             for (int c = 0; c < DP; c += 32) {
                 uint32_t o[32];
