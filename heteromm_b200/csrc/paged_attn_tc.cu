@@ -3,14 +3,14 @@
 //
 // A CTA takes 256 rows of one (sequence, KV head) - row = (new token, query head
 // of the group) - as two tiles of 128, and the keys they see in tiles of 128:
-//   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: scores from
+//   warps 0-7, 8-15 softmax of row tile 0 / 1, two threads per row: scores from
 //                   TMEM, running maximum and sum in registers, weights back to
 //                   TMEM; at the end the rows' results
-//   warp 8          TMA: K and V tiles in turn into a ring of stages, page by
+//   warp 16         TMA: K and V tiles in turn into a ring of stages, page by
 //                   page (boxes of up to 128 rows of one page and head; a box
 //                   that no row sees is asked for out of range and arrives as zeros)
-//   warp 10         zeros over V rows that no row of the CTA sees (a page's end)
-//   warp 9          MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
+//   warp 18         zeros over V rows that no row of the CTA sees (a page's end)
+//   warp 17         MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
 //                   P_w V with P_w from TMEM over S_w's columns
 // While one tile's rows are in the exponentials the tensor cores work on the
 // other.  S_w of the next key tile is issued after P_w V of this one, so one
@@ -43,12 +43,13 @@ constexpr int TC_ROWS = 128;                 // rows of a tile (MMA M, TMEM lane
 constexpr int TC_TILES = 2;
 constexpr int TC_CTA_ROWS = TC_ROWS * TC_TILES;
 constexpr int TC_KEYS = 128;                 // keys of a tile
-constexpr int TC_WARPS = 12;                 // three warpgroups, the last with two warps idle
+constexpr int TC_SOFTMAX_WARPS = 16;         // two row tiles x 32 rows x two parts of the columns
+constexpr int TC_WARPS = TC_SOFTMAX_WARPS + 4;
 constexpr int TC_THREADS = 32 * TC_WARPS;
-constexpr int TC_SOFTMAX = 256;              // threads of the softmax warps
-// Registers: 12 warps are launched with 168 each (64,512 in all); the two softmax
-// warpgroups take 224 (a row's 128 scores stay in registers), the third gives up to 56.
-constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
+constexpr int TC_SOFTMAX = 32 * TC_SOFTMAX_WARPS;
+// Registers: 640 threads are launched with 96 each (61,440 in all); the softmax warps
+// take 104 (half a row's scores stay in registers), the last warpgroup gives up to 56.
+constexpr int TC_REGS_LAUNCH = 96, TC_REGS_SOFTMAX = 104, TC_REGS_OTHER = 56;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
 // Of 8 pairs of exponentials, those that go to the FMA pipe.
@@ -72,12 +73,13 @@ struct TcCtrl {
     int64_t pre;
     int seq;
     uint32_t tmem;
-    uint32_t again[8];   // each softmax warp's rows that came out not finite
+    uint32_t again[TC_SOFTMAX_WARPS];   // each softmax warp's rows that came out not finite
+    float top[2][TC_CTA_ROWS];          // [part][row] a tile's largest scores; at the end sums
     int abort;
 };
 template <int DP>
 __host__ __device__ constexpr size_t tc_smem() {
-    return 1024 + tc_q_bytes<DP>() + tc_stages<DP>() * tc_tile_bytes<DP>() + sizeof(TcCtrl);
+    return tc_q_bytes<DP>() + tc_stages<DP>() * tc_tile_bytes<DP>() + sizeof(TcCtrl);
 }
 
 template <int N>
@@ -145,16 +147,12 @@ __device__ __forceinline__ uint32_t elect_one() {
     return one;
 }
 
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-        "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -219,6 +217,38 @@ __device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
     y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 
+// Weights exp2(sc (s - m)) of 32 of a row's scores, packed in pairs, and their sum (a
+// pair of partial sums).  m = -inf (no key seen yet) gives exp2(sc s).
+template <typename T>
+__device__ __forceinline__ void weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
+                                        uint64_t* sum) {
+    const float neg = m == -INFINITY ? 0.0f : -m * sc;
+    const uint64_t neg2 = pack_f2(neg, neg);
+    uint64_t s0 = pack_f2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
+        float x, y;
+        if (i % 8 < TC_POLY) {
+            exp2_pair(e, x, y);
+        } else {
+            unpack_f2(e, x, y);
+            x = ex2(x);
+            y = ex2(y);
+        }
+        if (i & 1) s1 = add_f2(s1, pack_f2(x, y));
+        else s0 = add_f2(s0, pack_f2(x, y));
+        // weights in the cache's type for the product: relative 2^-9 (bf16) or
+        // 2^-12, the size of the output's own rounding; the sum keeps fp32
+        p[i] = pack2<T>(x, y);
+    }
+    *sum = add_f2(s0, s1);
+}
+
+__device__ __forceinline__ void pair_sync(int id) {
+    asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
+}
+
 // CTAs of a sequence: row blocks x heads.
 struct TcLoad {
     int64_t blocks;
@@ -242,8 +272,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     constexpr int TILE = tc_tile_bytes<DP>();
     constexpr int HALVES = DP / 64;                    // 128-byte column blocks
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    unsigned char* Qs = smem;                          // [tile][half][128 rows][128 B], swizzled
+    // The swizzle needs 1,024-byte alignment, which the array's alignment gives (there is
+    // no room to round up to it); should it ever not, the call says so.
+    if ((smem_u32(smem_raw) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(t.a.status, HMM_STATUS_TIMEOUT);
+        return;
+    }
+    unsigned char* Qs = smem_raw;                      // [tile][half][128 rows][128 B], swizzled
     unsigned char* Rs = Qs + tc_q_bytes<DP>();         // ring: [stage][half][128 keys][128 B]
     TcCtrl* ctl = reinterpret_cast<TcCtrl*>(Rs + ST * TILE);
     const AttnArgs& a = t.a;
@@ -318,8 +353,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         for (int w = 0; w < TC_TILES; ++w) {
             mbar_init(&ctl->s_full[w], 1);
-            mbar_init(&ctl->p_full[w][0], 4);
-            mbar_init(&ctl->p_full[w][1], 4);
+            mbar_init(&ctl->p_full[w][0], TC_SOFTMAX_WARPS / 2);
+            mbar_init(&ctl->p_full[w][1], TC_SOFTMAX_WARPS / 2);
         }
         mbar_init(&ctl->v_mend, 1);
         mbar_init(&ctl->v_fixed, 1);
@@ -328,11 +363,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         ctl->abort = 0;
         fence_barrier_init();
     }
-    if (warp == 9) {
+    if (warp == TC_SOFTMAX_WARPS + 1) {
         tmem_alloc(&ctl->tmem, 512);
         tmem_relinquish();
     }
-    if (warp < 8) {
+    if (warp < TC_SOFTMAX_WARPS) {
         // q rows, swizzled; a negative scale turns their signs, so that the
         // largest score is the largest product
         constexpr int CH = DP / 8;
@@ -361,9 +396,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 
     // The same setmaxnreg for all warps of a warpgroup; what is outside of the roles runs
     // with the launch's registers again.
-    if (warp >= 8) {
+    if (warp >= TC_SOFTMAX_WARPS) {
         set_regs_down<TC_REGS_OTHER>();
-        if (warp == 8) {
+        if (warp == TC_SOFTMAX_WARPS) {
             // -------------------------------------------------------- producer
             const int br = t.box_rows, subs = TC_KEYS / br;
             if (lane == 0) {
@@ -418,7 +453,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 for (int i = max(0, issued - ST); i < issued; ++i)   // copies in flight land first
                     mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
             }
-        } else if (warp == 9) {
+        } else if (warp == TC_SOFTMAX_WARPS + 1) {
             // --------------------------------------------------------- MMA
             constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
             const uint32_t id_qk = idesc_f16(TC_ROWS, TC_KEYS, FMT);
@@ -497,7 +532,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
             }
             __syncwarp();
-        } else if (warp == 10) {
+        } else if (warp == TC_SOFTMAX_WARPS + 2) {
             // ------------------------------------------------ V's unseen rows
             // V rows that no row of the CTA sees, in boxes that were read, become zeros:
             // a weight of zero times what a slot of nobody holds is only zero then.
@@ -528,12 +563,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     } else {
         // --------------------------------------------------------- softmax
         set_regs_up<TC_REGS_SOFTMAX>();
-        const int w = warp >> 2;
+        // Two threads share a row: part p has the scores of keys [32 p, 32 p + 32) and
+        // [64 + 32 p, 96 + 32 p) of a tile, and half of the row's results.  Two warps per
+        // row tile on each scheduler keep the special-function unit busy where one, with
+        // the maxima and the conversions between, leaves it idle half of the time.
+        const int w = warp >> 3, part = (warp >> 2) & 1;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + lanes;
+        const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + part * (DP / 2) + lanes;
         const int r = w * TC_ROWS + (warp & 3) * 32 + lane;   // row of the CTA
         const int wr0 = r - lane;                              // the warp's rows: [wr0, wr1)
         const int wr1 = min(rows, wr0 + 32);
+        const int pair = 2 + w * 4 + (warp & 3);               // barrier of the two warps of these rows
         const int pos = row_pos(a, q, row0 + min(r, rows - 1));
         const int pos_first = row_pos(a, q, row0 + min(wr0, rows - 1));
         const int pos_last = row_pos(a, q, row0 + max(wr1, 1) - 1);
@@ -544,28 +584,45 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         bool ok = true, fine = true;
         const int nw = n_of[w];
         for (int j = 0; j < nw; ++j) {
-            if (!wait_warp(&ctl->s_full[w], j & 1, abort, t.wait_ns)) { ok = false; break; }
+            // (a warp that gave up keeps the pair's count of barriers: its partner may not
+            // have, or at another tile)
+            if (ok) ok = wait_warp(&ctl->s_full[w], j & 1, abort, t.wait_ns);
+            if (!ok) {
+                pair_sync(pair);
+                continue;
+            }
             tc_fence_after();
-            uint32_t v[TC_KEYS];
-#pragma unroll
-            for (int c = 0; c < TC_KEYS; c += 32) tmem_ld_x32(ts + c, v + c);
+            uint32_t v[64];
+            tmem_ld_x32(ts + 32 * part, v);
+            tmem_ld_x32(ts + 64 + 32 * part, v + 32);
             tmem_wait_ld();
             const int key0 = key0_of(j);
             if (!(key0 + TC_KEYS <= q.kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
                   (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
-                const int hi = (a.causal ? min(q.kv, pos + 1) : q.kv) - key0;
-                const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : -1;
-                const int sink = a.window > 0 ? a.sinks - key0 : 0;
+                const int at = key0 + 32 * part;
+                const int hi = (a.causal ? min(q.kv, pos + 1) : q.kv) - at;
+                const int lo = a.window > 0 ? max(0, pos - a.window + 1) - at : -TC_KEYS;
+                const int sink = a.window > 0 ? a.sinks - at : 0;
 #pragma unroll
-                for (int c = 0; c < TC_KEYS; ++c)
-                    if (c >= hi || (c < lo && c >= sink)) v[c] = 0xff800000u;
+                for (int i = 0; i < 64; ++i) {
+                    const int c = i < 32 ? i : i + 32;
+                    if (c >= hi || (c < lo && c >= sink)) v[i] = 0xff800000u;
+                }
             }
+            // The first half's weights with the maximum so far, while this tile's is found:
+            // that is right unless the row grew by more than TC_GROWTH, which is rare.
+            uint32_t p[16];
+            uint64_t sum;
+            weights<T>(v, sc2, m, sc, p, &sum);
             // NaN and +inf show in the maximum: such a row is computed again at the end
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < TC_KEYS; c += 2)
-                mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            for (int c = 0; c < 64; c += 2)
+                mx[(c >> 1) & 1] = max3(mx[(c >> 1) & 1], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+            float top = max3(mx[0], mx[1], mx[1]);
+            ctl->top[part][r] = top;   // read before the partner's weights, and so before the next tile
+            pair_sync(pair);
+            top = max3(top, ctl->top[part ^ 1][r], top);
             fine = fine && top < INFINITY;
             const bool grow = (top - m) * sc > TC_GROWTH;
             if (__any_sync(0xffffffffu, grow)) {
@@ -575,89 +632,77 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 l2[0] = fma_f2(l2[0], al2, pack_f2(0.0f, 0.0f));
                 l2[1] = fma_f2(l2[1], al2, pack_f2(0.0f, 0.0f));
                 if (j > 0) {
-#pragma unroll
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld_x32(to + c, o);
+#pragma unroll 1
+                    for (int c = 0; c < DP / 2; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_x16(to + c, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                        tmem_st_x32(to + c, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                        tmem_st_x16(to + c, o);
                     }
                 }
+                weights<T>(v, sc2, m, sc, p, &sum);
             }
-            const float neg = m == -INFINITY ? 0.0f : -m * sc;
-            const uint64_t neg2 = pack_f2(neg, neg);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t p[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int c = 64 * h + 2 * i;
-                    uint64_t e = fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2, neg2);
-                    float x, y;
-                    if (i % 8 < TC_POLY) {
-                        exp2_pair(e, x, y);
-                    } else {
-                        unpack_f2(e, x, y);
-                        x = ex2(x);
-                        y = ex2(y);
-                    }
-                    l2[i & 1] = add_f2(l2[i & 1], pack_f2(x, y));
-                    // weights in the cache's type for the product: relative 2^-9 (bf16) or
-                    // 2^-12, the size of the output's own rounding; the sum keeps fp32
-                    p[i] = pack2<T>(x, y);
-                }
-                // the first half's product starts while the second half is in the exponentials
-                tmem_st_x32(ts + 32 * h, p);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->p_full[w][h]);
-            }
+            // the first half's product starts while the second half is in the exponentials
+            tmem_st_x16(ts + 16 * part, p);
+            l2[0] = add_f2(l2[0], sum);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
+            weights<T>(v + 32, sc2, m, sc, p, &sum);
+            tmem_st_x16(ts + 32 + 16 * part, p);
+            l2[1] = add_f2(l2[1], sum);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[w][1]);
         }
         // ---- the rows' results
         if (ok && n > 0) ok = wait_warp(&ctl->o_full, 0, abort, t.wait_ns);
-        if (!ok) {
-            if (lane == 0) {
-                atomicExch(&ctl->abort, 1);
-                atomicOr(a.status, HMM_STATUS_TIMEOUT);
-            }
-        } else {
+        float l, lb;
+        unpack_f2(add_f2(l2[0], l2[1]), l, lb);
+        ctl->top[part][r] = l + lb;
+        if (!ok && lane == 0) {
+            atomicExch(&ctl->abort, 1);
+            atomicOr(a.status, HMM_STATUS_TIMEOUT);
+        }
+        pair_sync(pair);
+        if (ok) {
             tc_fence_after();
-            float l, lb;
-            unpack_f2(add_f2(l2[0], l2[1]), l, lb);
-            l += lb;
+            l = ctl->top[0][r] + ctl->top[1][r];
             const bool live = r < rows;
             const int at = row0 + (live ? r : 0);
             const int64_t orow = (int64_t)(q.begin + at / a.group) * a.hq + kvh * a.group + at % a.group;
             T* dst = reinterpret_cast<T*>(a.out) + orow * a.D;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             fine = fine && l == l;
-#pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-                uint32_t o[32];
+#pragma unroll 1
+            for (int c = 0; c < DP / 2; c += 16) {
+                const int d = part * (DP / 2) + c;
+                uint32_t o[16];
                 if (nw > 0) {
-                    tmem_ld_x32(to + c, o);
+                    tmem_ld_x16(to + c, o);
                     tmem_wait_ld();
                 }
                 if (live) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
+                    for (int i = 0; i < 16; i += 8) {
                         float f[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             f[e] = nw > 0 && l != 0.0f ? __uint_as_float(o[i + e]) * inv : 0.0f;
-                            if (c + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
+                            if (d + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
                         }
-                        if (c + i < a.D)
-                            *reinterpret_cast<uint4*>(dst + c + i) =
+                        if (d + i < a.D)
+                            *reinterpret_cast<uint4*>(dst + d + i) =
                                 make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
                                            pack2<T>(f[6], f[7]));
                     }
                 }
             }
-            if (live && a.lse)
+            if (live && a.lse && part == 0)
                 a.lse[orow] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * sc) + log2f(l)) * LN2;
             const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
             if (lane == 0) ctl->again[warp] = again;
@@ -667,9 +712,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         roles_done();
     }
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, 512);
-    if (warp < 8) {
-        unsigned again = ctl->abort ? 0u : ctl->again[warp];
+    if (warp == TC_SOFTMAX_WARPS + 1) tmem_dealloc(tmem, 512);
+    if (warp < TC_CTA_ROWS / 32) {   // rows [32 warp, 32 warp + 32)
+        const int at = (warp >> 2) * 8 + (warp & 3);
+        unsigned again = ctl->abort ? 0u : ctl->again[at] | ctl->again[at + 4];
         while (again) {
             const int i = __ffs(again) - 1;
             again &= again - 1;
