@@ -50,14 +50,6 @@ constexpr size_t rows_smem() {
     return (size_t)RW_WARPS * RW_STAGES * 2 * RW_KEYS * DP * 2;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void ldm4(uint32_t* r, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -546,6 +538,7 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     a.hq = (int)n_heads;
     a.hk = (int)cache->n_kv_heads;
     a.group = a.hq / a.hk;
+    a.by_group = FastDiv::of(a.group);
     a.D = (int)cache->D;
     a.page_tokens = (int)cache->page_tokens;
     a.n_pages = (int)cache->n_pages;

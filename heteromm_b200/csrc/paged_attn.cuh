@@ -11,6 +11,22 @@
 namespace hmm {
 namespace serve {
 
+// n / d for 0 <= n < 2^31 by a multiplication: mul = floor(2^(31 + s) / d) + 1 with 2^s
+// the power of two at or above d.
+struct FastDiv {
+    uint32_t mul;
+    int shift;
+    __host__ static FastDiv of(int d) {
+        int s = 0;
+        while ((int64_t(1) << s) < d) ++s;
+        if (s == 0) return FastDiv{0, 0};
+        return FastDiv{(uint32_t)((uint64_t(1) << (31 + s)) / (uint64_t)d + 1), s - 1};
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return mul == 0 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
+    }
+};
+
 struct AttnArgs {
     Batch b;
     Pages k, v;
@@ -21,6 +37,7 @@ struct AttnArgs {
     float scale, scale_log2;     // scale * log2(e)
     int causal, window, sinks;
     int hq, hk, group, D, page_tokens, n_pages;
+    FastDiv by_group;
     int64_t max_kv;
     int32_t* status;
 };
@@ -33,7 +50,7 @@ struct Span {                    // keys [0, sink) and [lo, hi) hold all that so
 
 // -1 for a row before the first cached token: it sees nothing.
 __device__ __forceinline__ int row_pos(const AttnArgs& a, const Seq& q, int row) {
-    return max(-1, q.kv - q.n_new + row / a.group);
+    return max(-1, q.kv - q.n_new + a.by_group(row));
 }
 
 __device__ __forceinline__ Span tile_span(const AttnArgs& a, const Seq& q, int row0, int row1) {
@@ -62,6 +79,14 @@ __device__ __forceinline__ int page_of(const AttnArgs& a, int s, int logical) {
     atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
     return -1;
 }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

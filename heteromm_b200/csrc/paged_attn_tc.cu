@@ -68,9 +68,10 @@ __host__ __device__ constexpr int tc_q_bytes() { return TC_CTA_ROWS * DP * 2; }
 
 struct TcCtrl {
     uint64_t full[8], empty[8];
-    uint64_t s_full[TC_TILES], p_full[TC_TILES][2], v_mend, v_fixed, o_full, drain;
+    uint64_t s_full[TC_TILES], p_full[TC_TILES][2], q_full, v_mend, v_fixed, o_full, drain;
     int64_t scan[TC_WARPS];
     int64_t pre;
+    Seq own;
     int seq;
     uint32_t tmem;
     uint32_t again[TC_SOFTMAX_WARPS];   // each softmax warp's rows that came out not finite
@@ -217,32 +218,45 @@ __device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
     y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 
-// Weights exp2(sc (s - m)) of 32 of a row's scores, packed in pairs, and their sum (a
-// pair of partial sums).  m = -inf (no key seen yet) gives exp2(sc s).
-template <typename T>
-__device__ __forceinline__ void weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
-                                        uint64_t* sum) {
+// Weights exp2(sc (s - m)) of 32 of a row's scores v, packed in pairs, and their sum (a
+// pair of partial sums); with TOP also the largest of the 64 scores from v on.  m = -inf
+// (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
+// and ALU) stand between the exponentials, which keep the special-function unit for 8
+// clocks each: apart, the two would take their times in turn.
+template <typename T, bool TOP>
+__device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
+                                         uint64_t* sum) {
+    constexpr int LAG = 2;   // pairs between a weight's exponential and its use
     const float neg = m == -INFINITY ? 0.0f : -m * sc;
     const uint64_t neg2 = pack_f2(neg, neg);
     uint64_t s0 = pack_f2(0.0f, 0.0f), s1 = s0;
+    float x[16], y[16], mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
-        float x, y;
-        if (i % 8 < TC_POLY) {
-            exp2_pair(e, x, y);
-        } else {
-            unpack_f2(e, x, y);
-            x = ex2(x);
-            y = ex2(y);
+    for (int i = 0; i < 16 + LAG; ++i) {
+        if (i < 16) {
+            const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
+            if (i % 8 < TC_POLY) {
+                exp2_pair(e, x[i], y[i]);
+            } else {
+                unpack_f2(e, x[i], y[i]);
+                x[i] = ex2(x[i]);
+                if (TOP) mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
+                y[i] = ex2(y[i]);
+            }
+            if (TOP && i % 8 < TC_POLY) mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
+            if (TOP) mx1 = max3(mx1, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
         }
-        if (i & 1) s1 = add_f2(s1, pack_f2(x, y));
-        else s0 = add_f2(s0, pack_f2(x, y));
-        // weights in the cache's type for the product: relative 2^-9 (bf16) or
-        // 2^-12, the size of the output's own rounding; the sum keeps fp32
-        p[i] = pack2<T>(x, y);
+        if (i >= LAG) {
+            const int u = i - LAG;
+            if (u & 1) s1 = add_f2(s1, pack_f2(x[u], y[u]));
+            else s0 = add_f2(s0, pack_f2(x[u], y[u]));
+            // weights in the cache's type for the product: relative 2^-9 (bf16) or
+            // 2^-12, the size of the output's own rounding; the sum keeps fp32
+            p[u] = pack2<T>(x[u], y[u]);
+        }
     }
     *sum = add_f2(s0, s1);
+    return TOP ? max3(mx0, mx1, mx1) : 0.0f;
 }
 
 __device__ __forceinline__ void pair_sync(int id) {
@@ -262,6 +276,13 @@ __device__ __forceinline__ TcLoad tc_load(const TcArgs& t, const Seq& q) {
     x.row_blocks = (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
     x.blocks = (int64_t)x.row_blocks * t.a.hk;
     return x;
+}
+
+// Byte of 16-byte piece c of row r of Q: [tile][64 columns][128 rows][128 B], swizzled.
+template <int DP>
+__device__ __forceinline__ uint32_t q_at(int r, int c) {
+    const int rr = r % TC_ROWS;
+    return (r / TC_ROWS) * (TC_ROWS * DP * 2) + (c >> 3) * (TC_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) * 16);
 }
 
 template <typename T, int DP>
@@ -291,7 +312,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int s0 = 0; s0 < a.b.n_seq; s0 += TC_THREADS) {
             const int s = s0 + threadIdx.x;
             int64_t v = 0;
-            if (s < a.b.n_seq) v = tc_load(t, load_seq(a.b, a.max_kv, s, a.status)).blocks;
+            Seq mine{0, 0, 0, false};
+            if (s < a.b.n_seq) {
+                mine = load_seq(a.b, a.max_kv, s, a.status);
+                v = tc_load(t, mine).blocks;
+            }
             int64_t incl = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -309,6 +334,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             incl += run;
             if (incl - v <= (int64_t)blockIdx.x && (int64_t)blockIdx.x < incl) {
                 ctl->seq = s;
+                ctl->own = mine;
                 ctl->pre = incl - v;
             }
             run += sum;
@@ -319,7 +345,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (!found) return;
     }
     const int s = ctl->seq;
-    const Seq q = load_seq(a.b, a.max_kv, s, a.status);
+    const Seq q = ctl->own;
     const TcLoad ld = tc_load(t, q);
     const int unit = (int)(blockIdx.x - ctl->pre);
     // a sequence's last rows see the most keys: they go first, so that the
@@ -356,6 +382,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             mbar_init(&ctl->p_full[w][0], TC_SOFTMAX_WARPS / 2);
             mbar_init(&ctl->p_full[w][1], TC_SOFTMAX_WARPS / 2);
         }
+        mbar_init(&ctl->q_full, TC_SOFTMAX_WARPS);
         mbar_init(&ctl->v_mend, 1);
         mbar_init(&ctl->v_fixed, 1);
         mbar_init(&ctl->o_full, 1);
@@ -366,28 +393,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (warp == TC_SOFTMAX_WARPS + 1) {
         tmem_alloc(&ctl->tmem, 512);
         tmem_relinquish();
-    }
-    if (warp < TC_SOFTMAX_WARPS) {
-        // q rows, swizzled; a negative scale turns their signs, so that the
-        // largest score is the largest product
-        constexpr int CH = DP / 8;
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < TC_CTA_ROWS * CH; i += TC_SOFTMAX) {
-            const int r = i / CH, c = i % CH;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (r < rows && c * 8 < a.D) {
-                const int at = row0 + r;
-                v = __ldg(reinterpret_cast<const uint4*>(
-                        a.q + (int64_t)(q.begin + at / a.group) * a.q_token +
-                        (int64_t)(kvh * a.group + at % a.group) * a.q_head) + c);
-                v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-            }
-            const int tile = r / TC_ROWS, rr = r % TC_ROWS;
-            *reinterpret_cast<uint4*>(Qs + tile * (TC_ROWS * DP * 2) + (c >> 3) * (TC_ROWS * 128) + rr * 128 +
-                                      (((c & 7) ^ (rr & 7)) * 16)) = v;
-        }
-        fence_proxy_async_smem();
     }
     tc_fence_before();
     __syncthreads();
@@ -480,7 +485,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             };
             if (nu > 0) {
                 int fixed = 0, sv = 1, pv = 0, sk = 2 % ST, pk = 2 / ST;   // stages of V_j, K_j+1 and their phases
-                bool ok = wait(&ctl->full[0], 0);
+                bool ok = wait(&ctl->q_full, 0) && wait(&ctl->full[0], 0);
                 if (ok) {
                     tc_fence_after();
 #pragma unroll
@@ -567,6 +572,33 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         // [64 + 32 p, 96 + 32 p) of a tile, and half of the row's results.  Two warps per
         // row tile on each scheduler keep the special-function unit busy where one, with
         // the maxima and the conversions between, leaves it idle half of the time.
+        {
+            // q rows, swizzled
+            constexpr int CH = DP / 8;
+            const uint32_t q0 = smem_u32(Qs);
+#pragma unroll
+            for (int i = 0; i < TC_CTA_ROWS * CH / TC_SOFTMAX; ++i) {
+                const int at = i * TC_SOFTMAX + threadIdx.x, r = at / CH, c = at % CH;
+                const bool real = r < rows && c * 8 < a.D;
+                const int tok = a.by_group(row0 + (real ? r : 0)), head = row0 + (real ? r : 0) - tok * a.group;
+                cp16(q0 + q_at<DP>(r, c),
+                     a.q + (int64_t)(q.begin + tok) * a.q_token + (int64_t)(kvh * a.group + head) * a.q_head + (real ? 16 * c : 0),
+                     real);
+            }
+            cp_commit();
+            cp_wait<0>();
+            if (a.scale < 0.0f) {   // turned signs: the largest score is the largest product
+#pragma unroll 1
+                for (int i = 0; i < TC_CTA_ROWS * CH / TC_SOFTMAX; ++i) {
+                    const int at = i * TC_SOFTMAX + threadIdx.x;
+                    uint4* x = reinterpret_cast<uint4*>(Qs + q_at<DP>(at / CH, at % CH));
+                    *x = make_uint4(x->x ^ 0x80008000u, x->y ^ 0x80008000u, x->z ^ 0x80008000u, x->w ^ 0x80008000u);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->q_full);
+        }
         const int w = warp >> 3, part = (warp >> 2) & 1;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + part * (DP / 2) + lanes;
@@ -613,13 +645,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // that is right unless the row grew by more than TC_GROWTH, which is rare.
             uint32_t p[16];
             uint64_t sum;
-            weights<T>(v, sc2, m, sc, p, &sum);
-            // NaN and +inf show in the maximum: such a row is computed again at the end
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 64; c += 2)
-                mx[(c >> 1) & 1] = max3(mx[(c >> 1) & 1], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-            float top = max3(mx[0], mx[1], mx[1]);
+            // NaN and +inf show in the maximum: such a row is computed again at the end.
+            float top = weights<T, true>(v, sc2, m, sc, p, &sum);
             ctl->top[part][r] = top;   // read before the partner's weights, and so before the next tile
             pair_sync(pair);
             top = max3(top, ctl->top[part ^ 1][r], top);
@@ -642,7 +669,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         tmem_st_x16(to + c, o);
                     }
                 }
-                weights<T>(v, sc2, m, sc, p, &sum);
+                weights<T, false>(v, sc2, m, sc, p, &sum);
             }
             // the first half's product starts while the second half is in the exponentials
             tmem_st_x16(ts + 16 * part, p);
@@ -651,7 +678,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-            weights<T>(v + 32, sc2, m, sc, p, &sum);
+            weights<T, false>(v + 32, sc2, m, sc, p, &sum);
             tmem_st_x16(ts + 32 + 16 * part, p);
             l2[1] = add_f2(l2[1], sum);
             tmem_wait_st();
@@ -669,38 +696,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             atomicOr(a.status, HMM_STATUS_TIMEOUT);
         }
         pair_sync(pair);
-        if (ok) {
+        // (after a wait that ran out, too: every warp passes the same barriers, and what it
+        // writes, in its own rows, is as invalid as the call says)
+        {
             tc_fence_after();
             l = ctl->top[0][r] + ctl->top[1][r];
             const bool live = r < rows;
-            const int at = row0 + (live ? r : 0);
-            const int64_t orow = (int64_t)(q.begin + at / a.group) * a.hq + kvh * a.group + at % a.group;
-            T* dst = reinterpret_cast<T*>(a.out) + orow * a.D;
+            const int tok = a.by_group(row0 + (live ? r : 0)), head = row0 + (live ? r : 0) - tok * a.group;
+            const int64_t orow = (int64_t)(q.begin + tok) * a.hq + kvh * a.group + head;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             fine = fine && l == l;
-#pragma unroll 1
+            // through shared memory (every product is complete), rows 16 bytes apart in
+            // their banks, so that whole rows go out at once
+            constexpr int OROW = DP * 2 + 16;
+            unsigned char* os = smem_raw + r * OROW + part * DP;
+#pragma unroll
             for (int c = 0; c < DP / 2; c += 16) {
-                const int d = part * (DP / 2) + c;
                 uint32_t o[16];
                 if (nw > 0) {
                     tmem_ld_x16(to + c, o);
                     tmem_wait_ld();
                 }
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        float f[8];
+                for (int i = 0; i < 16; i += 8) {
+                    float f[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            f[e] = nw > 0 && l != 0.0f ? __uint_as_float(o[i + e]) * inv : 0.0f;
-                            if (d + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
-                        }
-                        if (d + i < a.D)
-                            *reinterpret_cast<uint4*>(dst + d + i) =
-                                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
-                                           pack2<T>(f[6], f[7]));
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] = nw > 0 && l != 0.0f ? __uint_as_float(o[i + e]) * inv : 0.0f;
+                        if (part * (DP / 2) + c + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
                     }
+                    *reinterpret_cast<uint4*>(os + 2 * (c + i)) =
+                        make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
+                                   pack2<T>(f[6], f[7]));
                 }
+            }
+            pair_sync(pair);
+            constexpr int CH = DP / 8;                 // 16-byte pieces of a row
+            const int c = lane % CH;
+#pragma unroll
+            for (int i = 0; i < 16; i += 32 / CH) {    // this warp's half of the pair's rows
+                const int rr = 16 * part + i + lane / CH;
+                const int64_t to_row = __shfl_sync(0xffffffffu, orow, rr);
+                if (wr0 + rr < rows && c * 8 < a.D)
+                    *reinterpret_cast<uint4*>(a.out + 2 * (to_row * a.D + 8 * c)) =
+                        *reinterpret_cast<const uint4*>(smem_raw + (wr0 + rr) * OROW + 16 * c);
             }
             if (live && a.lse && part == 0)
                 a.lse[orow] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * sc) + log2f(l)) * LN2;
@@ -715,7 +754,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (warp == TC_SOFTMAX_WARPS + 1) tmem_dealloc(tmem, 512);
     if (warp < TC_CTA_ROWS / 32) {   // rows [32 warp, 32 warp + 32)
         const int at = (warp >> 2) * 8 + (warp & 3);
-        unsigned again = ctl->abort ? 0u : ctl->again[at] | ctl->again[at + 4];
+        unsigned again = *abort ? 0u : ctl->again[at] | ctl->again[at + 4];
         while (again) {
             const int i = __ffs(again) - 1;
             again &= again - 1;
