@@ -7,14 +7,19 @@
 //   values: neighbours (2i, 2i+1), or halves (i, i + rotary_dim / 2)
 //
 // The pass has to read and write every value once (2 B each way) and does a
-// handful of fp32 operations on it, so HBM bounds it.  One CTA takes one token
-// with all its heads: the token's sequence, page and angles are looked up once
-// and the loads of its rows are issued before that lookup, so its latency (four
-// dependent L2 reads) is hidden behind them.  A head's row lies in a group of
-// 2^n lanes, 16 bytes a lane; the sum of squares is a butterfly in the group,
-// the partner of a halves pair comes by a shuffle (its vector is rotary_dim/16
-// lanes away), or through shared memory where rotary_dim/2 is no multiple of 8
-// or a lane holds two vectors.  A lane's angles are the same for every head.  Everything is computed in fp32 and rounded once.
+// handful of fp32 operations on it: HBM and, at 16 values a lane and ~300
+// instructions a step, the issue slots bound it.  A warp keeps a list of tokens
+// and goes through each one's rows in steps (as many rows of one kind as its lane
+// groups hold); the loads of the next steps, over the token's end too, are in
+// flight meanwhile, and the token's sequence, page and angles are looked up once.
+// Few tokens are shared by several warps, down to a step each.  Two steps in
+// flight at 5 blocks per SM measured best (8,198 tokens of 48 heads of 128: 53 us,
+// 3.9 TB/s; 4 at 4 blocks 60 us; a block per token, without lists, 66 us).
+// A head's row lies in a group of 2^n lanes with one or two 16-byte vectors
+// each; the sum of squares is a butterfly in the group.  The partner of a halves
+// pair is in the lane's other vector (a head turned as a whole), a shuffle away
+// (rotary_dim a multiple of 16), or goes through shared memory.  A lane's angles
+// are the same for every head.  Everything is computed in fp32 and rounded once.
 #include <algorithm>
 
 #include "paged_serve.cuh"
@@ -39,8 +44,8 @@ hmm_status_t check_batch(const hmm_paged_cache_t* cache, const hmm_paged_batch_t
                 (long long)batch->n_seq);
     HMM_REQUIRE(batch->pages_per_seq >= 0 && batch->pages_per_seq < (int64_t(1) << 31),
                 "pages_per_seq must be in [0, 2^31)");
-    HMM_REQUIRE(batch->n_tokens >= 0 && batch->n_tokens < (int64_t(1) << 31),
-                "n_tokens must be in [0, 2^31)");
+    HMM_REQUIRE(batch->n_tokens >= 0 && batch->n_tokens <= (int64_t(1) << 30),
+                "n_tokens must be in [0, 2^30]");
     HMM_REQUIRE(batch->pages_per_seq * cache->page_tokens < (int64_t(1) << 31),
                 "pages_per_seq * page_tokens must be < 2^31");
     if (batch->n_seq > 0 && batch->n_tokens > 0) {
@@ -67,10 +72,11 @@ hmm_status_t check_batch(const hmm_paged_cache_t* cache, const hmm_paged_batch_t
 
 namespace {
 
-constexpr int AP_THREADS = 256;
-constexpr int AP_UNROLL = 4;   // rows a lane group has in flight
+constexpr int AP_THREADS = 128;
+constexpr int AP_MINB = 5;       // blocks per SM
+constexpr int AP_DEPTH = 2;      // steps whose loads are in flight
 
-enum RopeMode { ROPE_NONE, ROPE_PAIRS, ROPE_HALVES, ROPE_HALVES_SMEM };
+enum RopeMode { ROPE_NONE, ROPE_PAIRS, ROPE_HALVES, ROPE_HALVES_LANE, ROPE_HALVES_SMEM };
 
 struct Rows {                    // one of q, k, v, q_out: strides in bytes
     unsigned char* base;
@@ -89,218 +95,304 @@ struct AppendArgs {
     int64_t max_kv;
     int n_pages;
     int hq, hk, D, vecs, half, page_tokens;
-    int lpr;                     // lanes of a row's group
-    float eps;
+    int lpr_log2;                // lanes of a row's group
+    int steps_q, steps_k;        // a token's steps of queries, and of keys or values
+    int parts;                   // warps that share a token's steps
+    int tokens_at_once;          // tokens that the grid's warps hold at once
+    float eps, inv_d;
     int32_t* status;
 };
 
+// Pairs of fp32 values: one instruction for both.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 un2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& w, float* f) {
+__device__ __forceinline__ void unpack4(const uint4& w, uint64_t* f) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 p = unpack2<T>(u[i]);
-        f[2 * i] = p.x;
-        f[2 * i + 1] = p.y;
+        f[i] = f2(p.x, p.y);
     }
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-    return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
-                      pack2<T>(f[6], f[7]));
+__device__ __forceinline__ uint4 pack4(const uint64_t* f) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = un2(f[i]);
+        u[i] = pack2<T>(p.x, p.y);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-template <typename T, int VPL, int MODE>
-__global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
-    extern __shared__ float sm[];             // ROPE_HALVES_SMEM: a row of D values per group
-    __shared__ int sh_phys, sh_row, sh_pos;   // sh_pos -1: no such token
-    const int t = blockIdx.x;
-    const int lpr = a.lpr, group = threadIdx.x / lpr, gl = threadIdx.x % lpr;
-    const int n_groups = blockDim.x / lpr;
-    const int rows = a.hq + 2 * a.hk;
-    float2 cs[VPL][8];   // (cos, sin) of each value's pair: the same for every row of the token
+// A warp's place in its list: token t, step `it` of the token's steps.  A step is
+// the rows of one kind that a warp's lane groups hold at once.
+struct Cursor {
+    int t, it;
+};
 
-    for (int r0 = group; r0 < rows + group; r0 += AP_UNROLL * n_groups) {
-        // every row's loads, before anything that depends on the token's place
-        uint4 x[AP_UNROLL][VPL];
+template <typename T, int VPL, int MODE>
+__global__ void __launch_bounds__(AP_THREADS, AP_MINB) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+    extern __shared__ float sm[];   // ROPE_HALVES_SMEM: a row of D values per group
+    const int lane = threadIdx.x & 31;
+    const int id = blockIdx.x * (AP_THREADS / 32) + (threadIdx.x >> 5);
+    const int part = id % a.parts;
+    const int lpr = 1 << a.lpr_log2, n_groups = 32 >> a.lpr_log2, group = lane >> a.lpr_log2,
+              gl = lane & (lpr - 1);
+    const int steps = a.steps_q + 2 * a.steps_k;
+    auto next = [&](Cursor& c) {
+        if ((c.it += a.parts) >= steps) {
+            c.it = part;
+            c.t += a.tokens_at_once;
+        }
+    };
+    auto kind_of = [&](int it) { return it < a.steps_q ? 0 : it < a.steps_q + a.steps_k ? 1 : 2; };
+    auto head_of = [&](int it, int kind) {
+        return (it - (kind == 0 ? 0 : kind == 1 ? a.steps_q : a.steps_q + a.steps_k)) * n_groups + group;
+    };
+    Cursor at{id / a.parts, part};
+    if (at.t >= a.tokens_at_once) return;
+    Cursor ahead = at;
+    uint4 x[AP_DEPTH][VPL];
+    auto load = [&](uint4* v) {     // the rows of `ahead`, which moves on
+        if (ahead.t >= a.b.n_tokens) return;
+        const int kind = kind_of(ahead.it), h = head_of(ahead.it, kind);
+        const Rows& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+        const unsigned char* src = in.base + ahead.t * in.token + h * in.head + 16 * gl;
 #pragma unroll
-        for (int u = 0; u < AP_UNROLL; ++u) {
-            const int r = r0 + u * n_groups;
-            const bool is_q = r < a.hq, is_k = !is_q && r < a.hq + a.hk;
-            const Rows& in = is_q ? a.q : is_k ? a.k : a.v;
-            const int h = is_q ? r : is_k ? r - a.hq : r - a.hq - a.hk;
-            const unsigned char* src = in.base + t * in.token + h * in.head;
+        for (int j = 0; j < VPL; ++j)
+            v[j] = h < (kind == 0 ? a.hq : a.hk) && gl + j * lpr < a.vecs
+                       ? *reinterpret_cast<const uint4*>(src + 16 * j * lpr)
+                       : make_uint4(0u, 0u, 0u, 0u);
+        next(ahead);
+    };
+#pragma unroll
+    for (int u = 0; u < AP_DEPTH; ++u) load(x[u]);
+
+    int token = -1, weight_of = -1;
+    bool ok = false;
+    int slot = 0;
+    int64_t phys = 0;
+    const void* w = nullptr;
+    uint64_t wf[VPL][4];
+    // The angles of the lane's values, the same for every row.  ROPE_PAIRS: (cos, cos) and
+    // (-sin, sin) of each pair.  Else of values 2 i, 2 i + 1 as pairs, for the first vector
+    // alone where the second holds the partners.
+    constexpr int CV = MODE == ROPE_HALVES_LANE ? 1 : VPL;
+    uint64_t c[CV][4], sn[CV][4];
+
+    // The place and angles of token t; false for a padding row and one that is flagged.
+    auto place = [&](int t) {
+        const int s = warp_find_seq(a.b, t);
+        const int begin = __ldg(a.b.cu + s), end = __ldg(a.b.cu + s + 1), kv = __ldg(a.b.kv_len + s);
+        if (t < begin || t >= end) {
+            // a padding row, left as it is (or cu_new is not ascending)
+            if (lane == 0 && t >= __ldg(a.b.cu) && t < __ldg(a.b.cu + a.b.n_seq))
+                atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);
+            return false;
+        }
+        const int64_t p = (int64_t)kv - (end - begin) + (t - begin);
+        const int64_t ap = MODE == ROPE_NONE ? 0 : a.positions ? (int64_t)__ldg(a.positions + t) : p;
+        if (begin < 0 || end > a.b.n_tokens || kv < 0 || kv > a.max_kv || p < 0 ||
+            (MODE != ROPE_NONE && (ap < 0 || ap >= a.n_pos))) {
+            if (lane == 0) atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);
+            return false;
+        }
+        const int logical = (int)p / a.page_tokens;
+        slot = (int)p - logical * a.page_tokens;
+        phys = __ldg(a.b.table + (int64_t)s * a.b.pages_per_seq + logical);
+        if (phys < 0 || phys >= a.n_pages) {
+            if (lane == 0) atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
+            return false;
+        }
+        if (MODE != ROPE_NONE) {
+            const float2* row = reinterpret_cast<const float2*>(a.rope) + ap * a.half;
+#pragma unroll
+            for (int j = 0; j < CV; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * (gl + j * lpr) + 2 * i;
+                    if (MODE == ROPE_PAIRS) {   // a' = a c - b s, b' = b c + a s on (a, b)
+                        const float2 cs = e < 2 * a.half ? __ldg(row + (e >> 1)) : make_float2(1.0f, 0.0f);
+                        c[j][i] = f2(cs.x, cs.x);
+                        sn[j][i] = f2(-cs.y, cs.y);
+                    } else {                    // each value times cos, its partner times -sin (first half) or sin
+                        float2 cs[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            cs[k] = e + k < 2 * a.half ? __ldg(row + (e + k < a.half ? e + k : e + k - a.half))
+                                                       : make_float2(1.0f, 0.0f);
+                        c[j][i] = f2(cs[0].x, cs[1].x);
+                        sn[j][i] = f2(e < a.half ? -cs[0].y : cs[0].y, e + 1 < a.half ? -cs[1].y : cs[1].y);
+                    }
+                }
+        }
+        return true;
+    };
+
+    auto step = [&](const uint4* v) {   // the rows of `at`
+        if (at.t != token) {
+            token = at.t;
+            ok = place(token);
+        }
+        if (!ok) return;
+        const int kind = kind_of(at.it), h = head_of(at.it, kind);
+        const bool live = h < (kind == 0 ? a.hq : a.hk);
+        const Pages& pg = kind == 1 ? a.k_pages : a.v_pages;
+        unsigned char* dst = (kind == 0 ? a.out.base + token * a.out.token + h * a.out.head
+                                        : pg.base + phys * pg.page + slot * pg.token + h * pg.head) + 16 * gl;
+        if (kind == 2) {   // values are stored as they are
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (live && gl + j * lpr < a.vecs) *reinterpret_cast<uint4*>(dst + 16 * j * lpr) = v[j];
+            return;
+        }
+        if (kind != weight_of) {
+            weight_of = kind;
+            w = a.w[kind];
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int vi = min(gl + j * lpr, a.vecs - 1);
+                if (!w) {
+                } else if (a.w_f32) {
+                    const float4* p = reinterpret_cast<const float4*>(w) + 2 * vi;
+                    const float4 lo = __ldg(p), hi = __ldg(p + 1);
+                    wf[j][0] = f2(lo.x, lo.y); wf[j][1] = f2(lo.z, lo.w);
+                    wf[j][2] = f2(hi.x, hi.y); wf[j][3] = f2(hi.z, hi.w);
+                } else {
+                    unpack4<T>(__ldg(reinterpret_cast<const uint4*>(w) + vi), wf[j]);
+                }
+            }
+        }
+        uint64_t y[VPL][4];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) unpack4<T>(v[j], y[j]);
+        if (w) {
+            uint64_t s2 = mul2(y[0][0], y[0][0]);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i + j > 0) s2 = fma2(y[j][i], y[j][i], s2);
+            const float2 s1 = un2(s2);
+            float ss = s1.x + s1.y;
+            for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = rsqrtf(fmaf(ss, a.inv_d, a.eps));
+            const uint64_t inv2 = f2(inv, inv);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[j][i] = mul2(mul2(y[j][i], inv2), wf[j][i]);
+        }
+        if (MODE == ROPE_PAIRS) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (8 * (gl + j * lpr) + 2 * i >= 2 * a.half) continue;   // as it is, infinities too
+                    const float2 ab = un2(y[j][i]);
+                    y[j][i] = fma2(f2(ab.y, ab.x), sn[j][i], mul2(y[j][i], c[j][i]));
+                }
+        } else if (MODE == ROPE_HALVES_LANE) {
+            // vectors gl and gl + lpr of the row: value e and its partner e + half
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t p0 = y[0][i], p1 = y[VPL - 1][i];
+                const float2 sv = un2(sn[0][i]);
+                y[0][i] = fma2(p1, sn[0][i], mul2(p0, c[0][i]));
+                y[VPL - 1][i] = fma2(p0, f2(-sv.x, -sv.y), mul2(p1, c[0][i]));
+            }
+        } else if (MODE == ROPE_HALVES) {
+            // vector gl holds values [8 gl, 8 gl + 8); half is a multiple of 8
+            const int hv = a.half >> 3;
+            const bool turned = gl < 2 * hv;
+            const int partner = gl < hv ? gl + hv : turned ? gl - hv : gl;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 ab = un2(y[0][i]);
+                const float o0 = __shfl_sync(0xffffffffu, ab.x, partner, lpr);
+                const float o1 = __shfl_sync(0xffffffffu, ab.y, partner, lpr);
+                if (turned) y[0][i] = fma2(f2(o0, o1), sn[0][i], mul2(y[0][i], c[0][i]));
+            }
+        } else if (MODE == ROPE_HALVES_SMEM) {
+            float* row = sm + ((threadIdx.x >> 5) * n_groups + group) * a.D;
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
                 const int vi = gl + j * lpr;
-                x[u][j] = r < rows && vi < a.vecs ? *reinterpret_cast<const uint4*>(src + 16 * vi)
-                                                  : make_uint4(0u, 0u, 0u, 0u);
+                if (vi < a.vecs) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 ab = un2(y[j][i]);
+                        row[8 * vi + 2 * i] = ab.x;
+                        row[8 * vi + 2 * i + 1] = ab.y;
+                    }
+                }
             }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * (gl + j * lpr) + 2 * i;
+                    const float2 ab = un2(y[j][i]), cc = un2(c[j][i]), ss = un2(sn[j][i]);
+                    float2 r = ab;
+                    if (e < 2 * a.half) r.x = ab.x * cc.x + row[e < a.half ? e + a.half : e - a.half] * ss.x;
+                    if (e + 1 < 2 * a.half)
+                        r.y = ab.y * cc.y + row[e + 1 < a.half ? e + 1 + a.half : e + 1 - a.half] * ss.y;
+                    y[j][i] = f2(r.x, r.y);
+                }
+            __syncwarp();
         }
-        if (r0 == group) {
-            if (threadIdx.x < 32) {
-                const int s = warp_find_seq(a.b, t);
-                if (threadIdx.x == 0) {
-                    int phys = -1, row = 0, pos = -1;
-                    const int begin = __ldg(a.b.cu + s), end = __ldg(a.b.cu + s + 1);
-                    if (begin <= t && t < end) {
-                        const int kv = __ldg(a.b.kv_len + s);
-                        const int64_t p = (int64_t)kv - (end - begin) + (t - begin);
-                        if (begin < 0 || end > a.b.n_tokens || kv < 0 || kv > a.max_kv || p < 0) {
-                            atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);
-                        } else {
-                            const int e = __ldg(a.b.table + (int64_t)s * a.b.pages_per_seq +
-                                                p / a.page_tokens);
-                            const int64_t ap = a.positions ? (int64_t)__ldg(a.positions + t) : p;
-                            if (e < 0 || e >= a.n_pages) {
-                                atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
-                            } else if (MODE != ROPE_NONE && (ap < 0 || ap >= a.n_pos)) {
-                                atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);
-                            } else {
-                                phys = e;
-                                row = (int)(p % a.page_tokens);
-                                pos = MODE == ROPE_NONE ? 0 : (int)ap;
-                            }
-                        }
-                    } else if (t < __ldg(a.b.cu + a.b.n_seq) && t >= __ldg(a.b.cu)) {
-                        atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);   // cu_new is not ascending
-                    }
-                    sh_phys = phys;
-                    sh_row = row;
-                    sh_pos = pos;
-                }
-            }
-            __syncthreads();
-            if (sh_pos < 0) return;   // a padding row, or one that was flagged: left as it is
-            if (MODE != ROPE_NONE) {
-                const float2* row = reinterpret_cast<const float2*>(a.rope) + (int64_t)sh_pos * a.half;
+        if (live) {
 #pragma unroll
-                for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int e = 8 * (gl + j * lpr) + i;
-                        const int pair = MODE == ROPE_PAIRS ? e >> 1 : e < a.half ? e : e - a.half;
-                        if (MODE != ROPE_PAIRS || (i & 1) == 0)
-                            cs[j][i] = e < 2 * a.half ? __ldg(row + pair) : make_float2(1.0f, 0.0f);
-                    }
-            }
+            for (int j = 0; j < VPL; ++j)
+                if (gl + j * lpr < a.vecs) *reinterpret_cast<uint4*>(dst + 16 * j * lpr) = pack4<T>(y[j]);
         }
+    };
+    while (at.t < a.b.n_tokens) {
 #pragma unroll
-        for (int u = 0; u < AP_UNROLL; ++u) {
-            const int r = r0 + u * n_groups;
-            const bool live = r < rows;
-            const bool is_q = r < a.hq, is_k = !is_q && r < a.hq + a.hk;
-            if (live && !is_q && !is_k) {   // a value head: stored as it is
-                unsigned char* dst = a.v_pages.base + sh_phys * a.v_pages.page +
-                                     (r - a.hq - a.hk) * a.v_pages.head + sh_row * a.v_pages.token;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    const int vi = gl + j * lpr;
-                    if (vi < a.vecs) *reinterpret_cast<uint4*>(dst + 16 * vi) = x[u][j];
-                }
-            }
-            // (a group past the last row, or on a value head, goes through the shuffles with its warp)
-            float y[VPL][8];
-            float ss = 0.0f;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                unpack8<T>(x[u][j], y[j]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(y[j][i], y[j][i], ss);
-            }
-            const void* w = is_q ? a.w[0] : a.w[1];
-            if (a.w[0] || a.w[1]) {
-                for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (w) {
-                    const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-#pragma unroll
-                    for (int j = 0; j < VPL; ++j) {
-                        const int vi = gl + j * lpr;
-                        if (vi >= a.vecs) continue;
-                        float wf[8];
-                        if (a.w_f32) {
-                            const float4* p = reinterpret_cast<const float4*>(w) + 2 * vi;
-                            const float4 lo = __ldg(p), hi = __ldg(p + 1);
-                            wf[0] = lo.x; wf[1] = lo.y; wf[2] = lo.z; wf[3] = lo.w;
-                            wf[4] = hi.x; wf[5] = hi.y; wf[6] = hi.z; wf[7] = hi.w;
-                        } else {
-                            unpack8<T>(__ldg(reinterpret_cast<const uint4*>(w) + vi), wf);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[j][i] = y[j][i] * inv * wf[i];
-                    }
-                }
-            }
-            if (MODE == ROPE_PAIRS) {
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        if (8 * (gl + j * lpr) + i >= 2 * a.half) continue;   // as it is, infinities too
-                        const float p = y[j][i], q = y[j][i + 1];
-                        y[j][i] = p * cs[j][i].x - q * cs[j][i].y;
-                        y[j][i + 1] = q * cs[j][i].x + p * cs[j][i].y;
-                    }
-            } else if (MODE == ROPE_HALVES) {
-                // vector gl holds values [8 gl, 8 gl + 8); half is a multiple of 8
-                const int hv = a.half >> 3;
-                const bool first = gl < hv, turned = gl < 2 * hv;
-                const int partner = first ? gl + hv : turned ? gl - hv : gl;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float o = __shfl_sync(0xffffffffu, y[0][i], partner, lpr);
-                    if (turned) y[0][i] = y[0][i] * cs[0][i].x + (first ? -o : o) * cs[0][i].y;
-                }
-            } else if (MODE == ROPE_HALVES_SMEM) {
-                float* row = sm + group * a.D;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    const int vi = gl + j * lpr;
-                    if (vi < a.vecs) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) row[8 * vi + i] = y[j][i];
-                    }
-                }
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int e = 8 * (gl + j * lpr) + i;
-                        if (e >= 2 * a.half) continue;
-                        const bool first = e < a.half;
-                        const float o = row[first ? e + a.half : e - a.half];
-                        y[j][i] = y[j][i] * cs[j][i].x + (first ? -o : o) * cs[j][i].y;
-                    }
-                __syncwarp();
-            }
-            if (live && (is_q || is_k)) {
-                unsigned char* dst =
-                    is_q ? a.out.base + t * a.out.token + r * a.out.head
-                         : a.k_pages.base + sh_phys * a.k_pages.page +
-                               (r - a.hq) * a.k_pages.head + sh_row * a.k_pages.token;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    const int vi = gl + j * lpr;
-                    if (vi < a.vecs) *reinterpret_cast<uint4*>(dst + 16 * vi) = pack8<T>(y[j]);
-                }
-            }
+        for (int u = 0; u < AP_DEPTH; ++u) {
+            if (at.t >= a.b.n_tokens) break;
+            step(x[u]);
+            load(x[u]);
+            next(at);
         }
     }
 }
 
 template <typename T, int VPL>
-hmm_status_t launch_append(const AppendArgs& a, int mode, int threads, cudaStream_t st) {
-    const size_t smem = mode == ROPE_HALVES_SMEM ? sizeof(float) * (threads / a.lpr) * a.D : 0;
-    const unsigned grid = (unsigned)a.b.n_tokens;
+hmm_status_t launch_append(const AppendArgs& a, int mode, cudaStream_t st) {
+    const int64_t warps = (int64_t)a.tokens_at_once * a.parts;
+    const unsigned grid = (unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32));
+    const size_t smem = mode == ROPE_HALVES_SMEM ? sizeof(float) * (AP_THREADS >> a.lpr_log2) * a.D : 0;
+    constexpr int threads = AP_THREADS;
     switch (mode) {
         case ROPE_NONE: paged_append_kernel<T, VPL, ROPE_NONE><<<grid, threads, 0, st>>>(a); break;
         case ROPE_PAIRS: paged_append_kernel<T, VPL, ROPE_PAIRS><<<grid, threads, 0, st>>>(a); break;
-        case ROPE_HALVES_SMEM:
-            paged_append_kernel<T, VPL, ROPE_HALVES_SMEM><<<grid, threads, smem, st>>>(a);
-            break;
-        default: paged_append_kernel<T, 1, ROPE_HALVES><<<grid, threads, 0, st>>>(a); break;
+        case ROPE_HALVES: paged_append_kernel<T, 1, ROPE_HALVES><<<grid, threads, 0, st>>>(a); break;
+        case ROPE_HALVES_LANE: paged_append_kernel<T, 2, ROPE_HALVES_LANE><<<grid, threads, 0, st>>>(a); break;
+        default: paged_append_kernel<T, VPL, ROPE_HALVES_SMEM><<<grid, threads, smem, st>>>(a); break;
     }
     return check_launch("paged_append_kernel");
 }
@@ -360,18 +452,30 @@ extern "C" hmm_status_t hmm_paged_kv_append(
     a.vecs = a.D / 8;
     a.half = rope ? (int)(rotary_dim / 2) : 0;
     a.page_tokens = (int)cache->page_tokens;
-    a.lpr = std::min(32, next_pow2(a.vecs));
     a.eps = eps;
+    a.inv_d = 1.0f / (float)a.D;
     a.status = device_status;
-    const int mode = !rope ? ROPE_NONE : interleaved ? ROPE_PAIRS
-                     : a.half % 8 == 0 && a.vecs <= 32 ? ROPE_HALVES : ROPE_HALVES_SMEM;
-    // as many lane groups as give each AP_UNROLL rows
-    const int64_t groups = ((int64_t)a.hq + 2 * a.hk + AP_UNROLL - 1) / AP_UNROLL;
-    const int threads = (int)std::min<int64_t>(AP_THREADS, (groups * a.lpr + 31) / 32 * 32);
+    // Two vectors a lane where that pairs a value with its partner in the lane, or leaves
+    // no lane idle; else one, with the partner a shuffle away if vectors pair up.
+    const bool lane = rope && !interleaved && 2 * a.half == a.D && a.half % 8 == 0 &&
+                      (a.half & (a.half - 1)) == 0 && a.half <= 256;
+    const bool shuffle = rope && !interleaved && !lane && a.half % 8 == 0 && a.vecs <= 32;
+    const int vpl = !shuffle && (lane || a.vecs % 2 == 0 || a.vecs > 32) ? 2 : 1;
+    const int mode = !rope ? ROPE_NONE : interleaved ? ROPE_PAIRS : lane ? ROPE_HALVES_LANE
+                     : shuffle ? ROPE_HALVES : ROPE_HALVES_SMEM;
+    while ((vpl << a.lpr_log2) < a.vecs) ++a.lpr_log2;
+    const int n_groups = 32 >> a.lpr_log2;
+    a.steps_q = (a.hq + n_groups - 1) / n_groups;
+    a.steps_k = (a.hk + n_groups - 1) / n_groups;
+    // As many warps as stay on the GPU, each with a list of tokens; few tokens are shared
+    // by several warps, down to a step each.
+    const int64_t slots = (int64_t)device_sm_count() * AP_MINB * (AP_THREADS / 32);
+    const int64_t steps = a.steps_q + 2 * (int64_t)a.steps_k;
+    a.parts = (int)std::min(steps, std::max<int64_t>(1, slots / a.b.n_tokens));
+    a.tokens_at_once = (int)std::min<int64_t>(a.b.n_tokens, std::max<int64_t>(1, slots / a.parts));
     const cudaStream_t cs = (cudaStream_t)stream;
     if (cache->dtype == HMM_DTYPE_BF16)
-        return a.vecs > 32 ? launch_append<__nv_bfloat16, 2>(a, mode, threads, cs)
-                           : launch_append<__nv_bfloat16, 1>(a, mode, threads, cs);
-    return a.vecs > 32 ? launch_append<__half, 2>(a, mode, threads, cs)
-                       : launch_append<__half, 1>(a, mode, threads, cs);
+        return vpl == 2 ? launch_append<__nv_bfloat16, 2>(a, mode, cs)
+                        : launch_append<__nv_bfloat16, 1>(a, mode, cs);
+    return vpl == 2 ? launch_append<__half, 2>(a, mode, cs) : launch_append<__half, 1>(a, mode, cs);
 }

@@ -329,7 +329,8 @@ hmm_status_t hmm_status_read(const int32_t* device_status, void* stream);
  * cached tokens, the new ones among them.  The new tokens of sequence s are
  * rows [cu_new[s], cu_new[s+1]) of the packed arrays of n_tokens rows; new
  * token j has position kv_len[s] - n_new[s] + j.  Rows that no sequence owns
- * (before cu_new[0], from cu_new[n_seq] on) are neither read nor written. */
+ * (before cu_new[0], from cu_new[n_seq] on) are left as they are.  n_tokens <=
+ * 2^30. */
 #define HMM_DTYPE_BF16 0
 #define HMM_DTYPE_F16 1
 #define HMM_DTYPE_F32 2
