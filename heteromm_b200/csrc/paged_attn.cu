@@ -8,9 +8,12 @@
 //   - all units' key tiles form one list, cut into as many equal pieces as CTAs
 //     fit the GPU (ragged lengths balance by themselves); a CTA finds its piece
 //     from the lengths on the device, so no host value goes stale;
-//   - each warp owns 16 keys of a tile and its own ring of cp.async stages, with
-//     no barrier between warps: page lookup one stage ahead, 16-byte copies, zero
-//     fill for what no row of the tile sees;
+//   - each warp owns 16 keys of a tile and its own ring of TMA stages, with no
+//     barrier between warps: a box per 64 values of a page's rows (issued by as
+//     many lanes as there are boxes, their page looked up one stage ahead), zeros
+//     for the boxes that no row of the tile sees.  The copies cost a warp about 30
+//     instructions a tile; with 16-byte cp.async (about 400) the issue slots bound
+//     the kernel, not HBM;
 //   - scores and the product with V on mma.sync (m16n8k16, fp32 sums), the
 //     running maximum and sum in fp32 per warp, warps joined once per piece;
 //   - a unit that several CTAs share leaves (maximum, sum, unnormalised rows) per
@@ -22,6 +25,7 @@
 
 namespace hmm {
 namespace serve {
+using namespace sm100;
 namespace {
 
 constexpr int RW_WARPS = 4;
@@ -40,6 +44,8 @@ struct RowsArgs {
     AttnArgs a;
     RowsWork w;
     int max_rows;     // sequences of more rows are another kernel's
+    int box_rows;     // rows of a TMA box: a power of two that divides page_tokens
+    uint64_t wait_ns; // limit of every bounded wait
 };
 
 template <int DP>
@@ -47,7 +53,7 @@ constexpr int rows_ctas_per_sm() { return DP == 64 ? 4 : DP == 128 ? 2 : 1; }
 
 template <int DP>
 constexpr size_t rows_smem() {
-    return (size_t)RW_WARPS * RW_STAGES * 2 * RW_KEYS * DP * 2;
+    return 1024 + (size_t)RW_WARPS * RW_STAGES * 2 * RW_KEYS * DP * 2;
 }
 
 __device__ __forceinline__ void ldm4(uint32_t* r, uint32_t addr) {
@@ -158,18 +164,27 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP>())
-paged_rows_kernel(const __grid_constant__ RowsArgs r) {
-    extern __shared__ __align__(128) unsigned char smem[];
+paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ RowsArgs r) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t full[RW_WARPS][RW_STAGES];
     __shared__ int64_t wt[RW_WARPS];
     __shared__ int64_t sh_pre;
-    __shared__ int sh_seq, again;
-    constexpr int ROWB = DP * 2;                       // bytes of a staged row
-    constexpr int CH = DP / 8;                         // its 16-byte chunks
-    constexpr int STAGE = 2 * RW_KEYS * ROWB;          // K then V
+    __shared__ int sh_seq, again, abort;
+    constexpr int HALVES = DP / 64;                    // boxes of 64 values in a row
+    constexpr int BLOCK = RW_KEYS * 128;               // 16 rows of 64 values, swizzled
+    constexpr int STAGE = 2 * HALVES * BLOCK;          // K then V
     constexpr int MR = DP + 4;                         // joining rows: 4 banks apart
     const AttnArgs& a = r.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < RW_WARPS; ++w)
+            for (int i = 0; i < RW_STAGES; ++i) mbar_init(&full[w][i], 1);
+        abort = 0;
+        fence_barrier_init();
+    }
     // ---- this CTA's piece of the list of all units' tiles
     int64_t total = 0;
     for (int s0 = 0; s0 < a.b.n_seq; s0 += RW_THREADS) {
@@ -211,7 +226,13 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
     Seq q = load_seq(a.b, a.max_kv, s, a.status);
     Load ld = seq_load(r, q);
 
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * RW_STAGES * STAGE;
+    unsigned char* ring_p = smem + warp * RW_STAGES * STAGE;
+    const uint32_t ring = smem_u32(ring_p);
+    // lane: box rows [sub * box_rows, +box_rows) of the warp's 16 keys, and of the (K / V,
+    // 64 values) boxes there every (32 / subs)-th
+    const int subs = RW_KEYS / r.box_rows, sub = lane % subs, box0 = lane / subs, box_step = 32 / subs;
+    uint32_t done = 0;                                 // tiles that the ring has seen
+    bool dead = false;                                 // a wait gave up: no more copies
     while (cur < end) {
         while (cur >= pre + (int64_t)ld.units * ld.tiles) {
             pre += (int64_t)ld.units * ld.tiles;
@@ -234,40 +255,32 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
             const int t = t0 + i;
             return (t < sink_tiles ? t : first + t - sink_tiles) * RW_TILE + warp * RW_KEYS;
         };
-        // lanes 0-15: page and slot of key (key0 + lane), page -1 where no row sees it
-        int phys = -1, slot = 0;
+        int page = a.n_pages, row = 0;                 // this lane's box rows of the next tile
         auto lookup = [&](int i) {
-            phys = -1;
-            if (i < n && lane < RW_KEYS) {
-                const int key = key0_of(i) + lane;
-                if (span_has(sp, key)) {
-                    const int lp = key / a.page_tokens;
-                    phys = page_of(a, s, lp);
-                    slot = key - lp * a.page_tokens;
+            page = a.n_pages;                          // out of range: zeros
+            if (i < n) {
+                const int k0 = key0_of(i) + sub * r.box_rows;
+                if (k0 < sp.sink || (k0 + r.box_rows > sp.lo && k0 < sp.hi)) {
+                    const int lp = k0 / a.page_tokens;
+                    const int e = page_of(a, s, lp);
+                    if (e >= 0) {
+                        page = e;
+                        row = k0 - lp * a.page_tokens;
+                    }
                 }
             }
         };
-        auto issue = [&](int i) {                      // copies of tile i, whose lookup is in phys / slot
-            if (i < n) {
-                const uint32_t st = ring + (i % RW_STAGES) * STAGE;
-#pragma unroll
-                for (int it = 0; it < RW_KEYS * CH / 32; ++it) {
-                    const int idx = it * 32 + lane, row = idx / CH, c = idx % CH;
-                    const int ph = __shfl_sync(0xffffffffu, phys, row);
-                    const int sl = __shfl_sync(0xffffffffu, slot, row);
-                    const bool real = ph >= 0 && c * 8 < a.D;
-                    const unsigned char* kp = a.k.base;
-                    const unsigned char* vp = a.v.base;
-                    if (real) {
-                        kp += ph * a.k.page + kvh * a.k.head + sl * a.k.token + c * 16;
-                        vp += ph * a.v.page + kvh * a.v.head + sl * a.v.token + c * 16;
-                    }
-                    const uint32_t d = st + row * ROWB + ((c ^ (row & 7)) * 16);
-                    cp16(d, kp, real);
-                    cp16(d + RW_KEYS * ROWB, vp, real);
-                }
+        auto issue = [&](int i) {                      // copies of tile i, whose lookup is in page / row
+            if (i < n && !dead) {
+                const uint32_t st = (done + i) % RW_STAGES;
+                if (lane == 0) mbar_expect_tx(&full[warp][st], STAGE);
+                __syncwarp();
+                const uint32_t d = ring + st * STAGE + sub * r.box_rows * 128;
+#pragma unroll 2
+                for (int b = box0; b < 2 * HALVES; b += box_step)
+                    tma_load_page(d + b * BLOCK, b < HALVES ? &tmK : &tmV, &full[warp][st],
+                                  64 * (b < HALVES ? b : b - HALVES), row, kvh, page);
             }
-            cp_commit();
         };
 
         // q fragments: rows lane / 4 and lane / 4 + 8
@@ -304,22 +317,45 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
         for (int i = 0; i < n; ++i) {
-            cp_wait<RW_STAGES - 2>();
-            __syncwarp();
+            if (!dead) {
+                const uint32_t at = done + i;
+                dead = !__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][at % RW_STAGES],
+                                                                  (at / RW_STAGES) & 1, &abort, r.wait_ns));
+                if (dead) {
+                    if (lane == 0) {
+                        atomicExch(&abort, 1);
+                        atomicOr(a.status, HMM_STATUS_TIMEOUT);
+                    }
+                    for (int k = i; k < min(n, i + RW_STAGES - 1); ++k)   // copies in flight land first
+                        mbar_wait_drain(&full[warp][(done + k) % RW_STAGES], ((done + k) / RW_STAGES) & 1);
+                }
+            }
             issue(i + RW_STAGES - 1);                  // into the stage that tile i - 1 left
             lookup(i + RW_STAGES);
-            const uint32_t kt = ring + (i % RW_STAGES) * STAGE, vt = kt + RW_KEYS * ROWB;
+            const uint32_t so = ((done + i) % RW_STAGES) * STAGE;
+            const uint32_t kt = ring + so, vt = kt + HALVES * BLOCK;
+            const int key0 = key0_of(i);
+            if (!(key0 >= sp.lo && key0 + RW_KEYS <= sp.hi) && key0 + RW_KEYS > sp.sink) {
+                // V rows that no row of the unit sees, beside some that are seen, become
+                // zeros: a weight of zero times what a slot of nobody holds is only zero then
+                if (lane < RW_KEYS && !span_has(sp, key0 + lane)) {
+#pragma unroll
+                    for (int c = 0; c < HALVES * 8; ++c)
+                        *reinterpret_cast<uint4*>(ring_p + so + (HALVES + (c >> 3)) * BLOCK + lane * 128 + (c & 7) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
+            }
             float sc[2][4] = {};
             const int mi = lane >> 3, ml = lane & 7;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
                 uint32_t b[4];
                 const int row = ml + (mi >> 1) * 8, c = 2 * k + (mi & 1);
-                ldm4(b, kt + row * ROWB + ((c ^ (row & 7)) * 16));
+                ldm4(b, kt + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) * 16));
                 mma16816<T>(sc[0], qf[k], b[0], b[1]);
                 mma16816<T>(sc[1], qf[k], b[2], b[3]);
             }
-            const int key0 = key0_of(i);
             const bool all = key0 + RW_KEYS <= q.kv && (!a.causal || key0 + RW_KEYS - 1 <= sp.p0) &&
                              (a.window <= 0 || key0 > sp.p1 - a.window || key0 + RW_KEYS <= a.sinks);
             float mx[2] = {m[0], m[1]};
@@ -366,13 +402,13 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
             for (int d = 0; d < DP / 16; ++d) {
                 uint32_t b[4];
                 const int row = ml + (mi & 1) * 8, c = 2 * d + (mi >> 1);
-                ldm4t(b, vt + row * ROWB + ((c ^ (row & 7)) * 16));
+                ldm4t(b, vt + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) * 16));
                 mma16816<T>(o[2 * d], p, b[0], b[1]);
                 mma16816<T>(o[2 * d + 1], p, b[2], b[3]);
             }
             __syncwarp();                              // the stage may be overwritten
         }
-        cp_wait<0>();
+        if (n > 0) done += n;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -428,9 +464,10 @@ paged_rows_kernel(const __grid_constant__ RowsArgs r) {
             }
             if (t0 == 0 && threadIdx.x == 0)
                 r.w.joint[blockIdx.x] = make_int4(s, kvh, rt, 1 + (int)((ld.tiles - t1 + per - 1) / per));
-            __syncthreads();                           // the rings' memory is free again
         }
         cur += t1 - t0;
+        fence_proxy_async_smem();                      // the next copies come behind these writes
+        __syncthreads();
     }
 }
 
@@ -463,12 +500,12 @@ size_t rows_workspace(int dp) {
 }
 
 template <typename T, int DP>
-hmm_status_t launch_rows(const RowsArgs& r, cudaStream_t st) {
+hmm_status_t launch_rows(const RowsArgs& r, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
     const unsigned g = (unsigned)rows_ctas(DP);
     static std::atomic<uint64_t> done{0};
     hmm_status_t s = allow_smem(paged_rows_kernel<T, DP>, rows_smem<DP>(), &done);
     if (s != HMM_OK) return s;
-    paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(r);
+    paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(k, v, r);
     s = check_launch("paged_rows_kernel");
     if (s != HMM_OK) return s;
     paged_rows_join_kernel<T, DP><<<g, RW_THREADS, 0, st>>>(r);
@@ -478,9 +515,15 @@ hmm_status_t launch_rows(const RowsArgs& r, cudaStream_t st) {
 template <typename T>
 hmm_status_t run_rows(const AttnArgs& a, int max_rows, unsigned char* ws, cudaStream_t st) {
     const int dp = rows_dp(a.D);
-    RowsArgs r{a, {(int4*)ws, (float*)(ws + (size_t)rows_ctas(dp) * sizeof(int4))}, max_rows};
-    return dp == 64 ? launch_rows<T, 64>(r, st) : dp == 128 ? launch_rows<T, 128>(r, st)
-                                                            : launch_rows<T, 256>(r, st);
+    RowsArgs r{a, {(int4*)ws, (float*)(ws + (size_t)rows_ctas(dp) * sizeof(int4))}, max_rows,
+               box_rows_of(a.page_tokens, RW_KEYS), wait_limit_ns()};
+    CUtensorMap k, v;
+    hmm_status_t s = make_page_map(&k, a, a.k, r.box_rows);
+    if (s != HMM_OK) return s;
+    s = make_page_map(&v, a, a.v, r.box_rows);
+    if (s != HMM_OK) return s;
+    return dp == 64 ? launch_rows<T, 64>(r, k, v, st) : dp == 128 ? launch_rows<T, 128>(r, k, v, st)
+                                                                  : launch_rows<T, 256>(r, k, v, st);
 }
 
 }  // namespace
@@ -517,6 +560,13 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     HMM_REQUIRE(batch->n_tokens * n_heads / cache->n_kv_heads < (int64_t(1) << 31),
                 "n_tokens * (n_heads / n_kv_heads) must be < 2^31");
     if (batch->n_seq == 0 || batch->n_tokens == 0) return HMM_OK;
+    HMM_REQUIRE(cache->n_pages >= 1, "the cache has no pages");
+    const int64_t steps[6] = {cache->page_tokens > 1 ? cache->k_token : 8, cache->n_kv_heads > 1 ? cache->k_head : 8,
+                              cache->n_pages > 1 ? cache->k_page : 8, cache->page_tokens > 1 ? cache->v_token : 8,
+                              cache->n_kv_heads > 1 ? cache->v_head : 8, cache->n_pages > 1 ? cache->v_page : 8};
+    for (int64_t x : steps)
+        HMM_REQUIRE(x > 0 && x < (int64_t(1) << 39), "cache strides must be in [8, 2^39) elements, got %lld",
+                    (long long)x);
     HMM_REQUIRE(q && out, "null q or out");
     HMM_REQUIRE(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
     const size_t need = hmm_paged_attention_workspace_size(batch->n_seq, batch->n_tokens, n_heads,

@@ -24,7 +24,6 @@
 // Bound: 4 D FLOP per (row, key) on the tensor cores, against one exponential
 // per (row, key) on the special-function units, 16 a clock and SM: at D = 128
 // both take 1,024 clocks a tile.
-#include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -32,7 +31,6 @@
 
 #include "paged_attn.cuh"
 #include "paged_attn_tc.cuh"
-#include "sm100_ptx.cuh"
 
 namespace hmm {
 namespace serve {
@@ -98,14 +96,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, ns));
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
-                                            int z, int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-        : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
+                 : "memory");
 }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // One CTA's kind::f16 MMAs with the descriptors' halves apart: the upper words are
 // constants and the lower ones differ by constants (addresses are below 2^18, so a
@@ -443,7 +440,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
 #pragma unroll
                         for (int h = 0; h < HALVES; ++h)
-                            tma_load_4d(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
+                            tma_load_page(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
                                         kvh, page);
                     }
                 }
@@ -776,9 +773,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// A page array as a tensor (D, page_tokens, heads, pages) of boxes {64, rows, 1, 1},
-// 128-byte swizzle; values behind D and pages behind the last read as zeros.
-hmm_status_t make_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
+template <typename T, int DP>
+hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
+                          cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
+    if (s != HMM_OK) return s;
+    paged_chunk_kernel<T, DP><<<grid, TC_THREADS, tc_smem<DP>(), st>>>(k, v, t);
+    return check_launch("paged_chunk_kernel");
+}
+
+}  // namespace
+
+hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
     auto fn = encode_fn();
     if (!fn) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_tokens, (cuuint64_t)a.hk, (cuuint64_t)a.n_pages};
@@ -794,37 +801,16 @@ hmm_status_t make_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box
     return HMM_OK;
 }
 
-template <typename T, int DP>
-hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
-                          cudaStream_t st) {
-    static std::atomic<uint64_t> done{0};
-    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
-    if (s != HMM_OK) return s;
-    paged_chunk_kernel<T, DP><<<grid, TC_THREADS, tc_smem<DP>(), st>>>(k, v, t);
-    return check_launch("paged_chunk_kernel");
-}
-
-int box_rows_of(int64_t page_tokens) {
-    int64_t r = page_tokens & -page_tokens;   // the largest power of two that divides it
-    return (int)std::min<int64_t>(r, TC_KEYS);
-}
-
-}  // namespace
-
 bool chunk_applies(const AttnArgs& a) {
-    auto steps = [&](const Pages& p) {
-        return (a.page_tokens == 1 || p.token > 0) && (a.hk == 1 || p.head > 0) && (a.n_pages == 1 || p.page > 0) &&
-               p.token < (int64_t(1) << 40) && p.head < (int64_t(1) << 40) && p.page < (int64_t(1) << 40);
-    };
-    return a.D <= 128 && box_rows_of(a.page_tokens) >= 8 && a.n_pages > 0 && steps(a.k) && steps(a.v);
+    return a.D <= 128 && box_rows_of(a.page_tokens, TC_KEYS) >= 8;
 }
 
 hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, cudaStream_t st) {
-    TcArgs t{a, min_rows, box_rows_of(a.page_tokens), wait_limit_ns()};
+    TcArgs t{a, min_rows, box_rows_of(a.page_tokens, TC_KEYS), wait_limit_ns()};
     CUtensorMap k, v;
-    hmm_status_t s = make_map(&k, a, a.k, t.box_rows);
+    hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows);
     if (s != HMM_OK) return s;
-    s = make_map(&v, a, a.v, t.box_rows);
+    s = make_page_map(&v, a, a.v, t.box_rows);
     if (s != HMM_OK) return s;
     // every sequence's rows in blocks: one more than its share of the tokens at most
     const int64_t most = ((int64_t)a.b.n_tokens * a.group / TC_CTA_ROWS + a.b.n_seq) * a.hk;

@@ -1,10 +1,35 @@
-// paged_attn_tc.cuh — the tensor-core attention kernel's launcher.
+// paged_attn_tc.cuh — page arrays as TMA tensors, and the tensor-core attention
+// kernel's launcher.
 #pragma once
 
+#include <cuda.h>
+
 #include "paged_attn.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hmm {
 namespace serve {
+
+// A page array as a tensor (D, page_tokens, heads, pages) of boxes {64, rows, 1, 1},
+// 128-byte swizzle; values behind D and pages behind the last read as zeros.
+hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows);
+
+// Rows of a box: the largest power of two that divides page_tokens, at most `most`; a box
+// never crosses a page's end.
+inline int box_rows_of(int64_t page_tokens, int64_t most) {
+    const int64_t r = page_tokens & -page_tokens;
+    return (int)(r < most ? r : most);
+}
+
+// One box of a page array: values [x, x + 64) of rows y... of a head (z) and page (w).
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
+                                              int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
 
 struct TcArgs {
     AttnArgs a;
@@ -13,7 +38,7 @@ struct TcArgs {
     uint64_t wait_ns;    // limit of every bounded wait
 };
 
-// Whether the kernel can read this cache (head size, page size, strides).
+// Whether the kernel takes this head size and page size.
 bool chunk_applies(const AttnArgs& a);
 // Rows of every sequence with at least min_rows rows (n_new * group).
 hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, cudaStream_t st);
