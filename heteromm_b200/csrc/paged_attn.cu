@@ -46,6 +46,7 @@ struct RowsArgs {
     int max_rows;     // sequences of more rows are another kernel's
     int box_rows;     // rows of a TMA box: a power of two that divides page_tokens
     uint64_t wait_ns; // limit of every bounded wait
+    int* counter;     // set to 0 for the kernel behind, or null
 };
 
 template <int DP>
@@ -124,44 +125,6 @@ __device__ __forceinline__ int64_t scan_incl(int64_t v, int64_t* wt, int64_t* to
     return v + add;
 }
 
-// Joins (maximum, sum, row) pieces of the unit's rows and writes them out; rows
-// that come out not finite are computed again by attn_row_exact.  piece(i, row,
-// -1 / -2 / d) reads the maximum, sum or value of piece i.  Whole block.
-template <typename T, typename Piece>
-__device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
-                                            int rows, int pieces, Piece piece, int* again) {
-    if (threadIdx.x == 0) *again = 0;
-    __syncthreads();
-    const int pairs = a.D / 2;
-    for (int i = threadIdx.x; i < rows * pairs; i += blockDim.x) {
-        const int r = i / pairs, d = 2 * (i - r * pairs);
-        float m = -INFINITY;
-        for (int p = 0; p < pieces; ++p) m = fmaxf(m, piece(p, r, -1));
-        const float ms = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f, y = 0.0f;
-        for (int p = 0; p < pieces; ++p) {
-            const float wgt = ex2(piece(p, r, -1) - ms);
-            if (wgt == 0.0f) continue;   // a piece in which the row saw nothing
-            l = fmaf(wgt, piece(p, r, -2), l);
-            x = fmaf(wgt, piece(p, r, d), x);
-            y = fmaf(wgt, piece(p, r, d + 1), y);
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        x = l == 0.0f ? 0.0f : x * inv;
-        y = l == 0.0f ? 0.0f : y * inv;
-        if (!isfinite(x) || !isfinite(y) || l != l) atomicOr(again, 1 << r);
-        const int tok = q.begin + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
-        const int64_t at = (int64_t)tok * a.hq + head;
-        *reinterpret_cast<uint32_t*>(a.out + 2 * (at * a.D + d)) = pack2<T>(x, y);
-        if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
-    }
-    __syncthreads();
-    const int bits = *again;
-    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
-        if ((bits >> r) & 1) attn_row_exact<T>(a, s, q, kvh, row0 + r);
-    __syncthreads();
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP>())
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -178,6 +141,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     constexpr int MR = DP + 4;                         // joining rows: 4 banks apart
     const AttnArgs& a = r.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
         for (int w = 0; w < RW_WARPS; ++w)
@@ -200,7 +164,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const int64_t per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     int64_t cur = blockIdx.x * per;
     const int64_t end = min(total, cur + per);
-    if (threadIdx.x == 0) r.w.joint[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) {
+        r.w.joint[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (r.counter && blockIdx.x == 0) *r.counter = 0;
+    }
     if (cur >= end) return;
     {
         int64_t run = 0;
@@ -440,7 +407,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                              : jm[(w * RW_ROWS + row) * MR + d];
         };
         if (t0 == 0 && t1 == ld.tiles) {
-            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, piece, &again);
+            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, piece, jst + 2 * RW_WARPS * RW_ROWS, &again);
         } else {
             float* part = r.w.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * RW_ROWS * (DP + 2);
             for (int i = threadIdx.x; i < rows * a.D; i += RW_THREADS) {
@@ -474,7 +441,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 // Block c: the unit begun in CTA c and ended in a later one.
 template <typename T, int DP>
 __global__ void __launch_bounds__(RW_THREADS) paged_rows_join_kernel(const __grid_constant__ RowsArgs r) {
+    extern __shared__ float share[];
     __shared__ int again;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the rows kernel runs
     const int4 u = r.w.joint[blockIdx.x];
     if (u.w == 0) return;
     const Seq q = load_seq(r.a.b, r.a.max_kv, u.x, r.a.status);
@@ -485,7 +454,7 @@ __global__ void __launch_bounds__(RW_THREADS) paged_rows_join_kernel(const __gri
     finish_rows<T>(r.a, u.x, q, u.y, row0, rows, u.w, [&](int i, int row, int d) {
         const float* p = part + ((c + i) * 2 + (i == 0)) * RW_ROWS * (DP + 2);
         return d == -1 ? p[RW_ROWS * DP + row] : d == -2 ? p[RW_ROWS * (DP + 1) + row] : p[row * DP + d];
-    }, &again);
+    }, share, &again);
 }
 
 int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
@@ -493,6 +462,8 @@ int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 int64_t rows_ctas(int dp) {
     return (int64_t)device_sm_count() * (dp == 64 ? rows_ctas_per_sm<64>() : dp == 128 ? rows_ctas_per_sm<128>() : 1);
 }
+
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 size_t rows_workspace(int dp) {
     const size_t g = (size_t)rows_ctas(dp);
@@ -508,15 +479,18 @@ hmm_status_t launch_rows(const RowsArgs& r, const CUtensorMap& k, const CUtensor
     paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(k, v, r);
     s = check_launch("paged_rows_kernel");
     if (s != HMM_OK) return s;
-    paged_rows_join_kernel<T, DP><<<g, RW_THREADS, 0, st>>>(r);
-    return check_launch("paged_rows_join_kernel");
+    const size_t share = sizeof(float) * RW_ROWS * (g + 1);
+    static std::atomic<uint64_t> join_done{0};
+    s = allow_smem(paged_rows_join_kernel<T, DP>, share, &join_done);
+    if (s != HMM_OK) return s;
+    return launch_behind(paged_rows_join_kernel<T, DP>, dim3(g), RW_THREADS, share, st, r, "paged_rows_join_kernel");
 }
 
 template <typename T>
-hmm_status_t run_rows(const AttnArgs& a, int max_rows, unsigned char* ws, cudaStream_t st) {
+hmm_status_t run_rows(const AttnArgs& a, int max_rows, unsigned char* ws, int* counter, cudaStream_t st) {
     const int dp = rows_dp(a.D);
     RowsArgs r{a, {(int4*)ws, (float*)(ws + (size_t)rows_ctas(dp) * sizeof(int4))}, max_rows,
-               box_rows_of(a.page_tokens, RW_KEYS), wait_limit_ns()};
+               box_rows_of(a.page_tokens, RW_KEYS), wait_limit_ns(), counter};
     CUtensorMap k, v;
     hmm_status_t s = make_page_map(&k, a, a.k, r.box_rows);
     if (s != HMM_OK) return s;
@@ -536,7 +510,8 @@ using namespace hmm::serve;
 extern "C" size_t hmm_paged_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
                                                      int64_t n_kv_heads, int64_t D) {
     if (n_seq < 0 || n_tokens < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256) return 0;
-    return rows_workspace(rows_dp(D));
+    const int dp = rows_dp(D);
+    return up256(rows_workspace(dp)) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D);
 }
 
 extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
@@ -602,10 +577,13 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     const bool rows_too = few || !chunk || batch->n_seq > 1;
     const int split = !chunk || few ? INT32_MAX : batch->n_seq == 1 ? 0 : RW_ROWS;
     const bool bf16 = cache->dtype == HMM_DTYPE_BF16;
+    unsigned char* chunk_ws = (unsigned char*)workspace + up256(rows_workspace(rows_dp(a.D)));
     if (rows_too) {
-        s = bf16 ? run_rows<__nv_bfloat16>(a, split, (unsigned char*)workspace, st)
-                 : run_rows<__half>(a, split, (unsigned char*)workspace, st);
+        int* counter = chunk && !few ? (int*)chunk_ws : nullptr;
+        s = bf16 ? run_rows<__nv_bfloat16>(a, split, (unsigned char*)workspace, counter, st)
+                 : run_rows<__half>(a, split, (unsigned char*)workspace, counter, st);
         if (s != HMM_OK) return s;
     }
-    return chunk && !few ? run_chunk(a, bf16, split == 0 ? 1 : split + 1, st) : HMM_OK;
+    return chunk && !few ? run_chunk(a, bf16, split == 0 ? 1 : split + 1, chunk_ws, st)
+                         : HMM_OK;
 }

@@ -141,5 +141,86 @@ __device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const S
         a.lse[(int64_t)tok * a.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+// Joins (maximum, sum, row) pieces of up to 16 rows, which several warps or CTAs summed
+// over different keys, in their order, and writes the rows out; rows that come out not
+// finite are computed again by attn_row_exact.  piece(i, row, -1 / -2 / d) reads the
+// maximum, sum or value of piece i; `share` holds 16 x pieces floats.  Whole block.
+template <typename T, typename Piece>
+__device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
+                                            int rows, int pieces, Piece piece, float* share, int* again) {
+    if (threadIdx.x == 0) *again = 0;
+    const int lane = threadIdx.x & 31;
+    // each piece's share of the row: exp2(m_i - m) / sum_k exp2(m_k - m) l_k
+    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
+        float m = -INFINITY, l = 0.0f;
+        for (int p = lane; p < pieces; p += 32) m = fmaxf(m, piece(p, r, -1));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float ms = m == -INFINITY ? 0.0f : m;
+        for (int p = lane; p < pieces; p += 32) {
+            const float wgt = ex2(piece(p, r, -1) - ms);
+            share[r * pieces + p] = wgt;
+            if (wgt != 0.0f) l = fmaf(wgt, piece(p, r, -2), l);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        __syncwarp();
+        for (int p = lane; p < pieces; p += 32) {
+            const float wgt = share[r * pieces + p];
+            share[r * pieces + p] = wgt == 0.0f ? 0.0f : wgt * inv;   // (0: a piece in which the row saw nothing)
+        }
+        if (lane == 0) {
+            if (l != l) atomicOr(again, 1 << r);
+            if (a.lse) {
+                const int tok = a.by_group(row0 + r);
+                a.lse[(int64_t)(q.begin + tok) * a.hq + kvh * a.group + row0 + r - tok * a.group] =
+                    l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+            }
+        }
+    }
+    __syncthreads();
+    const int pairs = a.D / 2;
+    for (int i = threadIdx.x; i < rows * pairs; i += blockDim.x) {
+        const int r = i / pairs, d = 2 * (i - r * pairs);
+        float x = 0.0f, y = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < pieces; ++p) {
+            const float wgt = share[r * pieces + p];
+            const float u = piece(p, r, d), v = piece(p, r, d + 1);
+            x = wgt == 0.0f ? x : fmaf(wgt, u, x);
+            y = wgt == 0.0f ? y : fmaf(wgt, v, y);
+        }
+        if (!isfinite(x) || !isfinite(y)) atomicOr(again, 1 << r);
+        const int tok = a.by_group(row0 + r), head = kvh * a.group + row0 + r - tok * a.group;
+        *reinterpret_cast<uint32_t*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + d)) =
+            pack2<T>(x, y);
+    }
+    __syncthreads();
+    const int bits = *again;
+    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
+        if ((bits >> r) & 1) attn_row_exact<T>(a, s, q, kvh, row0 + r);
+    __syncthreads();
+}
+
+// Launches a kernel that begins with griddepcontrol.wait: its blocks may be set up while
+// the kernel before it on the stream still runs.
+template <typename F, typename A>
+hmm_status_t launch_behind(F fn, dim3 grid, int threads, size_t smem, cudaStream_t st, const A& args,
+                           const char* what) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    HMM_CUDA_TRY(cudaLaunchKernelEx(&c, fn, args));
+    return check_launch(what);
+}
+
 }  // namespace serve
 }  // namespace hmm

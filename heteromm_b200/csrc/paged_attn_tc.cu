@@ -3,14 +3,14 @@
 //
 // A CTA takes 256 rows of one (sequence, KV head) - row = (new token, query head
 // of the group) - as two tiles of 128, and the keys they see in tiles of 128:
-//   warps 0-7, 8-15 softmax of row tile 0 / 1, two threads per row: scores from
-//                   TMEM, running maximum and sum in registers, weights back to
-//                   TMEM; at the end the rows' results
-//   warp 16         TMA: K and V tiles in turn into a ring of stages, page by
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, a thread per row: scores from TMEM,
+//                   running maximum and sum in registers, weights back to TMEM; at
+//                   the end the rows' results
+//   warp 8          TMA: K and V tiles in turn into a ring of stages, page by
 //                   page (boxes of up to 128 rows of one page and head; a box
 //                   that no row sees is asked for out of range and arrives as zeros)
-//   warp 18         zeros over V rows that no row of the CTA sees (a page's end)
-//   warp 17         MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
+//   warp 10         zeros over V rows that no row of the CTA sees (a page's end)
+//   warp 9          MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
 //                   P_w V with P_w from TMEM over S_w's columns
 // While one tile's rows are in the exponentials the tensor cores work on the
 // other.  S_w of the next key tile is issued after P_w V of this one, so one
@@ -41,13 +41,13 @@ constexpr int TC_ROWS = 128;                 // rows of a tile (MMA M, TMEM lane
 constexpr int TC_TILES = 2;
 constexpr int TC_CTA_ROWS = TC_ROWS * TC_TILES;
 constexpr int TC_KEYS = 128;                 // keys of a tile
-constexpr int TC_SOFTMAX_WARPS = 16;         // two row tiles x 32 rows x two parts of the columns
+constexpr int TC_SOFTMAX_WARPS = 8;          // two row tiles, 32 rows a warp
 constexpr int TC_WARPS = TC_SOFTMAX_WARPS + 4;
 constexpr int TC_THREADS = 32 * TC_WARPS;
-constexpr int TC_SOFTMAX = 32 * TC_SOFTMAX_WARPS;
-// Registers: 640 threads are launched with 96 each (61,440 in all); the softmax warps
-// take 104 (half a row's scores stay in registers), the last warpgroup gives up to 56.
-constexpr int TC_REGS_LAUNCH = 96, TC_REGS_SOFTMAX = 104, TC_REGS_OTHER = 56;
+// Registers: 384 threads are launched with 168 each (64,512 in all); the softmax warps
+// take 224 (a row's scores stay in registers), the last warpgroup keeps 56.
+constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
+constexpr int TC_MIN_PIECE = 3;               // key tiles of a split unit's piece
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
 // Of 8 pairs of exponentials, those that go to the FMA pipe.
@@ -64,16 +64,45 @@ __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * DP * 2; }
 template <int DP>
 __host__ __device__ constexpr int tc_q_bytes() { return TC_CTA_ROWS * DP * 2; }
 
+struct TcArgs {
+    AttnArgs a;
+    int min_rows;        // sequences of fewer rows are another kernel's
+    int box_rows;        // rows of a TMA box: a power of two that divides page_tokens
+    int split;           // whether few units may be split over the keys
+    int* next;           // the next item, or null: the CTAs' rounds go to and fro
+    int* owner;          // [items] the CTA that took it (with `next`)
+    int q_tokens;        // new tokens of a row tile's TMA box, 0: queries by 16-byte copies
+    uint64_t wait_ns;    // limit of every bounded wait
+    uint32_t* again;     // [items][TC_SOFTMAX_WARPS] rows that came out not finite
+    int4* joint;         // [ctas] split unit that begins with this item: sequence, head, row block, pieces
+    float* part;         // [ctas][TC_CTA_ROWS * (DP + 2)]: a piece's rows, maxima, sums
+};
+
+// What a CTA works on at a time: 256 rows of a (sequence, KV head) and `n` key tiles of
+// those that they see, from the t0-th on.
+struct Unit {
+    int s, kvh, row0, rows;      // s < 0: no more
+    Seq q;
+    Span sp;
+    int sink_tiles, first;       // the seen tiles are [0, sink_tiles) and [first, ...)
+    int t0, n, n_of[TC_TILES];   // each row tile's key tiles: a prefix of the unit's
+    int pieces, item;
+    __device__ __forceinline__ int key0(int j) const {
+        return (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
+    }
+    // tiles with keys that no row sees beside some that are seen
+    __device__ __forceinline__ bool mends(int k0) const {
+        return !(k0 >= sp.lo && k0 + TC_KEYS <= sp.hi) && k0 + TC_KEYS > sp.sink;
+    }
+};
+
 struct TcCtrl {
     uint64_t full[8], empty[8];
-    uint64_t s_full[TC_TILES], p_full[TC_TILES][2], q_full, v_mend, v_fixed, o_full, drain;
-    int64_t scan[TC_WARPS];
-    int64_t pre;
-    Seq own;
-    int seq;
+    uint64_t s_full[TC_TILES], p_full[TC_TILES][2], o_free[TC_TILES];
+    uint64_t u_full[2], u_empty[2], q_full, q_empty, v_mend, v_fixed, o_full, drain;
+    Unit unit[2];
+    int per, any_again;
     uint32_t tmem;
-    uint32_t again[TC_SOFTMAX_WARPS];   // each softmax warp's rows that came out not finite
-    float top[2][TC_CTA_ROWS];          // [part][row] a tile's largest scores; at the end sums
     int abort;
 };
 template <int DP>
@@ -103,6 +132,15 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One box of the queries: values [x, x + 64) of heads y... of tokens z....
+__device__ __forceinline__ void tma_load_q(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
 
 // One CTA's kind::f16 MMAs with the descriptors' halves apart: the upper words are
 // constants and the lower ones differ by constants (addresses are below 2^18, so a
@@ -145,12 +183,16 @@ __device__ __forceinline__ uint32_t elect_one() {
     return one;
 }
 
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -215,8 +257,8 @@ __device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
     y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 
-// Weights exp2(sc (s - m)) of 32 of a row's scores v, packed in pairs, and their sum (a
-// pair of partial sums); with TOP also the largest of the 64 scores from v on.  m = -inf
+// Weights exp2(sc (s - m)) of 64 of a row's scores v, packed in pairs, and their sum (two
+// pairs of partial sums); with TOP also the largest of the 128 scores from v on.  m = -inf
 // (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
@@ -226,53 +268,184 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
     const float neg = m == -INFINITY ? 0.0f : -m * sc;
     const uint64_t neg2 = pack_f2(neg, neg);
-    uint64_t s0 = pack_f2(0.0f, 0.0f), s1 = s0;
-    float x[16], y[16], mx0 = -INFINITY, mx1 = -INFINITY;
+    sum[0] = sum[1] = pack_f2(0.0f, 0.0f);
+    float x[32], y[32], mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16 + LAG; ++i) {
-        if (i < 16) {
+    for (int i = 0; i < 32 + LAG; ++i) {
+        if (i < 32) {
             const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
             if (i % 8 < TC_POLY) {
                 exp2_pair(e, x[i], y[i]);
             } else {
                 unpack_f2(e, x[i], y[i]);
                 x[i] = ex2(x[i]);
-                if (TOP) mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
                 y[i] = ex2(y[i]);
             }
-            if (TOP && i % 8 < TC_POLY) mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
-            if (TOP) mx1 = max3(mx1, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            if (TOP) {
+                mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
+                mx1 = max3(mx1, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            }
         }
         if (i >= LAG) {
             const int u = i - LAG;
-            if (u & 1) s1 = add_f2(s1, pack_f2(x[u], y[u]));
-            else s0 = add_f2(s0, pack_f2(x[u], y[u]));
+            sum[u & 1] = add_f2(sum[u & 1], pack_f2(x[u], y[u]));
             // weights in the cache's type for the product: relative 2^-9 (bf16) or
             // 2^-12, the size of the output's own rounding; the sum keeps fp32
             p[u] = pack2<T>(x[u], y[u]);
         }
     }
-    *sum = add_f2(s0, s1);
     return TOP ? max3(mx0, mx1, mx1) : 0.0f;
 }
 
-__device__ __forceinline__ void pair_sync(int id) {
-    asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
-}
-
-// CTAs of a sequence: row blocks x heads.
+// Units of a sequence, and the key tiles of any of them (an upper bound).
 struct TcLoad {
-    int64_t blocks;
-    int row_blocks;
+    int64_t units;
+    int row_blocks, tiles;
 };
 
 __device__ __forceinline__ TcLoad tc_load(const TcArgs& t, const Seq& q) {
     const int64_t rows = (int64_t)q.n_new * t.a.group;
-    TcLoad x{0, 0};
+    TcLoad x{0, 0, 0};
     if (rows < t.min_rows) return x;
     x.row_blocks = (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
-    x.blocks = (int64_t)x.row_blocks * t.a.hk;
+    x.units = (int64_t)x.row_blocks * t.a.hk;
+    int64_t n = ((int64_t)q.kv + TC_KEYS - 1) / TC_KEYS;
+    if (t.a.window > 0) {
+        const int64_t near = ((int64_t)t.a.window + TC_CTA_ROWS / t.a.group + 1 + TC_KEYS) / TC_KEYS + 1;
+        n = min(n, near + ((int64_t)t.a.sinks + TC_KEYS - 1) / TC_KEYS);
+    }
+    x.tiles = (int)max(n, (int64_t)1);
     return x;
+}
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Key tiles of a piece: all of a unit's, unless the units leave CTAs without work; then
+// the smallest number at which the pieces are no more than the CTAs.  One warp.
+__device__ __forceinline__ int tiles_per_piece(const TcArgs& t) {
+    const int lane = threadIdx.x & 31;
+    const int64_t ctas = gridDim.x;
+    if (!t.split) return INT_MAX;
+    int64_t units = 0, tiles = 0;
+    for (int s = lane; s < t.a.b.n_seq; s += 32) {
+        const TcLoad x = tc_load(t, load_seq(t.a.b, t.a.max_kv, s, t.a.status));
+        units += x.units;
+        tiles += x.units * x.tiles;
+    }
+    units = warp_sum(units);
+    tiles = warp_sum(tiles);
+    if (units == 0 || units >= ctas) return INT_MAX;
+    int64_t per = max((int64_t)TC_MIN_PIECE, (tiles + ctas - 1) / ctas);
+    while (true) {
+        int64_t items = 0;
+        for (int s = lane; s < t.a.b.n_seq; s += 32) {
+            const TcLoad x = tc_load(t, load_seq(t.a.b, t.a.max_kv, s, t.a.status));
+            items += x.units * ((x.tiles + per - 1) / per);
+        }
+        if (warp_sum(items) <= ctas) return (int)per;
+        per += max((int64_t)1, per / 16);
+    }
+}
+
+// The item-th piece of all sequences' units, by one warp, into *u (s = -1: there is none).
+__device__ __forceinline__ void describe(const TcArgs& t, int64_t item, int per, Unit* u) {
+    const AttnArgs& a = t.a;
+    const int lane = threadIdx.x & 31;
+    int64_t run = 0;
+    for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
+        const int s = s0 + lane;
+        Seq q{0, 0, 0, false};
+        TcLoad x{0, 0, 0};
+        if (s < a.b.n_seq) {
+            q = load_seq(a.b, a.max_kv, s, a.status);
+            x = tc_load(t, q);
+        }
+        const int pieces = x.units > 0 ? (int)(((int64_t)x.tiles + per - 1) / per) : 0;
+        const int64_t v = x.units * pieces;
+        int64_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t w = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += w;
+        }
+        const bool here = run + incl - v <= item && item < run + incl;
+        if (here) {
+            const int at = (int)(item - (run + incl - v)), unit = at / pieces, piece = at - unit * pieces;
+            // a sequence's last rows see the most keys: they go first, so that the
+            // short blocks fill the end
+            const int kvh = unit % a.hk, rb = x.row_blocks - 1 - unit / a.hk;
+            const int row0 = rb * TC_CTA_ROWS;
+            const int rows = (int)min((int64_t)TC_CTA_ROWS, (int64_t)q.n_new * a.group - row0);
+            const Span sp = tile_span(a, q, row0, row0 + rows);
+            const int sink_tiles = (sp.sink + TC_KEYS - 1) / TC_KEYS;
+            const int first = max(sp.lo / TC_KEYS, sink_tiles);
+            const int t0 = pieces > 1 ? piece * per : 0;
+            u->s = s;
+            u->kvh = kvh;
+            u->row0 = row0;
+            u->rows = rows;
+            u->q = q;
+            u->sp = sp;
+            u->sink_tiles = sink_tiles;
+            u->first = first;
+            u->t0 = t0;
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < TC_TILES; ++w) {
+                const int r0 = row0 + w * TC_ROWS, r1 = min(row0 + rows, r0 + TC_ROWS);
+                int nw = 0;
+                if (r0 < r1) {
+                    const int hi = tile_span(a, q, r0, r1).hi;
+                    nw = sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - first) - t0;
+                    nw = max(0, min(nw, per));
+                }
+                u->n_of[w] = nw;
+                n = max(n, nw);
+            }
+            u->n = n;
+            u->pieces = pieces;
+            u->item = (int)item;
+            if (t.split && item < gridDim.x)
+                t.joint[item] = make_int4(s, kvh, rb, pieces > 1 && piece == 0 ? pieces : 0);
+        }
+        if (__any_sync(0xffffffffu, here)) {
+            __syncwarp();
+            return;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+        u->s = -1;
+        if (t.split && item < gridDim.x) t.joint[item] = make_int4(0, 0, 0, 0);
+    }
+    __syncwarp();
+}
+
+// A CTA's k-th item.  One sequence's items fall in size, so rounds in turn from the first
+// and the last CTA even out; of several sequences each CTA takes the next one left.
+__device__ __forceinline__ int64_t item_of(const TcArgs& t, int k) {
+    if (t.next) {
+        int x = 0;
+        if ((threadIdx.x & 31) == 0) x = atomicAdd(t.next, 1);
+        return __shfl_sync(0xffffffffu, x, 0);
+    }
+    return (int64_t)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// A full sector (32 bytes) or two halves of one.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v, bool whole) {
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                     "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
 }
 
 // Byte of 16-byte piece c of row r of Q: [tile][64 columns][128 rows][128 B], swizzled.
@@ -285,7 +458,7 @@ __device__ __forceinline__ uint32_t q_at(int r, int c) {
 template <typename T, int DP>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ TcArgs t) {
+                   const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ TcArgs t) {
     constexpr int ST = tc_stages<DP>();
     constexpr int TILE = tc_tile_bytes<DP>();
     constexpr int HALVES = DP / 64;                    // 128-byte column blocks
@@ -301,73 +474,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     TcCtrl* ctl = reinterpret_cast<TcCtrl*>(Rs + ST * TILE);
     const AttnArgs& a = t.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    // ---- this CTA's unit
-    {
-        int64_t run = 0;
-        bool found = false;
-        for (int s0 = 0; s0 < a.b.n_seq; s0 += TC_THREADS) {
-            const int s = s0 + threadIdx.x;
-            int64_t v = 0;
-            Seq mine{0, 0, 0, false};
-            if (s < a.b.n_seq) {
-                mine = load_seq(a.b, a.max_kv, s, a.status);
-                v = tc_load(t, mine).blocks;
-            }
-            int64_t incl = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += u;
-            }
-            if (lane == 31) ctl->scan[warp] = incl;
-            __syncthreads();
-            int64_t sum = 0;
-#pragma unroll
-            for (int w = 0; w < TC_WARPS; ++w) {
-                if (w < warp) incl += ctl->scan[w];
-                sum += ctl->scan[w];
-            }
-            incl += run;
-            if (incl - v <= (int64_t)blockIdx.x && (int64_t)blockIdx.x < incl) {
-                ctl->seq = s;
-                ctl->own = mine;
-                ctl->pre = incl - v;
-            }
-            run += sum;
-            found = run > (int64_t)blockIdx.x;
-            __syncthreads();
-            if (found) break;
-        }
-        if (!found) return;
-    }
-    const int s = ctl->seq;
-    const Seq q = ctl->own;
-    const TcLoad ld = tc_load(t, q);
-    const int unit = (int)(blockIdx.x - ctl->pre);
-    // a sequence's last rows see the most keys: they go first, so that the
-    // short blocks fill the end
-    const int kvh = unit % a.hk, rb = ld.row_blocks - 1 - unit / a.hk;
-    const int row0 = rb * TC_CTA_ROWS;
-    const int rows = (int)min((int64_t)TC_CTA_ROWS, (int64_t)q.n_new * a.group - row0);
-    const Span sp = tile_span(a, q, row0, row0 + rows);
-    const int sink_tiles = (sp.sink + TC_KEYS - 1) / TC_KEYS;
-    const int first = max(sp.lo / TC_KEYS, sink_tiles);
-    auto tiles_to = [&](int hi) { return sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - first); };
-    auto key0_of = [&](int j) { return (j < sink_tiles ? j : first + j - sink_tiles) * TC_KEYS; };
-    // tiles with keys that no row sees beside some that are seen
-    auto mends = [&](int key0) {
-        return !(key0 >= sp.lo && key0 + TC_KEYS <= sp.hi) && key0 + TC_KEYS > sp.sink;
-    };
-    // key tiles of each row tile: a prefix of the CTA's
-    int n_of[TC_TILES];
-#pragma unroll
-    for (int w = 0; w < TC_TILES; ++w) {
-        const int r0 = row0 + w * TC_ROWS, r1 = min(row0 + rows, r0 + TC_ROWS);
-        n_of[w] = r0 < r1 ? tiles_to(tile_span(a, q, r0, r1).hi) : 0;
-    }
-    const int n = max(n_of[0], n_of[1]);
     volatile int* abort = &ctl->abort;
+    if (t.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
@@ -378,12 +486,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             mbar_init(&ctl->s_full[w], 1);
             mbar_init(&ctl->p_full[w][0], TC_SOFTMAX_WARPS / 2);
             mbar_init(&ctl->p_full[w][1], TC_SOFTMAX_WARPS / 2);
+            mbar_init(&ctl->o_free[w], TC_SOFTMAX_WARPS / 2);
         }
-        mbar_init(&ctl->q_full, TC_SOFTMAX_WARPS);
+        for (int k = 0; k < 2; ++k) {
+            mbar_init(&ctl->u_full[k], 1);
+            mbar_init(&ctl->u_empty[k], TC_SOFTMAX_WARPS + 3);   // softmax, TMA, MMA, zeros
+        }
+        mbar_init(&ctl->q_full, 1);
+        mbar_init(&ctl->q_empty, 1);
         mbar_init(&ctl->v_mend, 1);
         mbar_init(&ctl->v_fixed, 1);
         mbar_init(&ctl->o_full, 1);
         mbar_init(&ctl->drain, 1);
+        ctl->any_again = 0;
         ctl->abort = 0;
         fence_barrier_init();
     }
@@ -395,6 +510,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem;   // S_w at 128 w, O_w at 256 + DP w
+    auto give_up = [&] {
+        if (lane == 0) {
+            atomicExch(&ctl->abort, 1);
+            atomicOr(a.status, HMM_STATUS_TIMEOUT);
+        }
+    };
+    // The k-th unit lies in ctl->unit[k & 1] between these two.
+    auto take = [&](int k) { return wait_warp(&ctl->u_full[k & 1], (k >> 1) & 1, abort, t.wait_ns); };
+    auto leave = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->u_empty[k & 1]);
+    };
 
     // The same setmaxnreg for all warps of a warpgroup; what is outside of the roles runs
     // with the launch's registers again.
@@ -407,53 +534,52 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 prefetch_tmap(&tmK);
                 prefetch_tmap(&tmV);
             }
-            auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
-                *page = a.n_pages;                            // out of range: zeros
-                *row = 0;
-                if (j < n && lane < subs) {
-                    const int k0 = key0_of(j) + lane * br;
-                    if (k0 < sp.sink || (k0 + br > sp.lo && k0 < sp.hi)) {
-                        const int e = page_of(a, s, k0 / a.page_tokens);
-                        if (e >= 0) {
-                            *page = e;
-                            *row = k0 % a.page_tokens;
+            uint32_t i = 0;                                   // boxes' tiles so far, K and V in turn
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                const Unit& u = ctl->unit[k & 1];
+                if (!(ok = take(k)) || u.s < 0) break;
+                auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
+                    *page = a.n_pages;                            // out of range: zeros
+                    *row = 0;
+                    if (j < u.n && lane < subs) {
+                        const int k0 = u.key0(j) + lane * br;
+                        if (k0 < u.sp.sink || (k0 + br > u.sp.lo && k0 < u.sp.hi)) {
+                            const int e = page_of(a, u.s, k0 / a.page_tokens);
+                            if (e >= 0) {
+                                *page = e;
+                                *row = k0 % a.page_tokens;
+                            }
                         }
                     }
-                }
-            };
-            int page, row, issued = 0;
-            bool ok = true;
-            lookup(0, &page, &row);
-            for (int j = 0; ok && j < n; ++j) {
-                int next_page, next_row;
-                lookup(j + 1, &next_page, &next_row);
-                for (int kv = 0; kv < 2; ++kv) {
-                    const int i = 2 * j + kv, st = i % ST;
-                    if (!wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
-                    __syncwarp();
-                    issued = i + 1;
-                    if (lane < subs) {
-                        const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
+                };
+                int page, row;
+                lookup(0, &page, &row);
+                for (int j = 0; ok && j < u.n; ++j) {
+                    int next_page, next_row;
+                    lookup(j + 1, &next_page, &next_row);
+                    for (int kv = 0; kv < 2; ++kv, ++i) {
+                        const uint32_t st = i % ST;
+                        if (!(ok = wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns))) break;
+                        if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
+                        __syncwarp();
+                        if (lane < subs) {
+                            const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
 #pragma unroll
-                        for (int h = 0; h < HALVES; ++h)
-                            tma_load_page(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h, row,
-                                        kvh, page);
+                            for (int h = 0; h < HALVES; ++h)
+                                tma_load_page(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h,
+                                              row, u.kvh, page);
+                        }
                     }
+                    page = next_page;
+                    row = next_row;
                 }
-                page = next_page;
-                row = next_row;
+                leave(k);
             }
             if (!ok) {
-                if (lane == 0) {
-                    atomicExch(&ctl->abort, 1);
-                    atomicOr(a.status, HMM_STATUS_TIMEOUT);
-                }
-                for (int i = max(0, issued - ST); i < issued; ++i)   // copies in flight land first
-                    mbar_wait_drain(&ctl->full[i % ST], (i / ST) & 1);
+                give_up();
+                for (uint32_t b = i > ST ? i - ST : 0; b < i; ++b)   // copies in flight land first
+                    mbar_wait_drain(&ctl->full[b % ST], (b / ST) & 1);
             }
         } else if (warp == TC_SOFTMAX_WARPS + 1) {
             // --------------------------------------------------------- MMA
@@ -466,8 +592,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const uint32_t khi = (uint32_t)(dk >> 32), vhi = (uint32_t)(dv >> 32);
             const uint32_t klo = (uint32_t)dk, vlo = (uint32_t)dv, qlo = (uint32_t)dq;
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-            const int nu = __shfl_sync(0xffffffffu, n, 0);
-            const int nu_of[2] = {__shfl_sync(0xffffffffu, n_of[0], 0), __shfl_sync(0xffffffffu, n_of[1], 0)};
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 return wait_warp(bar, parity, abort, t.wait_ns);
             };
@@ -480,30 +604,59 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
                 commit_one(one, &ctl->s_full[w]);
             };
-            if (nu > 0) {
-                int fixed = 0, sv = 1, pv = 0, sk = 2 % ST, pk = 2 / ST;   // stages of V_j, K_j+1 and their phases
-                bool ok = wait(&ctl->q_full, 0) && wait(&ctl->full[0], 0);
-                if (ok) {
-                    tc_fence_after();
+            int st = 0, ph = 0;                  // the ring's next tile
+            auto next = [&](int& x, int& p) {
+                if (++x == ST) {
+                    x = 0;
+                    p ^= 1;
+                }
+            };
+            int fixed = 0, busy = 0;             // tiles mended; units with keys so far
+            int tiles[TC_TILES] = {0, 0};        // key tiles of each row tile so far
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                if (!(ok = take(k))) break;
+                const Unit& u = ctl->unit[k & 1];
+                const int us = __shfl_sync(0xffffffffu, u.s, 0), n = __shfl_sync(0xffffffffu, u.n, 0);
+                const int n_of[2] = {__shfl_sync(0xffffffffu, u.n_of[0], 0), __shfl_sync(0xffffffffu, u.n_of[1], 0)};
+                // key tiles with rows that no row sees: found from the first and the last few
+                const int t0 = u.t0, sink_tiles = u.sink_tiles, first = u.first;
+                const int lo = u.sp.lo, hi = u.sp.hi, sink = u.sp.sink;
+                leave(k);
+                if (us < 0) break;
+                if (n == 0) continue;
+                if (!(ok = wait(&ctl->q_full, busy & 1) && wait(&ctl->full[st], ph))) break;
+                tc_fence_after();
+                {
+                    const uint32_t kl = klo + st * (TILE / 16);
 #pragma unroll
                     for (int w = 0; w < TC_TILES; ++w)
-                        if (nu_of[w] > 0) qk(w, klo);
-                    commit_one(one, &ctl->empty[0]);
+                        if (n_of[w] > 0) qk(w, kl);
                 }
-                for (int j = 0; ok && j < nu; ++j) {
-                    const uint32_t v = vlo + sv * (TILE / 16), k = klo + sk * (TILE / 16);
-                    if (!(ok = wait(&ctl->full[sv], pv))) break;
-                    if (mends(key0_of(j))) {
+                commit_one(one, &ctl->empty[st]);
+                if (n == 1) commit_one(one, &ctl->q_empty);
+                next(st, ph);
+                for (int j = 0; ok && j < n; ++j) {
+                    int sk = st, pk = ph;        // K_j+1, behind V_j
+                    next(sk, pk);
+                    const uint32_t v = vlo + st * (TILE / 16), kl = klo + sk * (TILE / 16);
+                    if (!(ok = wait(&ctl->full[st], ph))) break;
+                    const int key0 = (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
+                    if (!(key0 >= lo && key0 + TC_KEYS <= hi) && key0 + TC_KEYS > sink) {
                         if (lane == 0) mbar_arrive(&ctl->v_mend);
                         if (!(ok = wait(&ctl->v_fixed, fixed++ & 1))) break;
                     }
+                    // the results of the unit before have left TMEM
+                    if (j == 0 && busy > 0 &&
+                        !(ok = wait(&ctl->o_free[0], (busy - 1) & 1) && wait(&ctl->o_free[1], (busy - 1) & 1)))
+                        break;
                     bool k_ready = false;
 #pragma unroll
                     for (int w = 0; w < TC_TILES; ++w) {
-                        if (j >= nu_of[w]) continue;
+                        if (j >= n_of[w]) continue;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            if (!(ok = wait(&ctl->p_full[w][h], j & 1))) break;
+                            if (!(ok = wait(&ctl->p_full[w][h], (tiles[w] + j) & 1))) break;
                             tc_fence_after();
 #pragma unroll
                             for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
@@ -511,52 +664,118 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                                        j > 0 || ks > 0);
                         }
                         if (!ok) break;
-                        if (j + 1 < nu_of[w]) {
+                        if (j + 1 < n_of[w]) {
                             if (!k_ready && !(ok = wait(&ctl->full[sk], pk))) break;
                             k_ready = true;
-                            qk(w, k);
+                            qk(w, kl);
                         }
                     }
                     if (!ok) break;
-                    commit_one(one, &ctl->empty[sv]);
-                    if (j + 1 < nu) commit_one(one, &ctl->empty[sk]);
-                    else commit_one(one, &ctl->o_full);
-                    if ((sv += 2) >= ST) { sv -= ST; pv ^= 1; }
-                    if ((sk += 2) >= ST) { sk -= ST; pk ^= 1; }
-                }
-                if (!ok) {
-                    if (lane == 0) {
-                        atomicExch(&ctl->abort, 1);
-                        atomicOr(a.status, HMM_STATUS_TIMEOUT);
+                    commit_one(one, &ctl->empty[st]);
+                    if (j + 1 < n) {
+                        commit_one(one, &ctl->empty[sk]);
+                        if (j + 2 == n) commit_one(one, &ctl->q_empty);   // the unit's last scores
+                        next(st, ph);
+                    } else {
+                        commit_one(one, &ctl->o_full);
                     }
-                    commit_one(one, &ctl->drain);    // the MMAs issued end before TMEM is freed
-                    mbar_wait_drain(&ctl->drain, 0);
+                    next(st, ph);
                 }
+                tiles[0] += n_of[0];
+                tiles[1] += n_of[1];
+                ++busy;
+            }
+            if (!ok) {
+                give_up();
+                commit_one(one, &ctl->drain);    // the MMAs issued end before TMEM is freed
+                mbar_wait_drain(&ctl->drain, 0);
             }
             __syncwarp();
         } else if (warp == TC_SOFTMAX_WARPS + 2) {
             // ------------------------------------------------ V's unseen rows
             // V rows that no row of the CTA sees, in boxes that were read, become zeros:
             // a weight of zero times what a slot of nobody holds is only zero then.
-            // The MMA lane says when such a tile has arrived, and waits: this warp, which
+            // The MMA warp says when such a tile has arrived, and waits: this warp, which
             // skips the others, could not tell a stage's phases apart.
             int mended = 0;
-            for (int j = 0; j < n; ++j) {
-                const int key0 = key0_of(j), st = (2 * j + 1) % ST;
-                if (!mends(key0)) continue;
-                if (!wait_warp(&ctl->v_mend, mended++ & 1, abort, t.wait_ns)) break;
-                for (int r = lane; r < TC_KEYS; r += 32) {
-                    const int key = key0 + r, k0 = key - r % t.box_rows;
-                    if (!span_has(sp, key) && (k0 < sp.sink || (k0 + t.box_rows > sp.lo && k0 < sp.hi))) {
+            uint32_t base = 0;                   // the ring's tiles before this unit
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                const Unit& u = ctl->unit[k & 1];
+                if (!(ok = take(k)) || u.s < 0) break;
+                for (int j = 0; j < u.n; ++j) {
+                    const int key0 = u.key0(j);
+                    const uint32_t st = (base + 2 * j + 1) % ST;
+                    if (!u.mends(key0)) continue;
+                    if (!(ok = wait_warp(&ctl->v_mend, mended++ & 1, abort, t.wait_ns))) break;
+                    for (int r = lane; r < TC_KEYS; r += 32) {
+                        const int key = key0 + r, k0 = key - r % t.box_rows;
+                        if (!span_has(u.sp, key) &&
+                            (k0 < u.sp.sink || (k0 + t.box_rows > u.sp.lo && k0 < u.sp.hi))) {
 #pragma unroll
-                        for (int c = 0; c < HALVES * 8; ++c)
-                            *reinterpret_cast<uint4*>(Rs + st * TILE + (c >> 3) * (TC_KEYS * 128) + r * 128 +
-                                                      (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            for (int c = 0; c < HALVES * 8; ++c)
+                                *reinterpret_cast<uint4*>(Rs + st * TILE + (c >> 3) * (TC_KEYS * 128) + r * 128 +
+                                                          (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->v_fixed);
+                }
+                base += 2 * u.n;
+                leave(k);
+            }
+        } else {
+            // -------------------------------------- the units, and their queries
+            const int per = tiles_per_piece(t);
+            if (lane == 0) ctl->per = per;
+            int busy = 0;
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.wait_ns))) break;
+                Unit* u = &ctl->unit[k & 1];
+                const int64_t item = item_of(t, k);
+                describe(t, item, per, u);
+                if (t.next && u->s >= 0 && lane == 0) t.owner[item] = blockIdx.x;
+                const int s = u->s, n = u->n, row0 = u->row0, rows = u->rows, kvh = u->kvh, begin = u->q.begin;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->u_full[k & 1]);
+                if (s < 0) break;
+                if (n == 0) continue;
+                if (!(ok = wait_warp(&ctl->q_empty, (busy++ & 1) ^ 1, abort, t.wait_ns))) break;
+                constexpr int CH = DP / 8;
+                const uint32_t q0 = smem_u32(Qs);
+                if (t.q_tokens > 0) {   // a tile's 128 rows are whole tokens' groups: boxes of them
+                    if (lane == 0) mbar_expect_tx(&ctl->q_full, tc_q_bytes<DP>());
+                    __syncwarp();
+                    const int b = lane;
+                    if (b < TC_TILES * HALVES)
+                        tma_load_q(q0 + b * (TC_ROWS * 128), &tmQ, &ctl->q_full, 64 * (b % HALVES), kvh * a.group,
+                                   begin + a.by_group(row0) + (b / HALVES) * t.q_tokens);
+                    continue;
+                }
+#pragma unroll 8
+                for (int i = lane; i < TC_CTA_ROWS * CH; i += 32) {
+                    const int r = i / CH, c = i % CH;
+                    const bool real = r < rows && c * 8 < a.D;
+                    const int x = row0 + (real ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
+                    cp16(q0 + q_at<DP>(r, c),
+                         a.q + (int64_t)(begin + tok) * a.q_token + (int64_t)(kvh * a.group + head) * a.q_head +
+                             (real ? 16 * c : 0),
+                         real);
+                }
+                cp_commit();
+                cp_wait<0>();
+                if (a.scale < 0.0f) {   // turned signs: the largest score is the largest product
+#pragma unroll 1
+                    for (int i = lane; i < TC_CTA_ROWS * CH; i += 32) {
+                        uint4* x = reinterpret_cast<uint4*>(Qs + q_at<DP>(i / CH, i % CH));
+                        *x = make_uint4(x->x ^ 0x80008000u, x->y ^ 0x80008000u, x->z ^ 0x80008000u, x->w ^ 0x80008000u);
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->v_fixed);
+                if (lane == 0) mbar_arrive(&ctl->q_full);
             }
         }
         tc_fence_before();
@@ -565,199 +784,205 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     } else {
         // --------------------------------------------------------- softmax
         set_regs_up<TC_REGS_SOFTMAX>();
-        // Two threads share a row: part p has the scores of keys [32 p, 32 p + 32) and
-        // [64 + 32 p, 96 + 32 p) of a tile, and half of the row's results.  Two warps per
-        // row tile on each scheduler keep the special-function unit busy where one, with
-        // the maxima and the conversions between, leaves it idle half of the time.
-        {
-            // q rows, swizzled
-            constexpr int CH = DP / 8;
-            const uint32_t q0 = smem_u32(Qs);
-#pragma unroll
-            for (int i = 0; i < TC_CTA_ROWS * CH / TC_SOFTMAX; ++i) {
-                const int at = i * TC_SOFTMAX + threadIdx.x, r = at / CH, c = at % CH;
-                const bool real = r < rows && c * 8 < a.D;
-                const int tok = a.by_group(row0 + (real ? r : 0)), head = row0 + (real ? r : 0) - tok * a.group;
-                cp16(q0 + q_at<DP>(r, c),
-                     a.q + (int64_t)(q.begin + tok) * a.q_token + (int64_t)(kvh * a.group + head) * a.q_head + (real ? 16 * c : 0),
-                     real);
-            }
-            cp_commit();
-            cp_wait<0>();
-            if (a.scale < 0.0f) {   // turned signs: the largest score is the largest product
-#pragma unroll 1
-                for (int i = 0; i < TC_CTA_ROWS * CH / TC_SOFTMAX; ++i) {
-                    const int at = i * TC_SOFTMAX + threadIdx.x;
-                    uint4* x = reinterpret_cast<uint4*>(Qs + q_at<DP>(at / CH, at % CH));
-                    *x = make_uint4(x->x ^ 0x80008000u, x->y ^ 0x80008000u, x->z ^ 0x80008000u, x->w ^ 0x80008000u);
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->q_full);
-        }
-        const int w = warp >> 3, part = (warp >> 2) & 1;
+        const int w = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + part * (DP / 2) + lanes;
-        const int r = w * TC_ROWS + (warp & 3) * 32 + lane;   // row of the CTA
-        const int wr0 = r - lane;                              // the warp's rows: [wr0, wr1)
-        const int wr1 = min(rows, wr0 + 32);
-        const int pair = 2 + w * 4 + (warp & 3);               // barrier of the two warps of these rows
-        const int pos = row_pos(a, q, row0 + min(r, rows - 1));
-        const int pos_first = row_pos(a, q, row0 + min(wr0, rows - 1));
-        const int pos_last = row_pos(a, q, row0 + max(wr1, 1) - 1);
+        const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + lanes;
+        const int wr0 = warp * 32, r = wr0 + lane;             // the warp's first row of the unit, the thread's
         const float sc = fabsf(a.scale_log2);
         const uint64_t sc2 = pack_f2(sc, sc);
-        float m = -INFINITY;
-        uint64_t l2[2] = {pack_f2(0.0f, 0.0f), pack_f2(0.0f, 0.0f)};
-        bool ok = true, fine = true;
-        const int nw = n_of[w];
-        for (int j = 0; j < nw; ++j) {
-            // (a warp that gave up keeps the pair's count of barriers: its partner may not
-            // have, or at another tile)
-            if (ok) ok = wait_warp(&ctl->s_full[w], j & 1, abort, t.wait_ns);
-            if (!ok) {
-                pair_sync(pair);
-                continue;
-            }
-            tc_fence_after();
-            uint32_t v[64];
-            tmem_ld_x32(ts + 32 * part, v);
-            tmem_ld_x32(ts + 64 + 32 * part, v + 32);
-            tmem_wait_ld();
-            const int key0 = key0_of(j);
-            if (!(key0 + TC_KEYS <= q.kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
-                  (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
-                const int at = key0 + 32 * part;
-                const int hi = (a.causal ? min(q.kv, pos + 1) : q.kv) - at;
-                const int lo = a.window > 0 ? max(0, pos - a.window + 1) - at : -TC_KEYS;
-                const int sink = a.window > 0 ? a.sinks - at : 0;
+        int tiles = 0, busy = 0;                               // key tiles, units with keys so far
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            const Unit& u = ctl->unit[k & 1];
+            if (!(ok = take(k)) || u.s < 0) break;
+            const int rows = u.rows, n = u.n, nw = u.n_of[w];
+            const int pos = row_pos(a, u.q, u.row0 + min(r, rows - 1));
+            const int pos_first = row_pos(a, u.q, u.row0 + min(wr0, rows - 1));
+            const int pos_last = row_pos(a, u.q, u.row0 + min(wr0 + 31, rows - 1));
+            float m = -INFINITY;
+            uint64_t l2[2] = {pack_f2(0.0f, 0.0f), pack_f2(0.0f, 0.0f)};
+            bool fine = true;
+            for (int j = 0; j < nw; ++j) {
+                if (!(ok = wait_warp(&ctl->s_full[w], (tiles + j) & 1, abort, t.wait_ns))) break;
+                tc_fence_after();
+                uint32_t v[TC_KEYS];
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    const int c = i < 32 ? i : i + 32;
-                    if (c >= hi || (c < lo && c >= sink)) v[i] = 0xff800000u;
+                for (int c = 0; c < TC_KEYS; c += 32) tmem_ld_x32(ts + c, v + c);
+                tmem_wait_ld();
+                const int key0 = u.key0(j), kv = u.q.kv;
+                if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
+                      (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
+                    const int hi = (a.causal ? min(kv, pos + 1) : kv) - key0;
+                    const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : -1;
+                    const int sink = a.window > 0 ? a.sinks - key0 : 0;
+#pragma unroll
+                    for (int c = 0; c < TC_KEYS; ++c)
+                        if (c >= hi || (c < lo && c >= sink)) v[c] = 0xff800000u;
                 }
-            }
-            // The first half's weights with the maximum so far, while this tile's is found:
-            // that is right unless the row grew by more than TC_GROWTH, which is rare.
-            uint32_t p[16];
-            uint64_t sum;
-            // NaN and +inf show in the maximum: such a row is computed again at the end.
-            float top = weights<T, true>(v, sc2, m, sc, p, &sum);
-            ctl->top[part][r] = top;   // read before the partner's weights, and so before the next tile
-            pair_sync(pair);
-            top = max3(top, ctl->top[part ^ 1][r], top);
-            fine = fine && top < INFINITY;
-            const bool grow = (top - m) * sc > TC_GROWTH;
-            if (__any_sync(0xffffffffu, grow)) {
-                const float al = grow ? ex2((m - top) * sc) : 1.0f;
-                if (grow) m = top;
-                const uint64_t al2 = pack_f2(al, al);
-                l2[0] = fma_f2(l2[0], al2, pack_f2(0.0f, 0.0f));
-                l2[1] = fma_f2(l2[1], al2, pack_f2(0.0f, 0.0f));
-                if (j > 0) {
+                // The first half's weights with the maximum so far, while this tile's is found:
+                // that is right unless the row grew by more than TC_GROWTH, which is rare.
+                uint32_t p[32];
+                uint64_t sum[2];
+                // NaN and +inf show in the maximum: such a row is computed again at the end.
+                const float top = weights<T, true>(v, sc2, m, sc, p, sum);
+                fine = fine && top < INFINITY;
+                const bool grow = (top - m) * sc > TC_GROWTH;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float al = grow ? ex2((m - top) * sc) : 1.0f;
+                    if (grow) m = top;
+                    const uint64_t al2 = pack_f2(al, al);
+                    l2[0] = fma_f2(l2[0], al2, pack_f2(0.0f, 0.0f));
+                    l2[1] = fma_f2(l2[1], al2, pack_f2(0.0f, 0.0f));
+                    if (j > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < DP / 2; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld_x16(to + c, o);
-                        tmem_wait_ld();
+                        for (int c = 0; c < DP; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld_x32(to + c, o);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                        tmem_st_x16(to + c, o);
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                            tmem_st_x32(to + c, o);
+                        }
                     }
+                    weights<T, false>(v, sc2, m, sc, p, sum);
                 }
-                weights<T, false>(v, sc2, m, sc, p, &sum);
+                // the first half's product starts while the second half is in the exponentials
+                tmem_st_x32(ts, p);
+                l2[0] = add_f2(l2[0], sum[0]);
+                l2[1] = add_f2(l2[1], sum[1]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
+                weights<T, false>(v + 64, sc2, m, sc, p, sum);
+                tmem_st_x32(ts + 32, p);
+                l2[0] = add_f2(l2[0], sum[0]);
+                l2[1] = add_f2(l2[1], sum[1]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_full[w][1]);
             }
-            // the first half's product starts while the second half is in the exponentials
-            tmem_st_x16(ts + 16 * part, p);
-            l2[0] = add_f2(l2[0], sum);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-            weights<T, false>(v + 32, sc2, m, sc, p, &sum);
-            tmem_st_x16(ts + 32 + 16 * part, p);
-            l2[1] = add_f2(l2[1], sum);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->p_full[w][1]);
-        }
-        // ---- the rows' results
-        if (ok && n > 0) ok = wait_warp(&ctl->o_full, 0, abort, t.wait_ns);
-        float l, lb;
-        unpack_f2(add_f2(l2[0], l2[1]), l, lb);
-        ctl->top[part][r] = l + lb;
-        if (!ok && lane == 0) {
-            atomicExch(&ctl->abort, 1);
-            atomicOr(a.status, HMM_STATUS_TIMEOUT);
-        }
-        pair_sync(pair);
-        // (after a wait that ran out, too: every warp passes the same barriers, and what it
-        // writes, in its own rows, is as invalid as the call says)
-        {
+            // ---- the rows' results
+            if (ok && n > 0) ok = wait_warp(&ctl->o_full, busy & 1, abort, t.wait_ns);
+            if (!ok) break;
             tc_fence_after();
-            l = ctl->top[0][r] + ctl->top[1][r];
-            const bool live = r < rows;
-            const int tok = a.by_group(row0 + (live ? r : 0)), head = row0 + (live ? r : 0) - tok * a.group;
-            const int64_t orow = (int64_t)(q.begin + tok) * a.hq + kvh * a.group + head;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            tiles += nw;
+            float l, lb;
+            unpack_f2(add_f2(l2[0], l2[1]), l, lb);
+            l += lb;
+            const bool live = r < rows, some = nw > 0 && l != 0.0f, whole_unit = u.pieces == 1;
+            const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
+            const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
+            float* pt = t.part + (int64_t)u.item * TC_CTA_ROWS * (DP + 2);   // (split units)
             fine = fine && l == l;
-            // through shared memory (every product is complete), rows 16 bytes apart in
-            // their banks, so that whole rows go out at once
-            constexpr int OROW = DP * 2 + 16;
-            unsigned char* os = smem_raw + r * OROW + part * DP;
-#pragma unroll
-            for (int c = 0; c < DP / 2; c += 16) {
-                uint32_t o[16];
+            const float inv = !some ? 0.0f : whole_unit ? 1.0f / l : 1.0f;
+            const bool sectors = ((a.D & 15) | (reinterpret_cast<uintptr_t>(a.out) & 31)) == 0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < DP; c0 += 32) {
+                uint32_t o[32];
                 if (nw > 0) {
-                    tmem_ld_x16(to + c, o);
+                    tmem_ld_x32(to + c0, o);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int i = 0; i < 16; i += 8) {
-                    float f[8];
+                for (int c = 0; c < 32; ++c) {
+                    const float f = some ? __uint_as_float(o[c]) * inv : 0.0f;
+                    if (c0 + c < a.D) fine = fine && fabsf(f) < INFINITY;
+                    o[c] = __float_as_uint(f);
+                }
+                if (!live) continue;
+                if (!whole_unit) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] = nw > 0 && l != 0.0f ? __uint_as_float(o[i + e]) * inv : 0.0f;
-                        if (part * (DP / 2) + c + i < a.D) fine = fine && fabsf(f[e]) < INFINITY;
-                    }
-                    *reinterpret_cast<uint4*>(os + 2 * (c + i)) =
-                        make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
-                                   pack2<T>(f[6], f[7]));
+                    for (int c = 0; c < 32; c += 8) store32(pt + r * DP + c0 + c, o + c, true);
+                    continue;
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        h[e] = pack2<T>(__uint_as_float(o[c + 2 * e]), __uint_as_float(o[c + 2 * e + 1]));
+                    unsigned char* dst = a.out + 2 * (orow * a.D + c0 + c);
+                    if (c0 + c + 16 <= a.D) store32(dst, h, sectors);
+                    else if (c0 + c < a.D) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
-            pair_sync(pair);
-            constexpr int CH = DP / 8;                 // 16-byte pieces of a row
-            const int c = lane % CH;
-#pragma unroll
-            for (int i = 0; i < 16; i += 32 / CH) {    // this warp's half of the pair's rows
-                const int rr = 16 * part + i + lane / CH;
-                const int64_t to_row = __shfl_sync(0xffffffffu, orow, rr);
-                if (wr0 + rr < rows && c * 8 < a.D)
-                    *reinterpret_cast<uint4*>(a.out + 2 * (to_row * a.D + 8 * c)) =
-                        *reinterpret_cast<const uint4*>(smem_raw + (wr0 + rr) * OROW + 16 * c);
+            if (n > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->o_free[w]);
+                ++busy;
             }
-            if (live && a.lse && part == 0)
-                a.lse[orow] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * sc) + log2f(l)) * LN2;
+            if (live) {
+                const float top = m == -INFINITY ? (some ? 0.0f : -INFINITY) : m * sc;
+                if (!whole_unit) {
+                    pt[TC_CTA_ROWS * DP + r] = top;
+                    pt[TC_CTA_ROWS * (DP + 1) + r] = l;
+                } else if (a.lse) {
+                    a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
+                }
+            }
             const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
-            if (lane == 0) ctl->again[warp] = again;
+            if (lane == 0) {
+                t.again[(int64_t)u.item * TC_SOFTMAX_WARPS + warp] = again;
+                if (again) ctl->any_again = 1;
+            }
+            leave(k);
         }
+        if (!ok) give_up();
         set_regs_down<TC_REGS_LAUNCH>();
         tc_fence_before();
         roles_done();
     }
     tc_fence_after();
     if (warp == TC_SOFTMAX_WARPS + 1) tmem_dealloc(tmem, 512);
-    if (warp < TC_CTA_ROWS / 32) {   // rows [32 warp, 32 warp + 32)
-        const int at = (warp >> 2) * 8 + (warp & 3);
-        unsigned again = *abort ? 0u : ctl->again[at] | ctl->again[at + 4];
-        while (again) {
+    // Rows that came out not finite, from the definition.
+    if (*abort || !ctl->any_again || warp >= TC_SOFTMAX_WARPS) return;
+    Unit* u = reinterpret_cast<Unit*>(smem_raw) + warp;   // (nothing is left in the rings)
+    for (int64_t k = 0;; ++k) {
+        const int64_t item = t.next ? k : k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        describe(t, item, ctl->per, u);
+        const int s = u->s, kvh = u->kvh, row0 = u->row0 + 32 * warp, pieces = u->pieces;
+        const Seq q = u->q;
+        __syncwarp();
+        if (s < 0) break;
+        if (pieces > 1 || (t.next && __ldcg(t.owner + item) != (int)blockIdx.x)) continue;
+        unsigned again = __ldcg(t.again + item * TC_SOFTMAX_WARPS + warp);
+        while (again) {   // rows [32 warp, 32 warp + 32) of the unit
             const int i = __ffs(again) - 1;
             again &= again - 1;
-            attn_row_exact<T>(a, s, q, kvh, row0 + warp * 32 + i);
+            attn_row_exact<T>(a, s, q, kvh, row0 + i);
         }
     }
+}
+
+// Block (c, y): rows [16 y, 16 y + 16) of the split unit that begins with item c.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) paged_chunk_join_kernel(const __grid_constant__ TcArgs t) {
+    extern __shared__ float share[];
+    __shared__ int again;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the chunk kernel runs
+    const int4 u = t.joint[blockIdx.x];
+    if (u.w == 0) return;
+    const Seq q = load_seq(t.a.b, t.a.max_kv, u.x, t.a.status);
+    const int64_t left = (int64_t)q.n_new * t.a.group - (int64_t)u.z * TC_CTA_ROWS - 16 * blockIdx.y;
+    if (left <= 0) return;
+    const int64_t c = blockIdx.x;
+    const int r0 = 16 * blockIdx.y;
+    // rows that came out not finite in a piece: a NaN for its sum has them computed again
+    uint32_t bad = 0;
+    for (int i = 0; i < u.w; ++i) bad |= t.again[(c + i) * TC_SOFTMAX_WARPS + r0 / 32];
+    bad >>= r0 % 32;
+    finish_rows<T>(t.a, u.x, q, u.y, u.z * TC_CTA_ROWS + r0, (int)min((int64_t)16, left), u.w,
+                   [&](int i, int row, int d) {
+                       const float* p = t.part + (c + i) * TC_CTA_ROWS * (DP + 2);
+                       return d == -1   ? ((bad >> row) & 1 ? 0.0f : p[TC_CTA_ROWS * DP + r0 + row])
+                              : d == -2 ? ((bad >> row) & 1 ? __int_as_float(0x7fc00000)
+                                                            : p[TC_CTA_ROWS * (DP + 1) + r0 + row])
+                                        : p[(r0 + row) * DP + d];
+                   },
+                   share, &again);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -773,52 +998,101 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-template <typename T, int DP>
-hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
-                          cudaStream_t st) {
-    static std::atomic<uint64_t> done{0};
-    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
-    if (s != HMM_OK) return s;
-    paged_chunk_kernel<T, DP><<<grid, TC_THREADS, tc_smem<DP>(), st>>>(k, v, t);
-    return check_launch("paged_chunk_kernel");
-}
-
-}  // namespace
-
-hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
+// 16-bit values, boxes of 64 values in a row, 128-byte swizzle, zeros out of range.
+hmm_status_t encode_map(CUtensorMap* m, void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                        const cuuint32_t* box) {
     auto fn = encode_fn();
     if (!fn) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_tokens, (cuuint64_t)a.hk, (cuuint64_t)a.n_pages};
-    cuuint64_t strides[3] = {(cuuint64_t)p.token, (cuuint64_t)p.head, (cuuint64_t)p.page};
-    for (int i = 0; i < 3; ++i)
-        if (dims[i + 1] == 1) strides[i] = 16;   // never stepped over
-    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-    cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, p.base, dims, strides, box, ones,
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, base, dims, strides, box, ones,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return HMM_OK;
 }
 
+// Items that may be left: units at most one more per sequence and head than its share of
+// the tokens, or pieces, no more than CTAs.
+int64_t most_items(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk) {
+    return std::max<int64_t>((n_tokens * group / TC_CTA_ROWS + n_seq) * hk, device_sm_count());
+}
+
+// Units may be fewer than CTAs only if the tokens' row blocks are.
+bool may_split(int64_t n_tokens, int64_t group, int64_t hk) {
+    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk < device_sm_count();
+}
+
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+
+template <typename T, int DP>
+hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q,
+                          cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
+    if (s != HMM_OK) return s;
+    const unsigned ctas = (unsigned)device_sm_count();
+    paged_chunk_kernel<T, DP><<<ctas, TC_THREADS, tc_smem<DP>(), st>>>(k, v, q, t);
+    s = check_launch("paged_chunk_kernel");
+    if (s != HMM_OK || !t.split) return s;
+    const int64_t rows = std::min<int64_t>(TC_CTA_ROWS, (int64_t)t.a.b.n_tokens * t.a.group);
+    return launch_behind(paged_chunk_join_kernel<T, DP>, dim3(ctas, (unsigned)((rows + 15) / 16)), 128,
+                         sizeof(float) * 16 * ctas, st, t, "paged_chunk_join_kernel");
+}
+
+}  // namespace
+
+hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
+    const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_tokens, (cuuint64_t)a.hk, (cuuint64_t)a.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)p.token, (cuuint64_t)p.head, (cuuint64_t)p.page};
+    for (int i = 0; i < 3; ++i)
+        if (dims[i + 1] == 1) strides[i] = 16;   // never stepped over
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    return encode_map(m, p.base, 4, dims, strides, box);
+}
+
 bool chunk_applies(const AttnArgs& a) {
     return a.D <= 128 && box_rows_of(a.page_tokens, TC_KEYS) >= 8;
 }
 
-hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, cudaStream_t st) {
-    TcArgs t{a, min_rows, box_rows_of(a.page_tokens, TC_KEYS), wait_limit_ns()};
+size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D) {
+    if (D > 128) return 0;
+    const int64_t group = std::max<int64_t>(1, n_heads / n_kv_heads), ctas = device_sm_count();
+    size_t n = 256 + up256(4 * (size_t)most_items(n_seq, n_tokens, group, n_kv_heads) * (TC_SOFTMAX_WARPS + 1));
+    if (may_split(n_tokens, group, n_kv_heads))
+        n += up256(sizeof(int4) * ctas) + sizeof(float) * ctas * TC_CTA_ROWS * ((D <= 64 ? 64 : 128) + 2);
+    return n;
+}
+
+hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, unsigned char* ws, cudaStream_t st) {
+    const int64_t items = most_items(a.b.n_seq, a.b.n_tokens, a.group, a.hk);
+    HMM_REQUIRE(items < (int64_t(1) << 30), "n_tokens * n_heads is too large for one call");
+    int* owner = (int*)(ws + 256);
+    unsigned char* joint = ws + 256 + up256(4 * (size_t)items * (TC_SOFTMAX_WARPS + 1));
+    // A tile of 128 rows is a box of the queries where it is whole tokens; a negative scale
+    // turns the signs on the way, which a box cannot.
+    const bool boxes = a.group <= TC_ROWS && (a.group & (a.group - 1)) == 0 && a.scale >= 0.0f &&
+                       (a.hq == 1 || a.q_head > 0) && (a.b.n_tokens == 1 || a.q_token > 0) &&
+                       a.q_head < (int64_t(1) << 40) && a.q_token < (int64_t(1) << 40);
+    TcArgs t{a, min_rows, box_rows_of(a.page_tokens, TC_KEYS), may_split(a.b.n_tokens, a.group, a.hk),
+             a.b.n_seq > 1 ? (int*)ws : nullptr, owner, boxes ? TC_ROWS / a.group : 0, wait_limit_ns(),
+             (uint32_t*)(owner + items), (int4*)joint, (float*)(joint + up256(sizeof(int4) * device_sm_count()))};
     CUtensorMap k, v;
     hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows);
     if (s != HMM_OK) return s;
     s = make_page_map(&v, a, a.v, t.box_rows);
     if (s != HMM_OK) return s;
-    // every sequence's rows in blocks: one more than its share of the tokens at most
-    const int64_t most = ((int64_t)a.b.n_tokens * a.group / TC_CTA_ROWS + a.b.n_seq) * a.hk;
-    HMM_REQUIRE(most < (int64_t(1) << 31), "n_tokens * n_heads is too large for one call");
-    const unsigned grid = (unsigned)most;
+    CUtensorMap q{};
+    if (boxes) {
+        const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tokens};
+        const cuuint64_t strides[2] = {a.hq == 1 ? 16 : (cuuint64_t)a.q_head,
+                                       a.b.n_tokens == 1 ? 16 : (cuuint64_t)a.q_token};
+        const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(TC_ROWS / a.group)};
+        s = encode_map(&q, const_cast<unsigned char*>(a.q), 3, dims, strides, box);
+        if (s != HMM_OK) return s;
+    }
     if (a.D <= 64)
-        return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, grid, st) : launch_chunk<__half, 64>(t, k, v, grid, st);
-    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, grid, st) : launch_chunk<__half, 128>(t, k, v, grid, st);
+        return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, q, st) : launch_chunk<__half, 64>(t, k, v, q, st);
+    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, q, st) : launch_chunk<__half, 128>(t, k, v, q, st);
 }
 
 }  // namespace serve

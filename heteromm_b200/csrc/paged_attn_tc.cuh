@@ -31,17 +31,12 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-struct TcArgs {
-    AttnArgs a;
-    int min_rows;        // sequences of fewer rows are another kernel's
-    int box_rows;        // rows of a TMA box: a power of two that divides page_tokens
-    uint64_t wait_ns;    // limit of every bounded wait
-};
-
 // Whether the kernel takes this head size and page size.
 bool chunk_applies(const AttnArgs& a);
-// Rows of every sequence with at least min_rows rows (n_new * group).
-hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, cudaStream_t st);
+size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D);
+// Rows of every sequence with at least min_rows rows (n_new * group).  With more than one
+// sequence the first word of ws must be 0 (the rows kernel, which runs before, sees to it).
+hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, unsigned char* ws, cudaStream_t st);
 
 }  // namespace serve
 }  // namespace hmm
