@@ -17,7 +17,7 @@
 //   - scores and the product with V on mma.sync (m16n8k16, fp32 sums), the
 //     running maximum and sum in fp32 per warp, warps joined once per piece;
 //   - a unit that several CTAs share leaves (maximum, sum, unnormalised rows) per
-//     piece in the workspace, and paged_rows_join_kernel adds the pieces in order.
+//     piece in the workspace, and paged_join_kernel adds the pieces in order.
 #include <algorithm>
 
 #include "paged_attn.cuh"
@@ -36,7 +36,8 @@ constexpr int RW_ROWS = 16;
 constexpr int RW_STAGES = 3;
 
 struct RowsWork {
-    int4* joint;      // [ctas] unit begun in the CTA and ended in another: sequence, head, row tile, pieces
+    int4* joint;      // [ctas][2] unit begun in the CTA and ended in another: sequence, head, row tile,
+                      // pieces (0: none); the sequence's begin, n_new, kv
     float* part;      // [ctas][2][RW_ROWS * (DP + 2)]: rows, then maxima, then sums
 };
 
@@ -46,7 +47,6 @@ struct RowsArgs {
     int max_rows;     // sequences of more rows are another kernel's
     int box_rows;     // rows of a TMA box: a power of two that divides page_tokens
     uint64_t wait_ns; // limit of every bounded wait
-    int* counter;     // set to 0 for the kernel behind, or null
 };
 
 template <int DP>
@@ -164,10 +164,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const int64_t per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     int64_t cur = blockIdx.x * per;
     const int64_t end = min(total, cur + per);
-    if (threadIdx.x == 0) {
-        r.w.joint[blockIdx.x] = make_int4(0, 0, 0, 0);
-        if (r.counter && blockIdx.x == 0) *r.counter = 0;
-    }
+    if (threadIdx.x == 0) r.w.joint[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
     if (cur >= end) return;
     {
         int64_t run = 0;
@@ -401,36 +398,40 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
         }
         __syncthreads();
-        auto piece = [&](int w, int row, int d) {
-            return d == -1   ? jst[w * RW_ROWS + row]
-                   : d == -2 ? jst[(RW_WARPS + w) * RW_ROWS + row]
-                             : jm[(w * RW_ROWS + row) * MR + d];
+        auto stat = [&](int w, int row, int k) { return jst[(k * RW_WARPS + w) * RW_ROWS + row]; };
+        auto value = [&](int w, int row, int c) {
+            return *reinterpret_cast<const float4*>(jm + (w * RW_ROWS + row) * MR + 4 * c);
         };
         if (t0 == 0 && t1 == ld.tiles) {
-            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, piece, jst + 2 * RW_WARPS * RW_ROWS, &again);
+            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, stat, value, jst + 2 * RW_WARPS * RW_ROWS, &again);
         } else {
             float* part = r.w.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * RW_ROWS * (DP + 2);
-            for (int i = threadIdx.x; i < rows * a.D; i += RW_THREADS) {
-                const int row = i / a.D, d = i - row * a.D;
+            for (int i = threadIdx.x; i < rows * (DP / 4); i += RW_THREADS) {
+                const int row = i / (DP / 4), c = i % (DP / 4);
                 float mm = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < RW_WARPS; ++w) mm = fmaxf(mm, piece(w, row, -1));
+                for (int w = 0; w < RW_WARPS; ++w) mm = fmaxf(mm, stat(w, row, 0));
                 const float ms = mm == -INFINITY ? 0.0f : mm;
-                float x = 0.0f, sum = 0.0f;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < RW_WARPS; ++w) {
-                    const float wgt = ex2(piece(w, row, -1) - ms);
-                    x = fmaf(wgt, piece(w, row, d), x);
-                    sum = fmaf(wgt, piece(w, row, -2), sum);
+                    const float wgt = ex2(stat(w, row, 0) - ms);
+                    const float4 v = value(w, row, c);
+                    x.x = fmaf(wgt, v.x, x.x); x.y = fmaf(wgt, v.y, x.y);
+                    x.z = fmaf(wgt, v.z, x.z); x.w = fmaf(wgt, v.w, x.w);
+                    sum = fmaf(wgt, stat(w, row, 1), sum);
                 }
-                part[row * DP + d] = x;
-                if (d == 0) {
+                *reinterpret_cast<float4*>(part + row * DP + 4 * c) = x;
+                if (c == 0) {
                     part[RW_ROWS * DP + row] = mm;
                     part[RW_ROWS * (DP + 1) + row] = sum;
                 }
             }
-            if (t0 == 0 && threadIdx.x == 0)
-                r.w.joint[blockIdx.x] = make_int4(s, kvh, rt, 1 + (int)((ld.tiles - t1 + per - 1) / per));
+            if (t0 == 0 && threadIdx.x == 0) {
+                r.w.joint[2 * blockIdx.x] = make_int4(s, kvh, rt, 1 + (int)((ld.tiles - t1 + per - 1) / per));
+                r.w.joint[2 * blockIdx.x + 1] = make_int4(q.begin, q.n_new, q.kv, 0);
+            }
         }
         cur += t1 - t0;
         fence_proxy_async_smem();                      // the next copies come behind these writes
@@ -438,23 +439,44 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
 }
 
-// Block c: the unit begun in CTA c and ended in a later one.
-template <typename T, int DP>
-__global__ void __launch_bounds__(RW_THREADS) paged_rows_join_kernel(const __grid_constant__ RowsArgs r) {
+// What both kernels left in pieces.  Blocks [0, rows_ctas): 16 rows each, of the unit begun
+// in that CTA of the rows kernel; the rest: a group of 16 rows of a unit begun in a CTA of
+// the chunk kernel.
+struct JoinArgs {
+    AttnArgs a;
+    RowsWork rows;
+    int rows_ctas, dp;
+    ChunkJoin chunk;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_constant__ JoinArgs j) {
     extern __shared__ float share[];
     __shared__ int again;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the rows kernel runs
-    const int4 u = r.w.joint[blockIdx.x];
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before still runs
+    const bool few = (int)blockIdx.x < j.rows_ctas;
+    const int at = few ? blockIdx.x : blockIdx.x - j.rows_ctas;
+    const int64_t c = few ? at : at / j.chunk.groups;
+    const int r0 = few ? 0 : 16 * (at - (int)c * j.chunk.groups);
+    const int4* joint = (few ? j.rows.joint : j.chunk.joint) + 2 * c;
+    const int4 u = joint[0], x = joint[1];
     if (u.w == 0) return;
-    const Seq q = load_seq(r.a.b, r.a.max_kv, u.x, r.a.status);
-    const int row0 = u.z * RW_ROWS;
-    const int rows = (int)min((int64_t)RW_ROWS, (int64_t)q.n_new * r.a.group - row0);
-    const float* part = r.w.part;
-    const int64_t c = blockIdx.x;
-    finish_rows<T>(r.a, u.x, q, u.y, row0, rows, u.w, [&](int i, int row, int d) {
-        const float* p = part + ((c + i) * 2 + (i == 0)) * RW_ROWS * (DP + 2);
-        return d == -1 ? p[RW_ROWS * DP + row] : d == -2 ? p[RW_ROWS * (DP + 1) + row] : p[row * DP + d];
-    }, share, &again);
+    const Seq q{x.x, x.y, x.z, true};
+    const int rows = few ? RW_ROWS : TC_CTA_ROWS, row0 = u.z * rows + r0;
+    const int64_t left = (int64_t)q.n_new * j.a.group - row0;
+    if (left <= 0) return;
+    const int64_t size = (int64_t)rows * (j.dp + 2);
+    const float* part = (few ? j.rows.part : j.chunk.part) + c * 2 * size;
+    finish_rows<T>(j.a, u.x, q, u.y, row0, (int)min((int64_t)16, left), u.w,
+                   [&](int i, int row, int k) {
+                       return part[(2 * i + (i == 0)) * size + rows * (j.dp + k) + r0 + row];
+                   },
+                   [&](int i, int row, int col) {   // rows: [row][DP]; chunk: [DP / 4][row][4]
+                       return *reinterpret_cast<const float4*>(
+                           part + (2 * i + (i == 0)) * size +
+                           (few ? row * j.dp + 4 * col : (col * rows + r0 + row) * 4));
+                   },
+                   share, &again);
 }
 
 int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
@@ -467,37 +489,60 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 size_t rows_workspace(int dp) {
     const size_t g = (size_t)rows_ctas(dp);
-    return g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
+    return 2 * g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
 }
 
 template <typename T, int DP>
 hmm_status_t launch_rows(const RowsArgs& r, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-    const unsigned g = (unsigned)rows_ctas(DP);
     static std::atomic<uint64_t> done{0};
-    hmm_status_t s = allow_smem(paged_rows_kernel<T, DP>, rows_smem<DP>(), &done);
+    const hmm_status_t s = allow_smem(paged_rows_kernel<T, DP>, rows_smem<DP>(), &done);
     if (s != HMM_OK) return s;
-    paged_rows_kernel<T, DP><<<g, RW_THREADS, rows_smem<DP>(), st>>>(k, v, r);
-    s = check_launch("paged_rows_kernel");
-    if (s != HMM_OK) return s;
-    const size_t share = sizeof(float) * RW_ROWS * (g + 1);
-    static std::atomic<uint64_t> join_done{0};
-    s = allow_smem(paged_rows_join_kernel<T, DP>, share, &join_done);
-    if (s != HMM_OK) return s;
-    return launch_behind(paged_rows_join_kernel<T, DP>, dim3(g), RW_THREADS, share, st, r, "paged_rows_join_kernel");
+    return launch(paged_rows_kernel<T, DP>, dim3((unsigned)rows_ctas(DP)), RW_THREADS, rows_smem<DP>(), false, st,
+                  "paged_rows_kernel", k, v, r);
 }
 
 template <typename T>
-hmm_status_t run_rows(const AttnArgs& a, int max_rows, unsigned char* ws, int* counter, cudaStream_t st) {
-    const int dp = rows_dp(a.D);
-    RowsArgs r{a, {(int4*)ws, (float*)(ws + (size_t)rows_ctas(dp) * sizeof(int4))}, max_rows,
-               box_rows_of(a.page_tokens, RW_KEYS), wait_limit_ns(), counter};
+hmm_status_t run_rows(const RowsArgs& r, cudaStream_t st) {
     CUtensorMap k, v;
-    hmm_status_t s = make_page_map(&k, a, a.k, r.box_rows);
+    hmm_status_t s = make_page_map(&k, r.a, r.a.k, r.box_rows);
     if (s != HMM_OK) return s;
-    s = make_page_map(&v, a, a.v, r.box_rows);
+    s = make_page_map(&v, r.a, r.a.v, r.box_rows);
     if (s != HMM_OK) return s;
+    const int dp = rows_dp(r.a.D);
     return dp == 64 ? launch_rows<T, 64>(r, k, v, st) : dp == 128 ? launch_rows<T, 128>(r, k, v, st)
                                                                   : launch_rows<T, 256>(r, k, v, st);
+}
+
+template <typename T>
+hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
+    // A unit of up to 16 rows (one MMA's) reads its keys once either way and the many small
+    // CTAs of the rows kernel keep more reads in flight; more rows would read them again
+    // there.
+    const bool chunk = chunk_applies(a);
+    const bool few = max_new > 0 && (int64_t)std::min(max_new, a.b.n_tokens) * a.group <= RW_ROWS;
+    const bool with_rows = few || !chunk || a.b.n_seq > 1;
+    const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel
+    const int dp = rows_dp(a.D);
+    const int64_t ctas = rows_ctas(dp);
+    JoinArgs j{a, {(int4*)ws, (float*)(ws + 2 * (size_t)ctas * sizeof(int4))}, 0, dp, {}};
+    hmm_status_t s;
+    if (with_rows) {
+        j.rows_ctas = (int)ctas;
+        s = run_rows<T>(RowsArgs{a, j.rows, most, box_rows_of(a.page_tokens, RW_KEYS), wait_limit_ns()}, st);
+        if (s != HMM_OK) return s;
+    }
+    if (chunk && !few) {
+        s = run_chunk(a, std::is_same<T, __nv_bfloat16>::value, with_rows ? most + 1 : 1, with_rows,
+                      ws + up256(rows_workspace(dp)), st, &j.chunk);
+        if (s != HMM_OK) return s;
+    }
+    const int64_t blocks = j.rows_ctas + (int64_t)j.chunk.ctas * j.chunk.groups;
+    if (blocks == 0) return HMM_OK;
+    const size_t share = sizeof(float) * 32 * (std::max(j.rows_ctas, j.chunk.ctas) + 1);
+    static std::atomic<uint64_t> done{0};
+    s = allow_smem(paged_join_kernel<T>, sizeof(float) * 32 * 1024, &done);
+    if (s != HMM_OK) return s;
+    return launch(paged_join_kernel<T>, dim3((unsigned)blocks), RW_THREADS, share, true, st, "paged_join_kernel", j);
 }
 
 }  // namespace
@@ -568,22 +613,8 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     a.page_tokens = (int)cache->page_tokens;
     a.n_pages = (int)cache->n_pages;
     a.status = device_status;
-    const cudaStream_t st = (cudaStream_t)stream;
-    // A unit of up to 16 rows (one MMA's) reads its keys once either way and the
-    // many small CTAs of the rows kernel keep more reads in flight; more rows
-    // would read them again there.
-    const bool chunk = chunk_applies(a);
-    const bool few = max_new > 0 && std::min(max_new, batch->n_tokens) * a.group <= RW_ROWS;
-    const bool rows_too = few || !chunk || batch->n_seq > 1;
-    const int split = !chunk || few ? INT32_MAX : batch->n_seq == 1 ? 0 : RW_ROWS;
-    const bool bf16 = cache->dtype == HMM_DTYPE_BF16;
-    unsigned char* chunk_ws = (unsigned char*)workspace + up256(rows_workspace(rows_dp(a.D)));
-    if (rows_too) {
-        int* counter = chunk && !few ? (int*)chunk_ws : nullptr;
-        s = bf16 ? run_rows<__nv_bfloat16>(a, split, (unsigned char*)workspace, counter, st)
-                 : run_rows<__half>(a, split, (unsigned char*)workspace, counter, st);
-        if (s != HMM_OK) return s;
-    }
-    return chunk && !few ? run_chunk(a, bf16, split == 0 ? 1 : split + 1, chunk_ws, st)
-                         : HMM_OK;
+    const int hint = (int)std::min<int64_t>(max_new, INT32_MAX);
+    return cache->dtype == HMM_DTYPE_BF16
+               ? run_attention<__nv_bfloat16>(a, hint, (unsigned char*)workspace, (cudaStream_t)stream)
+               : run_attention<__half>(a, hint, (unsigned char*)workspace, (cudaStream_t)stream);
 }

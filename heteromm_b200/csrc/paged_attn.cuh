@@ -143,34 +143,44 @@ __device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const S
 
 // Joins (maximum, sum, row) pieces of up to 16 rows, which several warps or CTAs summed
 // over different keys, in their order, and writes the rows out; rows that come out not
-// finite are computed again by attn_row_exact.  piece(i, row, -1 / -2 / d) reads the
-// maximum, sum or value of piece i; `share` holds 16 x pieces floats.  Whole block.
-template <typename T, typename Piece>
+// finite are computed again by attn_row_exact.  stat(i, row, k) reads piece i's maximum
+// (k = 0) or sum (1), value(i, row, c) its columns 4 c ... 4 c + 3; `share` holds
+// 32 x pieces floats.  Whole block, 128 threads: all reads of a step are issued at once.
+template <typename T, typename Stat, typename Value>
 __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
-                                            int rows, int pieces, Piece piece, float* share, int* again) {
+                                            int rows, int pieces, Stat stat, Value value, float* share,
+                                            int* again) {
     if (threadIdx.x == 0) *again = 0;
-    const int lane = threadIdx.x & 31;
-    // each piece's share of the row: exp2(m_i - m) / sum_k exp2(m_k - m) l_k
-    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
+    float* top = share;                 // [row][piece] maxima, then the pieces' shares of the row
+    float* sum = share + 16 * pieces;
+    for (int i = threadIdx.x; i < rows * pieces; i += blockDim.x) {
+        const int r = i / pieces, p = i - r * pieces;
+        top[i] = stat(p, r, 0);
+        sum[i] = stat(p, r, 1);
+    }
+    __syncthreads();
+    // exp2(m_i - m) / sum_k exp2(m_k - m) l_k, eight threads a row
+    {
+        const int r = threadIdx.x >> 3, t = threadIdx.x & 7;
+        const bool live = r < rows;
         float m = -INFINITY, l = 0.0f;
-        for (int p = lane; p < pieces; p += 32) m = fmaxf(m, piece(p, r, -1));
+        for (int p = t; live && p < pieces; p += 8) m = fmaxf(m, top[r * pieces + p]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float ms = m == -INFINITY ? 0.0f : m;
-        for (int p = lane; p < pieces; p += 32) {
-            const float wgt = ex2(piece(p, r, -1) - ms);
-            share[r * pieces + p] = wgt;
-            if (wgt != 0.0f) l = fmaf(wgt, piece(p, r, -2), l);
+        for (int p = t; live && p < pieces; p += 8) {
+            const float w = ex2(top[r * pieces + p] - ms);
+            top[r * pieces + p] = w;
+            if (w != 0.0f) l = fmaf(w, sum[r * pieces + p], l);   // (0: a piece in which the row saw nothing)
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        __syncwarp();
-        for (int p = lane; p < pieces; p += 32) {
-            const float wgt = share[r * pieces + p];
-            share[r * pieces + p] = wgt == 0.0f ? 0.0f : wgt * inv;   // (0: a piece in which the row saw nothing)
+        for (int p = t; live && p < pieces; p += 8) {
+            const float w = top[r * pieces + p];
+            top[r * pieces + p] = w == 0.0f ? 0.0f : w * inv;
         }
-        if (lane == 0) {
+        if (live && t == 0) {
             if (l != l) atomicOr(again, 1 << r);
             if (a.lse) {
                 const int tok = a.by_group(row0 + r);
@@ -180,21 +190,44 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         }
     }
     __syncthreads();
-    const int pairs = a.D / 2;
-    for (int i = threadIdx.x; i < rows * pairs; i += blockDim.x) {
-        const int r = i / pairs, d = 2 * (i - r * pairs);
-        float x = 0.0f, y = 0.0f;
-#pragma unroll 4
-        for (int p = 0; p < pieces; ++p) {
-            const float wgt = share[r * pieces + p];
-            const float u = piece(p, r, d), v = piece(p, r, d + 1);
-            x = wgt == 0.0f ? x : fmaf(wgt, u, x);
-            y = wgt == 0.0f ? y : fmaf(wgt, v, y);
+    // four quads a thread and two pieces at a time: eight reads in flight
+    const int quads = a.D / 4, all = rows * quads;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * blockDim.x) {
+        float4 x[4];
+        int row[4], col[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = min(i0 + k * (int)blockDim.x, all - 1);
+            row[k] = i / quads;
+            col[k] = i - row[k] * quads;
+            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        if (!isfinite(x) || !isfinite(y)) atomicOr(again, 1 << r);
-        const int tok = a.by_group(row0 + r), head = kvh * a.group + row0 + r - tok * a.group;
-        *reinterpret_cast<uint32_t*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + d)) =
-            pack2<T>(x, y);
+        for (int p0 = 0; p0 < pieces; p0 += 2) {
+            float4 v[4][2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) v[k][p] = value(min(p0 + p, pieces - 1), row[k], col[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const float w = p0 + p < pieces ? top[row[k] * pieces + p0 + p] : 0.0f;
+                    if (w != 0.0f) {
+                        x[k].x = fmaf(w, v[k][p].x, x[k].x); x[k].y = fmaf(w, v[k][p].y, x[k].y);
+                        x[k].z = fmaf(w, v[k][p].z, x[k].z); x[k].w = fmaf(w, v[k][p].w, x[k].w);
+                    }
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k * (int)blockDim.x >= all) continue;
+            if (!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w))
+                atomicOr(again, 1 << row[k]);
+            const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
+            *reinterpret_cast<uint2*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + 4 * col[k])) =
+                make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
+        }
     }
     __syncthreads();
     const int bits = *again;
@@ -203,11 +236,11 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
     __syncthreads();
 }
 
-// Launches a kernel that begins with griddepcontrol.wait: its blocks may be set up while
-// the kernel before it on the stream still runs.
-template <typename F, typename A>
-hmm_status_t launch_behind(F fn, dim3 grid, int threads, size_t smem, cudaStream_t st, const A& args,
-                           const char* what) {
+// Launches a kernel; with `behind` its blocks may start while the kernel before it on the
+// stream, which lets them (griddepcontrol.launch_dependents), still runs.
+template <typename... P, typename... A>
+hmm_status_t launch(void (*fn)(P...), dim3 grid, int threads, size_t smem, bool behind, cudaStream_t st,
+                    const char* what, const A&... args) {
     cudaLaunchConfig_t c{};
     c.gridDim = grid;
     c.blockDim = dim3(threads);
@@ -217,8 +250,8 @@ hmm_status_t launch_behind(F fn, dim3 grid, int threads, size_t smem, cudaStream
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     c.attrs = &at;
-    c.numAttrs = 1;
-    HMM_CUDA_TRY(cudaLaunchKernelEx(&c, fn, args));
+    c.numAttrs = behind ? 1 : 0;
+    HMM_CUDA_TRY(cudaLaunchKernelEx(&c, fn, args...));
     return check_launch(what);
 }
 

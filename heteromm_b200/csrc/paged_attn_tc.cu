@@ -39,7 +39,7 @@ namespace {
 
 constexpr int TC_ROWS = 128;                 // rows of a tile (MMA M, TMEM lanes)
 constexpr int TC_TILES = 2;
-constexpr int TC_CTA_ROWS = TC_ROWS * TC_TILES;
+static_assert(TC_CTA_ROWS == TC_ROWS * TC_TILES, "a unit is its row tiles");
 constexpr int TC_KEYS = 128;                 // keys of a tile
 constexpr int TC_SOFTMAX_WARPS = 8;          // two row tiles, 32 rows a warp
 constexpr int TC_WARPS = TC_SOFTMAX_WARPS + 4;
@@ -47,7 +47,11 @@ constexpr int TC_THREADS = 32 * TC_WARPS;
 // Registers: 384 threads are launched with 168 each (64,512 in all); the softmax warps
 // take 224 (a row's scores stay in registers), the last warpgroup keeps 56.
 constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
-constexpr int TC_MIN_PIECE = 3;               // key tiles of a split unit's piece
+constexpr int TC_MIN_PIECE = 3;              // key tiles of a piece, at least
+constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start and end take the time of
+#ifndef TC_ROUNDS2
+#define TC_ROUNDS2 2
+#endif
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
 // Of 8 pairs of exponentials, those that go to the FMA pipe.
@@ -68,14 +72,11 @@ struct TcArgs {
     AttnArgs a;
     int min_rows;        // sequences of fewer rows are another kernel's
     int box_rows;        // rows of a TMA box: a power of two that divides page_tokens
-    int split;           // whether few units may be split over the keys
-    int* next;           // the next item, or null: the CTAs' rounds go to and fro
-    int* owner;          // [items] the CTA that took it (with `next`)
+    int split;           // whether few units may be cut into pieces
     int q_tokens;        // new tokens of a row tile's TMA box, 0: queries by 16-byte copies
     uint64_t wait_ns;    // limit of every bounded wait
-    uint32_t* again;     // [items][TC_SOFTMAX_WARPS] rows that came out not finite
-    int4* joint;         // [ctas] split unit that begins with this item: sequence, head, row block, pieces
-    float* part;         // [ctas][TC_CTA_ROWS * (DP + 2)]: a piece's rows, maxima, sums
+    uint32_t* again;     // [units][TC_SOFTMAX_WARPS] rows that came out not finite
+    ChunkJoin join;
 };
 
 // What a CTA works on at a time: 256 rows of a (sequence, KV head) and `n` key tiles of
@@ -86,7 +87,7 @@ struct Unit {
     Span sp;
     int sink_tiles, first;       // the seen tiles are [0, sink_tiles) and [first, ...)
     int t0, n, n_of[TC_TILES];   // each row tile's key tiles: a prefix of the unit's
-    int pieces, item;
+    int slot, id;                // where a piece's sums go (-1: the unit is whole); the unit's number
     __device__ __forceinline__ int key0(int j) const {
         return (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
     }
@@ -96,12 +97,19 @@ struct Unit {
     }
 };
 
+// The plan of a launch, the same for every CTA: with units for several rounds each CTA
+// takes whole ones; fewer are laid end to end and cut into equal pieces, one per CTA.
+struct Plan {
+    int64_t per, tiles;          // per = 0: whole units
+};
+
 struct TcCtrl {
     uint64_t full[8], empty[8];
     uint64_t s_full[TC_TILES], p_full[TC_TILES][2], o_free[TC_TILES];
     uint64_t u_full[2], u_empty[2], q_full, q_empty, v_mend, v_fixed, o_full, drain;
     Unit unit[2];
-    int per, any_again;
+    Plan plan;
+    int any_again;
     uint32_t tmem;
     int abort;
 };
@@ -297,24 +305,43 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
     return TOP ? max3(mx0, mx1, mx1) : 0.0f;
 }
 
-// Units of a sequence, and the key tiles of any of them (an upper bound).
-struct TcLoad {
-    int64_t units;
-    int row_blocks, tiles;
+// Row blocks of a sequence.
+__device__ __forceinline__ int row_blocks(const TcArgs& t, const Seq& q) {
+    const int64_t rows = (int64_t)q.n_new * t.a.group;
+    return rows < t.min_rows ? 0 : (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
+}
+
+// The seen key tiles of rows [row0, row1) of a sequence.
+struct Tiles {
+    Span sp;
+    int sink_tiles, first, n;
 };
 
-__device__ __forceinline__ TcLoad tc_load(const TcArgs& t, const Seq& q) {
-    const int64_t rows = (int64_t)q.n_new * t.a.group;
-    TcLoad x{0, 0, 0};
-    if (rows < t.min_rows) return x;
-    x.row_blocks = (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
-    x.units = (int64_t)x.row_blocks * t.a.hk;
-    int64_t n = ((int64_t)q.kv + TC_KEYS - 1) / TC_KEYS;
-    if (t.a.window > 0) {
-        const int64_t near = ((int64_t)t.a.window + TC_CTA_ROWS / t.a.group + 1 + TC_KEYS) / TC_KEYS + 1;
-        n = min(n, near + ((int64_t)t.a.sinks + TC_KEYS - 1) / TC_KEYS);
-    }
-    x.tiles = (int)max(n, (int64_t)1);
+__device__ __forceinline__ Tiles tiles_of(const AttnArgs& a, const Seq& q, int row0, int row1) {
+    Tiles x;
+    x.sp = tile_span(a, q, row0, row1);
+    x.sink_tiles = (x.sp.sink + TC_KEYS - 1) / TC_KEYS;
+    x.first = max(x.sp.lo / TC_KEYS, x.sink_tiles);
+    x.n = x.sink_tiles + max(0, (x.sp.hi + TC_KEYS - 1) / TC_KEYS - x.first);
+    return x;
+}
+
+__device__ __forceinline__ int last_row(const Seq& q, int group, int rb) {
+    return (int)min((int64_t)(rb + 1) * TC_CTA_ROWS, (int64_t)q.n_new * group);
+}
+
+// The length of row block rb's units in the plan: their key tiles behind the unit's own cost.
+__device__ __forceinline__ int block_length(const AttnArgs& a, const Seq& q, int rb) {
+    return TC_UNIT_COST + tiles_of(a, q, rb * TC_CTA_ROWS, last_row(q, a.group, rb)).n;
+}
+
+// Lane `src`'s sequence, for the warp.
+__device__ __forceinline__ Seq shared_seq(const Seq& q, int src) {
+    Seq x;
+    x.begin = __shfl_sync(0xffffffffu, q.begin, src);
+    x.n_new = __shfl_sync(0xffffffffu, q.n_new, src);
+    x.kv = __shfl_sync(0xffffffffu, q.kv, src);
+    x.ok = true;
     return x;
 }
 
@@ -324,116 +351,147 @@ __device__ __forceinline__ int64_t warp_sum(int64_t v) {
     return v;
 }
 
-// Key tiles of a piece: all of a unit's, unless the units leave CTAs without work; then
-// the smallest number at which the pieces are no more than the CTAs.  One warp.
-__device__ __forceinline__ int tiles_per_piece(const TcArgs& t) {
-    const int lane = threadIdx.x & 31;
-    const int64_t ctas = gridDim.x;
-    if (!t.split) return INT_MAX;
-    int64_t units = 0, tiles = 0;
-    for (int s = lane; s < t.a.b.n_seq; s += 32) {
-        const TcLoad x = tc_load(t, load_seq(t.a.b, t.a.max_kv, s, t.a.status));
-        units += x.units;
-        tiles += x.units * x.tiles;
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += w;
     }
-    units = warp_sum(units);
-    tiles = warp_sum(tiles);
-    if (units == 0 || units >= ctas) return INT_MAX;
-    int64_t per = max((int64_t)TC_MIN_PIECE, (tiles + ctas - 1) / ctas);
-    while (true) {
-        int64_t items = 0;
-        for (int s = lane; s < t.a.b.n_seq; s += 32) {
-            const TcLoad x = tc_load(t, load_seq(t.a.b, t.a.max_kv, s, t.a.status));
-            items += x.units * ((x.tiles + per - 1) / per);
-        }
-        if (warp_sum(items) <= ctas) return (int)per;
-        per += max((int64_t)1, per / 16);
-    }
+    return v;
 }
 
-// The item-th piece of all sequences' units, by one warp, into *u (s = -1: there is none).
-__device__ __forceinline__ void describe(const TcArgs& t, int64_t item, int per, Unit* u) {
+// One warp.
+__device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     const AttnArgs& a = t.a;
     const int lane = threadIdx.x & 31;
-    int64_t run = 0;
+    if (!t.split) return Plan{0, 0};
+    int64_t units = 0;
+    for (int s = lane; s < a.b.n_seq; s += 32)
+        units += (int64_t)row_blocks(t, load_seq(a.b, a.max_kv, s, a.status)) * a.hk;
+    if (2 * warp_sum(units) >= TC_ROUNDS2 * (int64_t)gridDim.x) return Plan{0, 0};
+    int64_t tiles = 0;   // (a few row blocks per CTA at most)
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
         const int s = s0 + lane;
         Seq q{0, 0, 0, false};
-        TcLoad x{0, 0, 0};
-        if (s < a.b.n_seq) {
-            q = load_seq(a.b, a.max_kv, s, a.status);
-            x = tc_load(t, q);
+        if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
+        const int rb = row_blocks(t, q);
+        unsigned busy = __ballot_sync(0xffffffffu, rb > 0);
+        while (busy) {
+            const int src = __ffs(busy) - 1;
+            busy &= busy - 1;
+            const Seq x = shared_seq(q, src);
+            const int n = __shfl_sync(0xffffffffu, rb, src);
+            for (int i = lane; i < n; i += 32) tiles += block_length(a, x, i);
         }
-        const int pieces = x.units > 0 ? (int)(((int64_t)x.tiles + per - 1) / per) : 0;
-        const int64_t v = x.units * pieces;
-        int64_t incl = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t w = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += w;
-        }
-        const bool here = run + incl - v <= item && item < run + incl;
-        if (here) {
-            const int at = (int)(item - (run + incl - v)), unit = at / pieces, piece = at - unit * pieces;
-            // a sequence's last rows see the most keys: they go first, so that the
-            // short blocks fill the end
-            const int kvh = unit % a.hk, rb = x.row_blocks - 1 - unit / a.hk;
-            const int row0 = rb * TC_CTA_ROWS;
-            const int rows = (int)min((int64_t)TC_CTA_ROWS, (int64_t)q.n_new * a.group - row0);
-            const Span sp = tile_span(a, q, row0, row0 + rows);
-            const int sink_tiles = (sp.sink + TC_KEYS - 1) / TC_KEYS;
-            const int first = max(sp.lo / TC_KEYS, sink_tiles);
-            const int t0 = pieces > 1 ? piece * per : 0;
-            u->s = s;
-            u->kvh = kvh;
-            u->row0 = row0;
-            u->rows = rows;
-            u->q = q;
-            u->sp = sp;
-            u->sink_tiles = sink_tiles;
-            u->first = first;
-            u->t0 = t0;
-            int n = 0;
-#pragma unroll
-            for (int w = 0; w < TC_TILES; ++w) {
-                const int r0 = row0 + w * TC_ROWS, r1 = min(row0 + rows, r0 + TC_ROWS);
-                int nw = 0;
-                if (r0 < r1) {
-                    const int hi = tile_span(a, q, r0, r1).hi;
-                    nw = sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - first) - t0;
-                    nw = max(0, min(nw, per));
-                }
-                u->n_of[w] = nw;
-                n = max(n, nw);
+    }
+    tiles = warp_sum(tiles) * a.hk;
+    return Plan{max((int64_t)TC_MIN_PIECE + TC_UNIT_COST, (tiles + gridDim.x - 1) / gridDim.x), tiles};
+}
+
+// The k-th unit (whole units) or, from tile `*pos` of all units' on, the next piece of this
+// CTA's share, into *u (s = -1: there is none); moves *pos on.  One warp.
+__device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int64_t k, int64_t* pos, Unit* u) {
+    const AttnArgs& a = t.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t cta = blockIdx.x, ctas = gridDim.x;
+    const bool cut = plan.per > 0;
+    // Whole units of a sequence fall in size, so rounds go from the first CTA and from the
+    // last one in turn.
+    const int64_t at = cut ? *pos : k * ctas + (k & 1 ? ctas - 1 - cta : cta);
+    const int64_t end = cut ? min(plan.tiles, (cta + 1) * plan.per) : INT64_MAX;
+    int64_t run = 0, unit_run = 0;   // tiles (cut) or units before, and units
+    for (int s0 = 0; s0 < a.b.n_seq && at < end; s0 += 32) {
+        const int s = s0 + lane;
+        Seq q{0, 0, 0, false};
+        if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
+        const int rb = row_blocks(t, q);
+        unsigned busy = __ballot_sync(0xffffffffu, rb > 0);
+        if (!cut) {   // past 32 sequences at once
+            const int64_t all = warp_sum((int64_t)rb * a.hk);
+            if (run + all <= at) {
+                run += all;
+                continue;
             }
-            u->n = n;
-            u->pieces = pieces;
-            u->item = (int)item;
-            if (t.split && item < gridDim.x)
-                t.joint[item] = make_int4(s, kvh, rb, pieces > 1 && piece == 0 ? pieces : 0);
         }
-        if (__any_sync(0xffffffffu, here)) {
+        while (busy) {
+            const int src = __ffs(busy) - 1;
+            busy &= busy - 1;
+            const Seq x = shared_seq(q, src);
+            const int n_rb = __shfl_sync(0xffffffffu, rb, src);
+            // a sequence's last rows see the most keys: they go first, so that the short
+            // blocks fill the end
+            int b = -1, kvh = 0, v0 = 0, n_all = 0;
+            if (!cut) {
+                const int64_t in = at - run;
+                if (in < (int64_t)n_rb * a.hk) {
+                    b = n_rb - 1 - (int)(in / a.hk);
+                    kvh = (int)(in % a.hk);
+                }
+                run += (int64_t)n_rb * a.hk;
+            } else {
+                for (int i0 = 0; i0 < n_rb && b < 0; i0 += 32) {
+                    const int n = i0 + lane < n_rb ? block_length(a, x, n_rb - 1 - i0 - lane) : 0;
+                    const int64_t v = (int64_t)n * a.hk, incl = warp_scan(v) + run;
+                    const unsigned here = __ballot_sync(0xffffffffu, incl - v <= at && at < incl);
+                    if (here) {
+                        const int l = __ffs(here) - 1;
+                        const int64_t in = at - __shfl_sync(0xffffffffu, incl - v, l);
+                        n_all = __shfl_sync(0xffffffffu, n, l);
+                        b = n_rb - 1 - i0 - l;
+                        kvh = (int)(in / n_all);
+                        v0 = (int)(in - (int64_t)kvh * n_all);
+                    }
+                    run = __shfl_sync(0xffffffffu, incl, 31);
+                }
+            }
+            if (b < 0) {
+                unit_run += (int64_t)n_rb * a.hk;
+                continue;
+            }
+            const int row0 = b * TC_CTA_ROWS, row1 = last_row(x, a.group, b);
+            const Tiles all = tiles_of(a, x, row0, row1);
+            const int take = cut ? (int)min((int64_t)(n_all - v0), end - at) : 0;   // of its length
+            const bool whole = !cut || (v0 == 0 && take == n_all);
+            const int t0 = cut ? max(0, v0 - TC_UNIT_COST) : 0;
+            const int most = cut ? max(0, v0 + take - TC_UNIT_COST) - t0 : INT_MAX;
+            if (lane == 0) {
+                u->s = s0 + src;
+                u->kvh = kvh;
+                u->row0 = row0;
+                u->rows = row1 - row0;
+                u->q = x;
+                u->sp = all.sp;
+                u->sink_tiles = all.sink_tiles;
+                u->first = all.first;
+                u->t0 = t0;
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < TC_TILES; ++w) {
+                    const int r0 = row0 + w * TC_ROWS, r1 = min(row1, r0 + TC_ROWS);
+                    int nw = 0;
+                    if (r0 < r1) {
+                        const int hi = tile_span(a, x, r0, r1).hi;
+                        nw = all.sink_tiles + max(0, (hi + TC_KEYS - 1) / TC_KEYS - all.first) - t0;
+                        nw = max(0, min(nw, most));
+                    }
+                    u->n_of[w] = nw;
+                    n = max(n, nw);
+                }
+                u->n = n;
+                u->slot = whole ? -1 : (int)(2 * cta + (v0 == 0));
+                u->id = (int)(cut ? unit_run + (int64_t)(n_rb - 1 - b) * a.hk + kvh : at);
+                if (!whole && v0 == 0) {   // its other pieces are the next CTAs' first ones
+                    t.join.joint[2 * cta] = make_int4(s0 + src, kvh, b, 1 + (int)((n_all - take + plan.per - 1) / plan.per));
+                    t.join.joint[2 * cta + 1] = make_int4(x.begin, x.n_new, x.kv, 0);
+                }
+            }
+            if (cut) *pos = at + take;
             __syncwarp();
             return;
         }
-        run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) {
-        u->s = -1;
-        if (t.split && item < gridDim.x) t.joint[item] = make_int4(0, 0, 0, 0);
-    }
+    if (lane == 0) u->s = -1;
     __syncwarp();
-}
-
-// A CTA's k-th item.  One sequence's items fall in size, so rounds in turn from the first
-// and the last CTA even out; of several sequences each CTA takes the next one left.
-__device__ __forceinline__ int64_t item_of(const TcArgs& t, int k) {
-    if (t.next) {
-        int x = 0;
-        if ((threadIdx.x & 31) == 0) x = atomicAdd(t.next, 1);
-        return __shfl_sync(0xffffffffu, x, 0);
-    }
-    return (int64_t)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 // A full sector (32 bytes) or two halves of one.
@@ -475,7 +533,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const AttnArgs& a = t.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort = &ctl->abort;
-    if (t.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
@@ -727,16 +785,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
         } else {
             // -------------------------------------- the units, and their queries
-            const int per = tiles_per_piece(t);
-            if (lane == 0) ctl->per = per;
+            if (t.split && lane == 0) t.join.joint[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+            const Plan plan = make_plan(t);
+            if (lane == 0) ctl->plan = plan;
+            int64_t pos = (int64_t)blockIdx.x * plan.per;
             int busy = 0;
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.wait_ns))) break;
                 Unit* u = &ctl->unit[k & 1];
-                const int64_t item = item_of(t, k);
-                describe(t, item, per, u);
-                if (t.next && u->s >= 0 && lane == 0) t.owner[item] = blockIdx.x;
+                describe(t, plan, k, &pos, u);
                 const int s = u->s, n = u->n, row0 = u->row0, rows = u->rows, kvh = u->kvh, begin = u->q.begin;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->u_full[k & 1]);
@@ -754,21 +812,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                                    begin + a.by_group(row0) + (b / HALVES) * t.q_tokens);
                     continue;
                 }
-#pragma unroll 8
-                for (int i = lane; i < TC_CTA_ROWS * CH; i += 32) {
-                    const int r = i / CH, c = i % CH;
-                    const bool real = r < rows && c * 8 < a.D;
-                    const int x = row0 + (real ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
+                // (rows behind the unit's keep what was there: they are nobody's)
+#pragma unroll 4
+                for (int i = lane; i < rows * CH; i += 32) {
+                    const int r = i / CH, c = i % CH, x = row0 + r, tok = a.by_group(x), head = x - tok * a.group;
                     cp16(q0 + q_at<DP>(r, c),
                          a.q + (int64_t)(begin + tok) * a.q_token + (int64_t)(kvh * a.group + head) * a.q_head +
-                             (real ? 16 * c : 0),
-                         real);
+                             (c * 8 < a.D ? 16 * c : 0),
+                         c * 8 < a.D);
                 }
                 cp_commit();
                 cp_wait<0>();
                 if (a.scale < 0.0f) {   // turned signs: the largest score is the largest product
 #pragma unroll 1
-                    for (int i = lane; i < TC_CTA_ROWS * CH; i += 32) {
+                    for (int i = lane; i < rows * CH; i += 32) {
                         uint4* x = reinterpret_cast<uint4*>(Qs + q_at<DP>(i / CH, i % CH));
                         *x = make_uint4(x->x ^ 0x80008000u, x->y ^ 0x80008000u, x->z ^ 0x80008000u, x->w ^ 0x80008000u);
                     }
@@ -871,13 +928,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             float l, lb;
             unpack_f2(add_f2(l2[0], l2[1]), l, lb);
             l += lb;
-            const bool live = r < rows, some = nw > 0 && l != 0.0f, whole_unit = u.pieces == 1;
+            const bool live = r < rows, some = nw > 0 && l != 0.0f, whole_unit = u.slot < 0;
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
             const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
-            float* pt = t.part + (int64_t)u.item * TC_CTA_ROWS * (DP + 2);   // (split units)
+            float* pt = t.join.part + (int64_t)u.slot * TC_CTA_ROWS * (DP + 2);   // (pieces)
             fine = fine && l == l;
             const float inv = !some ? 0.0f : whole_unit ? 1.0f / l : 1.0f;
             const bool sectors = ((a.D & 15) | (reinterpret_cast<uintptr_t>(a.out) & 31)) == 0;
+            uint32_t most = 0;   // an infinity or NaN has the largest bits behind the sign
 #pragma unroll 1
             for (int c0 = 0; c0 < DP; c0 += 32) {
                 uint32_t o[32];
@@ -887,14 +945,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
-                    const float f = some ? __uint_as_float(o[c]) * inv : 0.0f;
-                    if (c0 + c < a.D) fine = fine && fabsf(f) < INFINITY;
-                    o[c] = __float_as_uint(f);
+                    o[c] = some ? __float_as_uint(__uint_as_float(o[c]) * inv) : 0u;
+                    most = max(most, o[c] & 0x7fffffffu);
                 }
                 if (!live) continue;
-                if (!whole_unit) {
+                if (!whole_unit) {   // [DP / 4][row][4]: neighbouring rows' quads are neighbours
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) store32(pt + r * DP + c0 + c, o + c, true);
+                    for (int c = 0; c < 32; c += 4)
+                        *reinterpret_cast<uint4*>(pt + ((c0 + c) / 4 * TC_CTA_ROWS + r) * 4) =
+                            make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
                     continue;
                 }
 #pragma unroll
@@ -908,6 +967,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     else if (c0 + c < a.D) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
+            fine = fine && most < 0x7f800000u;
             if (n > 0) {
                 tc_fence_before();
                 __syncwarp();
@@ -917,15 +977,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (live) {
                 const float top = m == -INFINITY ? (some ? 0.0f : -INFINITY) : m * sc;
                 if (!whole_unit) {
-                    pt[TC_CTA_ROWS * DP + r] = top;
+                    // an infinite maximum joins to NaN: the row is computed again there
+                    pt[TC_CTA_ROWS * DP + r] = fine ? top : INFINITY;
                     pt[TC_CTA_ROWS * (DP + 1) + r] = l;
                 } else if (a.lse) {
                     a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
                 }
             }
             const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
-            if (lane == 0) {
-                t.again[(int64_t)u.item * TC_SOFTMAX_WARPS + warp] = again;
+            if (lane == 0 && whole_unit) {
+                t.again[(int64_t)u.id * TC_SOFTMAX_WARPS + warp] = again;
                 if (again) ctl->any_again = 1;
             }
             leave(k);
@@ -937,52 +998,27 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
     tc_fence_after();
     if (warp == TC_SOFTMAX_WARPS + 1) tmem_dealloc(tmem, 512);
+    if (warp == 0) asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows kernel may still run: not done before it
     // Rows that came out not finite, from the definition.
     if (*abort || !ctl->any_again || warp >= TC_SOFTMAX_WARPS) return;
     Unit* u = reinterpret_cast<Unit*>(smem_raw) + warp;   // (nothing is left in the rings)
+    const Plan plan = ctl->plan;
+    int64_t pos = (int64_t)blockIdx.x * plan.per;
     for (int64_t k = 0;; ++k) {
-        const int64_t item = t.next ? k : k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        describe(t, item, ctl->per, u);
-        const int s = u->s, kvh = u->kvh, row0 = u->row0 + 32 * warp, pieces = u->pieces;
+        describe(t, plan, k, &pos, u);
+        const int s = u->s, kvh = u->kvh, row0 = u->row0 + 32 * warp, slot = u->slot;
+        const int64_t id = u->id;
         const Seq q = u->q;
         __syncwarp();
         if (s < 0) break;
-        if (pieces > 1 || (t.next && __ldcg(t.owner + item) != (int)blockIdx.x)) continue;
-        unsigned again = __ldcg(t.again + item * TC_SOFTMAX_WARPS + warp);
+        if (slot >= 0) continue;
+        unsigned again = __ldcg(t.again + id * TC_SOFTMAX_WARPS + warp);
         while (again) {   // rows [32 warp, 32 warp + 32) of the unit
             const int i = __ffs(again) - 1;
             again &= again - 1;
             attn_row_exact<T>(a, s, q, kvh, row0 + i);
         }
     }
-}
-
-// Block (c, y): rows [16 y, 16 y + 16) of the split unit that begins with item c.
-template <typename T, int DP>
-__global__ void __launch_bounds__(128) paged_chunk_join_kernel(const __grid_constant__ TcArgs t) {
-    extern __shared__ float share[];
-    __shared__ int again;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the chunk kernel runs
-    const int4 u = t.joint[blockIdx.x];
-    if (u.w == 0) return;
-    const Seq q = load_seq(t.a.b, t.a.max_kv, u.x, t.a.status);
-    const int64_t left = (int64_t)q.n_new * t.a.group - (int64_t)u.z * TC_CTA_ROWS - 16 * blockIdx.y;
-    if (left <= 0) return;
-    const int64_t c = blockIdx.x;
-    const int r0 = 16 * blockIdx.y;
-    // rows that came out not finite in a piece: a NaN for its sum has them computed again
-    uint32_t bad = 0;
-    for (int i = 0; i < u.w; ++i) bad |= t.again[(c + i) * TC_SOFTMAX_WARPS + r0 / 32];
-    bad >>= r0 % 32;
-    finish_rows<T>(t.a, u.x, q, u.y, u.z * TC_CTA_ROWS + r0, (int)min((int64_t)16, left), u.w,
-                   [&](int i, int row, int d) {
-                       const float* p = t.part + (c + i) * TC_CTA_ROWS * (DP + 2);
-                       return d == -1   ? ((bad >> row) & 1 ? 0.0f : p[TC_CTA_ROWS * DP + r0 + row])
-                              : d == -2 ? ((bad >> row) & 1 ? __int_as_float(0x7fc00000)
-                                                            : p[TC_CTA_ROWS * (DP + 1) + r0 + row])
-                                        : p[(r0 + row) * DP + d];
-                   },
-                   share, &again);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -1011,32 +1047,27 @@ hmm_status_t encode_map(CUtensorMap* m, void* base, int rank, const cuuint64_t* 
     return HMM_OK;
 }
 
-// Items that may be left: units at most one more per sequence and head than its share of
-// the tokens, or pieces, no more than CTAs.
-int64_t most_items(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk) {
-    return std::max<int64_t>((n_tokens * group / TC_CTA_ROWS + n_seq) * hk, device_sm_count());
+// Units: at most one more per sequence and head than its share of the tokens.
+int64_t most_units(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk) {
+    return (n_tokens * group / TC_CTA_ROWS + n_seq) * hk;
 }
 
-// Units may be fewer than CTAs only if the tokens' row blocks are.
+// Whether the units can be too few for whole ones (the tokens' row blocks are as many at
+// least, if no sequence is another kernel's).
 bool may_split(int64_t n_tokens, int64_t group, int64_t hk) {
-    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk < device_sm_count();
+    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk * 2 < TC_ROUNDS2 * device_sm_count();
 }
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 template <typename T, int DP>
 hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q,
-                          cudaStream_t st) {
+                          bool behind, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
-    hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
+    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP>, tc_smem<DP>(), &done);
     if (s != HMM_OK) return s;
-    const unsigned ctas = (unsigned)device_sm_count();
-    paged_chunk_kernel<T, DP><<<ctas, TC_THREADS, tc_smem<DP>(), st>>>(k, v, q, t);
-    s = check_launch("paged_chunk_kernel");
-    if (s != HMM_OK || !t.split) return s;
-    const int64_t rows = std::min<int64_t>(TC_CTA_ROWS, (int64_t)t.a.b.n_tokens * t.a.group);
-    return launch_behind(paged_chunk_join_kernel<T, DP>, dim3(ctas, (unsigned)((rows + 15) / 16)), 128,
-                         sizeof(float) * 16 * ctas, st, t, "paged_chunk_join_kernel");
+    return launch(paged_chunk_kernel<T, DP>, dim3((unsigned)device_sm_count()), TC_THREADS, tc_smem<DP>(), behind, st,
+                  "paged_chunk_kernel", k, v, q, t);
 }
 
 }  // namespace
@@ -1057,31 +1088,41 @@ bool chunk_applies(const AttnArgs& a) {
 size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D) {
     if (D > 128) return 0;
     const int64_t group = std::max<int64_t>(1, n_heads / n_kv_heads), ctas = device_sm_count();
-    size_t n = 256 + up256(4 * (size_t)most_items(n_seq, n_tokens, group, n_kv_heads) * (TC_SOFTMAX_WARPS + 1));
+    size_t n = up256(4 * (size_t)most_units(n_seq, n_tokens, group, n_kv_heads) * TC_SOFTMAX_WARPS);
     if (may_split(n_tokens, group, n_kv_heads))
-        n += up256(sizeof(int4) * ctas) + sizeof(float) * ctas * TC_CTA_ROWS * ((D <= 64 ? 64 : 128) + 2);
+        n += up256(2 * sizeof(int4) * ctas) + sizeof(float) * 2 * ctas * TC_CTA_ROWS * ((D <= 64 ? 64 : 128) + 2);
     return n;
 }
 
-hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, unsigned char* ws, cudaStream_t st) {
-    const int64_t items = most_items(a.b.n_seq, a.b.n_tokens, a.group, a.hk);
-    HMM_REQUIRE(items < (int64_t(1) << 30), "n_tokens * n_heads is too large for one call");
-    int* owner = (int*)(ws + 256);
-    unsigned char* joint = ws + 256 + up256(4 * (size_t)items * (TC_SOFTMAX_WARPS + 1));
+hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, unsigned char* ws, cudaStream_t st,
+                       ChunkJoin* join) {
+    const int64_t units = most_units(a.b.n_seq, a.b.n_tokens, a.group, a.hk);
+    HMM_REQUIRE(units < (int64_t(1) << 30), "n_tokens * n_heads is too large for one call");
+    unsigned char* joint = ws + up256(4 * (size_t)units * TC_SOFTMAX_WARPS);
     // A tile of 128 rows is a box of the queries where it is whole tokens; a negative scale
     // turns the signs on the way, which a box cannot.
     const bool boxes = a.group <= TC_ROWS && (a.group & (a.group - 1)) == 0 && a.scale >= 0.0f &&
                        (a.hq == 1 || a.q_head > 0) && (a.b.n_tokens == 1 || a.q_token > 0) &&
                        a.q_head < (int64_t(1) << 40) && a.q_token < (int64_t(1) << 40);
-    TcArgs t{a, min_rows, box_rows_of(a.page_tokens, TC_KEYS), may_split(a.b.n_tokens, a.group, a.hk),
-             a.b.n_seq > 1 ? (int*)ws : nullptr, owner, boxes ? TC_ROWS / a.group : 0, wait_limit_ns(),
-             (uint32_t*)(owner + items), (int4*)joint, (float*)(joint + up256(sizeof(int4) * device_sm_count()))};
-    CUtensorMap k, v;
+    TcArgs t{};
+    t.a = a;
+    t.min_rows = min_rows;
+    t.box_rows = box_rows_of(a.page_tokens, TC_KEYS);
+    t.split = may_split(a.b.n_tokens, a.group, a.hk);
+    t.q_tokens = boxes ? TC_ROWS / a.group : 0;
+    t.wait_ns = wait_limit_ns();
+    t.again = (uint32_t*)ws;
+    if (t.split) {
+        const int64_t rows = std::min<int64_t>(TC_CTA_ROWS, (int64_t)a.b.n_tokens * a.group);
+        t.join = ChunkJoin{(int4*)joint, (float*)(joint + up256(2 * sizeof(int4) * device_sm_count())),
+                           device_sm_count(), (int)((rows + 15) / 16)};
+    }
+    *join = t.join;
+    CUtensorMap k, v, q{};
     hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows);
     if (s != HMM_OK) return s;
     s = make_page_map(&v, a, a.v, t.box_rows);
     if (s != HMM_OK) return s;
-    CUtensorMap q{};
     if (boxes) {
         const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tokens};
         const cuuint64_t strides[2] = {a.hq == 1 ? 16 : (cuuint64_t)a.q_head,
@@ -1091,8 +1132,10 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, unsigned char
         if (s != HMM_OK) return s;
     }
     if (a.D <= 64)
-        return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, q, st) : launch_chunk<__half, 64>(t, k, v, q, st);
-    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, q, st) : launch_chunk<__half, 128>(t, k, v, q, st);
+        return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, q, behind, st)
+                    : launch_chunk<__half, 64>(t, k, v, q, behind, st);
+    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, q, behind, st)
+                : launch_chunk<__half, 128>(t, k, v, q, behind, st);
 }
 
 }  // namespace serve
