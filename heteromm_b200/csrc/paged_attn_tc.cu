@@ -305,6 +305,11 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
     return TOP ? max3(mx0, mx1, mx1) : 0.0f;
 }
 
+// The lowest n bits, none for n < 0, all from 32 on.
+__device__ __forceinline__ uint32_t below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
 // Row blocks of a sequence.
 __device__ __forceinline__ int row_blocks(const TcArgs& t, const Seq& q) {
     const int64_t rows = (int64_t)q.n_new * t.a.group;
@@ -375,13 +380,14 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
         Seq q{0, 0, 0, false};
         if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
-        unsigned busy = __ballot_sync(0xffffffffu, rb > 0);
+        if (rb > 0) tiles += block_length(a, q, 0);
+        unsigned busy = __ballot_sync(0xffffffffu, rb > 1);
         while (busy) {
             const int src = __ffs(busy) - 1;
             busy &= busy - 1;
             const Seq x = shared_seq(q, src);
             const int n = __shfl_sync(0xffffffffu, rb, src);
-            for (int i = lane; i < n; i += 32) tiles += block_length(a, x, i);
+            for (int i = 1 + lane; i < n; i += 32) tiles += block_length(a, x, i);
         }
     }
     tiles = warp_sum(tiles) * a.hk;
@@ -412,6 +418,17 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                 run += all;
                 continue;
             }
+        } else if (!__any_sync(0xffffffffu, rb > 1)) {   // a block each: past them to the one that is meant
+            const int64_t v = rb > 0 ? (int64_t)block_length(a, q, 0) * a.hk : 0, incl = warp_scan(v) + run;
+            const unsigned here = __ballot_sync(0xffffffffu, incl - v <= at && at < incl);
+            const int stop = here ? __ffs(here) - 1 : 32;
+            unit_run += (int64_t)__popc(busy & ((stop < 32 ? 1u << stop : 0u) - 1u)) * a.hk;
+            if (!here) {
+                run = __shfl_sync(0xffffffffu, incl, 31);
+                continue;
+            }
+            run = __shfl_sync(0xffffffffu, incl - v, stop);
+            busy = 1u << stop;
         }
         while (busy) {
             const int src = __ffs(busy) - 1;
@@ -450,10 +467,14 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
             }
             const int row0 = b * TC_CTA_ROWS, row1 = last_row(x, a.group, b);
             const Tiles all = tiles_of(a, x, row0, row1);
-            const int take = cut ? (int)min((int64_t)(n_all - v0), end - at) : 0;   // of its length
-            const bool whole = !cut || (v0 == 0 && take == n_all);
+            // A piece is [v0, v1) of the unit's length; its own cost alone is none, and who begins
+            // within it begins the unit.
+            const int v1 = cut ? v0 + (int)min((int64_t)(n_all - v0), end - at) : 0;
+            if (cut) *pos = at + v1 - v0;
+            if (cut && v1 <= TC_UNIT_COST && v1 < n_all) break;
+            const bool begins = v0 <= TC_UNIT_COST, whole = !cut || (begins && v1 == n_all);
             const int t0 = cut ? max(0, v0 - TC_UNIT_COST) : 0;
-            const int most = cut ? max(0, v0 + take - TC_UNIT_COST) - t0 : INT_MAX;
+            const int most = cut ? max(0, v1 - TC_UNIT_COST) - t0 : INT_MAX;
             if (lane == 0) {
                 u->s = s0 + src;
                 u->kvh = kvh;
@@ -478,17 +499,17 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                     n = max(n, nw);
                 }
                 u->n = n;
-                u->slot = whole ? -1 : (int)(2 * cta + (v0 == 0));
+                u->slot = whole ? -1 : (int)(2 * cta + begins);
                 u->id = (int)(cut ? unit_run + (int64_t)(n_rb - 1 - b) * a.hk + kvh : at);
-                if (!whole && v0 == 0) {   // its other pieces are the next CTAs' first ones
-                    t.join.joint[2 * cta] = make_int4(s0 + src, kvh, b, 1 + (int)((n_all - take + plan.per - 1) / plan.per));
+                if (!whole && begins) {   // its other pieces are the next CTAs' first ones
+                    t.join.joint[2 * cta] = make_int4(s0 + src, kvh, b, 1 + (int)((n_all - v1 + plan.per - 1) / plan.per));
                     t.join.joint[2 * cta + 1] = make_int4(x.begin, x.n_new, x.kv, 0);
                 }
             }
-            if (cut) *pos = at + take;
             __syncwarp();
             return;
         }
+        if (cut && *pos != at) break;   // the share ended in a unit's own cost
     }
     if (lane == 0) u->s = -1;
     __syncwarp();
@@ -870,21 +891,27 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
                       (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
                     const int hi = (a.causal ? min(kv, pos + 1) : kv) - key0;
-                    const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : -1;
+                    const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : 0;
                     const int sink = a.window > 0 ? a.sinks - key0 : 0;
 #pragma unroll
-                    for (int c = 0; c < TC_KEYS; ++c)
-                        if (c >= hi || (c < lo && c >= sink)) v[c] = 0xff800000u;
+                    for (int c0 = 0; c0 < TC_KEYS; c0 += 32) {
+                        const uint32_t seen = below(hi - c0) & (~below(lo - c0) | below(sink - c0));
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!((seen >> c) & 1u)) v[c0 + c] = 0xff800000u;
+                    }
                 }
                 // The first half's weights with the maximum so far, while this tile's is found:
                 // that is right unless the row grew by more than TC_GROWTH, which is rare.
+                // NaN and +inf show in the maximum: such a row is computed again at the end.
                 uint32_t p[32];
                 uint64_t sum[2];
-                // NaN and +inf show in the maximum: such a row is computed again at the end.
-                const float top = weights<T, true>(v, sc2, m, sc, p, sum);
-                fine = fine && top < INFINITY;
-                const bool grow = (top - m) * sc > TC_GROWTH;
-                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+                while (true) {
+                    const float top = weights<T, true>(v, sc2, m, sc, p, sum);
+                    fine = fine && top < INFINITY;
+                    const bool grow = (top - m) * sc > TC_GROWTH && top < INFINITY;
+                    if (!__any_sync(0xffffffffu, grow)) break;
                     const float al = grow ? ex2((m - top) * sc) : 1.0f;
                     if (grow) m = top;
                     const uint64_t al2 = pack_f2(al, al);
@@ -900,8 +927,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
                             tmem_st_x32(to + c, o);
                         }
+                        tmem_wait_st();
                     }
-                    weights<T, false>(v, sc2, m, sc, p, sum);
                 }
                 // the first half's product starts while the second half is in the exponentials
                 tmem_st_x32(ts, p);
