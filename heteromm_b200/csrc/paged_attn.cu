@@ -150,17 +150,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         fence_barrier_init();
     }
     // ---- this CTA's piece of the list of all units' tiles
-    int64_t total = 0;
-    for (int s0 = 0; s0 < a.b.n_seq; s0 += RW_THREADS) {
-        const int s = s0 + threadIdx.x;
-        int64_t v = 0, sum;
-        if (s < a.b.n_seq) {
-            const Load x = seq_load(r, load_seq(a.b, a.max_kv, s, a.status));
-            v = (int64_t)x.units * x.tiles;
-        }
-        scan_incl(v, wt, &sum);
-        total += sum;
+    int64_t total = 0, own = 0;
+    for (int s = threadIdx.x; s < a.b.n_seq; s += RW_THREADS) {
+        const Load x = seq_load(r, load_seq(a.b, a.max_kv, s, a.status));
+        own += (int64_t)x.units * x.tiles;
     }
+    scan_incl(own, wt, &total);
     const int64_t per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     int64_t cur = blockIdx.x * per;
     const int64_t end = min(total, cur + per);
@@ -581,6 +576,8 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
                 "n_tokens * (n_heads / n_kv_heads) must be < 2^31");
     if (batch->n_seq == 0 || batch->n_tokens == 0) return HMM_OK;
     HMM_REQUIRE(cache->n_pages >= 1, "the cache has no pages");
+    HMM_REQUIRE(batch->pages_per_seq * cache->page_tokens <= (int64_t(1) << 31) - 1024,
+                "pages_per_seq * page_tokens must be <= 2^31 - 1024");   // ends of tiles stay in 31 bits
     const int64_t steps[6] = {cache->page_tokens > 1 ? cache->k_token : 8, cache->n_kv_heads > 1 ? cache->k_head : 8,
                               cache->n_pages > 1 ? cache->k_page : 8, cache->page_tokens > 1 ? cache->v_token : 8,
                               cache->n_kv_heads > 1 ? cache->v_head : 8, cache->n_pages > 1 ? cache->v_page : 8};

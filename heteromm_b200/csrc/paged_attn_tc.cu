@@ -49,15 +49,16 @@ constexpr int TC_THREADS = 32 * TC_WARPS;
 constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
 constexpr int TC_MIN_PIECE = 3;              // key tiles of a piece, at least
 constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start and end take the time of
-#ifndef TC_ROUNDS2
-#define TC_ROUNDS2 2
-#endif
+// Units are cut when they are fewer than the CTAs.  A cut costs a join (about 10 us): at 1.1
+// units a CTA (the window of 1,024 at 2,000 tokens) cutting up to 1.5 a CTA took 87 us, not
+// cutting 82; at 1.4 (a mixed step) 126 and 106.
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
-// Of 8 pairs of exponentials, those that go to the FMA pipe.
-#ifndef TC_POLY
-#define TC_POLY 0
-#endif
+// Of 8 pairs of exponentials, those that go to the FMA pipe.  At D = 64 the exponentials
+// bound a tile (8,192 tokens: 0 of 8 430 us, 1 413, 2 434); at D = 128 the products and
+// their reads do, and more instructions only cost (0: 486 us, 1 514, 2 528).
+template <int DP>
+__host__ __device__ constexpr int tc_poly() { return DP == 64 ? 1 : 0; }
 constexpr float EXP2_C1 = 0.6931470036506653f, EXP2_C2 = 0.24022242426872253f, EXP2_C3 = 0.05550733581185341f,
                 EXP2_C4 = 0.009671512991189957f, EXP2_C5 = 0.001326472731307149f;
 
@@ -76,6 +77,7 @@ struct TcArgs {
     int q_tokens;        // new tokens of a row tile's TMA box, 0: queries by 16-byte copies
     uint64_t wait_ns;    // limit of every bounded wait
     uint32_t* again;     // [units][TC_SOFTMAX_WARPS] rows that came out not finite
+    int units;           // sequences that overlap (a cu_new that descends) would be more units
     ChunkJoin join;
 };
 
@@ -270,7 +272,7 @@ __device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
 // (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
-template <typename T, bool TOP>
+template <typename T, int POLY, bool TOP>
 __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
                                          uint64_t* sum) {
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
@@ -282,7 +284,7 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
     for (int i = 0; i < 32 + LAG; ++i) {
         if (i < 32) {
             const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
-            if (i % 8 < TC_POLY) {
+            if (i % 8 < POLY) {
                 exp2_pair(e, x[i], y[i]);
             } else {
                 unpack_f2(e, x[i], y[i]);
@@ -373,7 +375,7 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     int64_t units = 0;
     for (int s = lane; s < a.b.n_seq; s += 32)
         units += (int64_t)row_blocks(t, load_seq(a.b, a.max_kv, s, a.status)) * a.hk;
-    if (2 * warp_sum(units) >= TC_ROUNDS2 * (int64_t)gridDim.x) return Plan{0, 0};
+    if (warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
         const int s = s0 + lane;
@@ -394,19 +396,31 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     return Plan{max((int64_t)TC_MIN_PIECE + TC_UNIT_COST, (tiles + gridDim.x - 1) / gridDim.x), tiles};
 }
 
-// The k-th unit (whole units) or, from tile `*pos` of all units' on, the next piece of this
-// CTA's share, into *u (s = -1: there is none); moves *pos on.  One warp.
-__device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int64_t k, int64_t* pos, Unit* u) {
+// Where a CTA has come to: the next tile of its share (cut units), and the 32 sequences where
+// its last unit lay, with the tiles or units and the units before them (the order is the
+// same for all, so a CTA's next unit is there or behind).
+struct Cursor {
+    int64_t pos;
+    int s0;
+    int64_t run, units;
+};
+
+// The k-th unit (whole units) or, from c->pos on, the next piece of this CTA's share, into
+// *u (s = -1: there is none); moves *c on.  One warp.
+__device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int64_t k, Cursor* c, Unit* u) {
     const AttnArgs& a = t.a;
     const int lane = threadIdx.x & 31;
     const int64_t cta = blockIdx.x, ctas = gridDim.x;
     const bool cut = plan.per > 0;
     // Whole units of a sequence fall in size, so rounds go from the first CTA and from the
     // last one in turn.
-    const int64_t at = cut ? *pos : k * ctas + (k & 1 ? ctas - 1 - cta : cta);
+    const int64_t at = cut ? c->pos : k * ctas + (k & 1 ? ctas - 1 - cta : cta);
     const int64_t end = cut ? min(plan.tiles, (cta + 1) * plan.per) : INT64_MAX;
-    int64_t run = 0, unit_run = 0;   // tiles (cut) or units before, and units
-    for (int s0 = 0; s0 < a.b.n_seq && at < end; s0 += 32) {
+    int64_t run = c->run, unit_run = c->units;
+    for (int s0 = c->s0; s0 < a.b.n_seq && at < end; s0 += 32) {
+        c->s0 = s0;
+        c->run = run;
+        c->units = unit_run;
         const int s = s0 + lane;
         Seq q{0, 0, 0, false};
         if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
@@ -470,7 +484,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
             // A piece is [v0, v1) of the unit's length; its own cost alone is none, and who begins
             // within it begins the unit.
             const int v1 = cut ? v0 + (int)min((int64_t)(n_all - v0), end - at) : 0;
-            if (cut) *pos = at + v1 - v0;
+            if (cut) c->pos = at + v1 - v0;
             if (cut && v1 <= TC_UNIT_COST && v1 < n_all) break;
             const bool begins = v0 <= TC_UNIT_COST, whole = !cut || (begins && v1 == n_all);
             const int t0 = cut ? max(0, v0 - TC_UNIT_COST) : 0;
@@ -509,7 +523,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
             __syncwarp();
             return;
         }
-        if (cut && *pos != at) break;   // the share ended in a unit's own cost
+        if (cut && c->pos != at) break;   // the share ended in a unit's own cost
     }
     if (lane == 0) u->s = -1;
     __syncwarp();
@@ -545,7 +559,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     // The swizzle needs 1,024-byte alignment, which the array's alignment gives (there is
     // no room to round up to it); should it ever not, the call says so.
     if ((smem_u32(smem_raw) & 1023u) != 0) {
-        if (threadIdx.x == 0) atomicOr(t.a.status, HMM_STATUS_TIMEOUT);
+        if (threadIdx.x == 0) {
+            atomicOr(t.a.status, HMM_STATUS_TIMEOUT);
+            if (t.split) t.join.joint[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     unsigned char* Qs = smem_raw;                      // [tile][half][128 rows][128 B], swizzled
@@ -655,11 +673,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
                 leave(k);
             }
-            if (!ok) {
-                give_up();
-                for (uint32_t b = i > ST ? i - ST : 0; b < i; ++b)   // copies in flight land first
-                    mbar_wait_drain(&ctl->full[b % ST], (b / ST) & 1);
-            }
+            if (!ok) give_up();
+            for (uint32_t b = i > ST ? i - ST : 0; b < i; ++b)   // copies in flight, if another role gave up
+                mbar_wait_drain(&ctl->full[b % ST], (b / ST) & 1);
         } else if (warp == TC_SOFTMAX_WARPS + 1) {
             // --------------------------------------------------------- MMA
             constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -764,11 +780,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 tiles[1] += n_of[1];
                 ++busy;
             }
-            if (!ok) {
-                give_up();
-                commit_one(one, &ctl->drain);    // the MMAs issued end before TMEM is freed
-                mbar_wait_drain(&ctl->drain, 0);
-            }
+            if (!ok) give_up();
+            commit_one(one, &ctl->drain);        // the MMAs issued end before TMEM is freed
+            mbar_wait_drain(&ctl->drain, 0);
             __syncwarp();
         } else if (warp == TC_SOFTMAX_WARPS + 2) {
             // ------------------------------------------------ V's unseen rows
@@ -804,24 +818,26 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 base += 2 * u.n;
                 leave(k);
             }
+            if (!ok) give_up();
         } else {
             // -------------------------------------- the units, and their queries
             if (t.split && lane == 0) t.join.joint[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
             const Plan plan = make_plan(t);
             if (lane == 0) ctl->plan = plan;
-            int64_t pos = (int64_t)blockIdx.x * plan.per;
-            int busy = 0;
+            Cursor at{(int64_t)blockIdx.x * plan.per, 0, 0, 0};
+            int loads = 0;                       // units' queries so far
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.wait_ns))) break;
                 Unit* u = &ctl->unit[k & 1];
-                describe(t, plan, k, &pos, u);
+                describe(t, plan, k, &at, u);
                 const int s = u->s, n = u->n, row0 = u->row0, rows = u->rows, kvh = u->kvh, begin = u->q.begin;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->u_full[k & 1]);
                 if (s < 0) break;
                 if (n == 0) continue;
-                if (!(ok = wait_warp(&ctl->q_empty, (busy++ & 1) ^ 1, abort, t.wait_ns))) break;
+                if (!(ok = wait_warp(&ctl->q_empty, (loads & 1) ^ 1, abort, t.wait_ns))) break;
+                ++loads;
                 constexpr int CH = DP / 8;
                 const uint32_t q0 = smem_u32(Qs);
                 if (t.q_tokens > 0) {   // a tile's 128 rows are whole tokens' groups: boxes of them
@@ -855,6 +871,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->q_full);
             }
+            if (!ok) give_up();
+            if (loads > 0) mbar_wait_drain(&ctl->q_full, (loads - 1) & 1);   // (as the producer's)
         }
         tc_fence_before();
         roles_done();
@@ -908,7 +926,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 uint64_t sum[2];
 #pragma unroll 1
                 while (true) {
-                    const float top = weights<T, true>(v, sc2, m, sc, p, sum);
+                    const float top = weights<T, tc_poly<DP>(), true>(v, sc2, m, sc, p, sum);
                     fine = fine && top < INFINITY;
                     const bool grow = (top - m) * sc > TC_GROWTH && top < INFINITY;
                     if (!__any_sync(0xffffffffu, grow)) break;
@@ -938,7 +956,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-                weights<T, false>(v + 64, sc2, m, sc, p, sum);
+                weights<T, tc_poly<DP>(), false>(v + 64, sc2, m, sc, p, sum);
                 tmem_st_x32(ts + 32, p);
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
@@ -1012,7 +1030,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
             }
             const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
-            if (lane == 0 && whole_unit) {
+            if (lane == 0 && whole_unit && (uint32_t)u.id < (uint32_t)t.units) {
                 t.again[(int64_t)u.id * TC_SOFTMAX_WARPS + warp] = again;
                 if (again) ctl->any_again = 1;
             }
@@ -1030,16 +1048,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (*abort || !ctl->any_again || warp >= TC_SOFTMAX_WARPS) return;
     Unit* u = reinterpret_cast<Unit*>(smem_raw) + warp;   // (nothing is left in the rings)
     const Plan plan = ctl->plan;
-    int64_t pos = (int64_t)blockIdx.x * plan.per;
+    Cursor at{(int64_t)blockIdx.x * plan.per, 0, 0, 0};
     for (int64_t k = 0;; ++k) {
-        describe(t, plan, k, &pos, u);
+        describe(t, plan, k, &at, u);
         const int s = u->s, kvh = u->kvh, row0 = u->row0 + 32 * warp, slot = u->slot;
-        const int64_t id = u->id;
+        const int id = u->id;
         const Seq q = u->q;
         __syncwarp();
         if (s < 0) break;
-        if (slot >= 0) continue;
-        unsigned again = __ldcg(t.again + id * TC_SOFTMAX_WARPS + warp);
+        if (slot >= 0 || (uint32_t)id >= (uint32_t)t.units) continue;
+        unsigned again = __ldcg(t.again + (int64_t)id * TC_SOFTMAX_WARPS + warp);
         while (again) {   // rows [32 warp, 32 warp + 32) of the unit
             const int i = __ffs(again) - 1;
             again &= again - 1;
@@ -1082,7 +1100,7 @@ int64_t most_units(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk) {
 // Whether the units can be too few for whole ones (the tokens' row blocks are as many at
 // least, if no sequence is another kernel's).
 bool may_split(int64_t n_tokens, int64_t group, int64_t hk) {
-    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk * 2 < TC_ROUNDS2 * device_sm_count();
+    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk < device_sm_count();
 }
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -1139,6 +1157,7 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     t.q_tokens = boxes ? TC_ROWS / a.group : 0;
     t.wait_ns = wait_limit_ns();
     t.again = (uint32_t*)ws;
+    t.units = (int)units;
     if (t.split) {
         const int64_t rows = std::min<int64_t>(TC_CTA_ROWS, (int64_t)a.b.n_tokens * a.group);
         t.join = ChunkJoin{(int4*)joint, (float*)(joint + up256(2 * sizeof(int4) * device_sm_count())),

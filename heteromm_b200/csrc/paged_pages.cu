@@ -645,7 +645,8 @@ extern "C" hmm_status_t hmm_paged_fork(const hmm_paged_state_t* state, const hmm
     if (e != HMM_OK) return e;
     HMM_REQUIRE(store->n_pages == state->n_pages, "the store has %lld pages, the state %lld",
                 (long long)store->n_pages, (long long)state->n_pages);
-    HMM_REQUIRE(page_tokens >= 1 && state->pages_per_seq * page_tokens < (int64_t(1) << 31),
+    HMM_REQUIRE(page_tokens >= 1 && page_tokens < (int64_t(1) << 31) &&
+                    state->pages_per_seq * page_tokens < (int64_t(1) << 31),
                 "page_tokens must be >= 1 and pages_per_seq * page_tokens < 2^31");
     HMM_REQUIRE(n >= 0 && n <= 65535, "n must be in [0, 65535], got %lld", (long long)n);
     HMM_REQUIRE(device_status && (n == 0 || (src && dst)), "null src, dst or device_status");
@@ -665,7 +666,8 @@ extern "C" hmm_status_t hmm_paged_grow(const hmm_paged_state_t* state, int64_t p
     Work w;
     hmm_status_t e = check_state(state, true, workspace, workspace_bytes, &s, &w);
     if (e != HMM_OK) return e;
-    HMM_REQUIRE(page_tokens >= 1 && state->pages_per_seq * page_tokens < (int64_t(1) << 31),
+    HMM_REQUIRE(page_tokens >= 1 && page_tokens < (int64_t(1) << 31) &&
+                    state->pages_per_seq * page_tokens < (int64_t(1) << 31),
                 "page_tokens must be >= 1 and pages_per_seq * page_tokens < 2^31");
     HMM_REQUIRE(device_status && (s.n_seq == 0 || n_new), "null n_new or device_status");
     const cudaStream_t st = (cudaStream_t)stream;

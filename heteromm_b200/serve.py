@@ -26,6 +26,7 @@ import functools
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch.cuda import current_device as _current_device
 
 from ._abi import HMM_DTYPE_BF16, HMM_DTYPE_F16, HMM_DTYPE_F32, PageStore, PagedBatch, PagedCache, \
     PagedState, call, load
@@ -113,14 +114,13 @@ def _on_device(f):
     """Runs the call with the device of its first tensor as the current one."""
     @functools.wraps(f)
     def g(*args, **kw):
-        for t in args:
-            if t is not None:
+        for t in args or kw.values():
+            if isinstance(t, torch.Tensor):
+                dev = t.get_device()   # -1 for a CPU tensor, which f refuses
+                if dev >= 0 and dev != _current_device():
+                    with torch.cuda.device(dev):
+                        return f(*args, **kw)
                 break
-        else:
-            t = None
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.get_device()):
-                return f(*args, **kw)
         return f(*args, **kw)
     return g
 

@@ -314,7 +314,8 @@ hmm_status_t hmm_status_read(const int32_t* device_status, void* stream);
  * HMM_STATUS_BATCH_BOUNDS for a length, position, offset or sequence number
  * outside its extent, HMM_STATUS_NO_PAGES for too few free pages;
  * hmm_status_read turns them into HMM_ERR_BOUNDS and HMM_ERR_OOM.  No kernel
- * follows such a value.
+ * follows such a value.  (Attention may also set HMM_STATUS_TIMEOUT: a bounded
+ * wait ran out, and the call's outputs are invalid.)
  *
  * hmm_paged_cache_t: the K and V page arrays [n_pages][n_kv_heads]
  * [page_tokens][D] of 16-bit floats, both 16-byte aligned, with page, head
@@ -392,7 +393,9 @@ hmm_status_t hmm_paged_kv_append(
  *   the same type, contiguous, 16-byte aligned; lse [n_tokens][n_heads] fp32 or NULL
  *   max_new: a bound on the new tokens of any sequence, or 0 for none known; it
  *   chooses between kernels and never changes which rows are computed
- * D % 8 == 0, 8 <= D <= 256; workspace 16-byte aligned. */
+ * D % 8 == 0, 8 <= D <= 256; at least one page, strides of dimensions longer
+ * than 1 in [8, 2^39), pages_per_seq * page_tokens <= 2^31 - 1024, n_tokens *
+ * n_heads / n_kv_heads < 2^31; workspace 16-byte aligned. */
 size_t hmm_paged_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
                                           int64_t n_kv_heads, int64_t D);
 hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
@@ -610,7 +613,7 @@ hmm_status_t hmm_profile_read(double* total_ms, int64_t* launches);
 
 /* Test hook, no reference counterpart.  Sets the limit of every bounded
  * pipeline wait inside the tensor-core kernels (tc_score_select_kernel,
- * dsa_scores_kernel) for the calls that follow, in nanoseconds; a negative
+ * dsa_scores_kernel, paged_rows_kernel, paged_chunk_kernel) for the calls that follow, in nanoseconds; a negative
  * value restores the default of 2 s.  A wait that runs out makes its CTA let
  * the copies and MMAs already in flight complete, then exit, and the entry
  * point returns HMM_ERR_TIMEOUT with its outputs invalid.  With 0, the first
