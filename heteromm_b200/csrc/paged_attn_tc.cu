@@ -49,9 +49,11 @@ constexpr int TC_THREADS = 32 * TC_WARPS;
 constexpr int TC_REGS_LAUNCH = 168, TC_REGS_SOFTMAX = 224, TC_REGS_OTHER = 56;
 constexpr int TC_MIN_PIECE = 3;              // key tiles of a piece, at least
 constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start and end take the time of
-// Units are cut when they are fewer than the CTAs.  A cut costs a join (about 10 us): at 1.1
-// units a CTA (the window of 1,024 at 2,000 tokens) cutting up to 1.5 a CTA took 87 us, not
-// cutting 82; at 1.4 (a mixed step) 126 and 106.
+// Units are cut when they are fewer than the CTAs (at 1.4 a CTA, a mixed step, cut took 121 us
+// and whole ones 106) and the longest is longer than an equal share by what the join costs, in
+// key tiles: 128 units of 2,000 tokens, a window of 1,024 (D = 64) took 55 us cut and 43 whole,
+// 64 units of 512 tokens over 4,096 (D = 128) 64 cut and 81 whole.
+constexpr int TC_JOIN_COST = 10;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
 // Of 8 pairs of exponentials, those that go to the FMA pipe.  At D = 64 the exponentials
@@ -377,23 +379,31 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
         units += (int64_t)row_blocks(t, load_seq(a.b, a.max_kv, s, a.status)) * a.hk;
     if (warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
+    int longest = 0;
+    auto add = [&](const Seq& q, int rb) {
+        const int n = block_length(a, q, rb);
+        tiles += n;
+        longest = max(longest, n);
+    };
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
         const int s = s0 + lane;
         Seq q{0, 0, 0, false};
         if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
-        if (rb > 0) tiles += block_length(a, q, 0);
+        if (rb > 0) add(q, 0);
         unsigned busy = __ballot_sync(0xffffffffu, rb > 1);
         while (busy) {
             const int src = __ffs(busy) - 1;
             busy &= busy - 1;
             const Seq x = shared_seq(q, src);
             const int n = __shfl_sync(0xffffffffu, rb, src);
-            for (int i = 1 + lane; i < n; i += 32) tiles += block_length(a, x, i);
+            for (int i = 1 + lane; i < n; i += 32) add(x, i);
         }
     }
     tiles = warp_sum(tiles) * a.hk;
-    return Plan{max((int64_t)TC_MIN_PIECE + TC_UNIT_COST, (tiles + gridDim.x - 1) / gridDim.x), tiles};
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const int64_t per = max((int64_t)TC_MIN_PIECE + TC_UNIT_COST, (tiles + gridDim.x - 1) / gridDim.x);
+    return longest <= per + TC_JOIN_COST ? Plan{0, 0} : Plan{per, tiles};
 }
 
 // Where a CTA has come to: the next tile of its share (cut units), and the 32 sequences where
