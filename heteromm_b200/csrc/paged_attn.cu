@@ -220,7 +220,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             if (i < n) {
                 const int k0 = key0_of(i) + sub * r.box_rows;
                 if (k0 < sp.sink || (k0 + r.box_rows > sp.lo && k0 < sp.hi)) {
-                    const int lp = k0 / a.page_tokens;
+                    const int lp = a.by_page(k0);
                     const int e = page_of(a, s, lp);
                     if (e >= 0) {
                         page = e;
@@ -606,6 +606,7 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     a.hk = (int)cache->n_kv_heads;
     a.group = a.hq / a.hk;
     a.by_group = FastDiv::of(a.group);
+    a.by_page = FastDiv::of((int)cache->page_tokens);
     a.D = (int)cache->D;
     a.page_tokens = (int)cache->page_tokens;
     a.n_pages = (int)cache->n_pages;

@@ -37,7 +37,7 @@ struct AttnArgs {
     float scale, scale_log2;     // scale * log2(e)
     int causal, window, sinks;
     int hq, hk, group, D, page_tokens, n_pages;
-    FastDiv by_group;
+    FastDiv by_group, by_page;   // n / group, key / page_tokens
     int64_t max_kv;
     int32_t* status;
 };
@@ -112,9 +112,9 @@ __device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const S
         if (key == sp.sink && key < sp.lo) key = sp.lo;
         if (key >= sp.hi) break;
         if (!sees(a, q.kv, pos, key)) continue;
-        const int phys = page_of(a, s, key / a.page_tokens);
+        const int lp = a.by_page(key), phys = page_of(a, s, lp);
         if (phys < 0) continue;
-        const int in = key % a.page_tokens;
+        const int in = key - lp * a.page_tokens;
         const T* kr = reinterpret_cast<const T*>(a.k.base + phys * a.k.page + kvh * a.k.head + in * a.k.token);
         const T* vr = reinterpret_cast<const T*>(a.v.base + phys * a.v.page + kvh * a.v.head + in * a.v.token);
         float x = 0.0f;

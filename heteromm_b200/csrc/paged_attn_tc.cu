@@ -90,11 +90,13 @@ struct Unit {
     Seq q;
     Span sp;
     int sink_tiles, first;       // the seen tiles are [0, sink_tiles) and [first, ...)
-    int t0, n, n_of[TC_TILES];   // each row tile's key tiles: a prefix of the unit's
+    int t0, n, n_of[TC_TILES];   // key tiles of each row tile, a prefix of the unit's; alone: of each half
     int slot, id;                // where a piece's sums go (-1: the unit is whole); the unit's number
     __device__ __forceinline__ int key0(int j) const {
         return (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
     }
+    // one row tile: both halves of the softmax warps work on it, on every second key tile
+    __device__ __forceinline__ bool alone() const { return rows <= TC_ROWS; }
     // tiles with keys that no row sees beside some that are seen
     __device__ __forceinline__ bool mends(int k0) const {
         return !(k0 >= sp.lo && k0 + TC_KEYS <= sp.hi) && k0 + TC_KEYS > sp.sink;
@@ -110,7 +112,8 @@ struct Plan {
 struct TcCtrl {
     uint64_t full[8], empty[8];
     uint64_t s_full[TC_TILES], p_full[TC_TILES][2], o_free[TC_TILES];
-    uint64_t u_full[2], u_empty[2], q_full, q_empty, v_mend, v_fixed, o_full, drain;
+    uint64_t u_full[2], u_empty[2], q_full, q_empty, v_mend, v_fixed, o_full, drain, half_full;
+    float2 half[TC_ROWS];        // alone: the second half's maxima (log2) and sums
     Unit unit[2];
     Plan plan;
     int any_again;
@@ -522,6 +525,10 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                     u->n_of[w] = nw;
                     n = max(n, nw);
                 }
+                if (u->alone()) {
+                    u->n_of[0] = (n + 1) / 2;
+                    u->n_of[1] = n / 2;
+                }
                 u->n = n;
                 u->slot = whole ? -1 : (int)(2 * cta + begins);
                 u->id = (int)(cut ? unit_run + (int64_t)(n_rb - 1 - b) * a.hk + kvh : at);
@@ -605,6 +612,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         mbar_init(&ctl->v_fixed, 1);
         mbar_init(&ctl->o_full, 1);
         mbar_init(&ctl->drain, 1);
+        mbar_init(&ctl->half_full, TC_SOFTMAX_WARPS / 2);
         ctl->any_again = 0;
         ctl->abort = 0;
         fence_barrier_init();
@@ -636,7 +644,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         set_regs_down<TC_REGS_OTHER>();
         if (warp == TC_SOFTMAX_WARPS) {
             // -------------------------------------------------------- producer
-            const int br = t.box_rows, subs = TC_KEYS / br;
+            // A lane looks up one box's page: of 32 boxes, that is of `ahead` key tiles, at once,
+            // and of the next 32 while these are asked for.
+            const int br = t.box_rows, subs = TC_KEYS / br, ahead = 32 / subs;
             if (lane == 0) {
                 prefetch_tmap(&tmK);
                 prefetch_tmap(&tmV);
@@ -646,36 +656,40 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             for (int k = 0; ok; ++k) {
                 const Unit& u = ctl->unit[k & 1];
                 if (!(ok = take(k)) || u.s < 0) break;
-                auto lookup = [&](int j, int* page, int* row) {   // lane: box `lane` of tile j
+                const int mine = lane / subs, sub = lane % subs;
+                auto lookup = [&](int j, int* page, int* row) {   // lane: box `sub` of tile j + mine
                     *page = a.n_pages;                            // out of range: zeros
                     *row = 0;
-                    if (j < u.n && lane < subs) {
-                        const int k0 = u.key0(j) + lane * br;
+                    if (j + mine < u.n) {
+                        const int k0 = u.key0(j + mine) + sub * br;
                         if (k0 < u.sp.sink || (k0 + br > u.sp.lo && k0 < u.sp.hi)) {
-                            const int e = page_of(a, u.s, k0 / a.page_tokens);
+                            const int lp = a.by_page(k0), e = page_of(a, u.s, lp);
                             if (e >= 0) {
                                 *page = e;
-                                *row = k0 % a.page_tokens;
+                                *row = k0 - lp * a.page_tokens;
                             }
                         }
                     }
                 };
                 int page, row;
                 lookup(0, &page, &row);
-                for (int j = 0; ok && j < u.n; ++j) {
+                for (int j0 = 0; ok && j0 < u.n; j0 += ahead) {
                     int next_page, next_row;
-                    lookup(j + 1, &next_page, &next_row);
-                    for (int kv = 0; kv < 2; ++kv, ++i) {
-                        const uint32_t st = i % ST;
-                        if (!(ok = wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns))) break;
-                        if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
-                        __syncwarp();
-                        if (lane < subs) {
-                            const uint32_t dst = smem_u32(Rs + st * TILE) + lane * br * 128;
+                    lookup(j0 + ahead, &next_page, &next_row);
+                    const int n = min(ahead, u.n - j0);
+                    for (int j = 0; ok && j < n; ++j) {
+                        for (int kv = 0; kv < 2; ++kv, ++i) {
+                            const uint32_t st = i % ST;
+                            if (!(ok = wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns))) break;
+                            if (lane == 0) mbar_expect_tx(&ctl->full[st], TILE);
+                            __syncwarp();
+                            if (mine == j) {
+                                const uint32_t dst = smem_u32(Rs + st * TILE) + sub * br * 128;
 #pragma unroll
-                            for (int h = 0; h < HALVES; ++h)
-                                tma_load_page(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h,
-                                              row, u.kvh, page);
+                                for (int h = 0; h < HALVES; ++h)
+                                    tma_load_page(dst + h * (TC_KEYS * 128), kv ? &tmV : &tmK, &ctl->full[st], 64 * h,
+                                                  row, u.kvh, page);
+                            }
                         }
                     }
                     page = next_page;
@@ -700,8 +714,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 return wait_warp(bar, parity, abort, t.wait_ns);
             };
-            auto qk = [&](int w, uint32_t k) {
-                const uint32_t ql = qlo + w * (TC_ROWS * DP * 2 / 16), d = tm + 128 * w;
+            auto qk = [&](int w, uint32_t k, int rows) {   // scores w of row tile `rows`
+                const uint32_t ql = qlo + rows * (TC_ROWS * DP * 2 / 16), d = tm + 128 * w;
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
                     const uint32_t off = ((ks >> 2) * (TC_ROWS * 128) + (ks & 3) * 32) / 16;
@@ -723,6 +737,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (!(ok = take(k))) break;
                 const Unit& u = ctl->unit[k & 1];
                 const int us = __shfl_sync(0xffffffffu, u.s, 0), n = __shfl_sync(0xffffffffu, u.n, 0);
+                const bool alone = u.alone();
                 const int n_of[2] = {__shfl_sync(0xffffffffu, u.n_of[0], 0), __shfl_sync(0xffffffffu, u.n_of[1], 0)};
                 // key tiles with rows that no row sees: found from the first and the last few
                 const int t0 = u.t0, sink_tiles = u.sink_tiles, first = u.first;
@@ -730,13 +745,69 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 leave(k);
                 if (us < 0) break;
                 if (n == 0) continue;
+                // V_j has arrived and is mended, the results of the unit before have left TMEM
+                auto ready = [&](int j) {
+                    if (!wait(&ctl->full[st], ph)) return false;
+                    const int key0 = (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
+                    if (!(key0 >= lo && key0 + TC_KEYS <= hi) && key0 + TC_KEYS > sink) {
+                        if (lane == 0) mbar_arrive(&ctl->v_mend);
+                        if (!wait(&ctl->v_fixed, fixed++ & 1)) return false;
+                    }
+                    return j > 0 || busy == 0 ||
+                           (wait(&ctl->o_free[0], (busy - 1) & 1) && wait(&ctl->o_free[1], (busy - 1) & 1));
+                };
+                // O_w += P_w V, its i-th product, as the halves of P_w arrive
+                auto pv = [&](int w, int i, uint32_t v) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!wait(&ctl->p_full[w][h], ((w ? tiles[1] : tiles[0]) + i) & 1)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+                            mma_ts(one, tm + 256 + DP * w, tm + 128 * w + 8 * ks, v + ks * 128, vhi, id_pv, i > 0 || ks > 0);
+                    }
+                    return true;
+                };
                 if (!(ok = wait(&ctl->q_full, busy & 1) && wait(&ctl->full[st], ph))) break;
                 tc_fence_after();
+                if (alone) {   // key tile j in scores and sums j & 1, which two tiles on are free again
+                    int sk = st, pk = ph;        // the next K
+                    for (int j = -2; j < n; ++j) {
+                        const int w = j & 1;
+                        if (j >= 0) {
+                            if (!(ok = ready(j) && pv(w, j >> 1, vlo + st * (TILE / 16)))) break;
+                            commit_one(one, &ctl->empty[st]);
+                            next(st, ph);
+                            next(st, ph);
+                        }
+                        if (j + 2 >= n) continue;
+                        if (!(ok = wait(&ctl->full[sk], pk))) break;
+                        tc_fence_after();
+                        qk(w, klo + sk * (TILE / 16), 0);
+                        commit_one(one, &ctl->empty[sk]);
+                        if (j + 3 == n) commit_one(one, &ctl->q_empty);
+                        next(sk, pk);
+                        if (j == -2) {
+                            st = sk;             // V_0
+                            ph = pk;
+                        }
+                        next(sk, pk);
+                    }
+                    if (!ok) break;
+                    commit_one(one, &ctl->o_full);
+                    // st is one past K_n: back to it
+                    st = sk;
+                    ph = pk;
+                    tiles[0] += n_of[0];
+                    tiles[1] += n_of[1];
+                    ++busy;
+                    continue;
+                }
                 {
                     const uint32_t kl = klo + st * (TILE / 16);
 #pragma unroll
                     for (int w = 0; w < TC_TILES; ++w)
-                        if (n_of[w] > 0) qk(w, kl);
+                        if (n_of[w] > 0) qk(w, kl, w);
                 }
                 commit_one(one, &ctl->empty[st]);
                 if (n == 1) commit_one(one, &ctl->q_empty);
@@ -745,34 +816,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     int sk = st, pk = ph;        // K_j+1, behind V_j
                     next(sk, pk);
                     const uint32_t v = vlo + st * (TILE / 16), kl = klo + sk * (TILE / 16);
-                    if (!(ok = wait(&ctl->full[st], ph))) break;
-                    const int key0 = (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
-                    if (!(key0 >= lo && key0 + TC_KEYS <= hi) && key0 + TC_KEYS > sink) {
-                        if (lane == 0) mbar_arrive(&ctl->v_mend);
-                        if (!(ok = wait(&ctl->v_fixed, fixed++ & 1))) break;
-                    }
-                    // the results of the unit before have left TMEM
-                    if (j == 0 && busy > 0 &&
-                        !(ok = wait(&ctl->o_free[0], (busy - 1) & 1) && wait(&ctl->o_free[1], (busy - 1) & 1)))
-                        break;
+                    if (!(ok = ready(j))) break;
                     bool k_ready = false;
 #pragma unroll
                     for (int w = 0; w < TC_TILES; ++w) {
                         if (j >= n_of[w]) continue;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (!(ok = wait(&ctl->p_full[w][h], (tiles[w] + j) & 1))) break;
-                            tc_fence_after();
-#pragma unroll
-                            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-                                mma_ts(one, tm + 256 + DP * w, tm + 128 * w + 8 * ks, v + ks * 128, vhi, id_pv,
-                                       j > 0 || ks > 0);
-                        }
-                        if (!ok) break;
+                        if (!(ok = pv(w, j, v))) break;
                         if (j + 1 < n_of[w]) {
                             if (!k_ready && !(ok = wait(&ctl->full[sk], pk))) break;
                             k_ready = true;
-                            qk(w, kl);
+                            qk(w, kl, w);
                         }
                     }
                     if (!ok) break;
@@ -893,7 +946,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int w = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + 128 * w + lanes, to = tmem + 256 + DP * w + lanes;
-        const int wr0 = warp * 32, r = wr0 + lane;             // the warp's first row of the unit, the thread's
         const float sc = fabsf(a.scale_log2);
         const uint64_t sc2 = pack_f2(sc, sc);
         int tiles = 0, busy = 0;                               // key tiles, units with keys so far
@@ -901,21 +953,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int k = 0; ok; ++k) {
             const Unit& u = ctl->unit[k & 1];
             if (!(ok = take(k)) || u.s < 0) break;
-            const int rows = u.rows, n = u.n, nw = u.n_of[w];
-            const int pos = row_pos(a, u.q, u.row0 + min(r, rows - 1));
-            const int pos_first = row_pos(a, u.q, u.row0 + min(wr0, rows - 1));
-            const int pos_last = row_pos(a, u.q, u.row0 + min(wr0 + 31, rows - 1));
+            // (what the loop does not need is read from the unit again behind it: registers)
+            auto row = [&] { return 32 * (u.alone() ? warp & 3 : warp) + lane; };   // the thread's of the unit
+            const int pos = row_pos(a, u.q, u.row0 + min(row(), u.rows - 1));
             float m = -INFINITY;
             uint64_t l2[2] = {pack_f2(0.0f, 0.0f), pack_f2(0.0f, 0.0f)};
             bool fine = true;
-            for (int j = 0; j < nw; ++j) {
+            for (int j = 0; j < u.n_of[w]; ++j) {
                 if (!(ok = wait_warp(&ctl->s_full[w], (tiles + j) & 1, abort, t.wait_ns))) break;
                 tc_fence_after();
                 uint32_t v[TC_KEYS];
 #pragma unroll
                 for (int c = 0; c < TC_KEYS; c += 32) tmem_ld_x32(ts + c, v + c);
                 tmem_wait_ld();
-                const int key0 = u.key0(j), kv = u.q.kv;
+                const int key0 = u.key0(u.alone() ? 2 * j + w : j), kv = u.q.kv;
+                const int pos_first = __shfl_sync(0xffffffffu, pos, 0), pos_last = __shfl_sync(0xffffffffu, pos, 31);
                 if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
                       (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
                     const int hi = (a.causal ? min(kv, pos + 1) : kv) - key0;
@@ -976,6 +1028,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (lane == 0) mbar_arrive(&ctl->p_full[w][1]);
             }
             // ---- the rows' results
+            const int n = u.n, nw = u.n_of[w], rows = u.rows, r = row();
+            const bool alone = u.alone();
             if (ok && n > 0) ok = wait_warp(&ctl->o_full, busy & 1, abort, t.wait_ns);
             if (!ok) break;
             tc_fence_after();
@@ -983,26 +1037,58 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             float l, lb;
             unpack_f2(add_f2(l2[0], l2[1]), l, lb);
             l += lb;
-            const bool live = r < rows, some = nw > 0 && l != 0.0f, whole_unit = u.slot < 0;
+            const bool live = r < rows && !(alone && w == 1), some = nw > 0 && l != 0.0f, whole_unit = u.slot < 0;
+            float top = m == -INFINITY ? (some ? 0.0f : -INFINITY) : m * sc, s0 = some ? 1.0f : 0.0f, s1 = 0.0f;
+            fine = fine && l == l;
+            if (n > 0 && w == 1) {
+                if (alone) ctl->half[r] = make_float2(top, fine ? l : NAN);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->half_full);
+            } else if (n > 0) {
+                if (!(ok = wait_warp(&ctl->half_full, busy & 1, abort, t.wait_ns))) break;
+                if (alone) {   // the halves' sums over different keys
+                    const float2 x = ctl->half[r];
+                    const float both = fmaxf(top, x.x);
+                    fine = fine && x.y == x.y;
+                    s0 = top == -INFINITY ? 0.0f : ex2(top - both);
+                    s1 = x.x == -INFINITY ? 0.0f : ex2(x.x - both);
+                    l = fmaf(l, s0, x.y * s1);
+                    top = both;
+                }
+            }
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
             const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
             float* pt = t.join.part + (int64_t)u.slot * TC_CTA_ROWS * (DP + 2);   // (pieces)
-            fine = fine && l == l;
-            const float inv = !some ? 0.0f : whole_unit ? 1.0f / l : 1.0f;
+            if (whole_unit && l != 0.0f) {
+                const float inv = 1.0f / l;
+                s0 *= inv;
+                s1 *= inv;
+            }
             const bool sectors = ((a.D & 15) | (reinterpret_cast<uintptr_t>(a.out) & 31)) == 0;
             uint32_t most = 0;   // an infinity or NaN has the largest bits behind the sign
 #pragma unroll 1
-            for (int c0 = 0; c0 < DP; c0 += 32) {
+            for (int c0 = 0; c0 < (alone && w == 1 ? 0 : DP); c0 += 32) {
                 uint32_t o[32];
                 if (nw > 0) {
                     tmem_ld_x32(to + c0, o);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    o[c] = some ? __float_as_uint(__uint_as_float(o[c]) * inv) : 0u;
-                    most = max(most, o[c] & 0x7fffffffu);
+                for (int c = 0; c < 32; ++c) o[c] = s0 != 0.0f ? __float_as_uint(__uint_as_float(o[c]) * s0) : 0u;
+                if (alone && u.n_of[1] > 0) {
+#pragma unroll
+                    for (int h = 0; h < 32; h += 8) {
+                        uint32_t o1[8];
+                        tmem_ld_x8(to + DP + c0 + h, o1);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (s1 != 0.0f)
+                                o[h + c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), s1, __uint_as_float(o[h + c])));
+                    }
                 }
+#pragma unroll
+                for (int c = 0; c < 32; ++c) most = max(most, o[c] & 0x7fffffffu);
                 if (!live) continue;
                 if (!whole_unit) {   // [DP / 4][row][4]: neighbouring rows' quads are neighbours
 #pragma unroll
@@ -1026,11 +1112,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (n > 0) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->o_free[w]);
+                if (lane == 0 && !(alone && w == 1)) mbar_arrive(&ctl->o_free[w]);
+                if (lane == 0 && alone && w == 0) mbar_arrive(&ctl->o_free[1]);   // (both read by this half)
                 ++busy;
             }
             if (live) {
-                const float top = m == -INFINITY ? (some ? 0.0f : -INFINITY) : m * sc;
                 if (!whole_unit) {
                     // an infinite maximum joins to NaN: the row is computed again there
                     pt[TC_CTA_ROWS * DP + r] = fine ? top : INFINITY;
