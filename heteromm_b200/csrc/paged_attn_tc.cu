@@ -1,29 +1,47 @@
 // paged_attn_tc.cu — attention of chunks of new tokens over a paged cache on
 // tcgen05 tensor cores.
 //
-// A CTA takes 256 rows of one (sequence, KV head) - row = (new token, query head
-// of the group) - as two tiles of 128, and the keys they see in tiles of 128:
-//   warps 0-3, 4-7  softmax of row tile 0 / 1, a thread per row: scores from TMEM,
-//                   running maximum and sum in registers, weights back to TMEM; at
-//                   the end the rows' results
-//   warp 8          TMA: K and V tiles in turn into a ring of stages, page by
-//                   page (boxes of up to 128 rows of one page and head; a box
-//                   that no row sees is asked for out of range and arrives as zeros)
-//   warp 10         zeros over V rows that no row of the CTA sees (a page's end)
-//   warp 9          MMA issue: S_w = Q_w K^T (both in shared memory), then O_w +=
-//                   P_w V with P_w from TMEM over S_w's columns
+// A persistent CTA takes units: 256 rows of one (sequence, KV head) - row = (new
+// token, query head of the group) - as two tiles of 128, and the keys they see in
+// tiles of 128.  Warps:
+//   0-3, 4-7  softmax of row tile 0 / 1, a thread per row: scores from TMEM, running
+//             maximum and sum in registers, weights back to TMEM (over the scores,
+//             in halves, so that the product starts on the first); at the end the
+//             rows' results.  A unit of up to 128 rows has one row tile: then both
+//             halves work on it, on every second key tile, and join their sums
+//             (32 drafted or 12 new tokens over 8,192, 64 sequences, 8 KV heads,
+//             D = 128: 472 us -> 392; with the second half idle a tile took as long
+//             as two)
+//   8         TMA: K and V tiles in turn into a ring of stages, page by page
+//             (boxes of up to 128 rows of one page and head; a box that no row sees
+//             is asked for out of range and arrives as zeros).  A lane looks up a
+//             box's page, 32 boxes ahead of those that are asked for; a tile's pages
+//             at a time left the read of the table in the chain (8,192 tokens, pages
+//             of 16: 505 -> 478 us)
+//   9         MMA issue: S_w = Q_w K^T (both in shared memory), then O_w += P_w V
+//             with P_w from TMEM
+//   10        zeros over V rows that no row of the CTA sees (a page's end)
+//   11        the next unit (from the lengths on the device) and its queries
 // While one tile's rows are in the exponentials the tensor cores work on the
 // other.  S_w of the next key tile is issued after P_w V of this one, so one
 // barrier per tile and direction is enough: scores that are ready imply that
-// the sum with the previous weights is complete.
+// the sum with the previous weights is complete.  (At D = 64 TMEM has room for
+// weights beside the scores, so that the next scores need not wait: 468 us
+// against 420; the two halves then keep step and want the same units at once.)
 //
 // The maximum that the weights refer to is only moved when a row's has grown by
 // more than 2^8: weights then stay below 256 (exact in the fp32 sums, a common
 // factor in the result), and the sums in TMEM are rescaled rarely.
 //
-// Bound: 4 D FLOP per (row, key) on the tensor cores, against one exponential
-// per (row, key) on the special-function units, 16 a clock and SM: at D = 128
-// both take 1,024 clocks a tile.
+// Bound: 4 D FLOP per (row, key) on the tensor cores, 2,048 clocks for the two row
+// tiles and a key tile at D = 128, and as many for their exponentials on the
+// special-function units, 16 a clock.  Measured, 32 query and 8 KV heads, 8,192
+// tokens, causal: D = 128 465-478 us (1,150-1,180 TFLOP/s, about 4,000 clocks a
+// tile); without the exponentials it is no faster, with the products and loads
+// alone 418: reading K and V into shared memory, 64 KB a tile and CTA, and their
+// reading by both row tiles' products bound it.  D = 64 424 us (650 TFLOP/s): the
+// softmax warps' instructions do; exponentials moved to the FMA pipe only add (1 of
+// 8: 437).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -55,14 +73,6 @@ constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start an
 // 64 units of 512 tokens over 4,096 (D = 128) 64 cut and 81 whole.
 constexpr int TC_JOIN_COST = 10;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
-
-// Of 8 pairs of exponentials, those that go to the FMA pipe.  At D = 64 the exponentials
-// bound a tile (8,192 tokens: 0 of 8 430 us, 1 413, 2 434); at D = 128 the products and
-// their reads do, and more instructions only cost (0: 486 us, 1 514, 2 528).
-template <int DP>
-__host__ __device__ constexpr int tc_poly() { return DP == 64 ? 1 : 0; }
-constexpr float EXP2_C1 = 0.6931470036506653f, EXP2_C2 = 0.24022242426872253f, EXP2_C3 = 0.05550733581185341f,
-                EXP2_C4 = 0.009671512991189957f, EXP2_C5 = 0.001326472731307149f;
 
 template <int DP>
 __host__ __device__ constexpr int tc_stages() { return DP == 64 ? 8 : 5; }
@@ -249,35 +259,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// 2^x of a pair on the FMA pipe, x <= 2^22: x = n + f with n the nearest whole number
-// (read off the low bits of x + 1.5 2^23), 2^f on [-1/2, 1/2] by the polynomial of
-// degree 5 with p(0) = 1 that is nearest in relative error (a weighted least-squares
-// fit: 2^-23.4), and n added to the exponent.  From -127 down it is 0 (p(0) = 1 makes
-// that exact).  A NaN is lost: the caller looks for it in the maximum.
-__device__ __forceinline__ void exp2_pair(uint64_t e, float& x, float& y) {
-    unpack_f2(e, x, y);
-    e = pack_f2(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
-    const uint64_t big = pack_f2(12582912.0f, 12582912.0f), nbig = pack_f2(-12582912.0f, -12582912.0f);
-    const uint64_t t = add_f2(e, big);
-    const uint64_t f = fma_f2(add_f2(t, nbig), pack_f2(-1.0f, -1.0f), e);
-    uint64_t p = fma_f2(f, pack_f2(EXP2_C5, EXP2_C5), pack_f2(EXP2_C4, EXP2_C4));
-    p = fma_f2(f, p, pack_f2(EXP2_C3, EXP2_C3));
-    p = fma_f2(f, p, pack_f2(EXP2_C2, EXP2_C2));
-    p = fma_f2(f, p, pack_f2(EXP2_C1, EXP2_C1));
-    p = fma_f2(f, p, pack_f2(1.0f, 1.0f));
-    float tx, ty;
-    unpack_f2(t, tx, ty);
-    unpack_f2(p, x, y);
-    x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
-    y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
-}
-
 // Weights exp2(sc (s - m)) of 64 of a row's scores v, packed in pairs, and their sum (two
 // pairs of partial sums); with TOP also the largest of the 128 scores from v on.  m = -inf
 // (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
-template <typename T, int POLY, bool TOP>
+template <typename T, bool TOP>
 __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
                                          uint64_t* sum) {
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
@@ -289,13 +276,9 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
     for (int i = 0; i < 32 + LAG; ++i) {
         if (i < 32) {
             const uint64_t e = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sc2, neg2);
-            if (i % 8 < POLY) {
-                exp2_pair(e, x[i], y[i]);
-            } else {
-                unpack_f2(e, x[i], y[i]);
-                x[i] = ex2(x[i]);
-                y[i] = ex2(y[i]);
-            }
+            unpack_f2(e, x[i], y[i]);
+            x[i] = ex2(x[i]);
+            y[i] = ex2(y[i]);
             if (TOP) {
                 mx0 = max3(mx0, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
                 mx1 = max3(mx1, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
@@ -988,7 +971,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 uint64_t sum[2];
 #pragma unroll 1
                 while (true) {
-                    const float top = weights<T, tc_poly<DP>(), true>(v, sc2, m, sc, p, sum);
+                    const float top = weights<T, true>(v, sc2, m, sc, p, sum);
                     fine = fine && top < INFINITY;
                     const bool grow = (top - m) * sc > TC_GROWTH && top < INFINITY;
                     if (!__any_sync(0xffffffffu, grow)) break;
@@ -1018,7 +1001,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-                weights<T, tc_poly<DP>(), false>(v + 64, sc2, m, sc, p, sum);
+                weights<T, false>(v + 64, sc2, m, sc, p, sum);
                 tmem_st_x32(ts + 32, p);
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
