@@ -8,6 +8,8 @@
   lib/heteromm_cpp_kernels<ext>  Python bindings of the steps under the names the
                             reference's pipeline generator calls
                             (src/py/heteromm_cpp_kernels.cpp, pybind11)
+  lib/heteromm_serve_calls<ext>  the serving entry points called with torch tensors
+                            (src/py/serve_calls.cpp, torch's headers)
 
 nvcc cross-compiles for sm_100a without a GPU; the built .so files travel with
 the repository snapshot to the GPU machine.
@@ -96,10 +98,32 @@ def build_py_kernels(force: bool = False) -> str:
     return out
 
 
+def serve_calls_path() -> str:
+    import sysconfig
+    return os.path.join(LIB_DIR, "heteromm_serve_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_serve_calls(force: bool = False) -> str:
+    """The module heteromm_serve_calls; torch's own libraries are loaded when it is."""
+    import sysconfig
+    import torch
+    src, out = os.path.join(PKG, "src", "py", "serve_calls.cpp"), serve_calls_path()
+    if force or _newer(out, [src, os.path.join(INC, "heteromm_cuda.h")]):
+        os.makedirs(LIB_DIR, exist_ok=True)
+        home = os.path.dirname(torch.__file__)
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              *(f"-isystem{os.path.join(home, 'include', d)}" for d in ("", "torch/csrc/api/include")),
+              "-I/usr/local/cuda/include", f"-I{sysconfig.get_paths()['include']}", f"-I{INC}", "-o", out, src,
+              f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+    return out
+
+
 def build(force: bool = False) -> None:
     build_cuda(force)
     build_steps(force)
     build_py_kernels(force)
+    build_serve_calls(force)
 
 
 if __name__ == "__main__":
