@@ -369,14 +369,24 @@ grow_rows_kernel(const State s, const Work w, int page_tokens, const int32_t* n_
         before += i < row ? max(v, 0) : 0;
     }
     bad = __syncthreads_or(bad);
-    __shared__ unsigned long long acc[2];
-    if (threadIdx.x == 0) acc[0] = acc[1] = 0;
+    // (a butterfly and a sum over the warps: 64-bit atomics of all threads took 10 us here)
+    __shared__ long long acc[2][PG_THREADS / 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        need += __shfl_xor_sync(0xffffffffu, need, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        acc[0][threadIdx.x >> 5] = need;
+        acc[1][threadIdx.x >> 5] = before;
+    }
     __syncthreads();
-    if (need) atomicAdd(&acc[0], (unsigned long long)need);
-    if (before) atomicAdd(&acc[1], (unsigned long long)before);
-    __syncthreads();
-    need = (long long)acc[0];
-    before = (long long)acc[1];
+    need = before = 0;
+#pragma unroll
+    for (int i = 0; i < PG_THREADS / 32; ++i) {
+        need += acc[0][i];
+        before += acc[1][i];
+    }
     const bool short_of = total_free(w, s.chunks, red) < need;
     if (bad || short_of) {
         if (row == 0 && threadIdx.x == 0)
