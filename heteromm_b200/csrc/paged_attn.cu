@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_con
     const int4 u = joint[0], x = joint[1];
     if (u.w == 0) return;
     const Seq q{x.x, x.y, x.z, true};
-    const int rows = few ? RW_ROWS : TC_CTA_ROWS, row0 = u.z * rows + r0;
+    const int rows = few ? RW_ROWS : j.chunk.rows, row0 = u.z * rows + r0;
     const int64_t left = (int64_t)q.n_new * j.a.group - row0;
     if (left <= 0) return;
     const int64_t size = (int64_t)rows * (j.dp + 2);

@@ -22,6 +22,9 @@
 //             with P_w from TMEM
 //   10        zeros over V rows that no row of the CTA sees (a page's end)
 //   11        the next unit (from the lengths on the device) and its queries
+// Heads of 129 to 256 values: units of one row tile, whose sums take half of TMEM, on
+// warps 0-3 and a ring of two stages (2,048 tokens, 16 query and 4 KV heads, D = 256:
+// 72 us; by the rows kernel 990).
 // While one tile's rows are in the exponentials the tensor cores work on the
 // other.  S_w of the next key tile is issued after P_w V of this one, so one
 // barrier per tile and direction is enough: scores that are ready imply that
@@ -74,15 +77,20 @@ constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start an
 constexpr int TC_JOIN_COST = 10;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
 
+// Rows of a unit: at D = 256 the sums of one row tile take the TMEM beside its scores, and
+// the second half of the softmax warps rests.
 template <int DP>
-__host__ __device__ constexpr int tc_stages() { return DP == 64 ? 8 : 5; }
+__host__ __device__ constexpr int tc_rows() { return DP == 256 ? TC_ROWS : TC_CTA_ROWS; }
+template <int DP>
+__host__ __device__ constexpr int tc_stages() { return DP == 64 ? 8 : DP == 128 ? 5 : 2; }
 template <int DP>
 __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * DP * 2; }
 template <int DP>
-__host__ __device__ constexpr int tc_q_bytes() { return TC_CTA_ROWS * DP * 2; }
+__host__ __device__ constexpr int tc_q_bytes() { return tc_rows<DP>() * DP * 2; }
 
 struct TcArgs {
     AttnArgs a;
+    int rows_log2;       // rows of a unit
     int min_rows;        // sequences of fewer rows are another kernel's
     int box_rows;        // rows of a TMA box: a power of two that divides page_tokens
     int split;           // whether few units may be cut into pieces
@@ -93,7 +101,7 @@ struct TcArgs {
     ChunkJoin join;
 };
 
-// What a CTA works on at a time: 256 rows of a (sequence, KV head) and `n` key tiles of
+// What a CTA works on at a time: 256 (D = 256: 128) rows of a (sequence, KV head) and `n` key tiles of
 // those that they see, from the t0-th on.
 struct Unit {
     int s, kvh, row0, rows;      // s < 0: no more
@@ -101,12 +109,11 @@ struct Unit {
     Span sp;
     int sink_tiles, first;       // the seen tiles are [0, sink_tiles) and [first, ...)
     int t0, n, n_of[TC_TILES];   // key tiles of each row tile, a prefix of the unit's; alone: of each half
+    bool alone;                  // one row tile: both halves of the softmax warps work on it, on every second key tile
     int slot, id;                // where a piece's sums go (-1: the unit is whole); the unit's number
     __device__ __forceinline__ int key0(int j) const {
         return (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * TC_KEYS;
     }
-    // one row tile: both halves of the softmax warps work on it, on every second key tile
-    __device__ __forceinline__ bool alone() const { return rows <= TC_ROWS; }
     // tiles with keys that no row sees beside some that are seen
     __device__ __forceinline__ bool mends(int k0) const {
         return !(k0 >= sp.lo && k0 + TC_KEYS <= sp.hi) && k0 + TC_KEYS > sp.sink;
@@ -303,7 +310,7 @@ __device__ __forceinline__ uint32_t below(int n) {
 // Row blocks of a sequence.
 __device__ __forceinline__ int row_blocks(const TcArgs& t, const Seq& q) {
     const int64_t rows = (int64_t)q.n_new * t.a.group;
-    return rows < t.min_rows ? 0 : (int)((rows + TC_CTA_ROWS - 1) / TC_CTA_ROWS);
+    return rows < t.min_rows ? 0 : (int)((rows + (1 << t.rows_log2) - 1) >> t.rows_log2);
 }
 
 // The seen key tiles of rows [row0, row1) of a sequence.
@@ -321,13 +328,13 @@ __device__ __forceinline__ Tiles tiles_of(const AttnArgs& a, const Seq& q, int r
     return x;
 }
 
-__device__ __forceinline__ int last_row(const Seq& q, int group, int rb) {
-    return (int)min((int64_t)(rb + 1) * TC_CTA_ROWS, (int64_t)q.n_new * group);
+__device__ __forceinline__ int last_row(const TcArgs& t, const Seq& q, int rb) {
+    return (int)min((int64_t)(rb + 1) << t.rows_log2, (int64_t)q.n_new * t.a.group);
 }
 
 // The length of row block rb's units in the plan: their key tiles behind the unit's own cost.
-__device__ __forceinline__ int block_length(const AttnArgs& a, const Seq& q, int rb) {
-    return TC_UNIT_COST + tiles_of(a, q, rb * TC_CTA_ROWS, last_row(q, a.group, rb)).n;
+__device__ __forceinline__ int block_length(const TcArgs& t, const Seq& q, int rb) {
+    return TC_UNIT_COST + tiles_of(t.a, q, rb << t.rows_log2, last_row(t, q, rb)).n;
 }
 
 // Lane `src`'s sequence, for the warp.
@@ -367,7 +374,7 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
     int longest = 0;
     auto add = [&](const Seq& q, int rb) {
-        const int n = block_length(a, q, rb);
+        const int n = block_length(t, q, rb);
         tiles += n;
         longest = max(longest, n);
     };
@@ -429,7 +436,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                 continue;
             }
         } else if (!__any_sync(0xffffffffu, rb > 1)) {   // a block each: past them to the one that is meant
-            const int64_t v = rb > 0 ? (int64_t)block_length(a, q, 0) * a.hk : 0, incl = warp_scan(v) + run;
+            const int64_t v = rb > 0 ? (int64_t)block_length(t, q, 0) * a.hk : 0, incl = warp_scan(v) + run;
             const unsigned here = __ballot_sync(0xffffffffu, incl - v <= at && at < incl);
             const int stop = here ? __ffs(here) - 1 : 32;
             unit_run += (int64_t)__popc(busy & ((stop < 32 ? 1u << stop : 0u) - 1u)) * a.hk;
@@ -457,7 +464,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                 run += (int64_t)n_rb * a.hk;
             } else {
                 for (int i0 = 0; i0 < n_rb && b < 0; i0 += 32) {
-                    const int n = i0 + lane < n_rb ? block_length(a, x, n_rb - 1 - i0 - lane) : 0;
+                    const int n = i0 + lane < n_rb ? block_length(t, x, n_rb - 1 - i0 - lane) : 0;
                     const int64_t v = (int64_t)n * a.hk, incl = warp_scan(v) + run;
                     const unsigned here = __ballot_sync(0xffffffffu, incl - v <= at && at < incl);
                     if (here) {
@@ -475,7 +482,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                 unit_run += (int64_t)n_rb * a.hk;
                 continue;
             }
-            const int row0 = b * TC_CTA_ROWS, row1 = last_row(x, a.group, b);
+            const int row0 = b << t.rows_log2, row1 = last_row(t, x, b);
             const Tiles all = tiles_of(a, x, row0, row1);
             // A piece is [v0, v1) of the unit's length; its own cost alone is none, and who begins
             // within it begins the unit.
@@ -508,7 +515,8 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
                     u->n_of[w] = nw;
                     n = max(n, nw);
                 }
-                if (u->alone()) {
+                u->alone = t.rows_log2 == 8 && row1 - row0 <= TC_ROWS;
+                if (u->alone) {
                     u->n_of[0] = (n + 1) / 2;
                     u->n_of[1] = n / 2;
                 }
@@ -555,6 +563,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     constexpr int ST = tc_stages<DP>();
     constexpr int TILE = tc_tile_bytes<DP>();
     constexpr int HALVES = DP / 64;                    // 128-byte column blocks
+    constexpr int UNIT = tc_rows<DP>();
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // The swizzle needs 1,024-byte alignment, which the array's alignment gives (there is
     // no room to round up to it); should it ever not, the call says so.
@@ -720,7 +729,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (!(ok = take(k))) break;
                 const Unit& u = ctl->unit[k & 1];
                 const int us = __shfl_sync(0xffffffffu, u.s, 0), n = __shfl_sync(0xffffffffu, u.n, 0);
-                const bool alone = u.alone();
+                const bool alone = u.alone;
                 const int n_of[2] = {__shfl_sync(0xffffffffu, u.n_of[0], 0), __shfl_sync(0xffffffffu, u.n_of[1], 0)};
                 // key tiles with rows that no row sees: found from the first and the last few
                 const int t0 = u.t0, sink_tiles = u.sink_tiles, first = u.first;
@@ -890,7 +899,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     if (lane == 0) mbar_expect_tx(&ctl->q_full, tc_q_bytes<DP>());
                     __syncwarp();
                     const int b = lane;
-                    if (b < TC_TILES * HALVES)
+                    if (b < UNIT / TC_ROWS * HALVES)
                         tma_load_q(q0 + b * (TC_ROWS * 128), &tmQ, &ctl->q_full, 64 * (b % HALVES), kvh * a.group,
                                    begin + a.by_group(row0) + (b / HALVES) * t.q_tokens);
                     continue;
@@ -937,7 +946,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const Unit& u = ctl->unit[k & 1];
             if (!(ok = take(k)) || u.s < 0) break;
             // (what the loop does not need is read from the unit again behind it: registers)
-            auto row = [&] { return 32 * (u.alone() ? warp & 3 : warp) + lane; };   // the thread's of the unit
+            auto row = [&] { return 32 * (u.alone ? warp & 3 : warp) + lane; };   // the thread's of the unit
             const int pos = row_pos(a, u.q, u.row0 + min(row(), u.rows - 1));
             float m = -INFINITY;
             uint64_t l2[2] = {pack_f2(0.0f, 0.0f), pack_f2(0.0f, 0.0f)};
@@ -949,7 +958,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
                 for (int c = 0; c < TC_KEYS; c += 32) tmem_ld_x32(ts + c, v + c);
                 tmem_wait_ld();
-                const int key0 = u.key0(u.alone() ? 2 * j + w : j), kv = u.q.kv;
+                const int key0 = u.key0(u.alone ? 2 * j + w : j), kv = u.q.kv;
                 const int pos_first = __shfl_sync(0xffffffffu, pos, 0), pos_last = __shfl_sync(0xffffffffu, pos, 31);
                 if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
                       (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
@@ -1012,7 +1021,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
             // ---- the rows' results
             const int n = u.n, nw = u.n_of[w], rows = u.rows, r = row();
-            const bool alone = u.alone();
+            const bool alone = u.alone;
             if (ok && n > 0) ok = wait_warp(&ctl->o_full, busy & 1, abort, t.wait_ns);
             if (!ok) break;
             tc_fence_after();
@@ -1041,7 +1050,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
             const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
-            float* pt = t.join.part + (int64_t)u.slot * TC_CTA_ROWS * (DP + 2);   // (pieces)
+            float* pt = t.join.part + (int64_t)u.slot * UNIT * (DP + 2);   // (pieces)
             if (whole_unit && l != 0.0f) {
                 const float inv = 1.0f / l;
                 s0 *= inv;
@@ -1076,7 +1085,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (!whole_unit) {   // [DP / 4][row][4]: neighbouring rows' quads are neighbours
 #pragma unroll
                     for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<uint4*>(pt + ((c0 + c) / 4 * TC_CTA_ROWS + r) * 4) =
+                        *reinterpret_cast<uint4*>(pt + ((c0 + c) / 4 * UNIT + r) * 4) =
                             make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
                     continue;
                 }
@@ -1102,8 +1111,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (live) {
                 if (!whole_unit) {
                     // an infinite maximum joins to NaN: the row is computed again there
-                    pt[TC_CTA_ROWS * DP + r] = fine ? top : INFINITY;
-                    pt[TC_CTA_ROWS * (DP + 1) + r] = l;
+                    pt[UNIT * DP + r] = fine ? top : INFINITY;
+                    pt[UNIT * (DP + 1) + r] = l;
                 } else if (a.lse) {
                     a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
                 }
@@ -1172,15 +1181,17 @@ hmm_status_t encode_map(CUtensorMap* m, void* base, int rank, const cuuint64_t* 
 }
 
 // Units: at most one more per sequence and head than its share of the tokens.
-int64_t most_units(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk) {
-    return (n_tokens * group / TC_CTA_ROWS + n_seq) * hk;
+int64_t most_units(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk, int64_t rows) {
+    return (n_tokens * group / rows + n_seq) * hk;
 }
 
 // Whether the units can be too few for whole ones (the tokens' row blocks are as many at
 // least, if no sequence is another kernel's).
-bool may_split(int64_t n_tokens, int64_t group, int64_t hk) {
-    return (n_tokens * group + TC_CTA_ROWS - 1) / TC_CTA_ROWS * hk < device_sm_count();
+bool may_split(int64_t n_tokens, int64_t group, int64_t hk, int64_t rows) {
+    return (n_tokens * group + rows - 1) / rows * hk < device_sm_count();
 }
+
+int unit_rows(int64_t D) { return D <= 128 ? tc_rows<128>() : tc_rows<256>(); }
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -1206,21 +1217,21 @@ hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, in
 }
 
 bool chunk_applies(const AttnArgs& a) {
-    return a.D <= 128 && box_rows_of(a.page_tokens, TC_KEYS) >= 8;
+    return box_rows_of(a.page_tokens, TC_KEYS) >= 8;
 }
 
 size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D) {
-    if (D > 128) return 0;
-    const int64_t group = std::max<int64_t>(1, n_heads / n_kv_heads), ctas = device_sm_count();
-    size_t n = up256(4 * (size_t)most_units(n_seq, n_tokens, group, n_kv_heads) * TC_SOFTMAX_WARPS);
-    if (may_split(n_tokens, group, n_kv_heads))
-        n += up256(2 * sizeof(int4) * ctas) + sizeof(float) * 2 * ctas * TC_CTA_ROWS * ((D <= 64 ? 64 : 128) + 2);
+    const int64_t group = std::max<int64_t>(1, n_heads / n_kv_heads), ctas = device_sm_count(), rows = unit_rows(D);
+    size_t n = up256(4 * (size_t)most_units(n_seq, n_tokens, group, n_kv_heads, rows) * TC_SOFTMAX_WARPS);
+    if (may_split(n_tokens, group, n_kv_heads, rows))
+        n += up256(2 * sizeof(int4) * ctas) +
+             sizeof(float) * 2 * ctas * rows * ((D <= 64 ? 64 : D <= 128 ? 128 : 256) + 2);
     return n;
 }
 
 hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, unsigned char* ws, cudaStream_t st,
                        ChunkJoin* join) {
-    const int64_t units = most_units(a.b.n_seq, a.b.n_tokens, a.group, a.hk);
+    const int64_t rows = unit_rows(a.D), units = most_units(a.b.n_seq, a.b.n_tokens, a.group, a.hk, rows);
     HMM_REQUIRE(units < (int64_t(1) << 30), "n_tokens * n_heads is too large for one call");
     unsigned char* joint = ws + up256(4 * (size_t)units * TC_SOFTMAX_WARPS);
     // A tile of 128 rows is a box of the queries where it is whole tokens; a negative scale
@@ -1230,17 +1241,18 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
                        a.q_head < (int64_t(1) << 40) && a.q_token < (int64_t(1) << 40);
     TcArgs t{};
     t.a = a;
+    t.rows_log2 = rows == 256 ? 8 : 7;
     t.min_rows = min_rows;
     t.box_rows = box_rows_of(a.page_tokens, TC_KEYS);
-    t.split = may_split(a.b.n_tokens, a.group, a.hk);
+    t.split = may_split(a.b.n_tokens, a.group, a.hk, rows);
     t.q_tokens = boxes ? TC_ROWS / a.group : 0;
     t.wait_ns = wait_limit_ns();
     t.again = (uint32_t*)ws;
     t.units = (int)units;
     if (t.split) {
-        const int64_t rows = std::min<int64_t>(TC_CTA_ROWS, (int64_t)a.b.n_tokens * a.group);
+        const int64_t most = std::min<int64_t>(rows, (int64_t)a.b.n_tokens * a.group);
         t.join = ChunkJoin{(int4*)joint, (float*)(joint + up256(2 * sizeof(int4) * device_sm_count())),
-                           device_sm_count(), (int)((rows + 15) / 16)};
+                           device_sm_count(), (int)((most + 15) / 16), (int)rows};
     }
     *join = t.join;
     CUtensorMap k, v, q{};
@@ -1259,8 +1271,11 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     if (a.D <= 64)
         return bf16 ? launch_chunk<__nv_bfloat16, 64>(t, k, v, q, behind, st)
                     : launch_chunk<__half, 64>(t, k, v, q, behind, st);
-    return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, q, behind, st)
-                : launch_chunk<__half, 128>(t, k, v, q, behind, st);
+    if (a.D <= 128)
+        return bf16 ? launch_chunk<__nv_bfloat16, 128>(t, k, v, q, behind, st)
+                    : launch_chunk<__half, 128>(t, k, v, q, behind, st);
+    return bf16 ? launch_chunk<__nv_bfloat16, 256>(t, k, v, q, behind, st)
+                : launch_chunk<__half, 256>(t, k, v, q, behind, st);
 }
 
 }  // namespace serve

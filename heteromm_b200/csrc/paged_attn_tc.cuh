@@ -31,17 +31,18 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-constexpr int TC_CTA_ROWS = 256;   // rows of a unit of the chunk kernel
+constexpr int TC_CTA_ROWS = 256;   // rows of a unit of the chunk kernel (D <= 128), at most
 
 // What the join needs of units that the chunk kernel cut into pieces.
 struct ChunkJoin {
     int4* joint;      // [ctas][2] unit begun in the CTA and ended in another: sequence, head, row block,
                       // pieces (0: none); the sequence's begin, n_new, kv
-    float* part;      // [ctas][2][TC_CTA_ROWS * (DP + 2)]: rows, then maxima, then sums
+    float* part;      // [ctas][2][rows * (DP + 2)]: rows, then maxima, then sums
     int ctas, groups; // CTAs, 16-row groups of a unit that there can be
+    int rows;         // of a unit
 };
 
-// Whether the kernel takes this head size and page size.
+// Whether the kernel takes this page size.
 bool chunk_applies(const AttnArgs& a);
 size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D);
 // Rows of every sequence with at least min_rows rows (n_new * group).  `behind`: the kernel

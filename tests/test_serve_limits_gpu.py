@@ -163,3 +163,29 @@ def test_wrappers_refuse(cuda):
         a.update(kw)
         with pytest.raises(exc):
             hmm.paged_kv_append(**a)
+
+
+@pytest.mark.parametrize("d,pt,dtype", [(256, 16, "bf16"), (200, 8, "fp16"), (136, 128, "bf16")])
+@pytest.mark.parametrize("new,kv,hq,hk", [
+    ([700, 1, 130, 0, 33], [900, 50, 4000, 7, 33], 6, 2),     # cut units
+    ([1500, 800], [1500, 2000], 16, 4),                       # whole ones
+    ([128, 129, 127, 17, 16], [128, 300, 127, 17, 400], 1, 1),
+])
+@pytest.mark.parametrize("window", [0, 300])
+def test_wide_heads(cuda, d, pt, dtype, new, kv, hq, hk, window):
+    """Heads of more than 128 values: units of 128 rows."""
+    run_case(cuda, 47, new, kv, hq, hk, d, pt, dtype, pad=2, window=window, sinks=5 if window else 0)
+
+
+def test_wide_heads_wait(cuda):
+    args = make(cuda, 48, [900, 300], [900, 1200], 8, 2, 256, 16, torch.float16)
+    want = hmm.paged_attention(*args)
+    _abi.set_wait_limit_ns(0)
+    try:
+        with pytest.raises(HmmError) as e:
+            hmm.paged_attention(*args)
+        assert e.value.status == HMM_ERR_TIMEOUT
+    finally:
+        torch.cuda.synchronize()
+        _abi.set_wait_limit_ns(-1)
+    assert torch.equal(hmm.paged_attention(*args), want)
