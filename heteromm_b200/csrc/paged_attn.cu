@@ -151,10 +151,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     // ---- this CTA's piece of the list of all units' tiles
     int64_t total = 0, own = 0;
-    for (int s = threadIdx.x; s < a.b.n_seq; s += RW_THREADS) {
-        const Load x = seq_load(r, load_seq(a.b, a.max_kv, s, a.status));
+    each_seq(a.b, a.max_kv, threadIdx.x, RW_THREADS, a.status, [&](const Seq& q) {
+        const Load x = seq_load(r, q);
         own += (int64_t)x.units * x.tiles;
-    }
+    });
     scan_incl(own, wt, &total);
     const int64_t per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     int64_t cur = blockIdx.x * per;
@@ -591,6 +591,10 @@ extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, cons
     if (!workspace || workspace_bytes < need)
         return set_error(HMM_ERR_OOM, "workspace too small: %zu < %zu", workspace_bytes, need);
     HMM_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+    const uintptr_t q0 = (uintptr_t)q, o0 = (uintptr_t)out;
+    HMM_REQUIRE(o0 >= q0 + 2 * (size_t)((batch->n_tokens - 1) * q_token + (n_heads - 1) * q_head + cache->D) ||
+                    q0 >= o0 + 2 * (size_t)(batch->n_tokens * n_heads * cache->D),
+                "out overlaps q");   // rows are read again where they come out not finite
     a.q = (const unsigned char*)q;
     a.q_token = 2 * q_token;
     a.q_head = 2 * q_head;

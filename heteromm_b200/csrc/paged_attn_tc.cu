@@ -368,8 +368,7 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     const int lane = threadIdx.x & 31;
     if (!t.split) return Plan{0, 0};
     int64_t units = 0;
-    for (int s = lane; s < a.b.n_seq; s += 32)
-        units += (int64_t)row_blocks(t, load_seq(a.b, a.max_kv, s, a.status)) * a.hk;
+    each_seq(a.b, a.max_kv, lane, 32, a.status, [&](const Seq& q) { units += (int64_t)row_blocks(t, q) * a.hk; });
     if (warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
     int longest = 0;

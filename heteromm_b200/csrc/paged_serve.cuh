@@ -42,18 +42,39 @@ struct Seq {
     bool ok;
 };
 
-__device__ __forceinline__ Seq load_seq(const Batch& b, int64_t max_kv, int s, int32_t* status) {
+__device__ __forceinline__ Seq check_seq(const Batch& b, int64_t max_kv, int begin, int end, int kv, int32_t* status) {
     Seq q;
-    q.begin = __ldg(b.cu + s);
-    const int end = __ldg(b.cu + s + 1);
-    q.kv = __ldg(b.kv_len + s);
-    q.n_new = end - q.begin;
+    q.begin = begin;
+    q.kv = kv;
+    q.n_new = end - begin;
     q.ok = q.begin >= 0 && end >= q.begin && end <= b.n_tokens && q.kv >= 0 && q.kv <= max_kv;
     if (!q.ok) {
         atomicOr(status, HMM_STATUS_BATCH_BOUNDS);
         q.begin = q.n_new = q.kv = 0;
     }
     return q;
+}
+
+__device__ __forceinline__ Seq load_seq(const Batch& b, int64_t max_kv, int s, int32_t* status) {
+    return check_seq(b, max_kv, __ldg(b.cu + s), __ldg(b.cu + s + 1), __ldg(b.kv_len + s), status);
+}
+
+// f(sequence) of every step-th sequence from s on, four sequences' loads in flight.
+template <typename F>
+__device__ __forceinline__ void each_seq(const Batch& b, int64_t max_kv, int s, int step, int32_t* status, F&& f) {
+    for (; s < b.n_seq; s += 4 * step) {
+        int begin[4], end[4], kv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = min(s + i * step, b.n_seq - 1);   // (65,535 sequences at most)
+            begin[i] = __ldg(b.cu + at);
+            end[i] = __ldg(b.cu + at + 1);
+            kv[i] = __ldg(b.kv_len + at);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i * step < b.n_seq) f(check_seq(b, max_kv, begin[i], end[i], kv[i], status));
+    }
 }
 
 // The last sequence s with cu[s] <= t, by one warp, 32 probes a step.  With a

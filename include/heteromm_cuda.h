@@ -390,7 +390,8 @@ hmm_status_t hmm_paged_kv_append(
  * Deterministic: the same call gives the same bits.
  *   q [n_tokens][n_heads][D] of the cache's type, 16-byte aligned, token and
  *   head strides in elements (multiples of 8); out [n_tokens][n_heads][D] of
- *   the same type, contiguous, 16-byte aligned; lse [n_tokens][n_heads] fp32 or NULL
+ *   the same type, contiguous, 16-byte aligned, not overlapping q; lse
+ *   [n_tokens][n_heads] fp32 or NULL
  *   max_new: a bound on the new tokens of any sequence, or 0 for none known; it
  *   chooses between kernels and never changes which rows are computed
  * D % 8 == 0, 8 <= D <= 256; at least one page, strides of dimensions longer

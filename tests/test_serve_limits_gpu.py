@@ -95,6 +95,26 @@ def test_a_batch_of_thousands(cuda):
     run_case(cuda, 44, new, kv, 2, 1, 64, 16, "bf16")
 
 
+def test_nothing_to_attend_to(cuda):
+    """No tokens, no sequences, no room: outputs as the formula has them, or untouched."""
+    q, k, v, table, cu, kv_len = make(cuda, 49, [3, 2], [20, 9], 4, 2, 64, 16, torch.bfloat16)
+    none = torch.zeros_like(cu)
+    assert hmm.paged_attention(q[:0], k, v, table, none, kv_len).shape == (0, 4, 64)
+    out = torch.full_like(q, 5.0)
+    hmm.paged_attention(q, k, v, table, none, kv_len, out=out)                      # no new tokens
+    hmm.paged_attention(q, k, v, table[:0], cu[:1], kv_len[:0], out=out)            # no sequences
+    assert (out == 5.0).all()
+    got, lse = hmm.paged_attention(q, k, v, table[:, :0].contiguous(), cu, torch.zeros_like(kv_len), return_lse=True)
+    assert (got == 0).all() and (lse == -np.inf).all()                              # nothing cached
+    assert hmm.paged_kv_append(q[:0], k[:0, :, 0], v[:0, :, 0], k, v, table, none, kv_len).shape == (0, 4, 64)
+
+
+def test_a_thousand_sequences(cuda):
+    new = [1] * 1000 + [300] + [0] * 30
+    kv = [(37 * i) % 90 + 1 for i in range(1000)] + [500] + [3] * 30
+    run_case(cuda, 50, new, kv, 4, 1, 128, 16, "bf16")
+
+
 def test_two_threads_on_two_streams(cuda):
     cases = [make(cuda, 45 + i, new, kv, 8, 2, 128, 16, torch.bfloat16)
              for i, (new, kv) in enumerate((([300, 2], [900, 700]), ([1] * 20, list(range(50, 1050, 50)))))]

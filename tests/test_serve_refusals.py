@@ -120,6 +120,14 @@ def test_bad_attention(kw, text):
     refused(attend(**kw), text)
 
 
+def test_out_over_q():
+    """Default calls here have out = q, which is refused last; rows of out would be read."""
+    refused(attend(), "overlaps")
+    span = (4 * 256 + 3 * 64 + 64) * 2                 # bytes of q
+    refused(attend(out=P + span - 16), "overlaps")
+    refused(attend(out=P - 5 * 4 * 64 * 2 + 16), "overlaps")
+
+
 def test_attention_workspace():
     lib = hmm.load()
     need = lib.hmm_paged_attention_workspace_size(2, 5, 4, 2, 64)
