@@ -398,7 +398,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             return *reinterpret_cast<const float4*>(jm + (w * RW_ROWS + row) * MR + 4 * c);
         };
         if (t0 == 0 && t1 == ld.tiles) {
-            finish_rows<T>(a, s, q, kvh, row0, rows, RW_WARPS, stat, value, jst + 2 * RW_WARPS * RW_ROWS, &again);
+            finish_rows<T, false>(a, s, q, kvh, row0, rows, RW_WARPS, stat, value, jst + 2 * RW_WARPS * RW_ROWS, &again);
         } else {
             float* part = r.w.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * RW_ROWS * (DP + 2);
             for (int i = threadIdx.x; i < rows * (DP / 4); i += RW_THREADS) {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_con
     if (left <= 0) return;
     const int64_t size = (int64_t)rows * (j.dp + 2);
     const float* part = (few ? j.rows.part : j.chunk.part) + c * 2 * size;
-    finish_rows<T>(j.a, u.x, q, u.y, row0, (int)min((int64_t)16, left), u.w,
+    finish_rows<T, true>(j.a, u.x, q, u.y, row0, (int)min((int64_t)16, left), u.w,
                    [&](int i, int row, int k) {
                        return part[(2 * i + (i == 0)) * size + rows * (j.dp + k) + r0 + row];
                    },

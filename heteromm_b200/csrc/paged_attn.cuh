@@ -141,18 +141,68 @@ __device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const S
         a.lse[(int64_t)tok * a.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+// The joined rows' values: K quads a thread and P pieces at a time, K * P reads in flight.
+#ifndef PF
+#define PF 8
+#endif
+template <typename T, int K, int P, typename Value>
+__device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int kvh, int row0, int rows, int pieces,
+                                            Value value, const float* top, int* again) {
+    const int quads = a.D / 4, all = rows * quads;
+    for (int i0 = threadIdx.x; i0 < all; i0 += K * blockDim.x) {
+        float4 x[K];
+        int row[K], col[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = min(i0 + k * (int)blockDim.x, all - 1);
+            row[k] = i / quads;
+            col[k] = i - row[k] * quads;
+            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        for (int p0 = 0; p0 < pieces; p0 += P) {
+            float4 v[K][P];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int p = 0; p < P; ++p) v[k][p] = value(min(p0 + p, pieces - 1), row[k], col[k]);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const float w = p0 + p < pieces ? top[row[k] * pieces + p0 + p] : 0.0f;
+                    if (w != 0.0f) {
+                        x[k].x = fmaf(w, v[k][p].x, x[k].x); x[k].y = fmaf(w, v[k][p].y, x[k].y);
+                        x[k].z = fmaf(w, v[k][p].z, x[k].z); x[k].w = fmaf(w, v[k][p].w, x[k].w);
+                    }
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (i0 + k * (int)blockDim.x >= all) continue;
+            if (!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w))
+                atomicOr(again, 1 << row[k]);
+            const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
+            *reinterpret_cast<uint2*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + 4 * col[k])) =
+                make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
+        }
+    }
+}
+
 // Joins (maximum, sum, row) pieces of up to 16 rows, which several warps or CTAs summed
 // over different keys, in their order, and writes the rows out; rows that come out not
 // finite are computed again by attn_row_exact.  stat(i, row, k) reads piece i's maximum
 // (k = 0) or sum (1), value(i, row, c) its columns 4 c ... 4 c + 3; `share` holds
-// 32 x pieces floats.  Whole block, 128 threads: all reads of a step are issued at once.
-template <typename T, typename Stat, typename Value>
+// 32 x pieces floats.  Whole block, 128 threads.  FAR: the pieces lie in memory, many of
+// them maybe, and their reads' latency is what it costs (one token over 4,000, 31 pieces:
+// two at a time 14 us, sixteen 4).
+template <typename T, bool FAR, typename Stat, typename Value>
 __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
                                             int rows, int pieces, Stat stat, Value value, float* share,
                                             int* again) {
     if (threadIdx.x == 0) *again = 0;
     float* top = share;                 // [row][piece] maxima, then the pieces' shares of the row
     float* sum = share + 16 * pieces;
+#pragma unroll 4
     for (int i = threadIdx.x; i < rows * pieces; i += blockDim.x) {
         const int r = i / pieces, p = i - r * pieces;
         top[i] = stat(p, r, 0);
@@ -190,45 +240,8 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         }
     }
     __syncthreads();
-    // four quads a thread and two pieces at a time: eight reads in flight
-    const int quads = a.D / 4, all = rows * quads;
-    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * blockDim.x) {
-        float4 x[4];
-        int row[4], col[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = min(i0 + k * (int)blockDim.x, all - 1);
-            row[k] = i / quads;
-            col[k] = i - row[k] * quads;
-            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        for (int p0 = 0; p0 < pieces; p0 += 2) {
-            float4 v[4][2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) v[k][p] = value(min(p0 + p, pieces - 1), row[k], col[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const float w = p0 + p < pieces ? top[row[k] * pieces + p0 + p] : 0.0f;
-                    if (w != 0.0f) {
-                        x[k].x = fmaf(w, v[k][p].x, x[k].x); x[k].y = fmaf(w, v[k][p].y, x[k].y);
-                        x[k].z = fmaf(w, v[k][p].z, x[k].z); x[k].w = fmaf(w, v[k][p].w, x[k].w);
-                    }
-                }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (i0 + k * (int)blockDim.x >= all) continue;
-            if (!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w))
-                atomicOr(again, 1 << row[k]);
-            const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
-            *reinterpret_cast<uint2*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + 4 * col[k])) =
-                make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
-        }
-    }
+    if (FAR && rows * (a.D / 4) <= (int)blockDim.x) join_values<T, 1, PF>(a, q, kvh, row0, rows, pieces, value, top, again);
+    else join_values<T, 4, 2>(a, q, kvh, row0, rows, pieces, value, top, again);
     __syncthreads();
     const int bits = *again;
     for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
