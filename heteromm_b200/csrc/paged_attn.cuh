@@ -142,9 +142,6 @@ __device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const S
 }
 
 // The joined rows' values: K quads a thread and P pieces at a time, K * P reads in flight.
-#ifndef PF
-#define PF 8
-#endif
 template <typename T, int K, int P, typename Value>
 __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int kvh, int row0, int rows, int pieces,
                                             Value value, const float* top, int* again) {
@@ -194,7 +191,7 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 // (k = 0) or sum (1), value(i, row, c) its columns 4 c ... 4 c + 3; `share` holds
 // 32 x pieces floats.  Whole block, 128 threads.  FAR: the pieces lie in memory, many of
 // them maybe, and their reads' latency is what it costs (one token over 4,000, 31 pieces:
-// two at a time 14 us, sixteen 4).
+// the call took 25 us with two at a time, 17 with eight; sixteen gave no more).
 template <typename T, bool FAR, typename Stat, typename Value>
 __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
                                             int rows, int pieces, Stat stat, Value value, float* share,
@@ -240,8 +237,10 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         }
     }
     __syncthreads();
-    if (FAR && rows * (a.D / 4) <= (int)blockDim.x) join_values<T, 1, PF>(a, q, kvh, row0, rows, pieces, value, top, again);
-    else join_values<T, 4, 2>(a, q, kvh, row0, rows, pieces, value, top, again);
+    if (FAR && rows * (a.D / 4) <= (int)blockDim.x)
+        join_values<T, 1, 8>(a, q, kvh, row0, rows, pieces, value, top, again);
+    else
+        join_values<T, 4, 2>(a, q, kvh, row0, rows, pieces, value, top, again);
     __syncthreads();
     const int bits = *again;
     for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
