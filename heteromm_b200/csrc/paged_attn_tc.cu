@@ -39,7 +39,7 @@
 // Bound: 4 D FLOP per (row, key) on the tensor cores, 2,048 clocks for the two row
 // tiles and a key tile at D = 128, and as many for their exponentials on the
 // special-function units, 16 a clock.  Measured, 32 query and 8 KV heads, 8,192
-// tokens, causal: D = 128 465-478 us (1,150-1,180 TFLOP/s, about 4,000 clocks a
+// tokens, causal: D = 128 455-478 us (1,150-1,210 TFLOP/s, about 4,000 clocks a
 // tile); without the exponentials it is no faster, with the products and loads
 // alone 418: reading K and V into shared memory, 64 KB a tile and CTA, and their
 // reading by both row tiles' products bound it.  D = 64 424 us (650 TFLOP/s): the
