@@ -391,7 +391,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 dst[8 * d + 1] = o[d][2 * h + 1];
             }
             if ((lane & 3) == 0) {
-                jst[warp * RW_ROWS + row] = m[h];
+                // fmaxf drops NaN, the sum keeps it: with an infinite maximum the row's share of
+                // every join is NaN, so that a NaN score shows in the result
+                jst[warp * RW_ROWS + row] = l[h] == l[h] ? m[h] : INFINITY;
                 jst[(RW_WARPS + warp) * RW_ROWS + row] = l[h];
             }
         }

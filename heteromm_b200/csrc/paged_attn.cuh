@@ -189,7 +189,8 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 // over different keys, in their order, and writes the rows out; rows that come out not
 // finite are computed again by attn_row_exact.  stat(i, row, k) reads piece i's maximum
 // (k = 0) or sum (1), value(i, row, c) its columns 4 c ... 4 c + 3; `share` holds
-// 32 x pieces floats.  Whole block, 128 threads.  FAR: the pieces lie in memory, many of
+// 32 x pieces floats.  A piece with a score of NaN or +inf has a maximum of +inf (and no
+// other has: a sum with it is NaN).  Whole block, 128 threads.  FAR: the pieces lie in memory, many of
 // them maybe, and their reads' latency is what it costs (one token over 4,000, 31 pieces:
 // the call took 25 us with two at a time, 17 with eight; sixteen gave no more).
 template <typename T, bool FAR, typename Stat, typename Value>
@@ -218,7 +219,7 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         for (int p = t; live && p < pieces; p += 8) {
             const float w = ex2(top[r * pieces + p] - ms);
             top[r * pieces + p] = w;
-            if (w != 0.0f) l = fmaf(w, sum[r * pieces + p], l);   // (0: a piece in which the row saw nothing)
+            if (w != 0.0f) l = fmaf(w, sum[r * pieces + p], l);   // (0: nothing seen in the piece, or nothing beside the others)
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);

@@ -382,7 +382,8 @@ hmm_status_t hmm_paged_kv_append(
  * i <= p; with a window > 0 (causal only) i > p - window or i < sinks (a few
  * first tokens that stay visible).  A token that sees no key (kv_len 0, or
  * fewer cached than new tokens) gives zeros and lse -inf, as does one whose
- * every score is -inf.  Keys and values that a token does not see never reach
+ * every score is -inf; a seen score of NaN or +inf gives NaN in out and lse.
+ * Keys and values that a token does not see never reach
  * its result, NaN and infinities included; page-table entries are read only
  * for pages that hold a seen key, so pages behind a window may be gone.
  * Query head h reads KV head h / (n_heads / n_kv_heads).  fp32 scores, softmax

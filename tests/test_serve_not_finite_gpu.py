@@ -1,0 +1,92 @@
+"""paged_attention where scores are not finite: a NaN in a query or in keys that a row
+sees is NaN in its result, in both kernels, whole units and joined pieces alike."""
+import numpy as np
+import pytest
+import torch
+
+import heteromm_b200 as hmm
+from test_serve_attention_gpu import DT, check, make, reference
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+
+BATCHES = [  # new, kv, hq, hk, d, pt
+    ([1, 1, 1, 1], [1, 17, 50, 64], 8, 2, 128, 16),       # rows kernel: a CTA has all of a unit
+    ([1, 1, 3], [33, 4000, 97], 16, 8, 64, 16),           # pieces of several CTAs
+    ([1], [2049], 4, 1, 256, 16),
+    ([5, 1], [700, 65], 6, 2, 80, 5),                     # pages that only the rows kernel takes, joined
+    ([40, 1, 130], [50, 1, 900], 8, 2, 128, 16),          # both kernels, the chunk kernel's units cut
+    ([300], [333], 16, 4, 64, 64),
+    ([2600, 700], [2600, 2049], 16, 8, 128, 16),          # whole units
+]
+
+
+def poison(kind, q, k, table, new, kv, pt):
+    """NaN scores of some rows of every sequence; returns nothing, changes q or k."""
+    first = 0
+    for s, (n, L) in enumerate(zip(new, kv)):
+        if kind == "a query":                     # one head of the last token
+            q[first + n - 1, -1, 3] = NAN
+        elif kind == "all queries":
+            q[first:first + n] = NAN
+        elif kind == "all keys":
+            k[table[s, :-(-L // pt)].long()] = NAN
+        elif kind == "a page":
+            k[table[s, (L - 1) // pt // 2].item()] = NAN
+        elif kind == "16 keys":                   # a warp's share of a tile, whatever the page size
+            for p in range(16, min(32, L)):
+                k[table[s, p // pt].item(), :, p % pt] = NAN
+        elif kind == "newest key":
+            k[table[s, (L - 1) // pt].item(), :, (L - 1) % pt, 0] = NAN
+        elif kind == "inf - inf":                 # keys that overflowed: products of both signs
+            k[table[s, (L - 1) // pt].item(), 0, (L - 1) % pt] = INF
+        first += n
+
+
+@pytest.mark.parametrize("kind", ["a query", "all queries", "all keys", "a page", "16 keys", "newest key", "inf - inf"])
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_nan_scores(cuda, batch, kind, dtype):
+    new, kv = batch[:2]
+    q, k, v, table, cu, kv_len = make(cuda, 60, *batch, DT[dtype])
+    poison(kind, q, k, table, new, kv, batch[5])
+    ref = reference(q, k, v, table, new, kv)
+    assert torch.isnan(ref[0]).any()
+    out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, return_lse=True)
+    check(out, lse, ref)
+    assert torch.equal(torch.isnan(lse).double(), torch.isnan(ref[1]).double())
+    hint = hmm.paged_attention(q, k, v, table, cu, kv_len, max_new=1)        # the rows kernel, however many rows
+    check(hint, None, ref)
+
+
+@pytest.mark.parametrize("at", [0, 15, 16, 48, 63, 64, 1000])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_nan_key_at_any_place_of_a_tile(cuda, at, window):
+    """The newest key, which is the only one that a warp sees at the start of its 16 keys."""
+    batch = ([1, 2, 40], [at + 1, at + 2, at + 40], 8, 2, 128, 16)
+    new, kv = batch[:2]
+    q, k, v, table, cu, kv_len = make(cuda, 61, *batch, torch.bfloat16)
+    for s in range(3):
+        k[table[s, at // 16].item(), :, at % 16] = NAN
+    kw = dict(window=window, sinks=3 if window else 0)
+    ref = reference(q, k, v, table, new, kv, **kw)
+    out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, return_lse=True, **kw)
+    check(out, lse, ref)
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+
+
+def test_infinite_scores_of_few_rows(cuda):
+    """+inf is NaN, -inf a weight of zero, only -inf zeros: the rows kernel as the formula."""
+    new, kv, d = [1, 1, 1, 2], [100, 40, 2000, 33], 64
+    q, k, v, table, cu, kv_len = make(cuda, 62, new, kv, 2, 1, d, 16, torch.bfloat16)
+    q = q.abs() + 0.1
+    k[table[0, 3].item(), 0, 5] = INF
+    k[table[1, :3].long()] = -INF
+    k[table[2, 100].item()] = -INF
+    k[table[3, :2].long()] = -INF
+    ref = reference(q, k, v, table, new, kv)
+    out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, return_lse=True)
+    check(out, lse, ref)
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+    assert (out[1] == 0).all() and (lse[1] == -np.inf).all() and torch.isfinite(out[2]).all()
