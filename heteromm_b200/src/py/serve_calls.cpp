@@ -364,6 +364,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (a[8] != Py_None) {
         const Tensor& r = dense(a[8], "rope", at::kFloat, c.dev);
         if (r.dim() != 3 || r.size(2) != 2) throw value_error("rope must be [n_pos, pairs, 2]");
+        // (an array of nothing has no address, which would read as no rotation)
+        if (r.numel() == 0 && n_tokens > 0) throw value_error("rope is empty; None is no rotation");
         rope = (const float*)r.data_ptr();
         n_pos = r.size(0);
         rotary = 2 * r.size(1);
