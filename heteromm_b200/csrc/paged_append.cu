@@ -21,6 +21,7 @@
 // (rotary_dim a multiple of 16), or goes through shared memory.  A lane's angles
 // are the same for every head.  Everything is computed in fp32 and rounded once.
 #include <algorithm>
+#include <cstdlib>
 
 #include "paged_serve.cuh"
 
@@ -397,6 +398,48 @@ hmm_status_t launch_append(const AppendArgs& a, int mode, cudaStream_t st) {
     return check_launch("paged_append_kernel");
 }
 
+// Rows of n tokens as a call lays them out: `bytes` at p + i token + j head.
+struct Laid {
+    int64_t p, token, head, heads;
+    int64_t extent(int64_t bytes) const { return (heads - 1) * head + bytes; }
+};
+
+// Whether rows `d` bytes apart share a byte for some pair of n tokens, `token` bytes apart.
+bool tokens_meet(int64_t d, int64_t token, int64_t n, int64_t bytes) {
+    if (n == 1 || token == 0) return std::abs(d) < bytes;
+    const int64_t down = d / token - (d % token < 0), rest = d - down * token;   // d = down * token + rest
+    return (rest < bytes && std::abs(down) < n) || (token - rest < bytes && std::abs(down + 1) < n);
+}
+
+// Whether a's rows share a byte with b's.  Heads of one projection's tokens (one token
+// stride) are told apart; rows of other strides whose ranges overlap are taken to meet.
+bool rows_meet(const Laid& a, const Laid& b, int64_t n, int64_t bytes) {
+    if (a.heads == 0 || b.heads == 0) return false;
+    if (a.p + (n - 1) * a.token + a.extent(bytes) <= b.p || b.p + (n - 1) * b.token + b.extent(bytes) <= a.p)
+        return false;
+    if (n > 1 && a.token != b.token) return true;
+    const int64_t d = b.p - a.p;
+    if (n > 1 && a.token > 0) {   // b's heads behind a's, within a token
+        const int64_t rest = (d % a.token + a.token) % a.token;
+        if (rest >= a.extent(bytes) && rest + b.extent(bytes) <= a.token) return false;
+    }
+    if (a.heads * b.heads > (1 << 20)) return true;
+    for (int64_t i = 0; i < a.heads; ++i)
+        for (int64_t j = 0; j < b.heads; ++j)
+            if (tokens_meet(d + j * b.head - i * a.head, a.token, n, bytes)) return true;
+    return false;
+}
+
+// Whether two of a's own rows share a byte.
+bool rows_meet_themselves(const Laid& a, int64_t n, int64_t bytes) {
+    if (a.heads == 0) return false;
+    if ((a.heads == 1 || a.head >= bytes) && (n == 1 || a.token >= a.extent(bytes))) return false;
+    if (n > 1 && a.token < bytes) return true;
+    for (int64_t j = 1; j < a.heads; ++j)
+        if (tokens_meet(j * a.head, a.token, n, bytes)) return true;
+    return false;
+}
+
 }  // namespace
 }  // namespace serve
 }  // namespace hmm
@@ -434,6 +477,19 @@ extern "C" hmm_status_t hmm_paged_kv_append(
     for (int64_t x : st)
         HMM_REQUIRE(x >= 0 && x % 8 == 0, "row strides must be multiples of 8 elements, got %lld",
                     (long long)x);
+    if (n_heads > 0) {
+        // Warps read rows steps ahead of those that they write, in no order: q_out's rows are
+        // q's own, each at its place, or nobody's.
+        const int64_t n = batch->n_tokens, bytes = 2 * cache->D;
+        const Laid lo{(int64_t)q_out, 2 * out_token, 2 * out_head, n_heads};
+        const bool is_q = q_out == q && (n == 1 || out_token == q_token) && (n_heads == 1 || out_head == q_head);
+        HMM_REQUIRE(!rows_meet_themselves(lo, n, bytes), "rows of q_out overlap one another");
+        HMM_REQUIRE(is_q || !rows_meet(lo, {(int64_t)q, 2 * q_token, 2 * q_head, n_heads}, n, bytes),
+                    "q_out overlaps q, and is not q itself");
+        HMM_REQUIRE(!rows_meet(lo, {(int64_t)k, 2 * k_token, 2 * k_head, cache->n_kv_heads}, n, bytes) &&
+                        !rows_meet(lo, {(int64_t)v, 2 * v_token, 2 * v_head, cache->n_kv_heads}, n, bytes),
+                    "q_out overlaps k or v");
+    }
     a.q = Rows{(unsigned char*)const_cast<void*>(q), 2 * q_token, 2 * q_head};
     a.k = Rows{(unsigned char*)const_cast<void*>(k), 2 * k_token, 2 * k_head};
     a.v = Rows{(unsigned char*)const_cast<void*>(v), 2 * v_token, 2 * v_head};

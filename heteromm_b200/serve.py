@@ -78,7 +78,8 @@ def paged_kv_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     """The step before attention in one pass: RMS norm of each query and key head (with
     q_weight, k_weight [D], fp32 or the cache's type), rotation of their first
     2 * rope.shape[1] values by rope [n_pos, pairs, 2] fp32 (cos, sin), and the store of
-    keys and values into the cache.  Returns the queries (in `out`, which may be q).
+    keys and values into the cache.  Returns the queries (in `out`, which may be q, or rows
+    that overlap neither q nor k nor v).
 
     q [n_tokens, n_heads, D] (or None: keys and values alone), k, v
     [n_tokens, n_kv_heads, D], views of one projection included.  Pairs are halves

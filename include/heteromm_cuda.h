@@ -358,9 +358,11 @@ typedef struct {
  * [D] fp32 or of the cache's type, NULL = no norm), position rotation of their
  * first rotary_dim values, and the store of keys and values at the tokens'
  * positions in the cache.  Computed in fp32, rounded once.
- *   q [n_tokens][n_heads][D] -> q_out (q itself is allowed; n_heads = 0 for
- *   none), k, v [n_tokens][n_kv_heads][D], all of the cache's type, 16-byte
- *   aligned, with token and head strides in elements (multiples of 8)
+ *   q [n_tokens][n_heads][D] -> q_out (n_heads = 0 for none), k, v
+ *   [n_tokens][n_kv_heads][D], all of the cache's type, 16-byte aligned, with
+ *   token and head strides in elements (multiples of 8).  q_out is q itself, at
+ *   the same strides, or shares no row with q, k, v and itself (heads of one
+ *   projection are told apart; rows of different token strides may not interleave)
  *   rope [n_pos][rotary_dim / 2][2] fp32 (cos, sin), 8-byte aligned, or NULL:
  *   no rotation; pair i is values (i, i + rotary_dim / 2), or with
  *   `interleaved` (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin)
