@@ -18,6 +18,7 @@
 // page data moves once through registers (read + write), which HBM bounds:
 // 16 bytes a thread, four loads in flight, 8 blocks per SM.
 #include <algorithm>
+#include <initializer_list>
 
 #include "paged_serve.cuh"
 
@@ -549,6 +550,32 @@ hmm_status_t check_state(const hmm_paged_state_t* st, bool with_kv, void* ws, si
     return HMM_OK;
 }
 
+struct Span {
+    const void* p;
+    size_t bytes;
+    bool meets(const Span& o) const {
+        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
+        return bytes > 0 && o.bytes > 0 && a < b + o.bytes && b < a + bytes;
+    }
+};
+
+// The last check of a call.  Both launches read the old state and the call's vectors, and
+// rely on finding the same: a new array is the old one itself, or apart from all of them
+// (`more`: another output, null if there is none).
+hmm_status_t check_apart(const State& s, std::initializer_list<Span> read, Span more = {}) {
+    const size_t size[3] = {4 * (size_t)s.n_seq * s.pps, 4 * (size_t)s.n_pages, s.kv ? 4 * (size_t)s.n_seq : 0};
+    const Span in[3] = {{s.table_in, size[0]}, {s.refs_in, size[1]}, {s.kv_in, size[2]}};
+    const Span out[4] = {{s.table, size[0]}, {s.refs, size[1]}, {s.kv, size[2]}, more};
+    for (int x = 0; x < 4; ++x) {
+        for (int y = 0; y < 3; ++y)
+            HMM_REQUIRE(!out[x].meets(in[y]) || (x == y && out[x].p == in[y].p),
+                        "a new array overlaps an old one, and is not that one itself");
+        for (int y = 0; y < x; ++y) HMM_REQUIRE(!out[x].meets(out[y]), "the new arrays overlap");
+        for (const Span& r : read) HMM_REQUIRE(!out[x].meets(r), "a new array overlaps what the call reads");
+    }
+    return HMM_OK;
+}
+
 hmm_status_t check_store(const hmm_page_store_t* st, Store* p) {
     HMM_REQUIRE(st, "null store");
     HMM_REQUIRE(st->n_pages >= 0 && st->n_pages < (int64_t(1) << 31), "n_pages must be in [0, 2^31)");
@@ -632,6 +659,8 @@ extern "C" hmm_status_t hmm_paged_free(const hmm_paged_state_t* state, const int
     if (e != HMM_OK) return e;
     HMM_REQUIRE(n >= 0 && n < (int64_t(1) << 31), "n must be in [0, 2^31), got %lld", (long long)n);
     HMM_REQUIRE(device_status && (n == 0 || seqs), "null seqs or device_status");
+    e = check_apart(s, {{seqs, 4 * (size_t)n}});
+    if (e != HMM_OK) return e;
     const cudaStream_t st = (cudaStream_t)stream;
     if (s.table != s.table_in || s.refs != s.refs_in || s.kv != s.kv_in) {
         e = state_pass<OP_COPY_STATE>(s, w, 1, nullptr, nullptr, 0, st);
@@ -660,6 +689,8 @@ extern "C" hmm_status_t hmm_paged_fork(const hmm_paged_state_t* state, const hmm
                 "page_tokens must be >= 1 and pages_per_seq * page_tokens < 2^31");
     HMM_REQUIRE(n >= 0 && n <= 65535, "n must be in [0, 65535], got %lld", (long long)n);
     HMM_REQUIRE(device_status && (n == 0 || (src && dst)), "null src, dst or device_status");
+    e = check_apart(s, {{src, 4 * (size_t)n}, {dst, 4 * (size_t)n}});
+    if (e != HMM_OK) return e;
     const cudaStream_t st = (cudaStream_t)stream;
     e = state_pass<OP_FORK>(s, w, page_tokens, src, dst, (int)n, st);
     if (e != HMM_OK || n == 0) return e;
@@ -680,6 +711,10 @@ extern "C" hmm_status_t hmm_paged_grow(const hmm_paged_state_t* state, int64_t p
                     state->pages_per_seq * page_tokens < (int64_t(1) << 31),
                 "page_tokens must be >= 1 and pages_per_seq * page_tokens < 2^31");
     HMM_REQUIRE(device_status && (s.n_seq == 0 || n_new), "null n_new or device_status");
+    // (lengths that double in place: a row's block reads its own number, then writes it)
+    const bool doubles = n_new == s.kv && s.kv == s.kv_in;
+    e = check_apart(s, {{n_new, doubles ? 0 : 4 * (size_t)s.n_seq}});
+    if (e != HMM_OK) return e;
     const cudaStream_t st = (cudaStream_t)stream;
     e = state_pass<OP_GROW>(s, w, page_tokens, n_new, nullptr, 0, st);
     if (e != HMM_OK || s.n_seq == 0) return e;
@@ -700,6 +735,8 @@ extern "C" hmm_status_t hmm_paged_compact(const hmm_paged_state_t* state, const 
     HMM_REQUIRE(store->n_pages == state->n_pages, "the store has %lld pages, the state %lld",
                 (long long)store->n_pages, (long long)state->n_pages);
     HMM_REQUIRE(out_live && device_status, "null out_live or device_status");
+    e = check_apart(s, {}, {out_live, 4});
+    if (e != HMM_OK) return e;
     const cudaStream_t st = (cudaStream_t)stream;
     if (s.n_pages == 0) {
         HMM_CUDA_TRY(cudaMemsetAsync(out_live, 0, sizeof(int32_t), st));

@@ -123,7 +123,8 @@ def paged_free(page_table: torch.Tensor, refs: torch.Tensor, kv_len: torch.Tenso
                seqs: torch.Tensor, *, out=None, status: torch.Tensor | None = None):
     """Frees the sequences of `seqs` (int32; one listed twice is freed once): their pages
     lose a reference each, their rows become -1 and their lengths 0.  Returns the new
-    (page_table, refs, kv_len): new tensors, or `out`, which may be the old ones."""
+    (page_table, refs, kv_len): new tensors, or `out`, each of which may be the old one
+    itself (or is apart from all that the call reads)."""
     return _calls.free(page_table, refs, kv_len, seqs, out, status)
 
 

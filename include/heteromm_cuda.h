@@ -411,7 +411,8 @@ hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged
 /* Page management.  The state is the page table [n_seq][pages_per_seq] (an
  * entry below 0 holds no page), the references [n_pages] of each page (0 =
  * free) and kv_len [n_seq].  Every call reads the state from *_in and writes
- * the whole new state to *_out; the two may be the same arrays (in place).
+ * the whole new state to *_out; each of these is the old array itself (in
+ * place), or apart from all that the call reads and writes.
  * New pages are always the lowest free ones.  A request that cannot be met as
  * a whole - a sequence number or length out of bounds, too few free pages -
  * sets its status bit and leaves the state (and the pages) as they were.

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 import heteromm_b200 as hmm
-from test_serve_refusals import P, batch, cache, refused
+from test_serve_refusals import P, batch, cache, refused, state, store
 
 FAR = 1 << 30
 
@@ -52,3 +52,53 @@ def test_out_over_keys_or_values(kw):
 ])
 def test_out_over_itself(kw):
     refused(append(out=P + 3 * FAR, **kw), "overlap")
+
+
+T, R, L, V = P, P + FAR, P + 2 * FAR, P + 3 * FAR        # table, references, lengths, vectors
+NEW = 8 * FAR                                            # the new state: apart
+
+
+def apart(**kw):
+    d = dict(table_in=T, refs_in=R, kv_len_in=L, table_out=T + NEW, refs_out=R + NEW, kv_len_out=L + NEW)
+    d.update(kw)
+    return state(**d)
+
+
+STATES = [   # [2][4] entries, 8 references, 2 lengths
+    dict(table_out=T + 16), dict(table_out=T - 28), dict(refs_out=R + 4), dict(refs_out=R - 28), dict(table_out=R),
+    dict(table_out=R + 28), dict(refs_out=T), dict(table_out=R + NEW - 4), dict(refs_out=T + NEW),
+    dict(table_out=T, refs_out=T + 28),
+]
+LENGTHS = [
+    dict(kv_len_out=L + 4), dict(kv_len_out=L - 4), dict(kv_len_out=T), dict(kv_len_out=R + 28), dict(table_out=L),
+    dict(refs_out=L + 4), dict(kv_len_out=T + NEW + 28), dict(kv_len_out=R + NEW),
+]
+VECTORS = [  # three numbers at V
+    dict(table_out=V - 28), dict(table_out=V + 8), dict(refs_out=V), dict(kv_len_out=V + 8), dict(kv_len_out=V - 4),
+    dict(table_out=V, table_in=V),
+]
+BIG = 1 << 30
+
+
+@pytest.mark.parametrize("change", STATES + LENGTHS + VECTORS)
+def test_states_that_overlap(change):
+    lib, st = hmm.load(), apart(**change)
+    refused(lib.hmm_paged_free(C.byref(st), V, 3, P, P, BIG, None), "overlap")
+    refused(lib.hmm_paged_fork(C.byref(st), C.byref(store()), 16, V, V, 3, P, P, BIG, None), "overlap")
+    if change not in (dict(table_out=V + 8), dict(kv_len_out=V + 8)):      # (two numbers here)
+        refused(lib.hmm_paged_grow(C.byref(st), 16, V, P, P, BIG, None), "overlap")
+    if change in STATES:
+        refused(lib.hmm_paged_compact(C.byref(st), C.byref(store()), V + FAR, P, P, BIG, None), "overlap")
+
+
+def test_one_vector_that_overlaps():
+    lib, st = hmm.load(), apart()
+    for out in (st.table_out, st.refs_out, st.kv_len_out):
+        refused(lib.hmm_paged_fork(C.byref(st), C.byref(store()), 16, V, out, 3, P, P, BIG, None), "overlap")
+        refused(lib.hmm_paged_fork(C.byref(st), C.byref(store()), 16, out, V, 3, P, P, BIG, None), "overlap")
+        refused(lib.hmm_paged_grow(C.byref(st), 16, out, P, P, BIG, None), "overlap")
+    for live in (st.table_out, st.refs_out + 28, T, R):
+        refused(lib.hmm_paged_compact(C.byref(st), C.byref(store()), live, P, P, BIG, None), "overlap")
+    # lengths that double: only in place
+    refused(lib.hmm_paged_grow(C.byref(apart(kv_len_out=L + NEW)), 16, L + NEW, P, P, BIG, None), "overlap")
+    refused(lib.hmm_paged_grow(C.byref(apart(kv_len_out=L)), 16, L + 4, P, P, BIG, None), "overlap")
