@@ -128,6 +128,12 @@ __device__ __forceinline__ int64_t scan_incl(int64_t v, int64_t* wt, int64_t* to
     return v + add;
 }
 
+// (apart from the kernel's code, which streams)
+template <typename T>
+__device__ __noinline__ void rows_exact(const AttnArgs& a, int s, const Seq& q, int kvh, int row0, unsigned rows) {
+    attn_rows_exact<T, 1>(a, s, q, kvh, row0, rows);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP>())
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -137,7 +143,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     __shared__ uint64_t full[RW_WARPS][RW_STAGES];
     __shared__ int64_t wt[RW_WARPS];
     __shared__ int64_t sh_pre;
-    __shared__ int sh_seq, again, abort;
+    __shared__ int sh_seq, again, any_again, abort;
     constexpr int HALVES = DP / 64;                    // boxes of 64 values in a row
     constexpr int BLOCK = RW_KEYS * 128;               // 16 rows of 64 values, swizzled
     constexpr int STAGE = 2 * HALVES * BLOCK;          // K then V
@@ -149,7 +155,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (threadIdx.x == 0) {
         for (int w = 0; w < RW_WARPS; ++w)
             for (int i = 0; i < RW_STAGES; ++i) mbar_init(&full[w][i], 1);
-        abort = 0;
+        abort = any_again = 0;
         fence_barrier_init();
     }
     // ---- this CTA's piece of the list of all units' tiles
@@ -404,6 +410,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         };
         if (t0 == 0 && t1 == ld.tiles) {
             finish_rows<T, false>(a, s, q, kvh, row0, rows, RW_WARPS, stat, value, jst + 2 * RW_WARPS * RW_ROWS, &again);
+            if (threadIdx.x == 0 && again) any_again = 1;
         } else {
             float* part = r.w.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * RW_ROWS * (DP + 2);
             for (int i = threadIdx.x; i < rows * (DP / 4); i += RW_THREADS) {
@@ -436,6 +443,28 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         cur += t1 - t0;
         fence_proxy_async_smem();                      // the next copies come behind these writes
         __syncthreads();
+    }
+    if (!any_again || abort) return;
+    // ---- rows that came out not finite, of the units that are whole here (out of the way of the
+    // loop: within it the decode batch took 349 us, not 345)
+    pre = sh_pre;
+    s = sh_seq;
+    for (cur = blockIdx.x * per; cur < end;) {
+        q = load_seq(a.b, a.max_kv, s, a.status);
+        ld = seq_load(r, q);
+        if (cur >= pre + (int64_t)ld.units * ld.tiles) {
+            pre += (int64_t)ld.units * ld.tiles;
+            ++s;
+            continue;
+        }
+        const int unit = (int)((cur - pre) / ld.tiles), t0 = (int)(cur - pre - (int64_t)unit * ld.tiles);
+        const int n = (int)min((int64_t)(ld.tiles - t0), end - cur);
+        if (n == ld.tiles) {                           // a warp's rows: four neighbours
+            const int kvh = unit / ld.row_tiles, row0 = (unit - kvh * ld.row_tiles) * RW_ROWS;
+            const int rows = (int)min((int64_t)RW_ROWS, (int64_t)q.n_new * a.group - row0);
+            rows_exact<T>(a, s, q, kvh, row0, ((1u << rows) - 1u) & 0xfu << 4 * warp);
+        }
+        cur += n;
     }
 }
 
@@ -477,6 +506,8 @@ __global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_con
                            (few ? row * j.dp + 4 * col : (col * rows + r0 + row) * 4));
                    },
                    share, &again);
+    if (again)   // (four neighbours a warp)
+        attn_rows_exact<T, 1>(j.a, u.x, q, u.y, row0, (unsigned)again & 0xfu << 4 * (threadIdx.x >> 5));
 }
 
 int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
@@ -517,8 +548,9 @@ template <typename T>
 hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
     // A unit of up to 16 rows (one MMA's) reads its keys once either way and the many small
     // CTAs of the rows kernel keep more reads in flight; more rows would read them again
-    // there.
-    const bool chunk = chunk_applies(a);
+    // there.  (A scale of zero is the rows kernel's, which scales before it masks: in the
+    // chunk kernel a masked score of -inf times zero would be NaN.)
+    const bool chunk = chunk_applies(a) && a.scale_log2 != 0.0f;
     const bool few = max_new > 0 && (int64_t)std::min(max_new, a.b.n_tokens) * a.group <= RW_ROWS;
     const bool with_rows = few || !chunk || a.b.n_seq > 1;
     const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel

@@ -88,57 +88,184 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr float LN2 = 0.693147180559945309417f;
 
-// One row from the definition, by one warp, key by key in fp32: the row's
-// result where the tiled product does not hold.  A tile multiplies weights of
-// zero with the values of keys that only other rows see, and a zero times an
-// infinity or NaN there is NaN; such a row comes here, so that what a row does
-// not see never reaches it.  (It also comes here, to the same NaN or infinity,
-// when what it sees is not finite.)
+// A key's K and V rows; null if its page is flagged.
+struct KeyRows {
+    const unsigned char *k, *v;
+};
+__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int s, int kvh, int key) {
+    const int lp = a.by_page(key), phys = page_of(a, s, lp), in = key - lp * a.page_tokens;
+    if (phys < 0) return KeyRows{nullptr, nullptr};
+    return KeyRows{a.k.base + phys * a.k.page + kvh * a.k.head + in * a.k.token,
+                   a.v.base + phys * a.v.page + kvh * a.v.head + in * a.v.token};
+}
+
 template <typename T>
-__device__ __forceinline__ void attn_row_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row) {
-    constexpr int NV = 8;   // 32 lanes x 8 = D <= 256
-    const int lane = threadIdx.x & 31;
-    const int tok = q.begin + row / a.group, head = kvh * a.group + row % a.group;
-    const int pos = row_pos(a, q, row);
-    const Span sp = tile_span(a, q, row, row + 1);
-    const T* qr = reinterpret_cast<const T*>(a.q + tok * a.q_token + head * a.q_head);
-    float qf[NV], acc[NV], m = -INFINITY, l = 0.0f;
+__device__ __forceinline__ void unpack8(const uint4& w, float* f) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        qf[i] = lane + 32 * i < a.D ? to_f32<T>(qr[lane + 32 * i]) : 0.0f;
-        acc[i] = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = unpack2<T>(u[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
     }
-    for (int key = sp.sink > 0 ? 0 : sp.lo; key < sp.hi; ++key) {
-        if (key == sp.sink && key < sp.lo) key = sp.lo;
-        if (key >= sp.hi) break;
-        if (!sees(a, q.kv, pos, key)) continue;
-        const int lp = a.by_page(key), phys = page_of(a, s, lp);
-        if (phys < 0) continue;
-        const int in = key - lp * a.page_tokens;
-        const T* kr = reinterpret_cast<const T*>(a.k.base + phys * a.k.page + kvh * a.k.head + in * a.k.token);
-        const T* vr = reinterpret_cast<const T*>(a.v.base + phys * a.v.page + kvh * a.v.head + in * a.v.token);
-        float x = 0.0f;
+}
+
+// Whether one of eight values is an infinity or NaN: all bits of its exponent.
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const uint4& w) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+    return (__vcmpeq2(w.x & E, E) | __vcmpeq2(w.y & E, E) | __vcmpeq2(w.z & E, E) | __vcmpeq2(w.w & E, E)) != 0u;
+}
+
+// The columns that came out not finite of rows row0 + i, bit i of `rows`, from the
+// definition, by one warp in fp32: what the tiled product cannot tell.  A tile multiplies
+// weights of zero with the values of keys that only other rows see, and a zero times an
+// infinity or NaN there is NaN; such rows come here, so that what a row does not see never
+// reaches it.  Their scores are finite or, all but one, -inf, and their other columns and
+// lse stand.  (A row whose columns are finite is passed over, and one with a NaN score,
+// whose columns are NaN, stays so.)
+//
+// First the values alone: a seen NaN decides its column, as do infinities of both signs, and
+// a product that is infinite is right if the row sees an infinity (an unseen one gives NaN).
+// The keys that all the rows see are gone through once.  So one bad value that many rows see
+// costs each little.  What is left is added up again, row by row: a lane scores one of 32
+// keys, and groups of lanes, eight columns each, add values.
+//
+// 4,096 tokens, 32/8 heads of 128, one NaN or infinity: 0.36 ms if the first key holds it, 0.9
+// in the middle (row by row and key by key 227 and 180; without it 0.15).  One that some rows
+// of a unit see and others do not, the last key's: 16 ms.
+// U: loops are unrolled so far.  The code is never reached as a rule, but its size is felt by
+// kernels that stream (the decode batch 351 -> 355 us with 16 in the join; 352 with 1).
+template <typename T, int U>
+__device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row0, unsigned rows) {
+    const int lane = threadIdx.x & 31, vecs = a.D / 8;
+    const int lanes = vecs > 1 ? 2 << (31 - __clz(vecs - 1)) : 1, groups = 32 / lanes;   // of a V row
+    const int gl = lane & (lanes - 1), group = lane / lanes;
+    auto result = [&](int i) {   // the lane's columns of row row0 + i
+        const int r = row0 + i, tok = a.by_group(r);
+        return a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + kvh * a.group + r - tok * a.group) * a.D + 8 * gl);
+    };
+    auto bad_columns = [&](int i, uint32_t* nan, uint32_t* inf) {   // a bit per column
+        float f[8];
+        unpack8<T>(gl < vecs ? *reinterpret_cast<const uint4*>(result(i)) : make_uint4(0u, 0u, 0u, 0u), f);
+        *nan = *inf = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < a.D) x = fmaf(qf[i], to_f32<T>(kr[lane + 32 * i]), x);
+        for (int c = 0; c < 8; ++c) {
+            *nan |= (f[c] != f[c] ? 1u : 0u) << c;
+            *inf |= (isinf(f[c]) ? 1u : 0u) << c;
+        }
+    };
+    auto values = [&](const unsigned char* v, int i) {   // of the i-th of a group's `lanes` keys
+        const unsigned char* p = reinterpret_cast<const unsigned char*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), i * groups + group));
+        return p && gl < vecs ? __ldg(reinterpret_cast<const uint4*>(p) + gl) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto rows_of = [&](int key, int end) { return key < end ? key_rows(a, s, kvh, key) : KeyRows{nullptr, nullptr}; };
+    uint32_t met = 0;   // NaN, inf, -inf seen in the lane's columns, a byte each
+    auto met_nan = [&] { return (met | (met >> 8 & met >> 16)) & 0xffu; };
+    auto undecided = [&](uint32_t nan, uint32_t inf) { return (nan | (inf & ~(met >> 8 | met >> 16))) & ~met_nan(); };
+    auto scan = [&](int k0, int k1, uint32_t nan, uint32_t inf) {   // keys [k0, k1), until the columns are decided
+        if (k0 >= k1 || !__any_sync(0xffffffffu, undecided(nan, inf) != 0)) return;
+        KeyRows r = rows_of(k0 + lane, k1);
+        for (; k0 < k1; k0 += 32) {
+            const KeyRows next = rows_of(k0 + 32 + lane, k1);
+#pragma unroll U
+            for (int i = 0; i < lanes; ++i) {
+                const uint4 w = values(r.v, i);
+                if (any_not_finite<T>(w)) {
+                    float f[8];
+                    unpack8<T>(w, f);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x *= a.scale_log2;
-        const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.0f : mn;
-        const float al = ex2(m - ms), p = ex2(x - ms);
-        l = l * al + p;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < a.D) acc[i] = acc[i] * al + p * to_f32<T>(vr[lane + 32 * i]);
+                    for (int c = 0; c < 8; ++c)
+                        met |= (f[c] != f[c] ? 1u : f[c] == INFINITY ? 0x100u : f[c] == -INFINITY ? 0x10000u : 0u) << c;
+                }
+            }
+            r = next;
+            for (int w = lanes; w < 32; w <<= 1) met |= __shfl_xor_sync(0xffffffffu, met, w);
+            if (!__any_sync(0xffffffffu, undecided(nan, inf) != 0)) break;
+        }
+    };
+    if (rows == 0) return;
+    // the keys [all0, all1) that all of them see
+    const int first = row0 + __ffs(rows) - 1, last = row0 + 31 - __clz(rows);
+    const int all0 = tile_span(a, q, last, last + 1).lo, all1 = max(all0, tile_span(a, q, first, first + 1).hi);
+    {
+        uint32_t nan = 0, inf = 0;
+        for (unsigned left = rows; left; left &= left - 1) {
+            uint32_t n, f;
+            bad_columns(__ffs(left) - 1, &n, &f);
+            nan |= n;
+            inf |= f;
+        }
+        scan(all0, all1, nan, inf);
     }
-    T* o = reinterpret_cast<T*>(a.out) + ((int64_t)tok * a.hq + head) * a.D;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint32_t met_all = met;
+    for (; rows; rows &= rows - 1) {
+        const int i = __ffs(rows) - 1, row = row0 + i;
+        const Span sp = tile_span(a, q, row, row + 1);   // all of it is seen
+        uint32_t nan, inf;
+        bad_columns(i, &nan, &inf);
+        met = met_all;
+#pragma unroll 1
+        for (int part = 0; part < 3; ++part)             // first tokens; behind and before the common ones
+            scan(part == 0 ? 0 : part == 1 ? sp.lo : max(all1, sp.lo),
+                 part == 0 ? sp.sink : part == 1 ? min(all0, sp.hi) : sp.hi, nan, inf);
+        const uint32_t left = undecided(nan, inf), is_nan = met_nan() & (nan | inf);
+        float acc[8], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (lane + 32 * i < a.D) o[lane + 32 * i] = l == 0.0f ? T(0.0f) : T(acc[i] * inv);
-    if (a.lse && lane == 0)
-        a.lse[(int64_t)tok * a.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+        for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
+        if (__any_sync(0xffffffffu, left != 0)) {
+            const int tok = a.by_group(row), n = sp.sink + sp.hi - sp.lo;
+            const uint4* qr = reinterpret_cast<const uint4*>(a.q + (q.begin + tok) * a.q_token +
+                                                             (kvh * a.group + row - tok * a.group) * a.q_head);
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int at = i0 + lane;
+                const KeyRows r = rows_of(at < sp.sink ? at : sp.lo + at - sp.sink, at < n ? INT32_MAX : 0);
+                float x = -INFINITY;
+                if (r.k) {
+                    x = 0.0f;
+#pragma unroll U < 8 ? U : 8
+                    for (int c = 0; c < vecs; ++c) {
+                        float kf[8], qf[8];
+                        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.k) + c), kf);
+                        unpack8<T>(__ldg(qr + c), qf);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x = fmaf(qf[e], kf[e], x);
+                    }
+                    x *= a.scale_log2;
+                }
+                float mn = fmaxf(m, x);
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
+                const float ms = mn == -INFINITY ? 0.0f : mn, al = ex2(m - ms), p = ex2(x - ms);
+                l = fmaf(l, al, p);                      // (a lane's share)
+                m = mn;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) acc[c] *= al;
+#pragma unroll U
+                for (int j = 0; j < lanes; ++j) {
+                    const float pj = __shfl_sync(0xffffffffu, p, j * groups + group);
+                    float f[8];
+                    unpack8<T>(values(r.v, j), f);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) acc[c] = fmaf(pj, f[c], acc[c]);
+                }
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                for (int w = lanes; w < 32; w <<= 1) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], w);
+        }
+        const float inv = 1.0f / l;
+        T* o = reinterpret_cast<T*>(result(i));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (group != 0) continue;
+            if (is_nan >> c & 1u) o[c] = T(NAN);
+            else if (left >> c & 1u) o[c] = l == 0.0f ? T(0.0f) : T(acc[c] * inv);
+        }
+    }
 }
 
 // The joined rows' values: K quads a thread and P pieces at a time, K * P reads in flight.
@@ -166,8 +293,8 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    const float w = p0 + p < pieces ? top[row[k] * pieces + p0 + p] : 0.0f;
-                    if (w != 0.0f) {
+                    const float w = p0 + p < pieces ? top[row[k] * pieces + p0 + p] : -1.0f;
+                    if (!(w < 0.0f)) {   // (a weight of zero too: an infinity behind it shows)
                         x[k].x = fmaf(w, v[k][p].x, x[k].x); x[k].y = fmaf(w, v[k][p].y, x[k].y);
                         x[k].z = fmaf(w, v[k][p].z, x[k].z); x[k].w = fmaf(w, v[k][p].w, x[k].w);
                     }
@@ -176,7 +303,8 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (i0 + k * (int)blockDim.x >= all) continue;
-            if (!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w))
+            if ((!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w)) &&
+                !isnan(top[row[k] * pieces]))
                 atomicOr(again, 1 << row[k]);
             const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
             *reinterpret_cast<uint2*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + 4 * col[k])) =
@@ -186,13 +314,14 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 }
 
 // Joins (maximum, sum, row) pieces of up to 16 rows, which several warps or CTAs summed
-// over different keys, in their order, and writes the rows out; rows that come out not
-// finite are computed again by attn_row_exact.  stat(i, row, k) reads piece i's maximum
-// (k = 0) or sum (1), value(i, row, c) its columns 4 c ... 4 c + 3; `share` holds
-// 32 x pieces floats.  A piece with a score of NaN or +inf has a maximum of +inf (and no
-// other has: a sum with it is NaN).  Whole block, 128 threads.  FAR: the pieces lie in memory, many of
-// them maybe, and their reads' latency is what it costs (one token over 4,000, 31 pieces:
-// the call took 25 us with two at a time, 17 with eight; sixteen gave no more).
+// over different keys, in their order, and writes the rows out.  Whole block, 128 threads;
+// behind it *again holds a bit per row for attn_rows_exact: some columns came out not finite,
+// although the scores were (a row with a score that was not is NaN).
+// stat(i, row, k) reads piece i's maximum (k = 0) or sum (1), value(i, row, c) its columns
+// 4 c ... 4 c + 3; `share` holds 32 x pieces floats.  A piece with a score of NaN or +inf has
+// a maximum of +inf (and no other has: a sum with it is NaN).  FAR: the pieces lie in memory,
+// many of them maybe, and their reads' latency is what it costs (one token over 4,000, 31
+// pieces: the call took 25 us with two at a time, 17 with eight; sixteen gave no more).
 template <typename T, bool FAR, typename Stat, typename Value>
 __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
                                             int rows, int pieces, Stat stat, Value value, float* share,
@@ -226,10 +355,10 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         for (int p = t; live && p < pieces; p += 8) {
             const float w = top[r * pieces + p];
-            top[r * pieces + p] = w == 0.0f ? 0.0f : w * inv;
+            // a row of no weight at all is zeros, one with a NaN sum NaN, whatever the values
+            top[r * pieces + p] = l == 0.0f ? -1.0f : w * inv;
         }
         if (live && t == 0) {
-            if (l != l) atomicOr(again, 1 << r);
             if (a.lse) {
                 const int tok = a.by_group(row0 + r);
                 a.lse[(int64_t)(q.begin + tok) * a.hq + kvh * a.group + row0 + r - tok * a.group] =
@@ -242,10 +371,6 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         join_values<T, 1, 8>(a, q, kvh, row0, rows, pieces, value, top, again);
     else
         join_values<T, 4, 2>(a, q, kvh, row0, rows, pieces, value, top, again);
-    __syncthreads();
-    const int bits = *again;
-    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
-        if ((bits >> r) & 1) attn_row_exact<T>(a, s, q, kvh, row0 + r);
     __syncthreads();
 }
 

@@ -96,7 +96,7 @@ struct TcArgs {
     int split;           // whether few units may be cut into pieces
     int q_tokens;        // new tokens of a row tile's TMA box, 0: queries by 16-byte copies
     uint64_t wait_ns;    // limit of every bounded wait
-    uint32_t* again;     // [units][TC_SOFTMAX_WARPS] rows that came out not finite
+    uint32_t* again;     // [units][TC_SOFTMAX_WARPS] rows of finite scores that came out not finite
     int units;           // sequences that overlap (a cu_new that descends) would be more units
     ChunkJoin join;
 };
@@ -974,7 +974,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
                 // The first half's weights with the maximum so far, while this tile's is found:
                 // that is right unless the row grew by more than TC_GROWTH, which is rare.
-                // NaN and +inf show in the maximum: such a row is computed again at the end.
+                // NaN and +inf show in the maximum: such a row is NaN.
                 uint32_t p[32];
                 uint64_t sum[2];
 #pragma unroll 1
@@ -1028,9 +1028,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             float l, lb;
             unpack_f2(add_f2(l2[0], l2[1]), l, lb);
             l += lb;
-            const bool live = r < rows && !(alone && w == 1), some = nw > 0 && l != 0.0f, whole_unit = u.slot < 0;
-            float top = m == -INFINITY ? (some ? 0.0f : -INFINITY) : m * sc, s0 = some ? 1.0f : 0.0f, s1 = 0.0f;
-            fine = fine && l == l;
+            const bool live = r < rows && !(alone && w == 1), whole_unit = u.slot < 0;
+            bool some = m != -INFINITY, other = false;   // whether this half saw a key, and the other one did
+            float top = some ? m * sc : -INFINITY, s0 = 1.0f, s1 = 0.0f;
+            fine = fine && (!some || l > 0.0f);          // (no sum of a maximum's weights: NaN, or scores beyond fp32)
             if (n > 0 && w == 1) {
                 if (alone) ctl->half[r] = make_float2(top, fine ? l : NAN);
                 __syncwarp();
@@ -1041,11 +1042,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     const float2 x = ctl->half[r];
                     const float both = fmaxf(top, x.x);
                     fine = fine && x.y == x.y;
-                    s0 = top == -INFINITY ? 0.0f : ex2(top - both);
-                    s1 = x.x == -INFINITY ? 0.0f : ex2(x.x - both);
+                    other = x.x != -INFINITY;
+                    s0 = some ? ex2(top - both) : 0.0f;
+                    s1 = other ? ex2(x.x - both) : 0.0f;
                     l = fmaf(l, s0, x.y * s1);
                     top = both;
                 }
+            }
+            if (!fine) {                                 // every column and lse
+                some = true;
+                s0 = l = NAN;
             }
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
             const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
@@ -1065,7 +1071,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = s0 != 0.0f ? __float_as_uint(__uint_as_float(o[c]) * s0) : 0u;
+                for (int c = 0; c < 32; ++c) o[c] = some ? __float_as_uint(__uint_as_float(o[c]) * s0) : 0u;
                 if (alone && u.n_of[1] > 0) {
 #pragma unroll
                     for (int h = 0; h < 32; h += 8) {
@@ -1074,7 +1080,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         tmem_wait_ld();
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            if (s1 != 0.0f)
+                            if (other)
                                 o[h + c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), s1, __uint_as_float(o[h + c])));
                     }
                 }
@@ -1099,7 +1105,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     else if (c0 + c < a.D) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
-            fine = fine && most < 0x7f800000u;
             if (n > 0) {
                 tc_fence_before();
                 __syncwarp();
@@ -1109,14 +1114,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
             if (live) {
                 if (!whole_unit) {
-                    // an infinite maximum joins to NaN: the row is computed again there
+                    // an infinite maximum joins to NaN
                     pt[UNIT * DP + r] = fine ? top : INFINITY;
                     pt[UNIT * (DP + 1) + r] = l;
                 } else if (a.lse) {
                     a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
                 }
             }
-            const unsigned again = __ballot_sync(0xffffffffu, live && !fine);
+            const unsigned again = __ballot_sync(0xffffffffu, live && fine && most >= 0x7f800000u);
             if (lane == 0 && whole_unit && (uint32_t)u.id < (uint32_t)t.units) {
                 t.again[(int64_t)u.id * TC_SOFTMAX_WARPS + warp] = again;
                 if (again) ctl->any_again = 1;
@@ -1131,7 +1136,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     tc_fence_after();
     if (warp == TC_SOFTMAX_WARPS + 1) tmem_dealloc(tmem, 512);
     if (warp == 0) asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows kernel may still run: not done before it
-    // Rows that came out not finite, from the definition.
+    // Rows of finite scores that came out not finite, from the definition.
     if (*abort || !ctl->any_again || warp >= TC_SOFTMAX_WARPS) return;
     Unit* u = reinterpret_cast<Unit*>(smem_raw) + warp;   // (nothing is left in the rings)
     const Plan plan = ctl->plan;
@@ -1144,12 +1149,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         __syncwarp();
         if (s < 0) break;
         if (slot >= 0 || (uint32_t)id >= (uint32_t)t.units) continue;
-        unsigned again = __ldcg(t.again + (int64_t)id * TC_SOFTMAX_WARPS + warp);
-        while (again) {   // rows [32 warp, 32 warp + 32) of the unit
-            const int i = __ffs(again) - 1;
-            again &= again - 1;
-            attn_row_exact<T>(a, s, q, kvh, row0 + i);
-        }
+        // rows [32 warp, 32 warp + 32) of the unit
+        attn_rows_exact<T, 16>(a, s, q, kvh, row0, __ldcg(t.again + (int64_t)id * TC_SOFTMAX_WARPS + warp));
     }
 }
 

@@ -90,3 +90,84 @@ def test_infinite_scores_of_few_rows(cuda):
     check(out, lse, ref)
     assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
     assert (out[1] == 0).all() and (lse[1] == -np.inf).all() and torch.isfinite(out[2]).all()
+
+
+def put(t, table, s, p, pt, col, value):
+    t[table[s, p // pt].item(), :, p % pt, col] = value
+
+
+@pytest.mark.parametrize("kind", ["first nan", "first inf", "inf in the middle", "inf of both signs", "inf and nan", "newest inf",
+                                  "many inf", "many nan", "not seen by all"])
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("dtype,window", [("bf16", 0), ("fp16", 0), ("bf16", 40)])
+def test_values_that_are_not_finite(cuda, batch, kind, dtype, window):
+    """Rows that see them have what the formula gives, the others are as if they were not there."""
+    new, kv, pt = batch[0], batch[1], batch[5]
+    q, k, v, table, cu, kv_len = make(cuda, 63, *batch, DT[dtype])
+    d = v.shape[-1]
+    for s, (n, L) in enumerate(zip(new, kv)):
+        if kind == "first nan":
+            put(v, table, s, 0, pt, 5, NAN)
+        elif kind == "first inf":
+            put(v, table, s, 0, pt, 5, INF)
+            put(v, table, s, 0, pt, d - 1, -INF)
+        elif kind == "inf in the middle":
+            put(v, table, s, L // 2, pt, 0, INF)
+        elif kind == "inf of both signs":
+            put(v, table, s, 0, pt, 1, INF)
+            put(v, table, s, L - 1, pt, 1, -INF)
+            put(v, table, s, L // 2, pt, 2, -INF)
+        elif kind == "inf and nan":
+            put(v, table, s, L // 3, pt, 7, INF)
+            put(v, table, s, 2 * L // 3, pt, 7, NAN)
+        elif kind == "newest inf":
+            put(v, table, s, L - 1, pt, 3, INF)
+        elif kind in ("many inf", "many nan"):
+            for p in range(L // 2, L // 2 + min(5, L - L // 2)):
+                v[table[s, p // pt].item(), :, p % pt] = INF if kind == "many inf" else NAN
+        else:                                     # seen by the second half of the new tokens
+            put(v, table, s, L - n // 2 - 1, pt, 4, INF)
+            put(v, table, s, L - n // 2 - 1, pt, 6, NAN)
+    kw = dict(window=window, sinks=2 if window else 0)
+    ref = reference(q, k, v, table, new, kv, **kw)
+    for hint in (0, 1):
+        out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, return_lse=True, max_new=hint, **kw)
+        check(out, lse, ref)
+        inf = torch.isinf(ref[0])
+        assert torch.equal(out.double()[inf], ref[0][inf])
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-30])
+def test_a_scale_of_nothing(cuda, scale):
+    """All seen keys weigh the same, whatever their scores; the rows that see none are zeros."""
+    for batch in BATCHES:
+        new, kv = batch[:2]
+        q, k, v, table, cu, kv_len = make(cuda, 64, *batch, torch.bfloat16)
+        kw = dict(scale=scale, window=50, sinks=1)
+        out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, return_lse=True, **kw)
+        check(out, lse, reference(q, k, v, table, new, kv, **kw))
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+@pytest.mark.parametrize("what", ["k", "v", "q", "late v"])
+def test_one_bad_value_costs_little(cuda, value, what):
+    """A NaN or infinity that a long prompt's rows see does not send them through their keys one
+    after another: 227 ms when it did, and 0.15 ms without it."""
+    n, pt = 4096, 16
+    q, k, v, table, cu, kv_len = make(cuda, 65, [n], [n], 32, 8, 128, pt, torch.bfloat16)
+    if what == "q":
+        q[:, :, 0] = value
+    elif what == "late v":
+        put(v, table, 0, n // 2, pt, 9, value)
+    else:
+        put(k if what == "k" else v, table, 0, 0, pt, 9, value)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    times = []
+    for _ in range(3):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        hmm.paged_attention(q, k, v, table, cu, kv_len, status=status)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    assert min(times) < 10, times
