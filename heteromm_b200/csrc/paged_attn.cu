@@ -148,6 +148,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     constexpr int BLOCK = RW_KEYS * 128;               // 16 rows of 64 values, swizzled
     constexpr int STAGE = 2 * HALVES * BLOCK;          // K then V
     constexpr int MR = DP + 4;                         // joining rows: 4 banks apart
+    // log2 of what weights are held by: the largest is 2^14 in fp16, whose range ends at 2^-25
+    // (a key 18 nats below the largest had no weight at all, and a long tail of them a share
+    // of the result).  It cancels against the sum, and lse takes it back with the maximum.
+    constexpr float UP = std::is_same<T, __half>::value ? 14.0f : 0.0f;
     const AttnArgs& a = r.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -345,7 +349,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 const float ms = mx[h] == -INFINITY ? 0.0f : mx[h];
                 al[h] = ex2(m[h] - ms);
                 m[h] = mx[h];
-                mx[h] = ms;
+                mx[h] = ms - UP;
             }
             if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
 #pragma unroll
@@ -362,8 +366,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 for (int h = 0; h < 2; ++h) {
                     const float e0 = ex2(sc[nb][2 * h] - mx[h]), e1 = ex2(sc[nb][2 * h + 1] - mx[h]);
                     l[h] += e0 + e1;
-                    // weights in the cache's type for the product: relative 2^-9 (bf16) or 2^-12,
-                    // the size of the output's own rounding; the sum keeps fp32
+                    // weights in the cache's type for the product: off by half a step, 2^-8 of a
+                    // weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
                     p[2 * nb + h] = pack2<T>(e0, e1);
                 }
 #pragma unroll
@@ -399,7 +403,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             if ((lane & 3) == 0) {
                 // fmaxf drops NaN, the sum keeps it: with an infinite maximum the row's share of
                 // every join is NaN, so that a NaN score shows in the result
-                jst[warp * RW_ROWS + row] = l[h] == l[h] ? m[h] : INFINITY;
+                jst[warp * RW_ROWS + row] = l[h] == l[h] ? m[h] - UP : INFINITY;
                 jst[(RW_WARPS + warp) * RW_ROWS + row] = l[h];
             }
         }

@@ -33,8 +33,8 @@
 // against 420; the two halves then keep step and want the same units at once.)
 //
 // The maximum that the weights refer to is only moved when a row's has grown by
-// more than 2^8: weights then stay below 256 (exact in the fp32 sums, a common
-// factor in the result), and the sums in TMEM are rescaled rarely.
+// more than 2^8: weights then stay below 256 (fp16: 2^15; exact in the fp32 sums, a
+// common factor in the result), and the sums in TMEM are rescaled rarely.
 //
 // Bound: 4 D FLOP per (row, key) on the tensor cores, 2,048 clocks for the two row
 // tiles and a key tile at D = 128, and as many for their exponentials on the
@@ -76,6 +76,10 @@ constexpr int TC_UNIT_COST = 3;              // key tiles that a unit's start an
 // 64 units of 512 tokens over 4,096 (D = 128) 64 cut and 81 whole.
 constexpr int TC_JOIN_COST = 10;
 constexpr float TC_GROWTH = 8.0f;            // log2 of the growth that moves a row's maximum
+// log2 of what weights are held by, beside that growth: fp16 ends at 2^16 and 2^-25, so the
+// largest are 2^15, and keys far below the largest keep a weight.
+template <typename T>
+__host__ __device__ constexpr float tc_up() { return std::is_same<T, __half>::value ? 7.0f : 0.0f; }
 
 // Rows of a unit: at D = 256 the sums of one row tile take the TMEM beside its scores, and
 // the second half of the softmax warps rests.
@@ -266,16 +270,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Weights exp2(sc (s - m)) of 64 of a row's scores v, packed in pairs, and their sum (two
-// pairs of partial sums); with TOP also the largest of the 128 scores from v on.  m = -inf
-// (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
+// Weights exp2(sc (s - m) + tc_up) of 64 of a row's scores v, packed in pairs, and their sum
+// (two pairs of partial sums); with TOP also the largest of the 128 scores from v on.
+// m = -inf (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
 template <typename T, bool TOP>
 __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
                                          uint64_t* sum) {
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
-    const float neg = m == -INFINITY ? 0.0f : -m * sc;
+    const float neg = m == -INFINITY ? 0.0f : fmaf(-m, sc, tc_up<T>());
     const uint64_t neg2 = pack_f2(neg, neg);
     sum[0] = sum[1] = pack_f2(0.0f, 0.0f);
     float x[32], y[32], mx0 = -INFINITY, mx1 = -INFINITY;
@@ -294,8 +298,8 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
         if (i >= LAG) {
             const int u = i - LAG;
             sum[u & 1] = add_f2(sum[u & 1], pack_f2(x[u], y[u]));
-            // weights in the cache's type for the product: relative 2^-9 (bf16) or
-            // 2^-12, the size of the output's own rounding; the sum keeps fp32
+            // weights in the cache's type for the product: off by half a step, 2^-8 of a
+            // weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
             p[u] = pack2<T>(x[u], y[u]);
         }
     }
@@ -1030,7 +1034,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             l += lb;
             const bool live = r < rows && !(alone && w == 1), whole_unit = u.slot < 0;
             bool some = m != -INFINITY, other = false;   // whether this half saw a key, and the other one did
-            float top = some ? m * sc : -INFINITY, s0 = 1.0f, s1 = 0.0f;
+            float top = some ? fmaf(m, sc, -tc_up<T>()) : -INFINITY, s0 = 1.0f, s1 = 0.0f;
             fine = fine && (!some || l > 0.0f);          // (no sum of a maximum's weights: NaN, or scores beyond fp32)
             if (n > 0 && w == 1) {
                 if (alone) ctl->half[r] = make_float2(top, fine ? l : NAN);

@@ -392,7 +392,8 @@ hmm_status_t hmm_paged_kv_append(
  * up to 256 of them, are computed again key by key: 16 ms over 4,096 cached
  * tokens, 32/8 heads of 128.)
  * Query head h reads KV head h / (n_heads / n_kv_heads).  fp32 scores, softmax
- * and sums; the weights are rounded to the cache's type for the product with V.
+ * and sums; the weights are rounded to the cache's type for the product with V
+ * (by half a step; in fp16 those below 2^-21 of the row's largest by 2^-32 of it).
  * Deterministic: the same call gives the same bits.
  *   q [n_tokens][n_heads][D] of the cache's type, 16-byte aligned, token and
  *   head strides in elements (multiples of 8); out [n_tokens][n_heads][D] of
