@@ -8,8 +8,8 @@
   lib/heteromm_cpp_kernels<ext>  Python bindings of the steps under the names the
                             reference's pipeline generator calls
                             (src/py/heteromm_cpp_kernels.cpp, pybind11)
-  lib/heteromm_serve_calls<ext>  the serving entry points called with torch tensors
-                            (src/py/serve_calls.cpp, torch's headers)
+  lib/heteromm_serve_calls-<torch>-<sources><ext>  the serving entry points called with
+                            torch tensors (src/py/serve_calls.cpp, torch's headers)
 
 nvcc cross-compiles for sm_100a without a GPU; the built .so files travel with
 the repository snapshot to the GPU machine.
@@ -17,9 +17,11 @@ the repository snapshot to the GPU machine.
 from __future__ import annotations
 
 import glob
+import hashlib
 import os
 import subprocess
 import sys
+import threading
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -99,23 +101,55 @@ def build_py_kernels(force: bool = False) -> str:
 
 
 def serve_calls_path() -> str:
+    """Where the module is for this torch, this Python and these sources: one built for or
+    from others has another name."""
     import sysconfig
-    return os.path.join(LIB_DIR, "heteromm_serve_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    import torch
+    digest = hashlib.sha256()
+    for f in _serve_calls_sources():
+        with open(f, "rb") as src:
+            digest.update(src.read())
+    return os.path.join(LIB_DIR, f"heteromm_serve_calls-torch{torch.__version__.replace('+', '_')}-"
+                                 f"{digest.hexdigest()[:12]}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+def _serve_calls_sources() -> list[str]:
+    return [os.path.join(PKG, "src", "py", "serve_calls.cpp"), os.path.join(INC, "heteromm_cuda.h")]
 
 
 def build_serve_calls(force: bool = False) -> str:
-    """The module heteromm_serve_calls; torch's own libraries are loaded when it is."""
+    """The module heteromm_serve_calls; torch's own libraries are loaded when it is.  "" where
+    torch's headers or its CUDA library are not: the C ABI does not need them."""
     import sysconfig
-    import torch
-    src, out = os.path.join(PKG, "src", "py", "serve_calls.cpp"), serve_calls_path()
-    if force or _newer(out, [src, os.path.join(INC, "heteromm_cuda.h")]):
+    try:
+        import torch
+    except ImportError:
+        return ""
+    home = os.path.dirname(torch.__file__)
+    include, lib = os.path.join(home, "include"), os.path.join(home, "lib")
+    if not os.path.exists(os.path.join(include, "torch", "csrc", "Exceptions.h")) or \
+            not os.path.exists(os.path.join(lib, "libc10_cuda.so")):
+        return ""
+    out = serve_calls_path()
+    if force or not os.path.exists(out):
         os.makedirs(LIB_DIR, exist_ok=True)
-        home = os.path.dirname(torch.__file__)
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-              *(f"-isystem{os.path.join(home, 'include', d)}" for d in ("", "torch/csrc/api/include")),
-              "-I/usr/local/cuda/include", f"-I{sysconfig.get_paths()['include']}", f"-I{INC}", "-o", out, src,
-              f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+        # (renamed when it is whole: another process may look for it, or build it too)
+        part = f"{out}.{os.getpid()}.{threading.get_ident()}"
+        try:
+            _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                  f"-isystem{include}", f"-isystem{os.path.join(include, 'torch', 'csrc', 'api', 'include')}",
+                  "-I/usr/local/cuda/include", f"-I{sysconfig.get_paths()['include']}", f"-I{INC}", "-o", part,
+                  _serve_calls_sources()[0], f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                  "-lc10_cuda"])
+            os.replace(part, out)
+        finally:
+            if os.path.exists(part):
+                os.remove(part)
+        kind = out[:-len(sysconfig.get_config_var("EXT_SUFFIX")) - 12]   # for this torch, from older sources
+        for old in glob.glob(glob.escape(kind) + "*" + sysconfig.get_config_var("EXT_SUFFIX")):
+            if old != out:
+                os.remove(old)
     return out
 
 

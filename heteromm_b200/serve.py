@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
-import os
+import threading
 
 import torch
 
@@ -44,17 +44,23 @@ def _raise(name: str, status: int):
 class _Calls:
     """The module heteromm_serve_calls, loaded (and built, if it is absent) at the first call."""
 
+    _lock = threading.Lock()
+
     def __getattr__(self, name: str):
-        path = _build.serve_calls_path()
-        if not os.path.exists(path):
-            _build.build_serve_calls()
-        spec = importlib.util.spec_from_file_location("heteromm_serve_calls", path)
-        native = importlib.util.module_from_spec(spec)
-        lib = load()
-        native.bind(*(C.cast(getattr(lib, e), C.c_void_p).value for e in _ENTRIES), _raise)
-        for f in ("attention", "append", "copy_pages", "free", "fork", "grow", "compact"):
-            setattr(self, f, getattr(native, f))
-        return getattr(native, name)
+        if name not in ("attention", "append", "copy_pages", "free", "fork", "grow", "compact"):
+            raise AttributeError(name)
+        with self._lock:
+            if name not in self.__dict__:     # (another thread's first call was quicker)
+                path = _build.build_serve_calls()
+                if not path:
+                    raise RuntimeError("the serving calls need torch's headers and its CUDA library to be built")
+                spec = importlib.util.spec_from_file_location("heteromm_serve_calls", path)
+                native = importlib.util.module_from_spec(spec)
+                lib = load()
+                native.bind(*(C.cast(getattr(lib, e), C.c_void_p).value for e in _ENTRIES), _raise)
+                for f in ("attention", "append", "copy_pages", "free", "fork", "grow", "compact"):
+                    setattr(self, f, getattr(native, f))
+        return self.__dict__[name]
 
 
 _calls = _Calls()
