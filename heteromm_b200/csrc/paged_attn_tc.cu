@@ -99,7 +99,8 @@ struct TcArgs {
     int box_rows;        // rows of a TMA box: a power of two that divides page_tokens
     int split;           // whether few units may be cut into pieces
     int q_tokens;        // new tokens of a row tile's TMA box, 0: queries by 16-byte copies
-    uint64_t wait_ns;    // limit of every bounded wait
+    uint64_t wait_ns;    // limit of a bounded wait for one step: copies, products, weights of a tile
+    uint64_t unit_ns;    // and of one for the end of a unit, or of the two before it
     uint32_t* again;     // [units][TC_SOFTMAX_WARPS] rows of finite scores that came out not finite
     int units;           // sequences that overlap (a cu_new that descends) would be more units
     ChunkJoin join;
@@ -627,7 +628,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
     };
     // The k-th unit lies in ctl->unit[k & 1] between these two.
-    auto take = [&](int k) { return wait_warp(&ctl->u_full[k & 1], (k >> 1) & 1, abort, t.wait_ns); };
+    auto take = [&](int k) { return wait_warp(&ctl->u_full[k & 1], (k >> 1) & 1, abort, t.unit_ns); };
     auto leave = [&](int k) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->u_empty[k & 1]);
@@ -858,7 +859,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     const int key0 = u.key0(j);
                     const uint32_t st = (base + 2 * j + 1) % ST;
                     if (!u.mends(key0)) continue;
-                    if (!(ok = wait_warp(&ctl->v_mend, mended++ & 1, abort, t.wait_ns))) break;
+                    if (!(ok = wait_warp(&ctl->v_mend, mended++ & 1, abort, t.unit_ns))) break;
                     for (int r = lane; r < TC_KEYS; r += 32) {
                         const int key = key0 + r, k0 = key - r % t.box_rows;
                         if (!span_has(u.sp, key) &&
@@ -886,7 +887,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             int loads = 0;                       // units' queries so far
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.wait_ns))) break;
+                if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.unit_ns))) break;
                 Unit* u = &ctl->unit[k & 1];
                 describe(t, plan, k, &at, u);
                 const int s = u->s, n = u->n, row0 = u->row0, rows = u->rows, kvh = u->kvh, begin = u->q.begin;
@@ -894,7 +895,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (lane == 0) mbar_arrive(&ctl->u_full[k & 1]);
                 if (s < 0) break;
                 if (n == 0) continue;
-                if (!(ok = wait_warp(&ctl->q_empty, (loads & 1) ^ 1, abort, t.wait_ns))) break;
+                if (!(ok = wait_warp(&ctl->q_empty, (loads & 1) ^ 1, abort, t.unit_ns))) break;
                 ++loads;
                 constexpr int CH = DP / 8;
                 const uint32_t q0 = smem_u32(Qs);
@@ -1025,7 +1026,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // ---- the rows' results
             const int n = u.n, nw = u.n_of[w], rows = u.rows, r = row();
             const bool alone = u.alone;
-            if (ok && n > 0) ok = wait_warp(&ctl->o_full, busy & 1, abort, t.wait_ns);
+            if (ok && n > 0) ok = wait_warp(&ctl->o_full, busy & 1, abort, t.unit_ns);
             if (!ok) break;
             tc_fence_after();
             tiles += nw;
@@ -1041,7 +1042,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->half_full);
             } else if (n > 0) {
-                if (!(ok = wait_warp(&ctl->half_full, busy & 1, abort, t.wait_ns))) break;
+                if (!(ok = wait_warp(&ctl->half_full, busy & 1, abort, t.unit_ns))) break;
                 if (alone) {   // the halves' sums over different keys
                     const float2 x = ctl->half[r];
                     const float both = fmaxf(top, x.x);
@@ -1251,6 +1252,8 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     t.split = may_split(a.b.n_tokens, a.group, a.hk, rows);
     t.q_tokens = boxes ? TC_ROWS / a.group : 0;
     t.wait_ns = wait_limit_ns();
+    // 16 us a key tile, which takes 2 to 4 (a limit of 0 stays one)
+    t.unit_ns = t.wait_ns == 0 ? 0 : t.wait_ns + 2 * ((uint64_t)a.max_kv / TC_KEYS + 4) * 16000;
     t.again = (uint32_t*)ws;
     t.units = (int)units;
     if (t.split) {

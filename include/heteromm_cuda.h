@@ -622,9 +622,11 @@ hmm_status_t hmm_profile_read(double* total_ms, int64_t* launches);
 
 /* Test hook, no reference counterpart.  Sets the limit of every bounded
  * pipeline wait inside the tensor-core kernels (tc_score_select_kernel,
- * dsa_scores_kernel, paged_rows_kernel, paged_chunk_kernel) for the calls that follow, in nanoseconds; a negative
- * value restores the default of 2 s.  A wait that runs out makes its CTA let
- * the copies and MMAs already in flight complete, then exit, and the entry
+ * dsa_scores_kernel, paged_rows_kernel, paged_chunk_kernel) for the calls that
+ * follow, in nanoseconds; a negative value restores the default of 2 s.  (Waits
+ * of paged_chunk_kernel for a whole unit of work have 32 us more for each 128
+ * tokens that a row of the page table can hold.)  A wait that runs out makes its
+ * CTA let the copies and MMAs already in flight complete, then exit, and the entry
  * point returns HMM_ERR_TIMEOUT with its outputs invalid.  With 0, the first
  * wait that finds its pipeline stage not yet ready gives up: tests use it to
  * exercise that path without a fault or a hang. */
