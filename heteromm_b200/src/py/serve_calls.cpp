@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <ATen/ops/empty.h>
 
@@ -429,11 +430,8 @@ hmm_page_store_t store(PyObject* k_pages, PyObject* v_pages, int* dev) {
 // The state's old arrays and its new ones: fresh, or those of `out`.
 struct State {
     hmm_paged_state_t s{};
-    PyObject* fresh[3] = {nullptr, nullptr, nullptr};   // new references: the result's entries
+    THPObjectPtr fresh[3];   // the result's entries (given back if a check throws here too)
     int count = 0;
-    ~State() {
-        for (PyObject* o : fresh) Py_XDECREF(o);
-    }
     State(PyObject* table, PyObject* refs, PyObject* kv_len, PyObject* out, int dev) {
         static const char* const names[3] = {"out page_table", "out refs", "out kv_len"};
         const Tensor& t = page_table(table, dev);
@@ -447,21 +445,17 @@ struct State {
             for (int i = 0; i < count; ++i) {
                 Tensor x = empty(old[i]->sizes(), at::kInt, dev);
                 to[i] = (int32_t*)x.data_ptr();
-                fresh[i] = THPVariable_Wrap(std::move(x));
+                fresh[i] = THPObjectPtr(THPVariable_Wrap(std::move(x)));
                 if (!fresh[i]) throw python_error();
             }
         } else {
-            PyObject* list = PySequence_Tuple(out);
+            const THPObjectPtr list(PySequence_Tuple(out));
             if (!list) throw python_error();
-            const bool fits = PyTuple_GET_SIZE(list) == count;
-            for (int i = 0; fits && i < count; ++i) {
-                fresh[i] = PyTuple_GET_ITEM(list, i);
-                Py_INCREF(fresh[i]);
+            if (PyTuple_GET_SIZE(list.get()) != count) throw value_error("out must hold %d tensors", count);
+            for (int i = 0; i < count; ++i) {
+                fresh[i] = THPObjectPtr(Py_NewRef(PyTuple_GET_ITEM(list.get(), i)));
+                to[i] = (int32_t*)dense(fresh[i].get(), names[i], at::kInt, dev, old[i]->sizes()).data_ptr();
             }
-            Py_DECREF(list);
-            if (!fits) throw value_error("out must hold %d tensors", count);
-            for (int i = 0; i < count; ++i)
-                to[i] = (int32_t*)dense(fresh[i], names[i], at::kInt, dev, old[i]->sizes()).data_ptr();
         }
         s = hmm_paged_state_t{(const int32_t*)t.data_ptr(), (const int32_t*)r.data_ptr(),
                               kv_len ? (const int32_t*)old[2]->data_ptr() : nullptr, to[0], to[1], to[2], t.size(0),
@@ -471,7 +465,7 @@ struct State {
     PyObject* result(PyObject* more = nullptr) {
         PyObject* r = PyTuple_New(count + (more != nullptr));
         if (!r) throw python_error();
-        for (int i = 0; i < count; ++i) PyTuple_SET_ITEM(r, i, std::exchange(fresh[i], nullptr));
+        for (int i = 0; i < count; ++i) PyTuple_SET_ITEM(r, i, fresh[i].release());
         if (more) PyTuple_SET_ITEM(r, count, more);
         return r;
     }

@@ -1,5 +1,7 @@
 """Page calls whose new state lies in the memory of the old one: refused, and nothing changed;
 in place, array by array, as anywhere else."""
+import sys
+
 import pytest
 import torch
 
@@ -48,3 +50,27 @@ def test_lengths_that_double_in_place(cuda):
     t, r, l, _, _ = dev(m, cuda)
     m.grow(m.kv.copy())
     same(m, *hmm.paged_grow(t, r, l, l, 4, out=(t, r, l)))
+
+
+def test_a_refused_out_is_given_back(cuda):
+    """Refusals keep no reference to the tensors of `out`."""
+    m = state(3, 6, 40, 8, 4, 25)
+    t, r, l, k, v = dev(m, cuda)
+    bad = (torch.empty_like(t), torch.empty_like(r), l[:3])
+    before = [sys.getrefcount(x) for x in bad]
+    for out in (bad, list(bad), bad[:2], bad + bad[:1]):
+        for _ in range(5):
+            with pytest.raises(ValueError):
+                hmm.paged_free(t, r, l, ints([1], cuda), out=out)
+            with pytest.raises(ValueError):
+                hmm.paged_grow(t, r, l, ints([1] * 6, cuda), 4, out=out)
+            with pytest.raises(ValueError):
+                hmm.paged_compact(t, r, k, v, out=(bad[0], bad[2]))
+    del out
+    assert [sys.getrefcount(x) for x in bad] == before
+    good = tuple(torch.empty_like(x) for x in (t, r, l))
+    before = [sys.getrefcount(x) for x in good]
+    got = hmm.paged_free(t, r, l, ints([1], cuda), out=good)
+    assert all(a is b for a, b in zip(got, good))
+    del got
+    assert [sys.getrefcount(x) for x in good] == before
