@@ -6,6 +6,8 @@
 //   (no window or i > p - window or i < sinks)
 #pragma once
 
+#include <float.h>
+
 #include "paged_serve.cuh"
 
 namespace hmm {
@@ -241,14 +243,17 @@ __device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const 
                 l = fmaf(l, al, p);                      // (a lane's share)
                 m = mn;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) acc[c] *= al;
+                for (int c = 0; c < 8; ++c) acc[c] = isinf(acc[c]) ? acc[c] : acc[c] * al;
+                // (a weight is above zero for every score but -inf, too small for fp32 or not)
+                const float some = x == -INFINITY ? 0.0f : fmaxf(p, FLT_MIN);
 #pragma unroll U
                 for (int j = 0; j < lanes; ++j) {
                     const float pj = __shfl_sync(0xffffffffu, p, j * groups + group);
+                    const float sj = __shfl_sync(0xffffffffu, some, j * groups + group);
                     float f[8];
                     unpack8<T>(values(r.v, j), f);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) acc[c] = fmaf(pj, f[c], acc[c]);
+                    for (int c = 0; c < 8; ++c) acc[c] = fmaf(isinf(f[c]) ? sj : pj, f[c], acc[c]);
                 }
             }
 #pragma unroll

@@ -171,3 +171,30 @@ def test_one_bad_value_costs_little(cuda, value, what):
         torch.cuda.synchronize()
         times.append(a.elapsed_time(b))
     assert min(times) < 10, times
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("new", [1, 3, 40, 300])
+@pytest.mark.parametrize("low", [40, 120, 600])
+def test_an_infinity_behind_a_small_weight(cuda, dtype, new, low):
+    """exp(-low) may be nothing in the weights' type or in fp32; it is above zero all the same.
+    Only a score of -inf has no weight: its product with an infinity is NaN."""
+    L, d, pt = 900, 64, 16
+    q, k, v, table, cu, kv_len = make(cuda, 66, [new], [L], 2, 1, d, pt, DT[dtype])
+    q[:] = 0
+    q[..., 0] = 1
+    k.clamp_(-2, 2)
+    ids = table[0].long()
+    for p, col, x in ((5, 1, INF), (300, 2, -INF), (L - new, 3, INF), (299, 4, INF), (500, 4, -INF)):
+        k[ids[p // pt], 0, p % pt, 0] = -low
+        put(v, table, 0, p, pt, col, x)
+    ref = reference(q, k, v, table, [new], [L], scale=1.0)
+    for hint in (0, 1):
+        out, lse = hmm.paged_attention(q, k, v, table, cu, kv_len, scale=1.0, return_lse=True, max_new=hint)
+        check(out, lse, ref)
+        inf = torch.isinf(ref[0])
+        assert inf[..., 1:4].all() and torch.isnan(ref[0][..., 4]).all() and torch.equal(out.double()[inf], ref[0][inf])
+    k[ids[0], 0, 5, 0] = -INF
+    out = hmm.paged_attention(q, k, v, table, cu, kv_len, scale=1.0)
+    check(out, None, reference(q, k, v, table, [new], [L], scale=1.0))
+    assert torch.isnan(out[..., 1]).all()
