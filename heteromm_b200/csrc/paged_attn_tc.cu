@@ -42,7 +42,8 @@
 // tokens, causal: D = 128 455-478 us (1,150-1,210 TFLOP/s, about 4,000 clocks a
 // tile); without the exponentials it is no faster, with the products and loads
 // alone 418: reading K and V into shared memory, 64 KB a tile and CTA, and their
-// reading by both row tiles' products bound it.  D = 64 424 us (650 TFLOP/s): the
+// reading by both row tiles' products bound it (bytes, not boxes: pages of 128 take 459
+// where pages of 16 take 456).  D = 64 424 us (650 TFLOP/s): the
 // softmax warps' instructions do; exponentials moved to the FMA pipe only add (1 of
 // 8: 437).
 #include <cudaTypedefs.h>

@@ -2,7 +2,7 @@
 // arguments, outputs and scratch memory from torch's allocator, the current stream, the
 // call.  A serving step makes a call per layer, on the host's critical path when few
 // tokens are decoded: through ctypes and checks in Python a call took 21 us of the host
-// (6.5 of them the two launches), more than the kernels of a small step; here about 9.
+// (6.5 of them the two launches), more than the kernels of a small step; here 8.
 //
 // Positional arguments only, in the order that serve.py documents and passes.  The C entry
 // points come as addresses (bind), so that the library is the one that _abi loads.
