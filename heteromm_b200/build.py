@@ -16,6 +16,7 @@ the repository snapshot to the GPU machine.
 """
 from __future__ import annotations
 
+import contextlib
 import glob
 import hashlib
 import os
@@ -100,21 +101,35 @@ def build_py_kernels(force: bool = False) -> str:
     return out
 
 
-def serve_calls_path() -> str:
-    """Where the module is for this torch, this Python and these sources: one built for or
-    from others has another name."""
+def _serve_calls_sources() -> list[str]:
+    return [os.path.join(PKG, "src", "py", "serve_calls.cpp"), os.path.join(INC, "heteromm_cuda.h")]
+
+
+def _serve_calls_name(digest: str) -> str:
+    """The module's file for this torch, this Python and sources of this digest: one built for
+    or from others has another name."""
     import sysconfig
     import torch
+    return os.path.join(LIB_DIR, f"heteromm_serve_calls-torch{torch.__version__.replace('+', '_')}-"
+                                 f"{digest}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+def _built_serve_calls() -> list[str]:
+    """Those built for this torch and Python, from whatever sources."""
+    before, after = _serve_calls_name("*").split("*")
+    return sorted(glob.glob(glob.escape(before) + "*" + glob.escape(after)))
+
+
+def serve_calls_path() -> str:
+    """Where the module for this torch, this Python and these sources is or will be; without
+    the sources, the one that was built ("" if there is none)."""
+    if not all(map(os.path.exists, _serve_calls_sources())):
+        return (_built_serve_calls() or [""])[-1]
     digest = hashlib.sha256()
     for f in _serve_calls_sources():
         with open(f, "rb") as src:
             digest.update(src.read())
-    return os.path.join(LIB_DIR, f"heteromm_serve_calls-torch{torch.__version__.replace('+', '_')}-"
-                                 f"{digest.hexdigest()[:12]}{sysconfig.get_config_var('EXT_SUFFIX')}")
-
-
-def _serve_calls_sources() -> list[str]:
-    return [os.path.join(PKG, "src", "py", "serve_calls.cpp"), os.path.join(INC, "heteromm_cuda.h")]
+    return _serve_calls_name(digest.hexdigest()[:12])
 
 
 def build_serve_calls(force: bool = False) -> str:
@@ -125,30 +140,31 @@ def build_serve_calls(force: bool = False) -> str:
         import torch
     except ImportError:
         return ""
+    out = serve_calls_path()
+    if out == "" or (not force and os.path.exists(out)):
+        return out
     home = os.path.dirname(torch.__file__)
     include, lib = os.path.join(home, "include"), os.path.join(home, "lib")
     if not os.path.exists(os.path.join(include, "torch", "csrc", "Exceptions.h")) or \
             not os.path.exists(os.path.join(lib, "libc10_cuda.so")):
         return ""
-    out = serve_calls_path()
-    if force or not os.path.exists(out):
-        os.makedirs(LIB_DIR, exist_ok=True)
-        # (renamed when it is whole: another process may look for it, or build it too)
-        part = f"{out}.{os.getpid()}.{threading.get_ident()}"
-        try:
-            _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                  f"-isystem{include}", f"-isystem{os.path.join(include, 'torch', 'csrc', 'api', 'include')}",
-                  "-I/usr/local/cuda/include", f"-I{sysconfig.get_paths()['include']}", f"-I{INC}", "-o", part,
-                  _serve_calls_sources()[0], f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
-                  "-lc10_cuda"])
-            os.replace(part, out)
-        finally:
-            if os.path.exists(part):
-                os.remove(part)
-        kind = out[:-len(sysconfig.get_config_var("EXT_SUFFIX")) - 12]   # for this torch, from older sources
-        for old in glob.glob(glob.escape(kind) + "*" + sysconfig.get_config_var("EXT_SUFFIX")):
-            if old != out:
+    os.makedirs(LIB_DIR, exist_ok=True)
+    # (renamed when it is whole: another process may look for it, or build it too)
+    part = f"{out}.{os.getpid()}.{threading.get_ident()}"
+    try:
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              f"-isystem{include}", f"-isystem{os.path.join(include, 'torch', 'csrc', 'api', 'include')}",
+              "-I/usr/local/cuda/include", f"-I{sysconfig.get_paths()['include']}", f"-I{INC}", "-o", part,
+              _serve_calls_sources()[0], f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+              "-lc10_cuda"])
+        os.replace(part, out)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    for old in _built_serve_calls():   # from older sources
+        if old != out:
+            with contextlib.suppress(FileNotFoundError):
                 os.remove(old)
     return out
 

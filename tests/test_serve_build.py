@@ -83,11 +83,21 @@ def test_two_builds_at_once(tree):
 
 def test_without_headers_the_rest_is_built(tree, monkeypatch, tmp_path):
     monkeypatch.setattr(torch, "__file__", str(tmp_path / "nowhere" / "__init__.py"))
+    assert not os.path.exists(B.LIB_DIR)
     assert B.build_serve_calls() == "" and tree[2] == []
     with pytest.raises(RuntimeError, match="headers"):
         serve._Calls().attention
     monkeypatch.setitem(sys.modules, "torch", None)   # import torch fails
     assert B.build_serve_calls() == ""
+
+
+def test_without_sources_what_was_built_is_taken(tree):
+    pkg, inc, runs = tree
+    out = B.build_serve_calls()
+    os.remove(inc / "heteromm_cuda.h")
+    assert B.build_serve_calls() == out and len(runs) == 1
+    os.remove(out)
+    assert B.build_serve_calls() == "" and len(runs) == 1
 
 
 def test_threads_that_call_first(monkeypatch):
