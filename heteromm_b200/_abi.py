@@ -24,13 +24,19 @@ _I = C.c_int64
 _F = C.c_float
 _S = C.c_size_t
 
-HMM_DTYPE_BF16, HMM_DTYPE_F16, HMM_DTYPE_F32 = 0, 1, 2
+HMM_DTYPE_BF16, HMM_DTYPE_F16, HMM_DTYPE_F32, HMM_DTYPE_E4M3, HMM_DTYPE_I8 = 0, 1, 2, 3, 4
 
 
 class PagedCache(C.Structure):     # hmm_paged_cache_t
     _fields_ = [("k", _P), ("v", _P)] + [(n, _I) for n in (
         "n_pages", "n_kv_heads", "page_tokens", "D", "k_page", "k_head", "k_token", "v_page",
         "v_head", "v_token")] + [("dtype", C.c_int32)]
+
+
+class PagedQuant(C.Structure):     # hmm_paged_quant_t
+    _fields_ = [("k", _P), ("v", _P)] + [(n, _I) for n in (
+        "n_pages", "n_kv_heads", "page_tokens", "D", "k_page", "k_head", "v_page", "v_head")] + \
+               [("codes", C.c_int32)]
 
 
 class PagedBatch(C.Structure):     # hmm_paged_batch_t
@@ -87,6 +93,9 @@ SIGNATURES = {
     "hmm_paged_attention_workspace_size": (_S, [_I, _I, _I, _I, _I]),
     "hmm_paged_attention": (C.c_int, [_P, _P, _P, _I, _I, _I, _F, C.c_int, _I, _I, _I, _P, _P, _P,
                                       _P, _S, _P]),
+    "hmm_paged_quant_append": (C.c_int, [_P, _P, C.c_int, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P,
+                                         C.c_int, _F, _P, _I, _I, C.c_int, _P, _P, _I, _I, _P, _P]),
+    "hmm_paged_quant_read": (C.c_int, [_P, _P, C.c_int, _P, _P, _P, _P]),
     "hmm_paged_state_workspace_size": (_S, [_I, _I]),
     "hmm_paged_copy_pages": (C.c_int, [_P, _P, _P, _I, _P, _P, _S, _P]),
     "hmm_paged_free": (C.c_int, [_P, _P, _I, _P, _P, _S, _P]),

@@ -34,7 +34,9 @@ from ._abi import HmmError, last_error, load
 # once per layer and token, where checks in Python take longer than the kernels.
 _ENTRIES = ("hmm_paged_kv_append", "hmm_paged_attention", "hmm_paged_attention_workspace_size",
             "hmm_paged_state_workspace_size", "hmm_paged_copy_pages", "hmm_paged_free", "hmm_paged_fork",
-            "hmm_paged_grow", "hmm_paged_compact", "hmm_status_read")
+            "hmm_paged_grow", "hmm_paged_compact", "hmm_status_read", "hmm_paged_quant_append",
+            "hmm_paged_quant_read")
+_CALLS = ("attention", "append", "copy_pages", "free", "fork", "grow", "compact", "quant_append", "quant_read")
 
 
 def _raise(name: str, status: int):
@@ -47,7 +49,7 @@ class _Calls:
     _lock = threading.Lock()
 
     def __getattr__(self, name: str):
-        if name not in ("attention", "append", "copy_pages", "free", "fork", "grow", "compact"):
+        if name not in _CALLS:
             raise AttributeError(name)
         with self._lock:
             if name not in self.__dict__:     # (another thread's first call was quicker)
@@ -57,8 +59,8 @@ class _Calls:
                 spec = importlib.util.spec_from_file_location("heteromm_serve_calls", path)
                 native = importlib.util.module_from_spec(spec)
                 lib = load()
-                native.bind(*(C.cast(getattr(lib, e), C.c_void_p).value for e in _ENTRIES), _raise)
-                for f in ("attention", "append", "copy_pages", "free", "fork", "grow", "compact"):
+                native.bind(tuple(C.cast(getattr(lib, e), C.c_void_p).value for e in _ENTRIES), _raise)
+                for f in _CALLS:
                     setattr(self, f, getattr(native, f))
         return self.__dict__[name]
 
@@ -111,6 +113,50 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     helps to choose the kernel (decoding: 1); results do not depend on it."""
     return _calls.attention(q, k_pages, v_pages, page_table, cu_new, kv_len, causal, window, sinks, scale, max_new,
                             return_lse, out, status)
+
+
+# ------------------------------------------------------------------ a cache held in 8 bits
+
+
+def quant_pages(n_pages: int, n_kv_heads: int, page_tokens: int, D: int, dtype=torch.float8_e4m3fn,
+                device="cuda") -> torch.Tensor:
+    """A page array (of keys, or of values) for a cache held in 8 bits, all zeros:
+    [n_pages, n_kv_heads, page_tokens, D + D / 32] of float8_e4m3fn or int8.
+
+    Of each page and head the first page_tokens * D bytes are the tokens' codes, the rest
+    the scale bytes s of each 32 values of a token: a value is code * 2^(s - 127).  D is a
+    multiple of 32 (to 256), page_tokens * D / 32 one of 16.  paged_copy_pages, paged_fork
+    and paged_compact move such pages as any others."""
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise TypeError(f"dtype must be torch.float8_e4m3fn or torch.int8, got {dtype}")
+    if D < 32 or D > 256 or D % 32:
+        raise ValueError(f"D must be a multiple of 32 in [32, 256], got {D}")
+    if page_tokens < 1 or page_tokens * (D // 32) % 16:
+        raise ValueError(f"page_tokens * D / 32 must be a multiple of 16, got pages of {page_tokens} tokens and D {D}")
+    return torch.zeros((n_pages, n_kv_heads, page_tokens, D + D // 32), dtype=torch.uint8, device=device).view(dtype)
+
+
+def paged_quant_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                       page_table: torch.Tensor, cu_new: torch.Tensor, kv_len: torch.Tensor,
+                       rope: torch.Tensor | None = None, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+                       interleaved: bool = False, positions=None, out: torch.Tensor | None = None,
+                       status: torch.Tensor | None = None):
+    """paged_kv_append into a cache held in 8 bits (quant_pages): q, k, v are bf16 or fp16
+    (int16: bf16 bits), the queries come back in that type, keys (normed and turned, in fp32)
+    and values are rounded to codes, each 32 with the smallest power of two that holds
+    them; a group with an infinity or NaN reads as NaN."""
+    return _calls.quant_append(q, k, v, k_pages, v_pages, page_table, cu_new, kv_len, rope, q_weight, k_weight, eps,
+                               interleaved, positions, out, status)
+
+
+def paged_quant_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu: torch.Tensor,
+                     kv_len: torch.Tensor, n_rows: int, *, dtype=torch.bfloat16, out=None,
+                     status: torch.Tensor | None = None):
+    """(k, v) [n_rows, n_kv_heads, D] of bf16, fp16 or fp32: the last cu[s + 1] - cu[s] tokens
+    of every sequence s as the cache holds them (exact in each type), in rows
+    [cu[s], cu[s + 1]).  With a step's cu_new those it appended, with the sums of kv_len
+    the whole cache.  `out` may hold the two tensors."""
+    return _calls.quant_read(k_pages, v_pages, page_table, cu, kv_len, n_rows, dtype, out, status)
 
 
 # ------------------------------------------------------------------ pages

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <cstring>
 #include <sstream>
 #include <utility>
 
@@ -45,20 +46,30 @@ struct Entry {
     decltype(&hmm_paged_grow) grow;
     decltype(&hmm_paged_compact) compact;
     decltype(&hmm_status_read) status_read;
+    decltype(&hmm_paged_quant_append) quant_append;
+    decltype(&hmm_paged_quant_read) quant_read;
 };
 Entry hmm_fn{};
 PyObject* raise_error = nullptr;   // (entry point's name, status): raises HmmError
 
+// (addresses in Entry's order, raise)
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long p[10];
-    PyObject* raise;
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKKO", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
-                          &raise))
+    PyObject *addresses, *raise;
+    if (!PyArg_ParseTuple(args, "O!O", &PyTuple_Type, &addresses, &raise)) return nullptr;
+    constexpr Py_ssize_t n = sizeof(Entry) / sizeof(void*);
+    void* p[n];
+    if (PyTuple_GET_SIZE(addresses) != n) {
+        PyErr_Format(PyExc_ValueError, "%zd addresses, not %zd", n, PyTuple_GET_SIZE(addresses));
         return nullptr;
-    hmm_fn = Entry{(decltype(Entry::append))p[0], (decltype(Entry::attention))p[1],
-                   (decltype(Entry::attention_workspace))p[2], (decltype(Entry::state_workspace))p[3],
-                   (decltype(Entry::copy))p[4], (decltype(Entry::free))p[5], (decltype(Entry::fork))p[6],
-                   (decltype(Entry::grow))p[7], (decltype(Entry::compact))p[8], (decltype(Entry::status_read))p[9]};
+    }
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, i));
+        if (!p[i]) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null address");
+            return nullptr;
+        }
+    }
+    memcpy(&hmm_fn, p, sizeof hmm_fn);
     Py_INCREF(raise);
     raise_error = raise;
     Py_RETURN_NONE;
@@ -223,6 +234,30 @@ Cache cache(PyObject* k_pages, PyObject* v_pages) {
                  k.scalar_type(), (int)k.get_device()};
 }
 
+// A cache held in 8 bits: [n_pages, n_kv_heads, page_tokens, D + D / 32], a block per page and head.
+struct QuantCache {
+    hmm_paged_quant_t c;
+    int dev;
+};
+
+QuantCache quant_cache(PyObject* k_pages, PyObject* v_pages) {
+    const Tensor &k = on_gpu(k_pages, "k_pages"), &v = on_gpu(v_pages, "v_pages");
+    const ScalarType t = k.scalar_type();
+    if (t != at::kFloat8_e4m3fn && t != at::kChar)
+        throw type_error("k_pages must be float8_e4m3fn or int8, got %s", name_of(t).c_str());
+    if (v.scalar_type() != t || v.sizes() != k.sizes() || v.get_device() != k.get_device())
+        throw value_error("k_pages and v_pages differ in shape, dtype or device");
+    const Four a = four(k, "k_pages"), b = four(v, "v_pages");
+    if (a.n[3] == 0 || a.n[3] % 33 != 0)
+        throw value_error("k_pages must be [n_pages, n_kv_heads, page_tokens, D + D / 32], got rows of %d", (int)a.n[3]);
+    for (const Four* f : {&a, &b})
+        if (f->n[2] > 1 && f->st[2] != f->n[3])
+            throw value_error("%s: a page and head must be one block of memory", f == &a ? "k_pages" : "v_pages");
+    return QuantCache{{k.data_ptr(), v.data_ptr(), a.n[0], a.n[1], a.n[2], a.n[3] / 33 * 32, a.st[0], a.st[1], b.st[0],
+                       b.st[1], t == at::kChar ? HMM_DTYPE_I8 : HMM_DTYPE_E4M3},
+                      (int)k.get_device()};
+}
+
 const Tensor& page_table(PyObject* o, int dev) {
     const Tensor& t = dense(o, "page_table", at::kInt, dev);
     if (t.dim() != 2) throw value_error("page_table must be [n_seq, pages_per_seq]");
@@ -321,13 +356,26 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 
 // q, k, v, k_pages, v_pages, page_table, cu_new, kv_len, rope, q_weight, k_weight, eps,
 // interleaved, positions, out, status
+// (QUANT: into a cache held in 8 bits, whose vectors are of k's type)
+template <bool QUANT>
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     arguments(n_args, 16);
-    const Cache c = cache(a[3], a[4]);
-    const int64_t d = c.c.D, hk = c.c.n_kv_heads;
     const Tensor& k = on_gpu(a[1], "k");
     if (k.dim() != 3) throw value_error("k must be [n_tokens, n_kv_heads, D]");
+    Cache c{};
+    QuantCache qc{};
+    if constexpr (QUANT) {
+        qc = quant_cache(a[3], a[4]);
+        c.dtype = k.scalar_type();
+        c.c.dtype = code_of(c.dtype, "k");
+        c.c.D = qc.c.D;
+        c.c.n_kv_heads = qc.c.n_kv_heads;
+        c.dev = qc.dev;
+    } else {
+        c = cache(a[3], a[4]);
+    }
+    const int64_t d = c.c.D, hk = c.c.n_kv_heads;
     const int64_t n_tokens = k.size(0);
     const Rows kr = rows(a[1], "k", c.dtype, c.dev, {n_tokens, hk, d}),
                vr = rows(a[2], "v", c.dtype, c.dev, {n_tokens, hk, d});
@@ -376,14 +424,58 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const bool interleaved = truth(a[12]);
     const Status status = status_word(a[15], c.dev, at.stream);
     finish(unlocked([&] {
+               if constexpr (QUANT)
+                   return hmm_fn.quant_append(&qc.c, &b, c.c.dtype, qr.p, qr.token, qr.head, heads, kr.p, kr.token, kr.head,
+                                              vr.p, vr.token, vr.head, w[0], w[1], wdt, eps, rope, n_pos, rotary, interleaved,
+                                              positions, outr.p, outr.token, outr.head, status.p, at.stream);
                return hmm_fn.append(&c.c, &b, qr.p, qr.token, qr.head, heads, kr.p, kr.token, kr.head, vr.p, vr.token,
                                     vr.head, w[0], w[1], wdt, eps, rope, n_pos, rotary, interleaved, positions, outr.p,
                                     outr.token, outr.head, status.p, at.stream);
            }),
-           "hmm_paged_kv_append", status, at.stream);
+           QUANT ? "hmm_paged_quant_append" : "hmm_paged_kv_append", status, at.stream);
     if (out.defined()) return THPVariable_Wrap(std::move(out));
     Py_INCREF(a[14]);
     return a[14];
+    END_HANDLE_TH_ERRORS
+}
+
+// k_pages, v_pages, page_table, cu, kv_len, n_rows, dtype, out, status
+PyObject* quant_read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    arguments(n_args, 9);
+    const QuantCache c = quant_cache(a[0], a[1]);
+    const int64_t n_rows = whole(a[5]);
+    if (n_rows < 0) throw value_error("n_rows must be >= 0, got %lld", (long long)n_rows);
+    if (!THPDtype_Check(a[6])) throw type_error("dtype must be a torch.dtype");
+    const ScalarType t = ((THPDtype*)a[6])->scalar_type;
+    if (t != at::kBFloat16 && t != at::kHalf && t != at::kFloat)
+        throw type_error("dtype must be torch.bfloat16, torch.float16 or torch.float32, got %s", name_of(t).c_str());
+    const hmm_paged_batch_t b = batch(a[2], a[3], a[4], n_rows, c.dev);
+    const Place at(c.dev);
+    const int64_t shape[3] = {n_rows, c.c.n_kv_heads, c.c.D};
+    THPObjectPtr out[2];
+    void* p[2];
+    if (a[7] == Py_None) {
+        for (int i = 0; i < 2; ++i) {
+            Tensor x = empty(shape, t, c.dev);
+            p[i] = x.data_ptr();
+            out[i] = THPObjectPtr(THPVariable_Wrap(std::move(x)));
+            if (!out[i]) throw python_error();
+        }
+    } else {
+        const THPObjectPtr list(PySequence_Tuple(a[7]));
+        if (!list) throw python_error();
+        if (PyTuple_GET_SIZE(list.get()) != 2) throw value_error("out must hold 2 tensors");
+        for (int i = 0; i < 2; ++i) {
+            out[i] = THPObjectPtr(Py_NewRef(PyTuple_GET_ITEM(list.get(), i)));
+            p[i] = dense(out[i].get(), i == 0 ? "out k" : "out v", t, c.dev, shape).data_ptr();
+        }
+    }
+    const Status status = status_word(a[8], c.dev, at.stream);
+    const int dtype = t == at::kBFloat16 ? HMM_DTYPE_BF16 : t == at::kHalf ? HMM_DTYPE_F16 : HMM_DTYPE_F32;
+    finish(unlocked([&] { return hmm_fn.quant_read(&c.c, &b, dtype, p[0], p[1], status.p, at.stream); }),
+           "hmm_paged_quant_read", status, at.stream);
+    return Py_BuildValue("(NN)", out[0].release(), out[1].release());
     END_HANDLE_TH_ERRORS
 }
 
@@ -577,7 +669,9 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"attention", FAST(attention)},
-                         {"append", FAST(append)},
+                         {"append", FAST(append<false>)},
+                         {"quant_append", FAST(append<true>)},
+                         {"quant_read", FAST(quant_read)},
                          {"copy_pages", FAST(copy_pages)},
                          {"free", FAST(free_)},
                          {"fork", FAST(fork_)},

@@ -412,6 +412,49 @@ hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged
                                  int64_t max_new, void* out, float* lse, int32_t* device_status,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* A paged cache held in 8 bits.  Of each page and head one block of
+ * page_tokens * (D + D / 32) bytes: the codes [page_tokens][D], then a scale
+ * byte s for each 32 values of a token [page_tokens][D / 32]:
+ *   value = code * 2^(s - 127), code e4m3 (HMM_DTYPE_E4M3) or int8 (HMM_DTYPE_I8)
+ * Page and head strides in bytes (multiples of 16), 16-byte aligned; D % 32 ==
+ * 0, 32 <= D <= 256; page_tokens * D / 32 a multiple of 16.  A page's bytes are
+ * moved as any page's (hmm_page_store_t).  A group of 32 is stored with the
+ * smallest scale that holds its largest magnitude A, A <= M 2^e (M = 448 or
+ * 127), e held to [-15, 7] (e4m3) or [-22, 7], and codes rounded to the nearest
+ * (ties to even) and saturated at M: values beyond 57,344 (16,256) are cut.  A
+ * group with an infinity or NaN has s = 255 and reads as NaN.  Every value is a
+ * bf16 and an fp16 number exactly.  (Codes of e4m3's NaN and other scale bytes
+ * than these, which no call writes, are not told apart.) */
+#define HMM_DTYPE_E4M3 3
+#define HMM_DTYPE_I8 4
+typedef struct {
+    void* k;
+    void* v;
+    int64_t n_pages, n_kv_heads, page_tokens, D;
+    int64_t k_page, k_head, v_page, v_head;   /* strides in bytes */
+    int32_t codes;                            /* HMM_DTYPE_E4M3 or HMM_DTYPE_I8 */
+} hmm_paged_quant_t;
+
+/* hmm_paged_kv_append into a cache held in 8 bits: q, k, v, q_out and the norm
+ * weights of `dtype` (HMM_DTYPE_BF16 or HMM_DTYPE_F16), all else as there; keys
+ * are rounded once, from fp32 to codes. */
+hmm_status_t hmm_paged_quant_append(
+    const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype, const void* q, int64_t q_token,
+    int64_t q_head, int64_t n_heads, const void* k, int64_t k_token, int64_t k_head, const void* v,
+    int64_t v_token, int64_t v_head, const void* q_weight, const void* k_weight, int weight_dtype,
+    float eps, const float* rope, int64_t n_pos, int64_t rotary_dim, int interleaved,
+    const int32_t* positions, void* q_out, int64_t out_token, int64_t out_head,
+    int32_t* device_status, void* stream);
+
+/* Reads tokens back: row cu_new[s] + j of k_out and v_out [n_tokens][n_kv_heads]
+ * [D] (contiguous, 16-byte aligned; HMM_DTYPE_BF16, _F16 or _F32: exact in each)
+ * is the token that an append of the same batch wrote, of sequence s at position
+ * kv_len[s] - n[s] + j; with n[s] = kv_len[s] all that is cached.  Rows that no
+ * sequence owns are left as they are; one whose page is out of bounds is flagged
+ * and skipped. */
+hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
+                                  void* k_out, void* v_out, int32_t* device_status, void* stream);
+
 /* Page management.  The state is the page table [n_seq][pages_per_seq] (an
  * entry below 0 holds no page), the references [n_pages] of each page (0 =
  * free) and kv_len [n_seq].  Every call reads the state from *_in and writes
