@@ -8,7 +8,7 @@
 
 #include <float.h>
 
-#include "paged_serve.cuh"
+#include "paged_quant.cuh"
 
 namespace hmm {
 namespace serve {
@@ -36,6 +36,8 @@ struct AttnArgs {
     int64_t q_token, q_head;
     unsigned char* out;          // [n_tokens][hq][D], contiguous
     float* lse;                  // [n_tokens][hq] or null
+    float* part;                 // null, or where rows go in fp32 instead of `out` (each part of a batch of shared prefixes)
+    QuantRows quant;             // of a cache in 8 bits
     float scale, scale_log2;     // scale * log2(e)
     int causal, window, sinks;
     int hq, hk, group, D, page_tokens, n_pages;
@@ -43,6 +45,26 @@ struct AttnArgs {
     int64_t max_kv;
     int32_t* status;
 };
+
+// A call's arguments beside the cache and the batch, as the ABI has them, and the bytes that
+// its workspace needs.
+struct AttnCall {
+    const void* q;
+    int64_t q_token, q_head, n_heads;
+    float scale;
+    int causal;
+    int64_t window, sinks, max_new;
+    void* out;
+    float* lse;
+    int32_t* status;
+    void* workspace;
+    size_t workspace_bytes, need;
+};
+
+// Checks them for a cache of `dims`, and fills *a but for the pages and a->b; *nothing: no
+// rows to compute.
+hmm_status_t plan_attention(const AttnCall& c, const hmm_paged_cache_t& dims, const hmm_paged_batch_t* batch, bool quant,
+                            AttnArgs* a, bool* nothing);
 
 // A row of a unit (sequence, KV head): row r is new token r / group, head r % group.
 struct Span {                    // keys [0, sink) and [lo, hi) hold all that some row of a tile sees
@@ -52,7 +74,7 @@ struct Span {                    // keys [0, sink) and [lo, hi) hold all that so
 
 // -1 for a row before the first cached token: it sees nothing.
 __device__ __forceinline__ int row_pos(const AttnArgs& a, const Seq& q, int row) {
-    return max(-1, q.kv - q.n_new + a.by_group(row));
+    return max(-1, q.pos0 + a.by_group(row));
 }
 
 __device__ __forceinline__ Span tile_span(const AttnArgs& a, const Seq& q, int row0, int row1) {
@@ -60,7 +82,7 @@ __device__ __forceinline__ Span tile_span(const AttnArgs& a, const Seq& q, int r
     s.p0 = row_pos(a, q, row0);
     s.p1 = row_pos(a, q, row1 - 1);
     s.hi = a.causal ? max(0, min(q.kv, s.p1 + 1)) : q.kv;
-    s.lo = a.window > 0 ? min(s.hi, max(0, s.p0 - a.window + 1)) : 0;
+    s.lo = min(s.hi, a.window > 0 ? max(0, s.p0 - a.window + 1) : q.lo);   // (not both)
     s.sink = a.window > 0 ? min(a.sinks, s.lo) : 0;
     return s;
 }
@@ -69,14 +91,14 @@ __device__ __forceinline__ bool span_has(const Span& s, int key) {
     return key < s.sink || (key >= s.lo && key < s.hi);
 }
 
-__device__ __forceinline__ bool sees(const AttnArgs& a, int kv, int pos, int key) {
-    return key < kv && (!a.causal || key <= pos) &&
-           (a.window <= 0 || key > pos - a.window || key < a.sinks);
+__device__ __forceinline__ bool sees(const AttnArgs& a, const Seq& q, int pos, int key) {
+    return key < q.kv && (!a.causal || key <= pos) &&
+           (a.window > 0 ? key > pos - a.window || key < a.sinks : key >= q.lo);
 }
 
-// The physical page of a token, or -1 with HMM_STATUS_PAGE_BOUNDS set.
-__device__ __forceinline__ int page_of(const AttnArgs& a, int s, int logical) {
-    const int e = __ldg(a.b.table + (int64_t)s * a.b.pages_per_seq + logical);
+// The physical page of a token in a row of the table, or -1 with HMM_STATUS_PAGE_BOUNDS set.
+__device__ __forceinline__ int page_of(const AttnArgs& a, int row, int logical) {
+    const int e = __ldg(a.b.table + (int64_t)row * a.b.pages_per_seq + logical);
     if (e >= 0 && e < a.n_pages) return e;
     atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
     return -1;
@@ -90,15 +112,18 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr float LN2 = 0.693147180559945309417f;
 
-// A key's K and V rows; null if its page is flagged.
+// A key's K and V rows and, in a cache of 8 bits, their scale bytes; null if its page is flagged.
 struct KeyRows {
-    const unsigned char *k, *v;
+    const unsigned char *k, *v, *ks, *vs;
 };
-__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int s, int kvh, int key) {
-    const int lp = a.by_page(key), phys = page_of(a, s, lp), in = key - lp * a.page_tokens;
-    if (phys < 0) return KeyRows{nullptr, nullptr};
-    return KeyRows{a.k.base + phys * a.k.page + kvh * a.k.head + in * a.k.token,
-                   a.v.base + phys * a.v.page + kvh * a.v.head + in * a.v.token};
+template <int C>
+__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int row, int kvh, int key) {
+    const int lp = a.by_page(key), phys = page_of(a, row, lp), in = key - lp * a.page_tokens;
+    if (phys < 0) return KeyRows{nullptr, nullptr, nullptr, nullptr};
+    const unsigned char *k = a.k.base + phys * a.k.page + kvh * a.k.head, *v = a.v.base + phys * a.v.page + kvh * a.v.head;
+    const int64_t s = a.quant.scales + (int64_t)in * a.quant.per_token;
+    return KeyRows{k + in * a.k.token, v + in * a.v.token, C == CODEC_NONE ? nullptr : k + s,
+                   C == CODEC_NONE ? nullptr : v + s};
 }
 
 template <typename T>
@@ -117,6 +142,28 @@ template <typename T>
 __device__ __forceinline__ bool any_not_finite(const uint4& w) {
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
     return (__vcmpeq2(w.x & E, E) | __vcmpeq2(w.y & E, E) | __vcmpeq2(w.z & E, E) | __vcmpeq2(w.w & E, E)) != 0u;
+}
+
+// Eight values of a row as they lie in the cache, and in fp32; of 8 bits: codes, and their
+// scale byte behind them.
+template <int C>
+__device__ __forceinline__ uint4 load_eight(const unsigned char* row, const unsigned char* scales, int c) {
+    if (C == CODEC_NONE) return __ldg(reinterpret_cast<const uint4*>(row) + c);
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(row) + c);
+    return make_uint4(w.x, w.y, __ldg(scales + (c >> 2)), 0u);
+}
+template <typename T, int C>
+__device__ __forceinline__ void eight(const uint4& w, float* f) {
+    if (C == CODEC_NONE) {
+        unpack8<T>(w, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = value_of<C>((i < 4 ? w.x : w.y) >> (8 * (i & 3)) & 255u, w.z);
+    }
+}
+template <typename T, int C>
+__device__ __forceinline__ bool eight_not_finite(const uint4& w) {
+    return C == CODEC_NONE ? any_not_finite<T>(w) : w.z == 255u;
 }
 
 // The columns that came out not finite of rows row0 + i, bit i of `rows`, from the
@@ -138,14 +185,14 @@ __device__ __forceinline__ bool any_not_finite(const uint4& w) {
 // of a unit see and others do not, the last key's: 16 ms.
 // U: loops are unrolled so far.  The code is never reached as a rule, but its size is felt by
 // kernels that stream (the decode batch 351 -> 355 us with 16 in the join; 352 with 1).
-template <typename T, int U>
-__device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const Seq q, int kvh, int row0, unsigned rows) {
+template <typename T, int C, int U>
+__device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, const Seq q, int kvh, int row0, unsigned rows) {
     const int lane = threadIdx.x & 31, vecs = a.D / 8;
     const int lanes = vecs > 1 ? 2 << (31 - __clz(vecs - 1)) : 1, groups = 32 / lanes;   // of a V row
     const int gl = lane & (lanes - 1), group = lane / lanes;
     auto result = [&](int i) {   // the lane's columns of row row0 + i
         const int r = row0 + i, tok = a.by_group(r);
-        return a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + kvh * a.group + r - tok * a.group) * a.D + 8 * gl);
+        return a.out + 2 * (((int64_t)(q.out + tok) * a.hq + kvh * a.group + r - tok * a.group) * a.D + 8 * gl);
     };
     auto bad_columns = [&](int i, uint32_t* nan, uint32_t* inf) {   // a bit per column
         float f[8];
@@ -157,12 +204,17 @@ __device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const 
             *inf |= (isinf(f[c]) ? 1u : 0u) << c;
         }
     };
-    auto values = [&](const unsigned char* v, int i) {   // of the i-th of a group's `lanes` keys
-        const unsigned char* p = reinterpret_cast<const unsigned char*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), i * groups + group));
-        return p && gl < vecs ? __ldg(reinterpret_cast<const uint4*>(p) + gl) : make_uint4(0u, 0u, 0u, 0u);
+    auto values = [&](const KeyRows& r, int i) {   // of the i-th of a group's `lanes` keys
+        auto from = [&](const unsigned char* p) {
+            return reinterpret_cast<const unsigned char*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), i * groups + group));
+        };
+        const unsigned char *p = from(r.v), *ps = C == CODEC_NONE ? nullptr : from(r.vs);
+        return p && gl < vecs ? load_eight<C>(p, ps, gl) : make_uint4(0u, 0u, 0u, 0u);
     };
-    auto rows_of = [&](int key, int end) { return key < end ? key_rows(a, s, kvh, key) : KeyRows{nullptr, nullptr}; };
+    auto rows_of = [&](int key, int end) {
+        return key < end ? key_rows<C>(a, q.row, kvh, key) : KeyRows{nullptr, nullptr, nullptr, nullptr};
+    };
     uint32_t met = 0;   // NaN, inf, -inf seen in the lane's columns, a byte each
     auto met_nan = [&] { return (met | (met >> 8 & met >> 16)) & 0xffu; };
     auto undecided = [&](uint32_t nan, uint32_t inf) { return (nan | (inf & ~(met >> 8 | met >> 16))) & ~met_nan(); };
@@ -173,10 +225,10 @@ __device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const 
             const KeyRows next = rows_of(k0 + 32 + lane, k1);
 #pragma unroll U
             for (int i = 0; i < lanes; ++i) {
-                const uint4 w = values(r.v, i);
-                if (any_not_finite<T>(w)) {
+                const uint4 w = values(r, i);
+                if (eight_not_finite<T, C>(w)) {
                     float f[8];
-                    unpack8<T>(w, f);
+                    eight<T, C>(w, f);
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
                         met |= (f[c] != f[c] ? 1u : f[c] == INFINITY ? 0x100u : f[c] == -INFINITY ? 0x10000u : 0u) << c;
@@ -229,7 +281,7 @@ __device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const 
 #pragma unroll U < 8 ? U : 8
                     for (int c = 0; c < vecs; ++c) {
                         float kf[8], qf[8];
-                        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(r.k) + c), kf);
+                        eight<T, C>(load_eight<C>(r.k, r.ks, c), kf);
                         unpack8<T>(__ldg(qr + c), qf);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x = fmaf(qf[e], kf[e], x);
@@ -251,7 +303,7 @@ __device__ __forceinline__ void attn_rows_exact(const AttnArgs& a, int s, const 
                     const float pj = __shfl_sync(0xffffffffu, p, j * groups + group);
                     const float sj = __shfl_sync(0xffffffffu, some, j * groups + group);
                     float f[8];
-                    unpack8<T>(values(r.v, j), f);
+                    eight<T, C>(values(r, j), f);
 #pragma unroll
                     for (int c = 0; c < 8; ++c) acc[c] = fmaf(isinf(f[c]) ? sj : pj, f[c], acc[c]);
                 }
@@ -308,12 +360,16 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (i0 + k * (int)blockDim.x >= all) continue;
+            const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
+            const int64_t at = ((int64_t)(q.out + tok) * a.hq + head) * a.D + 4 * col[k];
+            if (a.part) {   // (what joins the parts looks for rows that are not finite)
+                *reinterpret_cast<float4*>(a.part + at) = x[k];
+                continue;
+            }
             if ((!isfinite(x[k].x) || !isfinite(x[k].y) || !isfinite(x[k].z) || !isfinite(x[k].w)) &&
                 !isnan(top[row[k] * pieces]))
                 atomicOr(again, 1 << row[k]);
-            const int tok = a.by_group(row0 + row[k]), head = kvh * a.group + row0 + row[k] - tok * a.group;
-            *reinterpret_cast<uint2*>(a.out + 2 * (((int64_t)(q.begin + tok) * a.hq + head) * a.D + 4 * col[k])) =
-                make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
+            *reinterpret_cast<uint2*>(a.out + 2 * at) = make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
         }
     }
 }
@@ -328,7 +384,7 @@ __device__ __forceinline__ void join_values(const AttnArgs& a, const Seq& q, int
 // many of them maybe, and their reads' latency is what it costs (one token over 4,000, 31
 // pieces: the call took 25 us with two at a time, 17 with eight; sixteen gave no more).
 template <typename T, bool FAR, typename Stat, typename Value>
-__device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq& q, int kvh, int row0,
+__device__ __forceinline__ void finish_rows(const AttnArgs& a, const Seq& q, int kvh, int row0,
                                             int rows, int pieces, Stat stat, Value value, float* share,
                                             int* again) {
     if (threadIdx.x == 0) *again = 0;
@@ -366,7 +422,7 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, int s, const Seq&
         if (live && t == 0) {
             if (a.lse) {
                 const int tok = a.by_group(row0 + r);
-                a.lse[(int64_t)(q.begin + tok) * a.hq + kvh * a.group + row0 + r - tok * a.group] =
+                a.lse[(int64_t)(q.out + tok) * a.hq + kvh * a.group + row0 + r - tok * a.group] =
                     l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
             }
         }

@@ -350,6 +350,10 @@ __device__ __forceinline__ Seq shared_seq(const Seq& q, int src) {
     x.n_new = __shfl_sync(0xffffffffu, q.n_new, src);
     x.kv = __shfl_sync(0xffffffffu, q.kv, src);
     x.ok = true;
+    x.pos0 = __shfl_sync(0xffffffffu, q.pos0, src);
+    x.lo = __shfl_sync(0xffffffffu, q.lo, src);
+    x.row = __shfl_sync(0xffffffffu, q.row, src);
+    x.out = __shfl_sync(0xffffffffu, q.out, src);
     return x;
 }
 
@@ -385,7 +389,7 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     };
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
         const int s = s0 + lane;
-        Seq q{0, 0, 0, false};
+        Seq q{};
         if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
         if (rb > 0) add(q, 0);
@@ -430,7 +434,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
         c->run = run;
         c->units = unit_run;
         const int s = s0 + lane;
-        Seq q{0, 0, 0, false};
+        Seq q{};
         if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
         unsigned busy = __ballot_sync(0xffffffffu, rb > 0);
@@ -660,7 +664,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     if (j + mine < u.n) {
                         const int k0 = u.key0(j + mine) + sub * br;
                         if (k0 < u.sp.sink || (k0 + br > u.sp.lo && k0 < u.sp.hi)) {
-                            const int lp = a.by_page(k0), e = page_of(a, u.s, lp);
+                            const int lp = a.by_page(k0), e = page_of(a, u.q.row, lp);
                             if (e >= 0) {
                                 *page = e;
                                 *row = k0 - lp * a.page_tokens;
@@ -966,9 +970,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 const int key0 = u.key0(u.alone ? 2 * j + w : j), kv = u.q.kv;
                 const int pos_first = __shfl_sync(0xffffffffu, pos, 0), pos_last = __shfl_sync(0xffffffffu, pos, 31);
                 if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
-                      (a.window <= 0 || key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks))) {
+                      (a.window > 0 ? key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks : key0 >= u.q.lo))) {
                     const int hi = (a.causal ? min(kv, pos + 1) : kv) - key0;
-                    const int lo = a.window > 0 ? max(0, pos - a.window + 1) - key0 : 0;
+                    const int lo = (a.window > 0 ? max(0, pos - a.window + 1) : u.q.lo) - key0;
                     const int sink = a.window > 0 ? a.sinks - key0 : 0;
 #pragma unroll
                     for (int c0 = 0; c0 < TC_KEYS; c0 += 32) {
@@ -1060,7 +1064,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 s0 = l = NAN;
             }
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
-            const int64_t orow = (int64_t)(u.q.begin + tok) * a.hq + u.kvh * a.group + head;
+            const int64_t orow = (int64_t)(u.q.out + tok) * a.hq + u.kvh * a.group + head;
             float* pt = t.join.part + (int64_t)u.slot * UNIT * (DP + 2);   // (pieces)
             if (whole_unit && l != 0.0f) {
                 const float inv = 1.0f / l;
@@ -1100,6 +1104,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                             make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
                     continue;
                 }
+                if (a.part) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8)
+                        if (c0 + c < a.D) store32(a.part + orow * a.D + c0 + c, o + c, false);
+                    continue;
+                }
 #pragma unroll
                 for (int c = 0; c < 32; c += 16) {
                     uint32_t h[8];
@@ -1127,7 +1137,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
                 }
             }
-            const unsigned again = __ballot_sync(0xffffffffu, live && fine && most >= 0x7f800000u);
+            const unsigned again = __ballot_sync(0xffffffffu, live && fine && !a.part && most >= 0x7f800000u);
             if (lane == 0 && whole_unit && (uint32_t)u.id < (uint32_t)t.units) {
                 t.again[(int64_t)u.id * TC_SOFTMAX_WARPS + warp] = again;
                 if (again) ctl->any_again = 1;
@@ -1156,7 +1166,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (s < 0) break;
         if (slot >= 0 || (uint32_t)id >= (uint32_t)t.units) continue;
         // rows [32 warp, 32 warp + 32) of the unit
-        attn_rows_exact<T, 16>(a, s, q, kvh, row0, __ldcg(t.again + (int64_t)id * TC_SOFTMAX_WARPS + warp));
+        attn_rows_exact<T, CODEC_NONE, 16>(a, q, kvh, row0, __ldcg(t.again + (int64_t)id * TC_SOFTMAX_WARPS + warp));
     }
 }
 
@@ -1173,14 +1183,15 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// 16-bit values, boxes of 64 values in a row, 128-byte swizzle, zeros out of range.
+// 16-bit values (or bytes) in boxes of 128 or 64 bytes of a row, swizzled over as many, zeros out of range.
 hmm_status_t encode_map(CUtensorMap* m, void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                        const cuuint32_t* box) {
+                        const cuuint32_t* box, bool bytes = false) {
     auto fn = encode_fn();
     if (!fn) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, base, dims, strides, box, ones,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult r = fn(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank,
+                          base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          bytes && box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(HMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return HMM_OK;
@@ -1213,13 +1224,13 @@ hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorM
 
 }  // namespace
 
-hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows) {
+hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows, bool codes) {
     const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_tokens, (cuuint64_t)a.hk, (cuuint64_t)a.n_pages};
     cuuint64_t strides[3] = {(cuuint64_t)p.token, (cuuint64_t)p.head, (cuuint64_t)p.page};
     for (int i = 0; i < 3; ++i)
         if (dims[i + 1] == 1) strides[i] = 16;   // never stepped over
-    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-    return encode_map(m, p.base, 4, dims, strides, box);
+    const cuuint32_t box[4] = {codes && a.D > 64 ? 128u : 64u, (cuuint32_t)box_rows, 1, 1};
+    return encode_map(m, p.base, 4, dims, strides, box, codes);
 }
 
 bool chunk_applies(const AttnArgs& a) {
@@ -1264,9 +1275,9 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     }
     *join = t.join;
     CUtensorMap k, v, q{};
-    hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows);
+    hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows, false);
     if (s != HMM_OK) return s;
-    s = make_page_map(&v, a, a.v, t.box_rows);
+    s = make_page_map(&v, a, a.v, t.box_rows, false);
     if (s != HMM_OK) return s;
     if (boxes) {
         const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tokens};

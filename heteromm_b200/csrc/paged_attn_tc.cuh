@@ -10,9 +10,10 @@
 namespace hmm {
 namespace serve {
 
-// A page array as a tensor (D, page_tokens, heads, pages) of boxes {64, rows, 1, 1},
-// 128-byte swizzle; values behind D and pages behind the last read as zeros.
-hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows);
+// A page array as a tensor (D, page_tokens, heads, pages) of boxes {64, rows, 1, 1} of 16-bit
+// values or (codes) {128, rows, 1, 1} of bytes, 128-byte swizzle; for codes of D <= 64 {64,
+// rows, 1, 1}, 64-byte swizzle.  Values behind D and pages behind the last read as zeros.
+hmm_status_t make_page_map(CUtensorMap* m, const AttnArgs& a, const Pages& p, int box_rows, bool codes);
 
 // Rows of a box: the largest power of two that divides page_tokens, at most `most`; a box
 // never crosses a page's end.
@@ -21,7 +22,7 @@ inline int box_rows_of(int64_t page_tokens, int64_t most) {
     return (int)(r < most ? r : most);
 }
 
-// One box of a page array: values [x, x + 64) of rows y... of a head (z) and page (w).
+// One box of a page array: values from x on of rows y... of a head (z) and page (w).
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
                                               int z, int w) {
     asm volatile(

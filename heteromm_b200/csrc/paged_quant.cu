@@ -19,14 +19,7 @@ hmm_status_t check_quant(const hmm_paged_quant_t* cache, const hmm_paged_batch_t
                 "codes must be HMM_DTYPE_E4M3 or HMM_DTYPE_I8, got %d", (int)cache->codes);
     HMM_REQUIRE(cache->D >= Q_GROUP && cache->D <= 256 && cache->D % Q_GROUP == 0,
                 "D must be a multiple of 32 in [32, 256], got %lld", (long long)cache->D);
-    hmm_paged_cache_t dims{};
-    dims.k = cache->k;
-    dims.v = cache->v;
-    dims.n_pages = cache->n_pages;
-    dims.n_kv_heads = cache->n_kv_heads;
-    dims.page_tokens = cache->page_tokens;
-    dims.D = cache->D;
-    dims.dtype = HMM_DTYPE_BF16;
+    const hmm_paged_cache_t dims = quant_dims(*cache);
     const hmm_status_t s = check_batch(&dims, batch, b, k, v);
     if (s != HMM_OK) return s;
     const int64_t per = cache->D / Q_GROUP, block = cache->page_tokens * (cache->D + per);
@@ -192,11 +185,7 @@ extern "C" hmm_status_t hmm_paged_quant_append(
     if (s != HMM_OK) return s;
     HMM_REQUIRE(dtype == HMM_DTYPE_BF16 || dtype == HMM_DTYPE_F16,
                 "dtype must be HMM_DTYPE_BF16 or HMM_DTYPE_F16, got %d", dtype);
-    hmm_paged_cache_t dims{};
-    dims.n_pages = cache->n_pages;
-    dims.n_kv_heads = cache->n_kv_heads;
-    dims.page_tokens = cache->page_tokens;
-    dims.D = cache->D;
+    hmm_paged_cache_t dims = quant_dims(*cache);
     dims.dtype = dtype;
     int mode, vpl;
     s = plan_append({q, q_token, q_head, n_heads, k, k_token, k_head, v, v_token, v_head, q_weight, k_weight, weight_dtype,

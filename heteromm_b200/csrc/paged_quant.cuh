@@ -142,6 +142,19 @@ __device__ __forceinline__ float value_of(uint32_t code, uint32_t s) {
 
 // ------------------------------------------------------------ host helpers
 
+// The sizes of a cache as those of one of 16-bit values.
+inline hmm_paged_cache_t quant_dims(const hmm_paged_quant_t& c) {
+    hmm_paged_cache_t d{};
+    d.k = c.k;
+    d.v = c.v;
+    d.n_pages = c.n_pages;
+    d.n_kv_heads = c.n_kv_heads;
+    d.page_tokens = c.page_tokens;
+    d.D = c.D;
+    d.dtype = HMM_DTYPE_BF16;
+    return d;
+}
+
 // Fills `b`, `k`, `v` (token strides: D) and `rows` from the ABI's descriptions, or returns the error.
 hmm_status_t check_quant(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, Batch* b, Pages* k, Pages* v,
                          QuantRows* rows);

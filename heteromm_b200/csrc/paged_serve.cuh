@@ -25,7 +25,8 @@ struct Batch {
     const int32_t* table;    // [n_seq][pages_per_seq]
     const int32_t* cu;       // [n_seq + 1]
     const int32_t* kv_len;   // [n_seq]
-    int n_seq;
+    const int4* shared;      // null, or two per sequence (Seq's fields): the parts of a batch of shared prefixes
+    int n_seq;               // (with `shared`: of such parts)
     int pages_per_seq;
     int n_tokens;            // rows of the packed batch (padding rows behind the last sequence included)
 };
@@ -35,33 +36,50 @@ struct Pages {               // one page array
     int64_t page, head, token;   // strides in bytes
 };
 
-// One sequence of the batch.  A cu_new / kv_len entry outside its extent sets
+// One sequence of the batch: its rows begin at `begin` and their results at `out`, its first new
+// token is at position pos0, its pages are listed in row `row` of the table, and of its keys
+// [lo, kv) count.  A cu_new / kv_len entry outside its extent sets
 // HMM_STATUS_BATCH_BOUNDS and makes the sequence empty (ok == false).
 struct Seq {
     int begin, n_new, kv;
     bool ok;
+    int pos0, lo, row, out;
 };
 
-__device__ __forceinline__ Seq check_seq(const Batch& b, int64_t max_kv, int begin, int end, int kv, int32_t* status) {
-    Seq q;
-    q.begin = begin;
-    q.kv = kv;
-    q.n_new = end - begin;
-    q.ok = q.begin >= 0 && end >= q.begin && end <= b.n_tokens && q.kv >= 0 && q.kv <= max_kv;
-    if (!q.ok) {
+__device__ __forceinline__ Seq seq_of(int s, int begin, int n_new, int kv) {
+    return Seq{begin, n_new, kv, true, kv - n_new, 0, s, begin};
+}
+
+__device__ __forceinline__ Seq check_seq(const Batch& b, int64_t max_kv, int s, int begin, int end, int kv,
+                                         int32_t* status) {
+    const bool ok = begin >= 0 && end >= begin && end <= b.n_tokens && kv >= 0 && kv <= max_kv;
+    if (!ok) {
         atomicOr(status, HMM_STATUS_BATCH_BOUNDS);
-        q.begin = q.n_new = q.kv = 0;
+        Seq q = seq_of(s, 0, 0, 0);
+        q.ok = false;
+        return q;
     }
-    return q;
+    return seq_of(s, begin, end - begin, kv);
+}
+
+// (checked where it was made)
+__device__ __forceinline__ Seq shared_part(const Batch& b, int s) {
+    const int4 x = __ldg(b.shared + 2 * (int64_t)s), y = __ldg(b.shared + 2 * (int64_t)s + 1);
+    return Seq{x.x, x.y, x.z, true, x.w, y.x, y.y, y.z};
 }
 
 __device__ __forceinline__ Seq load_seq(const Batch& b, int64_t max_kv, int s, int32_t* status) {
-    return check_seq(b, max_kv, __ldg(b.cu + s), __ldg(b.cu + s + 1), __ldg(b.kv_len + s), status);
+    if (b.shared) return shared_part(b, s);
+    return check_seq(b, max_kv, s, __ldg(b.cu + s), __ldg(b.cu + s + 1), __ldg(b.kv_len + s), status);
 }
 
 // f(sequence) of every step-th sequence from s on, four sequences' loads in flight.
 template <typename F>
 __device__ __forceinline__ void each_seq(const Batch& b, int64_t max_kv, int s, int step, int32_t* status, F&& f) {
+    if (b.shared) {
+        for (; s < b.n_seq; s += step) f(shared_part(b, s));
+        return;
+    }
     for (; s < b.n_seq; s += 4 * step) {
         int begin[4], end[4], kv[4];
 #pragma unroll
@@ -73,7 +91,7 @@ __device__ __forceinline__ void each_seq(const Batch& b, int64_t max_kv, int s, 
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (s + i * step < b.n_seq) f(check_seq(b, max_kv, begin[i], end[i], kv[i], status));
+            if (s + i * step < b.n_seq) f(check_seq(b, max_kv, s + i * step, begin[i], end[i], kv[i], status));
     }
 }
 

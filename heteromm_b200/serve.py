@@ -35,8 +35,9 @@ from ._abi import HmmError, last_error, load
 _ENTRIES = ("hmm_paged_kv_append", "hmm_paged_attention", "hmm_paged_attention_workspace_size",
             "hmm_paged_state_workspace_size", "hmm_paged_copy_pages", "hmm_paged_free", "hmm_paged_fork",
             "hmm_paged_grow", "hmm_paged_compact", "hmm_status_read", "hmm_paged_quant_append",
-            "hmm_paged_quant_read")
-_CALLS = ("attention", "append", "copy_pages", "free", "fork", "grow", "compact", "quant_append", "quant_read")
+            "hmm_paged_quant_read", "hmm_paged_quant_attention", "hmm_paged_quant_attention_workspace_size")
+_CALLS = ("attention", "append", "copy_pages", "free", "fork", "grow", "compact", "quant_append", "quant_read",
+          "quant_attention")
 
 
 def _raise(name: str, status: int):
@@ -147,6 +148,17 @@ def paged_quant_append(q, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tenso
     them; a group with an infinity or NaN reads as NaN."""
     return _calls.quant_append(q, k, v, k_pages, v_pages, page_table, cu_new, kv_len, rope, q_weight, k_weight, eps,
                                interleaved, positions, out, status)
+
+
+def paged_quant_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                          cu_new: torch.Tensor, kv_len: torch.Tensor, *, causal: bool = True, window: int = 0,
+                          sinks: int = 0, scale: float | None = None, max_new: int = 0, return_lse: bool = False,
+                          out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """paged_attention over a cache held in 8 bits, with q and the result of bf16 or fp16
+    (int16: bf16 bits): what it gives over a cache of that type that holds the same values
+    (paged_quant_read), up to the order of its sums."""
+    return _calls.quant_attention(q, k_pages, v_pages, page_table, cu_new, kv_len, causal, window, sinks, scale, max_new,
+                                  return_lse, out, status)
 
 
 def paged_quant_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu: torch.Tensor,

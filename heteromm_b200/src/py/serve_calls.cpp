@@ -48,6 +48,8 @@ struct Entry {
     decltype(&hmm_status_read) status_read;
     decltype(&hmm_paged_quant_append) quant_append;
     decltype(&hmm_paged_quant_read) quant_read;
+    decltype(&hmm_paged_quant_attention) quant_attention;
+    decltype(&hmm_paged_quant_attention_workspace_size) quant_attention_workspace;
 };
 Entry hmm_fn{};
 PyObject* raise_error = nullptr;   // (entry point's name, status): raises HmmError
@@ -258,6 +260,17 @@ QuantCache quant_cache(PyObject* k_pages, PyObject* v_pages) {
                       (int)k.get_device()};
 }
 
+// What the checks ask of a cache whose vectors are of this type, the one of `name`.
+Cache of_quant(const QuantCache& q, ScalarType dtype, const char* name) {
+    Cache c{};
+    c.c.n_kv_heads = q.c.n_kv_heads;
+    c.c.D = q.c.D;
+    c.c.dtype = code_of(dtype, name);
+    c.dtype = dtype;
+    c.dev = q.dev;
+    return c;
+}
+
 const Tensor& page_table(PyObject* o, int dev) {
     const Tensor& t = dense(o, "page_table", at::kInt, dev);
     if (t.dim() != 2) throw value_error("page_table must be [n_seq, pages_per_seq]");
@@ -323,11 +336,14 @@ void arguments(Py_ssize_t got, Py_ssize_t need) {
 
 // q, k_pages, v_pages, page_table, cu_new, kv_len, causal, window, sinks, scale, max_new,
 // return_lse, out, status
+// (QUANT: over a cache held in 8 bits)
+template <bool QUANT>
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     arguments(n_args, 14);
-    const Cache c = cache(a[1], a[2]);
     const Tensor& q = on_gpu(a[0], "q");
+    QuantCache qc{};
+    const Cache c = QUANT ? of_quant(qc = quant_cache(a[1], a[2]), q.scalar_type(), "q") : cache(a[1], a[2]);
     if (q.dim() != 3) throw value_error("q must be [n_tokens, n_heads, D]");
     const int64_t n_tokens = q.size(0), heads = q.size(1), d = q.size(2);
     if (d != c.c.D) throw value_error("q has heads of %d, the cache of %d", (int)d, (int)c.c.D);
@@ -341,14 +357,19 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     Tensor lse;
     if (with_lse) lse = empty({n_tokens, heads}, at::kFloat, c.dev);
     const Status status = status_word(a[13], c.dev, at.stream);
-    const size_t bytes = hmm_fn.attention_workspace(b.n_seq, n_tokens, heads, c.c.n_kv_heads, d);
+    const size_t bytes = (QUANT ? hmm_fn.quant_attention_workspace : hmm_fn.attention_workspace)(b.n_seq, n_tokens, heads,
+                                                                                                 c.c.n_kv_heads, d);
     const c10::DataPtr ws = scratch(bytes);
     finish(unlocked([&] {
+               if constexpr (QUANT)
+                   return hmm_fn.quant_attention(&qc.c, &b, c.c.dtype, qr.p, qr.token, qr.head, heads, scale, causal, window,
+                                                 sinks, max_new, out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr,
+                                                 status.p, ws.get(), bytes, at.stream);
                return hmm_fn.attention(&c.c, &b, qr.p, qr.token, qr.head, heads, scale, causal, window, sinks, max_new,
                                        out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, status.p, ws.get(),
                                        bytes, at.stream);
            }),
-           "hmm_paged_attention", status, at.stream);
+           QUANT ? "hmm_paged_quant_attention" : "hmm_paged_attention", status, at.stream);
     if (!with_lse) return THPVariable_Wrap(std::move(out));
     return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
     END_HANDLE_TH_ERRORS
@@ -363,18 +384,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     arguments(n_args, 16);
     const Tensor& k = on_gpu(a[1], "k");
     if (k.dim() != 3) throw value_error("k must be [n_tokens, n_kv_heads, D]");
-    Cache c{};
     QuantCache qc{};
-    if constexpr (QUANT) {
-        qc = quant_cache(a[3], a[4]);
-        c.dtype = k.scalar_type();
-        c.c.dtype = code_of(c.dtype, "k");
-        c.c.D = qc.c.D;
-        c.c.n_kv_heads = qc.c.n_kv_heads;
-        c.dev = qc.dev;
-    } else {
-        c = cache(a[3], a[4]);
-    }
+    const Cache c = QUANT ? of_quant(qc = quant_cache(a[3], a[4]), k.scalar_type(), "k") : cache(a[3], a[4]);
     const int64_t d = c.c.D, hk = c.c.n_kv_heads;
     const int64_t n_tokens = k.size(0);
     const Rows kr = rows(a[1], "k", c.dtype, c.dev, {n_tokens, hk, d}),
@@ -668,10 +679,11 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
-                         {"attention", FAST(attention)},
+                         {"attention", FAST(attention<false>)},
                          {"append", FAST(append<false>)},
                          {"quant_append", FAST(append<true>)},
                          {"quant_read", FAST(quant_read)},
+                         {"quant_attention", FAST(attention<true>)},
                          {"copy_pages", FAST(copy_pages)},
                          {"free", FAST(free_)},
                          {"fork", FAST(fork_)},

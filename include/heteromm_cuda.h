@@ -455,6 +455,17 @@ hmm_status_t hmm_paged_quant_append(
 hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
                                   void* k_out, void* v_out, int32_t* device_status, void* stream);
 
+/* hmm_paged_attention over a cache held in 8 bits: q and out of `dtype`
+ * (HMM_DTYPE_BF16 or HMM_DTYPE_F16), all else as there.  The result is that of a
+ * cache that holds the values in `dtype`; a seen group with s = 255 gives NaN. */
+size_t hmm_paged_quant_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
+                                                int64_t n_kv_heads, int64_t D);
+hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
+                                       const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
+                                       float scale, int causal, int64_t window, int64_t sinks, int64_t max_new,
+                                       void* out, float* lse, int32_t* device_status, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
 /* Page management.  The state is the page table [n_seq][pages_per_seq] (an
  * entry below 0 holds no page), the references [n_pages] of each page (0 =
  * free) and kv_len [n_seq].  Every call reads the state from *_in and writes
