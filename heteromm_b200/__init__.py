@@ -14,7 +14,7 @@ from .paged import (block_pages, block_sparse_attention_bf16, block_sparse_atten
                     block_select_minmax, block_sparse_decode_bf16, paged_kv_minmax_bf16,
                     paged_kv_summary_bf16, paged_kv_summary_f32)
 from .serve import (paged_attention, paged_compact, paged_copy_pages, paged_fork, paged_free,  # noqa: F401,E501
-                    paged_grow, paged_kv_append, paged_quant_append,
+                    paged_grow, paged_kv_append, paged_prefix_attention, paged_quant_append,
                     paged_quant_attention, paged_quant_read, quant_pages, rope_table)
 
 __version__ = "0.1.0"

@@ -68,6 +68,13 @@ hmm_status_t plan_attention(const AttnCall& c, const hmm_paged_cache_t& dims, co
     return HMM_OK;
 }
 
+size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared) {
+    return up256(rows_workspace(rows_dp(D))) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared);
+}
+
+template hmm_status_t run_attention<__nv_bfloat16, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template hmm_status_t run_attention<__half, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+
 }  // namespace serve
 }  // namespace hmm
 
@@ -77,8 +84,7 @@ using namespace hmm::serve;
 extern "C" size_t hmm_paged_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
                                                      int64_t n_kv_heads, int64_t D) {
     if (n_seq < 0 || n_tokens < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256) return 0;
-    const int dp = rows_dp(D);
-    return up256(rows_workspace(dp)) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D);
+    return attention_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, false);
 }
 
 extern "C" hmm_status_t hmm_paged_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,

@@ -66,6 +66,15 @@ struct AttnCall {
 hmm_status_t plan_attention(const AttnCall& c, const hmm_paged_cache_t& dims, const hmm_paged_batch_t* batch, bool quant,
                             AttnArgs* a, bool* nothing);
 
+inline size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// The kernels of a call over caches of this codec (paged_rows.cuh), with the host's bound on the
+// new tokens of any sequence (0: none known), and the bytes that they need (shared: for the parts
+// of a batch of shared prefixes, in which a token counts twice).
+template <typename T, int C>
+hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st);
+size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared);
+
 // A row of a unit (sequence, KV head): row r is new token r / group, head r % group.
 struct Span {                    // keys [0, sink) and [lo, hi) hold all that some row of a tile sees
     int p0, p1;                  // positions of the tile's first and last row

@@ -1210,8 +1210,6 @@ bool may_split(int64_t n_tokens, int64_t group, int64_t hk, int64_t rows) {
 
 int unit_rows(int64_t D) { return D <= 128 ? tc_rows<128>() : tc_rows<256>(); }
 
-size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
-
 template <typename T, int DP>
 hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q,
                           bool behind, cudaStream_t st) {
@@ -1237,10 +1235,11 @@ bool chunk_applies(const AttnArgs& a) {
     return box_rows_of(a.page_tokens, TC_KEYS) >= 8;
 }
 
-size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D) {
+size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared) {
     const int64_t group = std::max<int64_t>(1, n_heads / n_kv_heads), ctas = device_sm_count(), rows = unit_rows(D);
-    size_t n = up256(4 * (size_t)most_units(n_seq, n_tokens, group, n_kv_heads, rows) * TC_SOFTMAX_WARPS);
-    if (may_split(n_tokens, group, n_kv_heads, rows))
+    size_t n = up256(4 * (size_t)most_units(n_seq, shared ? 2 * n_tokens : n_tokens, group, n_kv_heads, rows) *
+                     TC_SOFTMAX_WARPS);
+    if (shared || may_split(n_tokens, group, n_kv_heads, rows))
         n += up256(2 * sizeof(int4) * ctas) +
              sizeof(float) * 2 * ctas * rows * ((D <= 64 ? 64 : D <= 128 ? 128 : 256) + 2);
     return n;
@@ -1248,7 +1247,8 @@ size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t
 
 hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, unsigned char* ws, cudaStream_t st,
                        ChunkJoin* join) {
-    const int64_t rows = unit_rows(a.D), units = most_units(a.b.n_seq, a.b.n_tokens, a.group, a.hk, rows);
+    const int64_t rows = unit_rows(a.D), tokens = (a.b.shared ? 2 : 1) * (int64_t)a.b.n_tokens,
+                  units = most_units(a.b.n_seq, tokens, a.group, a.hk, rows);
     HMM_REQUIRE(units < (int64_t(1) << 30), "n_tokens * n_heads is too large for one call");
     unsigned char* joint = ws + up256(4 * (size_t)units * TC_SOFTMAX_WARPS);
     // A tile of 128 rows is a box of the queries where it is whole tokens; a negative scale
@@ -1261,7 +1261,7 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     t.rows_log2 = rows == 256 ? 8 : 7;
     t.min_rows = min_rows;
     t.box_rows = box_rows_of(a.page_tokens, TC_KEYS);
-    t.split = may_split(a.b.n_tokens, a.group, a.hk, rows);
+    t.split = a.b.shared || may_split(a.b.n_tokens, a.group, a.hk, rows);
     t.q_tokens = boxes ? TC_ROWS / a.group : 0;
     t.wait_ns = wait_limit_ns();
     // 16 us a key tile, which takes 2 to 4 (a limit of 0 stays one)

@@ -47,7 +47,8 @@ struct ChunkJoin {
 // look up a tile's boxes, which boxes of 4 rows would just fit (not tried) and smaller ones
 // not (2,048 tokens, 32/8 heads of 128: pages of 8 58 us here, of 4 837 in the rows kernel).
 bool chunk_applies(const AttnArgs& a);
-size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D);
+// (shared: the parts of a batch of shared prefixes, in which a token counts twice)
+size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared);
 // Rows of every sequence with at least min_rows rows (n_new * group).  `behind`: the kernel
 // before it on the stream is the rows kernel, which it may overlap and does not end before.
 // *join says what is left to join (ctas = 0: nothing).

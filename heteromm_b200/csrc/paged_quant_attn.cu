@@ -2,6 +2,17 @@
 // bits: the entry point.
 #include "paged_rows.cuh"
 
+namespace hmm {
+namespace serve {
+
+template hmm_status_t run_attention<__nv_bfloat16, CODEC_E4M3>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template hmm_status_t run_attention<__half, CODEC_E4M3>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template hmm_status_t run_attention<__nv_bfloat16, CODEC_I8>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template hmm_status_t run_attention<__half, CODEC_I8>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+
+}  // namespace serve
+}  // namespace hmm
+
 using namespace hmm;
 using namespace hmm::serve;
 

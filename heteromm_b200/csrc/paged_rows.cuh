@@ -330,17 +330,17 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                                        (int64_t)(kvh * a.group + at % a.group) * a.q_head;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
-                if (QUANT) {
+                if constexpr (QUANT) {
                     const int d = code_of_step<DP>(k, lane & 3);
                     const uint2 x = real && d < a.D ? __ldg(reinterpret_cast<const uint2*>(src + 2 * d)) : make_uint2(0u, 0u);
                     qf[k][h] = __byte_perm(x.x, x.y, 0x5410);
                     qf[k][h + 2] = __byte_perm(x.x, x.y, 0x7632);
-                    continue;
-                }
+                } else {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int d = k * 16 + j * 8 + (lane & 3) * 2;
-                    qf[k][h + 2 * j] = real && d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(src + 2 * d)) : 0u;
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = k * 16 + j * 8 + (lane & 3) * 2;
+                        qf[k][h + 2 * j] = real && d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(src + 2 * d)) : 0u;
+                    }
                 }
             }
         }
@@ -661,8 +661,6 @@ inline int64_t rows_ctas(int dp) {
     return (int64_t)device_sm_count() * (dp == 64 ? rows_ctas_per_sm<64>() : dp == 128 ? rows_ctas_per_sm<128>() : 1);
 }
 
-inline size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
-
 inline size_t rows_workspace(int dp) {
     const size_t g = (size_t)rows_ctas(dp);
     return 2 * g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
@@ -699,7 +697,8 @@ hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cu
     // the chunk kernel, 32 rows 67 in both (over 777: 34 and 30, 25 and 29).  (A scale of zero is the rows kernel's, which scales before it masks: in the
     // chunk kernel a masked score of -inf times zero would be NaN.)
     const bool chunk = C == CODEC_NONE && chunk_applies(a) && a.scale_log2 != 0.0f;
-    const bool few = max_new > 0 && (int64_t)std::min(max_new, a.b.n_tokens) * a.group <= RW_ROWS;
+    const int bound = a.b.shared ? a.b.n_tokens : max_new;       // (a group's rows are those of its sequences)
+    const bool few = bound > 0 && (int64_t)std::min(bound, a.b.n_tokens) * a.group <= RW_ROWS;
     const bool with_rows = few || !chunk || a.b.n_seq > 1;
     const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel
     const int dp = rows_dp(a.D);

@@ -35,9 +35,11 @@ from ._abi import HmmError, last_error, load
 _ENTRIES = ("hmm_paged_kv_append", "hmm_paged_attention", "hmm_paged_attention_workspace_size",
             "hmm_paged_state_workspace_size", "hmm_paged_copy_pages", "hmm_paged_free", "hmm_paged_fork",
             "hmm_paged_grow", "hmm_paged_compact", "hmm_status_read", "hmm_paged_quant_append",
-            "hmm_paged_quant_read", "hmm_paged_quant_attention", "hmm_paged_quant_attention_workspace_size")
+            "hmm_paged_quant_read", "hmm_paged_quant_attention", "hmm_paged_quant_attention_workspace_size",
+            "hmm_paged_prefix_attention", "hmm_paged_prefix_attention_workspace_size",
+            "hmm_paged_quant_prefix_attention")
 _CALLS = ("attention", "append", "copy_pages", "free", "fork", "grow", "compact", "quant_append", "quant_read",
-          "quant_attention")
+          "quant_attention", "prefix_attention")
 
 
 def _raise(name: str, status: int):
@@ -114,6 +116,23 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     helps to choose the kernel (decoding: 1); results do not depend on it."""
     return _calls.attention(q, k_pages, v_pages, page_table, cu_new, kv_len, causal, window, sinks, scale, max_new,
                             return_lse, out, status)
+
+
+def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                           cu_new: torch.Tensor, kv_len: torch.Tensor, cu_group: torch.Tensor, prefix_len: torch.Tensor, *,
+                           scale: float | None = None, max_new: int = 0, return_lse: bool = False,
+                           out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """paged_attention (causal) of a batch in which sequences share a prefix, as paged_fork
+    leaves them, over a 16-bit cache or one held in 8 bits: sequences [cu_group[g],
+    cu_group[g + 1]) have their first prefix_len[g] tokens in common (int32, read on the
+    device; sequences may be left out), whose keys are read once for the whole group.
+
+    Every row of page_table lists all of its sequence's pages.  A prefix may end within a
+    page, and reaches no further than what its sequences held before their new tokens.
+    The result is paged_attention's up to the order of its sums; max_new is taken as there
+    and not needed."""
+    return _calls.prefix_attention(q, k_pages, v_pages, page_table, cu_new, kv_len, cu_group, prefix_len, scale, max_new,
+                                   return_lse, out, status)
 
 
 # ------------------------------------------------------------------ a cache held in 8 bits

@@ -50,6 +50,9 @@ struct Entry {
     decltype(&hmm_paged_quant_read) quant_read;
     decltype(&hmm_paged_quant_attention) quant_attention;
     decltype(&hmm_paged_quant_attention_workspace_size) quant_attention_workspace;
+    decltype(&hmm_paged_prefix_attention) prefix_attention;
+    decltype(&hmm_paged_prefix_attention_workspace_size) prefix_attention_workspace;
+    decltype(&hmm_paged_quant_prefix_attention) quant_prefix_attention;
 };
 Entry hmm_fn{};
 PyObject* raise_error = nullptr;   // (entry point's name, status): raises HmmError
@@ -375,6 +378,49 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// q, k_pages, v_pages, page_table, cu_new, kv_len, cu_group, prefix_len, scale, max_new,
+// return_lse, out, status; the dtype of k_pages says which cache it is
+PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    arguments(n_args, 13);
+    const Tensor& q = on_gpu(a[0], "q");
+    const ScalarType pt = on_gpu(a[1], "k_pages").scalar_type();
+    const bool quant = pt == at::kFloat8_e4m3fn || pt == at::kChar;
+    QuantCache qc{};
+    const Cache c = quant ? of_quant(qc = quant_cache(a[1], a[2]), q.scalar_type(), "q") : cache(a[1], a[2]);
+    if (q.dim() != 3) throw value_error("q must be [n_tokens, n_heads, D]");
+    const int64_t n_tokens = q.size(0), heads = q.size(1), d = q.size(2);
+    if (d != c.c.D) throw value_error("q has heads of %d, the cache of %d", (int)d, (int)c.c.D);
+    const Rows qr = rows(a[0], "q", c.dtype, c.dev, q.sizes());
+    const hmm_paged_batch_t b = batch(a[3], a[4], a[5], n_tokens, c.dev);
+    const Tensor& prefix = int_vector(a[7], "prefix_len", c.dev);
+    const int64_t groups = prefix.size(0);
+    const int32_t* cu_group = ints(a[6], "cu_group", c.dev, {groups + 1});
+    const float scale = a[8] == Py_None ? (float)std::pow((double)d, -0.5) : (float)real(a[8]);
+    if (whole(a[9]) < 0) throw value_error("max_new must be >= 0");
+    const bool with_lse = truth(a[10]);
+    const Place at(c.dev);
+    Tensor out = a[11] == Py_None ? empty(q.sizes(), c.dtype, c.dev) : dense(a[11], "out", c.dtype, c.dev, q.sizes());
+    Tensor lse;
+    if (with_lse) lse = empty({n_tokens, heads}, at::kFloat, c.dev);
+    float* lp = with_lse ? lse.data_ptr<float>() : nullptr;
+    const Status status = status_word(a[12], c.dev, at.stream);
+    const size_t bytes = hmm_fn.prefix_attention_workspace(b.n_seq, n_tokens, groups, heads, c.c.n_kv_heads, d);
+    const c10::DataPtr ws = scratch(bytes);
+    const int32_t* pl = (const int32_t*)prefix.data_ptr();
+    finish(unlocked([&] {
+               return quant ? hmm_fn.quant_prefix_attention(&qc.c, &b, c.c.dtype, cu_group, pl, groups, qr.p, qr.token, qr.head,
+                                                            heads, scale, out.data_ptr(), lp, status.p, ws.get(), bytes,
+                                                            at.stream)
+                            : hmm_fn.prefix_attention(&c.c, &b, cu_group, pl, groups, qr.p, qr.token, qr.head, heads, scale,
+                                                      out.data_ptr(), lp, status.p, ws.get(), bytes, at.stream);
+           }),
+           quant ? "hmm_paged_quant_prefix_attention" : "hmm_paged_prefix_attention", status, at.stream);
+    if (!with_lse) return THPVariable_Wrap(std::move(out));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+    END_HANDLE_TH_ERRORS
+}
+
 // q, k, v, k_pages, v_pages, page_table, cu_new, kv_len, rope, q_weight, k_weight, eps,
 // interleaved, positions, out, status
 // (QUANT: into a cache held in 8 bits, whose vectors are of k's type)
@@ -684,6 +730,7 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"quant_append", FAST(append<true>)},
                          {"quant_read", FAST(quant_read)},
                          {"quant_attention", FAST(attention<true>)},
+                         {"prefix_attention", FAST(prefix_attention)},
                          {"copy_pages", FAST(copy_pages)},
                          {"free", FAST(free_)},
                          {"fork", FAST(fork_)},

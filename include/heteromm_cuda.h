@@ -466,6 +466,36 @@ hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache, const hmm
                                        void* out, float* lse, int32_t* device_status, void* workspace,
                                        size_t workspace_bytes, void* stream);
 
+/* hmm_paged_attention (causal, no window) of a batch in which groups of sequences
+ * share a prefix, as hmm_paged_fork leaves them: sequences [cu_group[g],
+ * cu_group[g+1]) have their first prefix_len[g] tokens in common, which are gone
+ * through once for all of the group's rows.  The result is that of
+ * hmm_paged_attention, up to the order of its sums and one more rounding in
+ * fp32.  cu_group [n_groups + 1] ascending in [0, n_seq] and prefix_len
+ * [n_groups] in [0, pages_per_seq * page_tokens] (int32, on the device) may
+ * leave sequences out, and a prefix may end within a page.  Every sequence's
+ * row of the page table lists all its pages; those of a prefix are read
+ * from the row of the group's first sequence that has new tokens.  (Where that
+ * reads an infinity or NaN, a row that does not come out finite is computed
+ * again from its own.)  A prefix longer than what a sequence with new tokens
+ * held before them ends there.
+ * Workspace: 8 (D + 1) bytes for each row (token and query head) more than the
+ * plain call's, about. */
+size_t hmm_paged_prefix_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_groups,
+                                                 int64_t n_heads, int64_t n_kv_heads, int64_t D);
+hmm_status_t hmm_paged_prefix_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
+                                        const int32_t* cu_group, const int32_t* prefix_len, int64_t n_groups,
+                                        const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
+                                        float scale, void* out, float* lse, int32_t* device_status,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+/* The same over a cache held in 8 bits (and the same workspace). */
+hmm_status_t hmm_paged_quant_prefix_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch,
+                                              int dtype, const int32_t* cu_group, const int32_t* prefix_len,
+                                              int64_t n_groups, const void* q, int64_t q_token, int64_t q_head,
+                                              int64_t n_heads, float scale, void* out, float* lse,
+                                              int32_t* device_status, void* workspace, size_t workspace_bytes,
+                                              void* stream);
+
 /* Page management.  The state is the page table [n_seq][pages_per_seq] (an
  * entry below 0 holds no page), the references [n_pages] of each page (0 =
  * free) and kv_len [n_seq].  Every call reads the state from *_in and writes

@@ -7,9 +7,10 @@ import pytest
 import torch
 
 import heteromm_b200 as hmm
-from heteromm_b200._abi import (HMM_DTYPE_BF16, HMM_DTYPE_E4M3, HMM_DTYPE_F16, HMM_DTYPE_F32, HMM_DTYPE_I8, HMM_OK,
+from heteromm_b200._abi import (HMM_DTYPE_BF16, HMM_DTYPE_E4M3, HMM_DTYPE_F16, HMM_DTYPE_F32, HMM_DTYPE_I8, HMM_ERR_OOM,
+                                HMM_OK,
                                 PagedQuant)
-from test_serve_refusals import BAD_BATCH, P, batch, refused
+from test_serve_refusals import BAD_BATCH, BAD_CACHE, P, batch, cache, refused
 
 FAR = 1 << 30
 
@@ -46,16 +47,94 @@ def read(c=None, b=None, dtype=HMM_DTYPE_BF16, k=P + FAR, v=P + 2 * FAR, status=
     return hmm.load().hmm_paged_quant_read(C.byref(c or quant()), C.byref(b or batch()), dtype, k, v, status, None)
 
 
+def attend(c=None, b=None, dtype=HMM_DTYPE_BF16, q=P, q_token=256, q_head=64, n_heads=4, scale=0.125, causal=1, window=0,
+           sinks=0, max_new=0, out=P + FAR, status=P, ws=P, nbytes=1 << 40):
+    return hmm.load().hmm_paged_quant_attention(C.byref(c or quant()), C.byref(b or batch()), dtype, q, q_token, q_head,
+                                                n_heads, scale, causal, window, sinks, max_new, out, None, status, ws,
+                                                nbytes, None)
+
+
+def shared(c=None, b=None, cu_group=P, prefix=P, n_groups=2, q=P, q_token=256, q_head=64, n_heads=4, scale=0.125,
+           out=P + FAR, status=P, ws=P, nbytes=1 << 40):
+    return hmm.load().hmm_paged_prefix_attention(C.byref(c or cache()), C.byref(b or batch()), cu_group, prefix, n_groups, q,
+                                                 q_token, q_head, n_heads, scale, out, None, status, ws, nbytes, None)
+
+
+def shared_quant(c=None, b=None, dtype=HMM_DTYPE_BF16, cu_group=P, prefix=P, n_groups=2, q=P, q_token=256, q_head=64,
+                 n_heads=4, scale=0.125, out=P + FAR, status=P, ws=P, nbytes=1 << 40):
+    return hmm.load().hmm_paged_quant_prefix_attention(C.byref(c or quant()), C.byref(b or batch()), dtype, cu_group, prefix,
+                                                       n_groups, q, q_token, q_head, n_heads, scale, out, None, status, ws,
+                                                       nbytes, None)
+
+
 @pytest.mark.parametrize("change,text", BAD_QUANT)
 def test_bad_cache(change, text):
-    refused(append(quant(**change)), text)
-    refused(read(quant(**change)), text)
+    for call in (append, read, attend, shared_quant):
+        refused(call(quant(**change)), text)
+
+
+@pytest.mark.parametrize("change,text", BAD_CACHE)
+def test_bad_cache_of_16_bits(change, text):
+    refused(shared(cache(**change)), text)
 
 
 @pytest.mark.parametrize("change,text", BAD_BATCH)
 def test_bad_batch(change, text):
-    refused(append(b=batch(**change)), text)
-    refused(read(b=batch(**change)), text)
+    for call in (append, read, attend, shared, shared_quant):
+        refused(call(b=batch(**change)), text)
+
+
+BAD_ATTENTION = [
+    (dict(n_heads=0), "n_heads"), (dict(n_heads=3), "n_heads"), (dict(n_heads=65538), "n_heads"),
+    (dict(status=None), "device_status"), (dict(q_token=100), "q strides"), (dict(q_head=-64), "q strides"),
+    (dict(q=None), "null q"), (dict(out=None), "null q or out"), (dict(q=P + 2), "aligned"), (dict(out=P + FAR + 8), "aligned"),
+    (dict(ws=P + 8), "aligned"), (dict(out=P), "out overlaps q"),
+]
+
+
+@pytest.mark.parametrize("kw,text", BAD_ATTENTION)
+def test_bad_attention(kw, text):
+    for call in (attend, shared, shared_quant):
+        refused(call(**kw), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(dtype=HMM_DTYPE_F32), "dtype must"), (dict(dtype=HMM_DTYPE_E4M3), "dtype must"), (dict(window=-1), "window"),
+    (dict(sinks=-1), "sinks"), (dict(causal=0, window=4), "causal"), (dict(causal=0, sinks=4), "causal"), (dict(max_new=-1), "max_new"),
+    (dict(c=quant(n_pages=0)), "no pages"), (dict(c=quant(page_tokens=(1 << 31) - 512, k_page=1 << 39, k_head=1 << 38, v_page=1 << 39,
+                                                          v_head=1 << 38), b=batch(pages_per_seq=1)), "2^31 - 1024"),
+    (dict(c=quant(n_kv_heads=1), b=batch(n_tokens=1 << 30), n_heads=4), "2^31"),
+])
+def test_bad_quant_attention(kw, text):
+    refused(attend(**kw), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(n_groups=-1), "n_groups"), (dict(n_groups=3), "n_groups"), (dict(cu_group=None), "null cu_group"),
+    (dict(prefix=None), "null cu_group"),
+])
+def test_bad_groups(kw, text):
+    refused(shared(**kw), text)
+    refused(shared_quant(**kw), text)
+
+
+def test_workspaces():
+    lib = hmm.load()
+    for n_seq, n_tokens, heads, hk, d in ((2, 5, 4, 2, 64), (64, 64, 32, 8, 128), (3, 2000, 7, 1, 256), (1, 1, 1, 1, 32)):
+        need = lib.hmm_paged_quant_attention_workspace_size(n_seq, n_tokens, heads, hk, d)
+        assert need > 0
+        for n in (0, need - 1):
+            r = attend(quant(n_kv_heads=hk, D=d, page_tokens=64, k_page=1 << 20, k_head=1 << 15, v_page=1 << 20, v_head=1 << 15),
+                       batch(n_seq=n_seq, n_tokens=n_tokens), n_heads=heads, q_token=heads * d, q_head=d, nbytes=n)
+            refused(r, "workspace too small", HMM_ERR_OOM)
+        for groups in (0, n_seq):
+            more = lib.hmm_paged_prefix_attention_workspace_size(n_seq, n_tokens, groups, heads, hk, d)
+            assert more >= need + 8 * n_tokens * heads * (d + 1)
+            r = shared(cache(n_kv_heads=hk, D=d), batch(n_seq=n_seq, n_tokens=n_tokens), n_groups=groups, n_heads=heads,
+                       q_token=heads * d, q_head=d, nbytes=more - 1)
+            refused(r, "workspace too small", HMM_ERR_OOM)
+    assert lib.hmm_paged_quant_attention_workspace_size(1, 1, 1, 1, 257) == 0
+    assert lib.hmm_paged_prefix_attention_workspace_size(1, 1, -1, 1, 1, 64) == 0
 
 
 @pytest.mark.parametrize("kw,text", [
@@ -82,7 +161,8 @@ def test_bad_read(kw, text):
 
 def test_nothing_to_do():
     for b in (batch(n_seq=0), batch(n_tokens=0)):
-        assert append(b=b) == HMM_OK and read(b=b) == HMM_OK
+        assert append(b=b) == HMM_OK and read(b=b) == HMM_OK and attend(b=b) == HMM_OK
+        assert shared(b=b, n_groups=0) == HMM_OK and shared_quant(b=b, n_groups=0) == HMM_OK
 
 
 def test_wrappers_refuse():
@@ -91,6 +171,10 @@ def test_wrappers_refuse():
         hmm.paged_quant_read(x, x, x, x, x, 4)
     with pytest.raises(ValueError, match="must be a CUDA tensor"):
         hmm.paged_quant_append(x, x, x, x, x, x, x, x)
+    with pytest.raises(ValueError, match="q must be a CUDA tensor"):
+        hmm.paged_quant_attention(x, x, x, x, x, x)
+    with pytest.raises(ValueError, match="q must be a CUDA tensor"):
+        hmm.paged_prefix_attention(x, x, x, x, x, x, x, x)
     for kw, error in ((dict(dtype=torch.uint8), TypeError), (dict(D=80), ValueError), (dict(D=288), ValueError),
                       (dict(page_tokens=4), ValueError), (dict(page_tokens=0), ValueError)):
         with pytest.raises(error):
