@@ -53,7 +53,7 @@ def build_cuda(force: bool = False, verbose: bool = False) -> str:
     deps = srcs + glob.glob(os.path.join(PKG, "csrc", "*.cuh")) + [os.path.join(INC, "heteromm_cuda.h")]
     if force or _newer(CUDA_LIB, deps):
         os.makedirs(LIB_DIR, exist_ok=True)
-        cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+        cmd = [NVCC, f"--threads={os.cpu_count() or 1}", *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
                f"-I{INC}", "-o", CUDA_LIB, *srcs]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")

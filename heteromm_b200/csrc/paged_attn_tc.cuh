@@ -32,6 +32,14 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
+// Scale bytes of a box's rows: 16-byte aligned, a multiple of 16 of them.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+        "r"(bytes), "r"(sm100::smem_u32(bar))
+        : "memory");
+}
+
 constexpr int TC_CTA_ROWS = 256;   // rows of a unit of the chunk kernel (D <= 128), at most
 
 // What the join needs of units that the chunk kernel cut into pieces.
@@ -52,8 +60,14 @@ size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t
 // Rows of every sequence with at least min_rows rows (n_new * group).  `behind`: the kernel
 // before it on the stream is the rows kernel, which it may overlap and does not end before.
 // *join says what is left to join (ctas = 0: nothing).
+template <int C>
 hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, unsigned char* ws, cudaStream_t st,
                        ChunkJoin* join);
+
+// The tensor maps' encoder, and units' bounds (paged_attn_tc.cu).
+hmm_status_t make_query_map(CUtensorMap* m, const AttnArgs& a, int box_heads, int box_tokens);
+int64_t most_units(int64_t n_seq, int64_t n_tokens, int64_t group, int64_t hk, int64_t rows);
+bool may_split(int64_t n_tokens, int64_t group, int64_t hk, int64_t rows);
 
 }  // namespace serve
 }  // namespace hmm

@@ -97,14 +97,6 @@ __device__ __forceinline__ void mma16816<__half>(float* d, const uint32_t* a, ui
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A box of a page array's codes, and scale bytes (16-byte aligned, a multiple of 16).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-        "r"(bytes), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // Units and key tiles of a sequence.  `tiles` is the same for each of its
 // units, an upper bound of what a unit's rows see.
 struct Load {
@@ -696,7 +688,7 @@ hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cu
     // there: 64 rows of 4 KV heads over 5,000, 16 sequences, D = 128, 113 us there and 69 in
     // the chunk kernel, 32 rows 67 in both (over 777: 34 and 30, 25 and 29).  (A scale of zero is the rows kernel's, which scales before it masks: in the
     // chunk kernel a masked score of -inf times zero would be NaN.)
-    const bool chunk = C == CODEC_NONE && chunk_applies(a) && a.scale_log2 != 0.0f;
+    const bool chunk = chunk_applies(a) && a.scale_log2 != 0.0f;
     const int bound = a.b.shared ? a.b.n_tokens : max_new;       // (a group's rows are those of its sequences)
     const bool few = bound > 0 && (int64_t)std::min(bound, a.b.n_tokens) * a.group <= RW_ROWS;
     const bool with_rows = few || !chunk || a.b.n_seq > 1;
@@ -711,7 +703,7 @@ hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cu
         if (s != HMM_OK) return s;
     }
     if (chunk && !few) {
-        s = run_chunk(a, std::is_same<T, __nv_bfloat16>::value, with_rows ? most + 1 : 1, with_rows,
+        s = run_chunk<C>(a, std::is_same<T, __nv_bfloat16>::value, with_rows ? most + 1 : 1, with_rows,
                       ws + up256(rows_workspace(dp)), st, &j.chunk);
         if (s != HMM_OK) return s;
     }
