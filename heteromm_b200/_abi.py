@@ -96,11 +96,12 @@ SIGNATURES = {
     "hmm_paged_quant_append": (C.c_int, [_P, _P, C.c_int, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P,
                                          C.c_int, _F, _P, _I, _I, C.c_int, _P, _P, _I, _I, _P, _P]),
     "hmm_paged_quant_read": (C.c_int, [_P, _P, C.c_int, _P, _P, _P, _P]),
-    "hmm_paged_quant_attention_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "hmm_paged_quant_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
     "hmm_paged_quant_attention": (C.c_int, [_P, _P, C.c_int, _P, _I, _I, _I, _F, C.c_int, _I, _I, _I, _P, _P, _P,
                                             _P, _S, _P]),
     "hmm_paged_prefix_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
     "hmm_paged_prefix_attention": (C.c_int, [_P, _P, _P, _P, _I, _P, _I, _I, _I, _F, _P, _P, _P, _P, _S, _P]),
+    "hmm_paged_quant_prefix_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
     "hmm_paged_quant_prefix_attention": (C.c_int, [_P, _P, C.c_int, _P, _P, _I, _P, _I, _I, _I, _F, _P, _P, _P, _P, _S,
                                                    _P]),
     "hmm_paged_state_workspace_size": (_S, [_I, _I]),

@@ -72,8 +72,14 @@ size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int
     return up256(rows_workspace(rows_dp(D))) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared);
 }
 
-template hmm_status_t run_attention<__nv_bfloat16, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
-template hmm_status_t run_attention<__half, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <>
+hmm_status_t run_attention<__nv_bfloat16, CODEC_NONE>(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
+    return run_kernels<__nv_bfloat16, CODEC_NONE>(a, max_new, ws, st);
+}
+template <>
+hmm_status_t run_attention<__half, CODEC_NONE>(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
+    return run_kernels<__half, CODEC_NONE>(a, max_new, ws, st);
+}
 
 }  // namespace serve
 }  // namespace hmm

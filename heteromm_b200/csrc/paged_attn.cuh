@@ -38,6 +38,7 @@ struct AttnArgs {
     float* lse;                  // [n_tokens][hq] or null
     float* part;                 // null, or where rows go in fp32 instead of `out` (each part of a batch of shared prefixes)
     QuantRows quant;             // of a cache in 8 bits
+    int min_rows;                // 0, or what the caller knows every sequence with rows to have
     float scale, scale_log2;     // scale * log2(e)
     int causal, window, sinks;
     int hq, hk, group, D, page_tokens, n_pages;
@@ -68,12 +69,21 @@ hmm_status_t plan_attention(const AttnCall& c, const hmm_paged_cache_t& dims, co
 
 inline size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// The kernels of a call over caches of this codec (paged_rows.cuh), with the host's bound on the
-// new tokens of any sequence (0: none known), and the bytes that they need (shared: for the parts
-// of a batch of shared prefixes, in which a token counts twice).
+// The kernels of a call over caches of this codec, with the host's bound on the new tokens of any
+// sequence (0: none known), and the bytes that they need (shared: for the parts of a batch of
+// shared prefixes, in which a token counts twice).
 template <typename T, int C>
 hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st);
+template <> hmm_status_t run_attention<__nv_bfloat16, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <> hmm_status_t run_attention<__half, CODEC_NONE>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <> hmm_status_t run_attention<__nv_bfloat16, CODEC_E4M3>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <> hmm_status_t run_attention<__half, CODEC_E4M3>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <> hmm_status_t run_attention<__nv_bfloat16, CODEC_I8>(const AttnArgs&, int, unsigned char*, cudaStream_t);
+template <> hmm_status_t run_attention<__half, CODEC_I8>(const AttnArgs&, int, unsigned char*, cudaStream_t);
 size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared);
+// (over a cache in 8 bits; max_kv: the tokens that a row of the page table can hold)
+size_t quant_attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D,
+                                 int64_t max_kv, int64_t max_new, bool shared);
 
 // A row of a unit (sequence, KV head): row r is new token r / group, head r % group.
 struct Span {                    // keys [0, sink) and [lo, hi) hold all that some row of a tile sees

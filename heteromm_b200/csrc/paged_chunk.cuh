@@ -67,7 +67,7 @@ template <int C>
 __host__ __device__ constexpr int tc_threads() { return 32 * (TC_SOFTMAX_WARPS + 4 + (C == CODEC_NONE ? 0 : TC_WIDEN_WARPS)); }
 // Registers: 384 threads are launched with 168 each (64,512 in all); the softmax warps
 // take 224 (a row's scores stay in registers), the last warpgroup keeps 56.  512 threads are
-// launched with 128 (65,536); the softmax warps take 208, the others 48.
+// launched with 128 (65,536): the softmax warps take 208, the others 48.
 template <int C>
 __host__ __device__ constexpr int tc_regs_launch() { return C == CODEC_NONE ? 168 : 128; }
 template <int C>
@@ -93,16 +93,16 @@ template <int DP>
 __host__ __device__ constexpr int tc_rows() { return DP == 256 ? TC_ROWS : TC_CTA_ROWS; }
 template <int DP, int C>
 __host__ __device__ constexpr int tc_stages() {
-    return C == CODEC_NONE ? (DP == 64 ? 8 : DP == 128 ? 5 : 2) : DP == 64 ? 6 : DP == 128 ? 3 : 2;
+    return C == CODEC_NONE ? (DP == 64 ? 8 : DP == 128 ? 5 : 2) : DP == 64 ? 6 : DP == 128 ? 4 : 2;
 }
-// A cache in 8 bits: the ring of codes as they are loaded, 128 keys by 128 codes (D = 64: 64) and the
-// scale bytes of those keys.
+// A cache in 8 bits: the ring of codes and scale bytes as they lie in the cache, a tile's keys a
+// stage (D = 256: half of them).
 template <int DP>
-__host__ __device__ constexpr int tc_code_stages() { return DP == 64 ? 6 : DP == 128 ? 3 : 2; }
+__host__ __device__ constexpr int tc_code_keys() { return DP == 256 ? TC_KEYS / 2 : TC_KEYS; }
 template <int DP>
-__host__ __device__ constexpr int tc_code_bytes() { return TC_KEYS * (DP < 128 ? DP : 128); }
+__host__ __device__ constexpr int tc_code_stages() { return DP == 64 ? 6 : 2; }
 template <int DP>
-__host__ __device__ constexpr int tc_scale_bytes() { return TC_KEYS * DP / Q_GROUP; }
+__host__ __device__ constexpr int tc_code_bytes() { return tc_code_keys<DP>() * (DP + DP / Q_GROUP); }
 template <int DP>
 __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * DP * 2; }
 template <int DP>
@@ -163,7 +163,7 @@ struct TcCtrl {
 template <int DP, int C>
 __host__ __device__ constexpr size_t tc_smem() {
     return tc_q_bytes<DP>() + tc_stages<DP, C>() * tc_tile_bytes<DP>() +
-           (C == CODEC_NONE ? 0 : tc_code_stages<DP>() * (tc_code_bytes<DP>() + tc_scale_bytes<DP>())) + sizeof(TcCtrl<DP>);
+           (C == CODEC_NONE ? 0 : tc_code_stages<DP>() * tc_code_bytes<DP>()) + sizeof(TcCtrl<DP>);
 }
 
 template <int N>
@@ -252,6 +252,13 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
         "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -291,18 +298,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Weights exp2(sc (s - m) + tc_up) of 64 of a row's scores v, packed in pairs, and their sum
-// (two pairs of partial sums); with TOP also the largest of the 128 scores from v on.
+// Weights exp2(sc (s - m) + tc_up) of 64 of a row's scores v, packed in pairs, to TMEM, and their
+// sum (two pairs of partial sums), AT of 32 registers at a time (the warps that widen leave
+// fewer); with TOP also the largest of the 128 scores from v on.
 // m = -inf (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
-template <typename T, bool TOP>
-__device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t* p,
+template <typename T, bool TOP, int AT>
+__device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t to,
                                          uint64_t* sum) {
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
     const float neg = m == -INFINITY ? 0.0f : fmaf(-m, sc, tc_up<T>());
     const uint64_t neg2 = pack_f2(neg, neg);
     sum[0] = sum[1] = pack_f2(0.0f, 0.0f);
+    uint32_t p[AT];
     float x[32], y[32], mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 32 + LAG; ++i) {
@@ -321,9 +330,11 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
             sum[u & 1] = add_f2(sum[u & 1], pack_f2(x[u], y[u]));
             // weights in the cache's type for the product: off by half a step, 2^-8 of a
             // weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
-            p[u] = pack2<T>(x[u], y[u]);
+            p[u % AT] = pack2<T>(x[u], y[u]);
+            if (AT == 16 && u % 16 == 15) tmem_st_x16(to + u - 15, p);
         }
     }
+    if (AT == 32) tmem_st_x32(to, p);
     return TOP ? max3(mx0, mx1, mx1) : 0.0f;
 }
 
@@ -398,7 +409,8 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     if (!t.split) return Plan{0, 0};
     int64_t units = 0;
     each_seq(a.b, a.max_kv, lane, 32, a.status, [&](const Seq& q) { units += (int64_t)row_blocks(t, q) * a.hk; });
-    if (warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
+    // (A shared prefix is a long unit beside many short ones.)
+    if (!a.b.shared && warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
     int longest = 0;
     auto add = [&](const Seq& q, int rb) {
@@ -584,49 +596,53 @@ __device__ __forceinline__ uint32_t q_at(int r, int c) {
     return (r / TC_ROWS) * (TC_ROWS * DP * 2) + (c >> 3) * (TC_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) * 16);
 }
 
-// Byte of 16-byte piece p (of 16 codes) of row r of a tile of codes.
-template <int DP>
-__device__ __forceinline__ int code_at(int r, int p) {
-    return DP == 64 ? r * 64 + ((p ^ (r >> 1 & 3)) * 16) : r * 128 + ((p ^ (r & 7)) * 16);
-}
-
-// Codes to a tile of T as the tensor cores read it, by one warp of four: a thread takes 16
-// codes of a row at a time, eight neighbours (D = 64: two rows of four) whose reads and writes
-// meet in no bank.  V rows that no row of the CTA sees become zeros: a weight of zero times what a
-// slot of nobody holds is only zero then.
-template <typename T, int DP, int C, typename Seen>
-__device__ __forceinline__ void widen_block(const unsigned char* codes, const unsigned char* scales, int per, int block,
-                                            unsigned char* tile, int warp, int lane, Seen seen) {
-    constexpr int PIECES = DP < 128 ? DP / 16 : 8, ROWS = 32 / PIECES;   // of a row here; rows of a warp's step
-    const int p = lane % PIECES;
-#pragma unroll 2
-    for (int r = warp * ROWS + lane / PIECES; r < TC_KEYS; r += TC_WIDEN_WARPS * ROWS) {
-        uint4 w = *reinterpret_cast<const uint4*>(codes + code_at<DP>(r, p));
-        uint32_t s = scales[r * per + min(4 * block + (p >> 1), per - 1)];
-        if (!seen(r)) {
-            w = make_uint4(0u, 0u, 0u, 0u);
-            s = 127;
-        }
-        const uint32_t m = multiplier<T, C>(s | s << 16), u[4] = {w.x, w.y, w.z, w.w};
-        uint32_t v[8];
+// Codes to (a half of) a tile of T as the tensor cores read it, by one warp of four.  The codes lie in
+// boxes of 2^box_log2 rows: the rows' codes, then their scale bytes.  A thread takes 16 codes of a
+// row at a time; of a row pair one half of the lanes takes the other row, so that eight
+// neighbours' writes (16-byte pieces 0, 2, 4, 6 of a 128-byte row, swizzled by its number)
+// meet in no bank.  Rows that `seen` denies become zeros.
+template <typename T, int DP, int C, bool SOME, typename Seen>
+__device__ __forceinline__ void widen_rows(const unsigned char* codes, const AttnArgs& a, int box_log2, unsigned char* tile,
+                                           int warp, int lane, Seen seen) {
+    constexpr int PIECES = DP / 16, ROWS = 32 / PIECES, STEP = TC_WIDEN_WARPS * ROWS, STEPS = tc_code_keys<DP>() / STEP;
+    constexpr int AHEAD = 4;                             // rows whose codes are read at once
+    static_assert(STEP % 8 == 0 && STEPS % AHEAD == 0, "a thread's rows are swizzled alike");
+    const int p = lane % PIECES, r0 = (warp * ROWS + lane / PIECES) ^ (PIECES >= 8 ? p >> 2 & 1 : 0);
+    const int per = a.quant.per_token, row_bytes = a.D, box_bytes = (row_bytes + per) << box_log2, in_box = (1 << box_log2) - 1;
+    const bool real = 16 * p < row_bytes;
+    unsigned char* to = tile + (p >> 2) * (TC_KEYS * 128) + r0 * 128;
+    const int at0 = ((2 * p & 7) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
+    const unsigned char *row = codes + 16 * p, *scale = codes + (row_bytes << box_log2) + (p >> 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t even, odd;
-            widen<T, C>(u[i], even, odd);
-            even = mul_pair<T>(even, m);
-            odd = mul_pair<T>(odd, m);
-            v[2 * i] = in_order_lo(even, odd);
-            v[2 * i + 1] = in_order_hi(even, odd);
-        }
-        // two pieces of 8 values; of a row's first and last eight pieces' writes one half takes the
-        // second piece first
-        const int c = 16 * block + 2 * p, first = PIECES == 8 ? p >> 2 & 1 : 0;
+    for (int i0 = 0; i0 < STEPS; i0 += AHEAD) {
+        uint4 w[AHEAD];
+        uint32_t s[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int x = c + (i ^ first);
-            const bool hi = (i ^ first) != 0;
-            *reinterpret_cast<uint4*>(tile + (x >> 3) * (TC_KEYS * 128) + r * 128 + (((x & 7) ^ (r & 7)) * 16)) =
-                make_uint4(hi ? v[4] : v[0], hi ? v[5] : v[1], hi ? v[6] : v[2], hi ? v[7] : v[3]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int r = r0 + (i0 + i) * STEP, box = (r >> box_log2) * box_bytes, in = r & in_box;
+            w[i] = make_uint4(0u, 0u, 0u, 0u);
+            s[i] = 127;
+            if (real && (!SOME || seen(r))) {
+                w[i] = *reinterpret_cast<const uint4*>(row + box + in * row_bytes);
+                s[i] = scale[box + in * per];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t m = multiplier<T, C>(s[i] * 0x00010001u), u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t v[8];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t even, odd;
+                widen<T, C>(u[x], even, odd);
+                even = mul_pair<T>(even, m);
+                odd = mul_pair<T>(odd, m);
+                v[2 * x] = in_order_lo(even, odd);
+                v[2 * x + 1] = in_order_hi(even, odd);
+            }
+            unsigned char* dst = to + (i0 + i) * STEP * 128;
+            *reinterpret_cast<uint4*>(dst + at0) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(dst + at1) = make_uint4(v[4], v[5], v[6], v[7]);
         }
     }
 }
@@ -637,9 +653,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ TcArgs t) {
     constexpr bool QUANT = C != CODEC_NONE;
     constexpr int ST = tc_stages<DP, C>();
-    // codes: stages, column blocks of a tile, bytes of a block's codes and scales
-    constexpr int CST = tc_code_stages<DP>(), BLOCKS = DP == 256 ? 2 : 1;
-    constexpr int CODES = tc_code_bytes<DP>(), SCALES = tc_scale_bytes<DP>();
+    // codes: stages, a stage's keys and bytes, stages of a tile
+    constexpr int CST = tc_code_stages<DP>(), CKEYS = tc_code_keys<DP>(), CODES = tc_code_bytes<DP>(), PARTS = TC_KEYS / CKEYS;
     constexpr int TILE = tc_tile_bytes<DP>();
     constexpr int HALVES = DP / 64;                    // 128-byte column blocks
     constexpr int UNIT = tc_rows<DP>();
@@ -656,9 +671,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
     unsigned char* Qs = smem_raw;                      // [tile][half][128 rows][128 B], swizzled
     unsigned char* Rs = Qs + tc_q_bytes<DP>();         // ring: [stage][half][128 keys][128 B]
-    unsigned char* Cs = Rs + ST * TILE;                // codes: [stage][128 keys][128 B], swizzled; their scale bytes
-    unsigned char* Ss = Cs + (QUANT ? CST * CODES : 0);
-    TcCtrl<DP>* ctl = reinterpret_cast<TcCtrl<DP>*>(Ss + (QUANT ? CST * SCALES : 0));
+    unsigned char* Cs = Rs + ST * TILE;                // codes: [stage][box][rows' codes, their scale bytes]
+    TcCtrl<DP>* ctl = reinterpret_cast<TcCtrl<DP>*>(Cs + (QUANT ? CST * CODES : 0));
     const AttnArgs& a = t.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort = &ctl->abort;
@@ -759,24 +773,27 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     const int n = min(ahead, u.n - j0);
                     for (int j = 0; ok && j < n; ++j) {
                         if constexpr (QUANT) {
-                            const Pages* of[2] = {&a.k, &a.v};
-                            const bool real = mine == j && page < a.n_pages;
-                            const uint32_t bytes = CODES + br * a.quant.per_token * __popc(__ballot_sync(0xffffffffu, real));
+                            // (a box of a page out of range is not asked for: nothing of it is seen)
+                            const int per = a.quant.per_token, box_bytes = br * (a.D + per);
+                            const int64_t in_page = (int64_t)row * a.D, scale_at = a.quant.scales + (int64_t)row * per;
 #pragma unroll 1
-                            for (int x = 0; x < 2 * BLOCKS; ++x, ++i) {
+                            for (int x = 0; x < 2 * PARTS; ++x, ++i) {
                                 const uint32_t st = i % CST;
-                                const int kv = x / BLOCKS, block = x % BLOCKS;
+                                const bool in = mine == j && page < a.n_pages && (PARTS == 1 || sub * br / CKEYS == x % PARTS);
+                                const Pages& p = x < PARTS ? a.k : a.v;
+                                const unsigned char* src = p.base + page * p.page + u.kvh * p.head;
+                                const uint32_t dst = smem_u32(Cs + st * CODES) + (PARTS == 1 ? sub : sub & (CKEYS / br - 1)) * box_bytes;
+                                const uint32_t bytes = box_bytes * __popc(__ballot_sync(0xffffffffu, in));
                                 if (!(ok = wait_warp(&ctl->c_empty[st], ((i / CST) & 1) ^ 1, abort, t.wait_ns))) break;
                                 if (lane == 0) mbar_expect_tx(&ctl->c_full[st], bytes);
                                 __syncwarp();
-                                if (mine == j)
-                                    tma_load_page(smem_u32(Cs + st * CODES) + sub * br * (CODES / TC_KEYS), kv ? &tmV : &tmK,
-                                                  &ctl->c_full[st], 128 * block, row, u.kvh, page);
-                                if (real)   // (scale bytes of pages out of range are not asked for)
-                                    bulk_load(smem_u32(Ss + st * SCALES) + sub * br * a.quant.per_token,
-                                              of[kv]->base + page * of[kv]->page + u.kvh * of[kv]->head + a.quant.scales +
-                                                  (int64_t)row * a.quant.per_token,
-                                              br * a.quant.per_token, &ctl->c_full[st]);
+                                if (!in) continue;
+                                if (br == a.page_tokens) {   // all of a page and head: one block
+                                    bulk_load(dst, src, box_bytes, &ctl->c_full[st]);
+                                } else {
+                                    bulk_load(dst, src + in_page, br * a.D, &ctl->c_full[st]);
+                                    bulk_load(dst + br * a.D, src + scale_at, br * per, &ctl->c_full[st]);
+                                }
                             }
                         } else {
                             for (int kv = 0; kv < 2; ++kv, ++i) {
@@ -952,8 +969,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             __syncwarp();
         } else if (QUANT && warp >= TC_SOFTMAX_WARPS + 4) {
             // ------------------------------------------- codes to 16-bit tiles
-            const int mine = warp - TC_SOFTMAX_WARPS - 4, per = a.quant.per_token;
-            uint32_t i = 0, c = 0;               // tiles, and blocks of codes so far
+            // V rows that no row of the CTA sees become zeros: a weight of zero times what a slot of nobody
+            // holds is only zero then.
+            const int mine = warp - TC_SOFTMAX_WARPS - 4, box_log2 = 31 - __clz(t.box_rows);
+            uint32_t i = 0, c = 0;               // tiles, and stages of codes so far
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 const Unit& u = ctl->unit[k & 1];
@@ -964,13 +983,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     const uint32_t st = i % ST;
                     if (!(ok = wait_warp(&ctl->empty[st], ((i / ST) & 1) ^ 1, abort, t.wait_ns))) break;
                     const int key0 = u.key0(j >> 1);
-                    const bool mends = (j & 1) && u.mends(key0);
+                    const bool some = (j & 1) && u.mends(key0);
 #pragma unroll 1
-                    for (int b = 0; b < BLOCKS; ++b, ++c) {
+                    for (int x = 0; x < PARTS; ++x, ++c) {
                         const uint32_t cs = c % CST;
                         if (!(ok = wait_warp(&ctl->c_full[cs], (c / CST) & 1, abort, t.wait_ns))) break;
-                        widen_block<T, DP, C>(Cs + cs * CODES, Ss + cs * SCALES, per, b, Rs + st * TILE, mine, lane,
-                                              [&](int r) { return !mends || span_has(u.sp, key0 + r); });
+                        unsigned char* to = Rs + st * TILE + x * CKEYS * 128;
+                        auto seen = [&](int r) { return span_has(u.sp, key0 + x * CKEYS + r); };
+                        if (some) widen_rows<T, DP, C, true>(Cs + cs * CODES, a, box_log2, to, mine, lane, seen);
+                        else widen_rows<T, DP, C, false>(Cs + cs * CODES, a, box_log2, to, mine, lane, seen);
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&ctl->c_empty[cs]);
                     }
@@ -1121,11 +1142,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 // The first half's weights with the maximum so far, while this tile's is found:
                 // that is right unless the row grew by more than TC_GROWTH, which is rare.
                 // NaN and +inf show in the maximum: such a row is NaN.
-                uint32_t p[32];
+                // (They go over the scores, which are in registers, and are written again if it was not.)
                 uint64_t sum[2];
 #pragma unroll 1
                 while (true) {
-                    const float top = weights<T, true>(v, sc2, m, sc, p, sum);
+                    const float top = weights<T, true, QUANT ? 16 : 32>(v, sc2, m, sc, ts, sum);
                     fine = fine && top < INFINITY;
                     const bool grow = (top - m) * sc > TC_GROWTH && top < INFINITY;
                     if (!__any_sync(0xffffffffu, grow)) break;
@@ -1148,15 +1169,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     }
                 }
                 // the first half's product starts while the second half is in the exponentials
-                tmem_st_x32(ts, p);
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-                weights<T, false>(v + 64, sc2, m, sc, p, sum);
-                tmem_st_x32(ts + 32, p);
+                weights<T, false, QUANT ? 16 : 32>(v + 64, sc2, m, sc, ts + 32, sum);
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
                 tmem_wait_st();
@@ -1334,7 +1353,7 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
     t.a = a;
     t.rows_log2 = rows == 256 ? 8 : 7;
     t.min_rows = min_rows;
-    t.box_rows = box_rows_of(a.page_tokens, TC_KEYS);
+    t.box_rows = box_rows_of(a.page_tokens, C != CODEC_NONE && a.D > 128 ? tc_code_keys<256>() : TC_KEYS);
     t.split = a.b.shared || may_split(a.b.n_tokens, a.group, a.hk, rows);
     t.q_tokens = boxes ? TC_ROWS / a.group : 0;
     t.wait_ns = wait_limit_ns();

@@ -149,10 +149,11 @@ __global__ void __launch_bounds__(MG_THREADS) paged_merge_kernel(const __grid_co
 struct PrefixSpace {
     size_t attention, parts, of_group, part, lse, all;
 };
-PrefixSpace prefix_space(int64_t n_seq, int64_t n_tokens, int64_t n_groups, int64_t n_heads, int64_t n_kv_heads,
-                                int64_t D) {
+PrefixSpace prefix_space(int64_t n_seq, int64_t n_tokens, int64_t n_groups, int64_t n_heads, int64_t n_kv_heads, int64_t D,
+                         bool quant, int64_t max_kv) {
     PrefixSpace w;
-    w.attention = up256(attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, true));
+    w.attention = up256(quant ? quant_attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, max_kv, 0, true)
+                              : attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, true));
     w.parts = up256(2 * sizeof(int4) * (size_t)(n_seq + n_groups));
     w.of_group = up256(3 * sizeof(int32_t) * (size_t)n_groups);
     w.part = up256(2 * sizeof(float) * (size_t)(n_tokens * n_heads * D));
@@ -199,7 +200,7 @@ using namespace hmm::serve;
 extern "C" size_t hmm_paged_prefix_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_groups,
                                                             int64_t n_heads, int64_t n_kv_heads, int64_t D) {
     if (n_seq < 0 || n_tokens < 0 || n_groups < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256) return 0;
-    return prefix_space(n_seq, n_tokens, n_groups, n_heads, n_kv_heads, D).all;
+    return prefix_space(n_seq, n_tokens, n_groups, n_heads, n_kv_heads, D, false, 0).all;
 }
 
 extern "C" hmm_status_t hmm_paged_prefix_attention(const hmm_paged_cache_t* cache, const hmm_paged_batch_t* batch,
@@ -217,11 +218,19 @@ extern "C" hmm_status_t hmm_paged_prefix_attention(const hmm_paged_cache_t* cach
     s = plan_attention({q, q_token, q_head, n_heads, scale, 1, 0, 0, 0, out, lse, device_status, workspace, workspace_bytes,
                         need}, *cache, batch, false, &a, &nothing);
     if (s != HMM_OK || nothing) return s;
-    const PrefixSpace w = prefix_space(batch->n_seq, batch->n_tokens, n_groups, n_heads, cache->n_kv_heads, cache->D);
+    const PrefixSpace w = prefix_space(batch->n_seq, batch->n_tokens, n_groups, n_heads, cache->n_kv_heads, cache->D,
+                                       false, 0);
     return cache->dtype == HMM_DTYPE_BF16 ? run_prefix<__nv_bfloat16, CODEC_NONE>(a, cu_group, prefix_len, n_groups, w,
                                                                                   (unsigned char*)workspace, (cudaStream_t)stream)
                                           : run_prefix<__half, CODEC_NONE>(a, cu_group, prefix_len, n_groups, w,
                                                                            (unsigned char*)workspace, (cudaStream_t)stream);
+}
+
+extern "C" size_t hmm_paged_quant_prefix_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_groups,
+                                                                  int64_t n_heads, int64_t n_kv_heads, int64_t D,
+                                                                  int64_t max_kv) {
+    if (n_seq < 0 || n_tokens < 0 || n_groups < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256 || max_kv < 0) return 0;
+    return prefix_space(n_seq, n_tokens, n_groups, n_heads, n_kv_heads, D, true, max_kv).all;
 }
 
 extern "C" hmm_status_t hmm_paged_quant_prefix_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch,
@@ -237,13 +246,15 @@ extern "C" hmm_status_t hmm_paged_quant_prefix_attention(const hmm_paged_quant_t
                 "dtype must be HMM_DTYPE_BF16 or HMM_DTYPE_F16, got %d", dtype);
     s = check_groups(cu_group, prefix_len, n_groups, batch->n_seq);
     if (s != HMM_OK) return s;
-    const size_t need = hmm_paged_prefix_attention_workspace_size(batch->n_seq, batch->n_tokens, n_groups, n_heads,
-                                                                  cache->n_kv_heads, cache->D);
+    const int64_t max_kv = batch->pages_per_seq * cache->page_tokens;
+    const size_t need = hmm_paged_quant_prefix_attention_workspace_size(batch->n_seq, batch->n_tokens, n_groups, n_heads,
+                                                                        cache->n_kv_heads, cache->D, max_kv);
     bool nothing;
     s = plan_attention({q, q_token, q_head, n_heads, scale, 1, 0, 0, 0, out, lse, device_status, workspace, workspace_bytes,
                         need}, quant_dims(*cache), batch, true, &a, &nothing);
     if (s != HMM_OK || nothing) return s;
-    const PrefixSpace w = prefix_space(batch->n_seq, batch->n_tokens, n_groups, n_heads, cache->n_kv_heads, cache->D);
+    const PrefixSpace w = prefix_space(batch->n_seq, batch->n_tokens, n_groups, n_heads, cache->n_kv_heads, cache->D,
+                                       true, max_kv);
     unsigned char* ws = (unsigned char*)workspace;
     const cudaStream_t st = (cudaStream_t)stream;
     if (cache->codes == HMM_DTYPE_E4M3)

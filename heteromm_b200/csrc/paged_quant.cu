@@ -55,33 +55,6 @@ struct ReadArgs {
     int32_t* status;
 };
 
-// Sixteen codes of one scale as values of O at dst.
-template <typename O, int C>
-__device__ __forceinline__ void store16(O* dst, const uint4& w, uint32_t s) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    if constexpr (std::is_same<O, float>::value) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            reinterpret_cast<float4*>(dst)[i] =
-                make_float4(value_of<C>(u[i] & 255u, s), value_of<C>(u[i] >> 8 & 255u, s),
-                            value_of<C>(u[i] >> 16 & 255u, s), value_of<C>(u[i] >> 24, s));
-    } else {
-        const uint32_t m = multiplier<O, C>(s | s << 16);
-        uint32_t r[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t even, odd;
-            widen<O, C>(u[i], even, odd);
-            even = mul_pair<O>(even, m);
-            odd = mul_pair<O>(odd, m);
-            r[2 * i] = in_order_lo(even, odd);
-            r[2 * i + 1] = in_order_hi(even, odd);
-        }
-        reinterpret_cast<uint4*>(dst)[0] = make_uint4(r[0], r[1], r[2], r[3]);
-        reinterpret_cast<uint4*>(dst)[1] = make_uint4(r[4], r[5], r[6], r[7]);
-    }
-}
-
 template <typename O, int C>
 __global__ void __launch_bounds__(RD_THREADS) paged_quant_read_kernel(const __grid_constant__ ReadArgs a) {
     const int lane = threadIdx.x & 31, warps = gridDim.x * (RD_THREADS / 32);

@@ -140,6 +140,33 @@ __device__ __forceinline__ float value_of(uint32_t code, uint32_t s) {
     return __uint_as_float((code & 0x80u) << 24 | (code & 0x7fu) << 20) * 0x1p120f * scale;
 }
 
+// Sixteen codes of one scale as values of O at dst.
+template <typename O, int C>
+__device__ __forceinline__ void store16(O* dst, const uint4& w, uint32_t s) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (std::is_same<O, float>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(dst)[i] =
+                make_float4(value_of<C>(u[i] & 255u, s), value_of<C>(u[i] >> 8 & 255u, s),
+                            value_of<C>(u[i] >> 16 & 255u, s), value_of<C>(u[i] >> 24, s));
+    } else {
+        const uint32_t m = multiplier<O, C>(s | s << 16);
+        uint32_t r[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t even, odd;
+            widen<O, C>(u[i], even, odd);
+            even = mul_pair<O>(even, m);
+            odd = mul_pair<O>(odd, m);
+            r[2 * i] = in_order_lo(even, odd);
+            r[2 * i + 1] = in_order_hi(even, odd);
+        }
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    }
+}
+
 // ------------------------------------------------------------ host helpers
 
 // The sizes of a cache as those of one of 16-bit values.

@@ -682,7 +682,7 @@ hmm_status_t run_rows(const RowsArgs& r, cudaStream_t st) {
 }
 
 template <typename T, int C>
-hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
+hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
     // A unit of up to 16 rows (one MMA's) reads its keys once either way and the many small
     // CTAs of the rows kernel keep more reads in flight; more rows would read them again
     // there: 64 rows of 4 KV heads over 5,000, 16 sequences, D = 128, 113 us there and 69 in
@@ -691,7 +691,7 @@ hmm_status_t run_attention(const AttnArgs& a, int max_new, unsigned char* ws, cu
     const bool chunk = chunk_applies(a) && a.scale_log2 != 0.0f;
     const int bound = a.b.shared ? a.b.n_tokens : max_new;       // (a group's rows are those of its sequences)
     const bool few = bound > 0 && (int64_t)std::min(bound, a.b.n_tokens) * a.group <= RW_ROWS;
-    const bool with_rows = few || !chunk || a.b.n_seq > 1;
+    const bool with_rows = few || !chunk || (a.b.n_seq > 1 && a.min_rows <= RW_ROWS);
     const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel
     const int dp = rows_dp(a.D);
     const int64_t ctas = rows_ctas(dp);

@@ -53,6 +53,7 @@ struct Entry {
     decltype(&hmm_paged_prefix_attention) prefix_attention;
     decltype(&hmm_paged_prefix_attention_workspace_size) prefix_attention_workspace;
     decltype(&hmm_paged_quant_prefix_attention) quant_prefix_attention;
+    decltype(&hmm_paged_quant_prefix_attention_workspace_size) quant_prefix_attention_workspace;
 };
 Entry hmm_fn{};
 PyObject* raise_error = nullptr;   // (entry point's name, status): raises HmmError
@@ -360,8 +361,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     Tensor lse;
     if (with_lse) lse = empty({n_tokens, heads}, at::kFloat, c.dev);
     const Status status = status_word(a[13], c.dev, at.stream);
-    const size_t bytes = (QUANT ? hmm_fn.quant_attention_workspace : hmm_fn.attention_workspace)(b.n_seq, n_tokens, heads,
-                                                                                                 c.c.n_kv_heads, d);
+    const size_t bytes = QUANT ? hmm_fn.quant_attention_workspace(b.n_seq, n_tokens, heads, c.c.n_kv_heads, d,
+                                                                  b.pages_per_seq * qc.c.page_tokens, max_new)
+                               : hmm_fn.attention_workspace(b.n_seq, n_tokens, heads, c.c.n_kv_heads, d);
     const c10::DataPtr ws = scratch(bytes);
     finish(unlocked([&] {
                if constexpr (QUANT)
@@ -405,7 +407,9 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (with_lse) lse = empty({n_tokens, heads}, at::kFloat, c.dev);
     float* lp = with_lse ? lse.data_ptr<float>() : nullptr;
     const Status status = status_word(a[12], c.dev, at.stream);
-    const size_t bytes = hmm_fn.prefix_attention_workspace(b.n_seq, n_tokens, groups, heads, c.c.n_kv_heads, d);
+    const size_t bytes = quant ? hmm_fn.quant_prefix_attention_workspace(b.n_seq, n_tokens, groups, heads, c.c.n_kv_heads, d,
+                                                                         b.pages_per_seq * qc.c.page_tokens)
+                               : hmm_fn.prefix_attention_workspace(b.n_seq, n_tokens, groups, heads, c.c.n_kv_heads, d);
     const c10::DataPtr ws = scratch(bytes);
     const int32_t* pl = (const int32_t*)prefix.data_ptr();
     finish(unlocked([&] {

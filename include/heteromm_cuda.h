@@ -457,9 +457,12 @@ hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, const hmm_page
 
 /* hmm_paged_attention over a cache held in 8 bits: q and out of `dtype`
  * (HMM_DTYPE_BF16 or HMM_DTYPE_F16), all else as there.  The result is that of a
- * cache that holds the values in `dtype`; a seen group with s = 255 gives NaN. */
+ * cache that holds the values in `dtype`; a seen group with s = 255 gives NaN.
+ * Workspace: with max_kv = pages_per_seq * page_tokens and the call's max_new (a
+ * bound keeps it small: chunks of 512 rows (new tokens * query heads of a group)
+ * and more have their keys widened into it, up to 1 GiB of them). */
 size_t hmm_paged_quant_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
-                                                int64_t n_kv_heads, int64_t D);
+                                                int64_t n_kv_heads, int64_t D, int64_t max_kv, int64_t max_new);
 hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
                                        const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
                                        float scale, int causal, int64_t window, int64_t sinks, int64_t max_new,
@@ -488,7 +491,10 @@ hmm_status_t hmm_paged_prefix_attention(const hmm_paged_cache_t* cache, const hm
                                         const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
                                         float scale, void* out, float* lse, int32_t* device_status,
                                         void* workspace, size_t workspace_bytes, void* stream);
-/* The same over a cache held in 8 bits (and the same workspace). */
+/* The same over a cache held in 8 bits (max_kv = pages_per_seq * page_tokens). */
+size_t hmm_paged_quant_prefix_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_groups,
+                                                       int64_t n_heads, int64_t n_kv_heads, int64_t D,
+                                                       int64_t max_kv);
 hmm_status_t hmm_paged_quant_prefix_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch,
                                               int dtype, const int32_t* cu_group, const int32_t* prefix_len,
                                               int64_t n_groups, const void* q, int64_t q_token, int64_t q_head,

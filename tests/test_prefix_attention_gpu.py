@@ -73,6 +73,7 @@ BATCHES = [  # groups (first, end, prefix), new, kv, hq, hk, d, pt
     ([(0, 1, 100), (1, 2, 50)], [1, 3], [200, 100], 4, 2, 64, 16),                           # alone: nothing shared
     ([(0, 40, 1111)], [3] * 40, [1114 + (53 * i) % 400 for i in range(40)], 7, 1, 128, 32),
     ([(0, 3, 250)], [130, 7, 300], [400, 300, 550], 8, 2, 64, 16),                           # chunks
+    ([(0, 70, 600), (70, 75, 100)], [2] * 75, [610 + (7 * i) % 90 for i in range(70)] + [110] * 5, 4, 1, 128, 16),  # 560 rows
     ([(0, 9, 333)], [1] * 9, [340 + i for i in range(9)], 4, 2, 256, 16),
     ([(0, 5, 90)], [1] * 5, [100 + i for i in range(5)], 6, 2, 80, 5),                       # pages of the rows kernel alone
     ([(0, 2, 0)], [1, 1], [33, 20], 2, 1, 64, 16),

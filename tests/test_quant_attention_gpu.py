@@ -91,6 +91,27 @@ def test_all_keys_and_scale(cuda, shape):
     run_case(cuda, 9, *shape, "fp16", "e4m3", scale=0.0)
 
 
+@pytest.mark.parametrize("kind,dtype", [("e4m3", "bf16"), ("int8", "fp16")])
+@pytest.mark.parametrize("shape", [
+    ([600], [600], 2, 1, 64, 16),                                 # one sequence, widened whatever it holds
+    ([0], [40], 4, 2, 64, 16),
+    ([700, 1, 300, 3, 130], [900, 50, 301, 700, 2000], 8, 2, 128, 16),
+    ([256, 200, 260], [300, 1000, 261], 2, 1, 128, 4),            # 512 rows, 400, 520; small pages
+    ([520, 40], [530, 400], 3, 3, 96, 16),
+    ([128, 128, 1], [128, 700, 9], 8, 2, 256, 2),
+])
+def test_chunks_of_many_rows(cuda, shape, kind, dtype):
+    """Their keys are widened into the workspace first, beside sequences that are not."""
+    run_case(cuda, 13, *shape, dtype, kind, pad=3)
+    run_case(cuda, 13, *shape, dtype, kind, max_new=max(shape[0]), window=100, sinks=5)
+    run_case(cuda, 13, *shape, dtype, kind, causal=False, scale=0.2)
+
+
+def test_what_the_workspace_has_no_room_for(cuda):
+    """64 KV heads of 256: room for 16,384 widened tokens, and three chunks over 8,000 each."""
+    run_case(cuda, 14, [512, 530, 3, 515], [8000, 8100, 70, 8001], 64, 64, 256, 64, "bf16", "e4m3")
+
+
 @pytest.mark.parametrize("max_new", [0, 1, 4, 1000])
 def test_hint_is_only_a_hint(cuda, max_new):
     run_case(cuda, 10, [1, 50, 1, 4], [300, 50, 1000, 4], 8, 2, 128, 16, "bf16", "e4m3", max_new=max_new)

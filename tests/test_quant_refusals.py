@@ -120,21 +120,29 @@ def test_bad_groups(kw, text):
 
 def test_workspaces():
     lib = hmm.load()
-    for n_seq, n_tokens, heads, hk, d in ((2, 5, 4, 2, 64), (64, 64, 32, 8, 128), (3, 2000, 7, 1, 256), (1, 1, 1, 1, 32)):
-        need = lib.hmm_paged_quant_attention_workspace_size(n_seq, n_tokens, heads, hk, d)
-        assert need > 0
+    for n_seq, n_tokens, heads, hk, d, max_new in ((2, 5, 4, 2, 64, 0), (64, 64, 32, 8, 128, 1), (64, 200, 32, 8, 128, 0),
+                                                   (3, 2000, 7, 1, 256, 0), (1, 1, 1, 1, 32, 0)):
+        c = quant(n_kv_heads=hk, D=d, page_tokens=64, k_page=1 << 20, k_head=1 << 15, v_page=1 << 20, v_head=1 << 15)
+        b, kw = batch(n_seq=n_seq, n_tokens=n_tokens), dict(n_heads=heads, q_token=heads * d, q_head=d)
+        plain = lib.hmm_paged_attention_workspace_size(n_seq, n_tokens, heads, hk, d)
+        need = lib.hmm_paged_quant_attention_workspace_size(n_seq, n_tokens, heads, hk, d, 4 * 64, max_new)
+        assert plain > 0 and need >= plain
+        wide = n_tokens * heads // hk >= 512 and max_new == 0       # rows whose keys may be widened into the workspace
+        assert wide == (need > plain + 4 * 256 * hk * d)
         for n in (0, need - 1):
-            r = attend(quant(n_kv_heads=hk, D=d, page_tokens=64, k_page=1 << 20, k_head=1 << 15, v_page=1 << 20, v_head=1 << 15),
-                       batch(n_seq=n_seq, n_tokens=n_tokens), n_heads=heads, q_token=heads * d, q_head=d, nbytes=n)
-            refused(r, "workspace too small", HMM_ERR_OOM)
+            refused(attend(c, b, max_new=max_new, nbytes=n, **kw), "workspace too small", HMM_ERR_OOM)
         for groups in (0, n_seq):
             more = lib.hmm_paged_prefix_attention_workspace_size(n_seq, n_tokens, groups, heads, hk, d)
-            assert more >= need + 8 * n_tokens * heads * (d + 1)
-            r = shared(cache(n_kv_heads=hk, D=d), batch(n_seq=n_seq, n_tokens=n_tokens), n_groups=groups, n_heads=heads,
-                       q_token=heads * d, q_head=d, nbytes=more - 1)
-            refused(r, "workspace too small", HMM_ERR_OOM)
-    assert lib.hmm_paged_quant_attention_workspace_size(1, 1, 1, 1, 257) == 0
+            assert more >= plain + 8 * n_tokens * heads * (d + 1)
+            refused(shared(cache(n_kv_heads=hk, D=d), b, n_groups=groups, nbytes=more - 1, **kw), "workspace too small", HMM_ERR_OOM)
+            more = lib.hmm_paged_quant_prefix_attention_workspace_size(n_seq, n_tokens, groups, heads, hk, d, 4 * 64)
+            refused(shared_quant(c, b, n_groups=groups, nbytes=more - 1, **kw), "workspace too small", HMM_ERR_OOM)
+    assert lib.hmm_paged_quant_attention_workspace_size(1, 1, 1, 1, 257, 64, 0) == 0
+    assert lib.hmm_paged_quant_attention_workspace_size(1, 1, 1, 1, 64, -1, 0) == 0
     assert lib.hmm_paged_prefix_attention_workspace_size(1, 1, -1, 1, 1, 64) == 0
+    assert lib.hmm_paged_quant_prefix_attention_workspace_size(1, 1, -1, 1, 1, 64, 64) == 0
+    # a long table takes no more than the limit
+    assert lib.hmm_paged_quant_attention_workspace_size(64, 65536, 32, 8, 128, 1 << 20, 0) < 3 << 30
 
 
 @pytest.mark.parametrize("kw,text", [
