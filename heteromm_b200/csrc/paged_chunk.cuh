@@ -601,28 +601,30 @@ __device__ __forceinline__ uint32_t q_at(int r, int c) {
 // row at a time; of a row pair one half of the lanes takes the other row, so that eight
 // neighbours' writes (16-byte pieces 0, 2, 4, 6 of a 128-byte row, swizzled by its number)
 // meet in no bank.  Rows that `seen` denies become zeros.
-template <typename T, int DP, int C, bool SOME, typename Seen>
+// The loop is short on purpose: next to the softmax's straight code, a longer one (all rows
+// unrolled) did not stay in the instruction cache, and every role ran at a fifth of its speed.
+template <typename T, int DP, int C, typename Seen>
 __device__ __forceinline__ void widen_rows(const unsigned char* codes, const AttnArgs& a, int box_log2, unsigned char* tile,
-                                           int warp, int lane, Seen seen) {
-    constexpr int PIECES = DP / 16, ROWS = 32 / PIECES, STEP = TC_WIDEN_WARPS * ROWS, STEPS = tc_code_keys<DP>() / STEP;
-    constexpr int AHEAD = 4;                             // rows whose codes are read at once
-    static_assert(STEP % 8 == 0 && STEPS % AHEAD == 0, "a thread's rows are swizzled alike");
+                                           int warp, int lane, bool some, Seen seen) {
+    constexpr int PIECES = DP / 16, ROWS = 32 / PIECES, STEP = TC_WIDEN_WARPS * ROWS;
+    constexpr int AHEAD = 2;                             // rows whose codes are read at once
+    static_assert(STEP % 8 == 0 && tc_code_keys<DP>() % (STEP * AHEAD) == 0, "a thread's rows are swizzled alike");
     const int p = lane % PIECES, r0 = (warp * ROWS + lane / PIECES) ^ (PIECES >= 8 ? p >> 2 & 1 : 0);
     const int per = a.quant.per_token, row_bytes = a.D, box_bytes = (row_bytes + per) << box_log2, in_box = (1 << box_log2) - 1;
     const bool real = 16 * p < row_bytes;
     unsigned char* to = tile + (p >> 2) * (TC_KEYS * 128) + r0 * 128;
     const int at0 = ((2 * p & 7) ^ (r0 & 7)) * 16, at1 = at0 ^ 16;
     const unsigned char *row = codes + 16 * p, *scale = codes + (row_bytes << box_log2) + (p >> 1);
-#pragma unroll
-    for (int i0 = 0; i0 < STEPS; i0 += AHEAD) {
+#pragma unroll 1
+    for (int r = r0; r < tc_code_keys<DP>(); r += AHEAD * STEP, to += AHEAD * STEP * 128) {
         uint4 w[AHEAD];
         uint32_t s[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int r = r0 + (i0 + i) * STEP, box = (r >> box_log2) * box_bytes, in = r & in_box;
+            const int x = r + i * STEP, box = (x >> box_log2) * box_bytes, in = x & in_box;
             w[i] = make_uint4(0u, 0u, 0u, 0u);
             s[i] = 127;
-            if (real && (!SOME || seen(r))) {
+            if (real && (!some || seen(x))) {
                 w[i] = *reinterpret_cast<const uint4*>(row + box + in * row_bytes);
                 s[i] = scale[box + in * per];
             }
@@ -640,9 +642,8 @@ __device__ __forceinline__ void widen_rows(const unsigned char* codes, const Att
                 v[2 * x] = in_order_lo(even, odd);
                 v[2 * x + 1] = in_order_hi(even, odd);
             }
-            unsigned char* dst = to + (i0 + i) * STEP * 128;
-            *reinterpret_cast<uint4*>(dst + at0) = make_uint4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<uint4*>(dst + at1) = make_uint4(v[4], v[5], v[6], v[7]);
+            *reinterpret_cast<uint4*>(to + i * STEP * 128 + at0) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(to + i * STEP * 128 + at1) = make_uint4(v[4], v[5], v[6], v[7]);
         }
     }
 }
@@ -989,9 +990,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         const uint32_t cs = c % CST;
                         if (!(ok = wait_warp(&ctl->c_full[cs], (c / CST) & 1, abort, t.wait_ns))) break;
                         unsigned char* to = Rs + st * TILE + x * CKEYS * 128;
-                        auto seen = [&](int r) { return span_has(u.sp, key0 + x * CKEYS + r); };
-                        if (some) widen_rows<T, DP, C, true>(Cs + cs * CODES, a, box_log2, to, mine, lane, seen);
-                        else widen_rows<T, DP, C, false>(Cs + cs * CODES, a, box_log2, to, mine, lane, seen);
+                        widen_rows<T, DP, C>(Cs + cs * CODES, a, box_log2, to, mine, lane, some,
+                                             [&](int r) { return span_has(u.sp, key0 + x * CKEYS + r); });
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&ctl->c_empty[cs]);
                     }

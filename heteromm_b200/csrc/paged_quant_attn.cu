@@ -7,8 +7,10 @@
 // more are widened once, into a cache of the workspace, and attended to there
 // (8,192 tokens, 32/8 heads of 128, int8: 830 us within the chunk kernel, 500 so; a key
 // costs 6 KB of memory traffic once, and 80 ps per head and 256 rows more within the kernel: as
-// much at a block and a half, 384 rows).  What the workspace has no room for stays with the kernels
-// that widen.
+// much at a block and a half, 384 rows).  The kernels for it cost 25 us beside, so a call that cannot
+// come to LONG_TILES products of 256 rows and 128 keys (1.6 us more each on one of the SMs, 43 us in
+// all) has none (8 sequences, a chunk of 1,001 tokens among them, a window of 1,024: 64 us, 117
+// widened first).  What the workspace has no room for stays with the kernels that widen.
 #include "paged_rows.cuh"
 
 namespace hmm {
@@ -16,6 +18,7 @@ namespace serve {
 namespace {
 
 constexpr int LONG_ROWS = 512;
+constexpr int64_t LONG_TILES = 4096;
 constexpr int WIDE_TOKENS = 128;                     // tokens of a page of the workspace's cache
 constexpr int64_t WIDE_BYTES = int64_t(1) << 30;     // of that cache, at most
 constexpr int CL_THREADS = 1024, WD_THREADS = 256;
@@ -28,11 +31,13 @@ struct WidePlan {
     size_t bytes() const { return kernels + parts + wide_parts + owner + table + wide_kernels + 2 * cache; }
 };
 
-WidePlan wide_plan(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t hk, int64_t D, int64_t max_kv, int64_t max_new,
-                   bool shared) {
+WidePlan wide_plan(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t hk, int64_t D, int64_t max_kv, int64_t window,
+                   int64_t max_new, bool shared) {
     WidePlan w{};
     const int64_t group = std::max<int64_t>(1, n_heads / hk), rows = n_tokens * group;
-    const bool never = n_seq == 0 || (max_new > 0 && std::min(max_new, n_tokens) * group < LONG_ROWS) || rows < LONG_ROWS;
+    const int64_t keys = window > 0 ? std::min(max_kv, window + 256) : max_kv;   // of 256 rows, about
+    const bool never = n_seq == 0 || (max_new > 0 && std::min(max_new, n_tokens) * group < LONG_ROWS) || rows < LONG_ROWS ||
+                       (shared ? 2 : 1) * rows / 256 * hk * ((keys + 127) / 128) < LONG_TILES;
     if (!never) {
         const int64_t per_seq = (max_kv + WIDE_TOKENS - 1) / WIDE_TOKENS;
         w.most = std::min(n_seq, (shared ? 2 : 1) * rows / LONG_ROWS);
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(WD_THREADS) paged_widen_kernel(const __grid_co
 
 template <typename T, int C>
 hmm_status_t run_quant(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
-    const WidePlan p = wide_plan(a.b.n_seq, a.b.n_tokens, a.hq, a.hk, a.D, a.max_kv, max_new, a.b.shared != nullptr);
+    const WidePlan p = wide_plan(a.b.n_seq, a.b.n_tokens, a.hq, a.hk, a.D, a.max_kv, a.window, max_new, a.b.shared != nullptr);
     if (p.pages == 0) return run_kernels<T, C>(a, max_new, ws, st);
     WideArgs w{};
     unsigned char* at = ws + p.kernels;
@@ -218,7 +223,9 @@ hmm_status_t run_attention<__half, CODEC_I8>(const AttnArgs& a, int max_new, uns
 
 size_t quant_attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D,
                                  int64_t max_kv, int64_t max_new, bool shared) {
-    return wide_plan(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, max_new, shared).bytes();
+    // (a window may need less)
+    const size_t wide = wide_plan(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, 0, max_new, shared).bytes();
+    return std::max(wide, attention_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared));
 }
 
 }  // namespace serve

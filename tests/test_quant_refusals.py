@@ -121,13 +121,13 @@ def test_bad_groups(kw, text):
 def test_workspaces():
     lib = hmm.load()
     for n_seq, n_tokens, heads, hk, d, max_new in ((2, 5, 4, 2, 64, 0), (64, 64, 32, 8, 128, 1), (64, 200, 32, 8, 128, 0),
-                                                   (3, 2000, 7, 1, 256, 0), (1, 1, 1, 1, 32, 0)):
+                                                   (3, 99000, 7, 1, 256, 0), (1, 1, 1, 1, 32, 0), (3, 99000, 7, 1, 128, 16)):
         c = quant(n_kv_heads=hk, D=d, page_tokens=64, k_page=1 << 20, k_head=1 << 15, v_page=1 << 20, v_head=1 << 15)
         b, kw = batch(n_seq=n_seq, n_tokens=n_tokens), dict(n_heads=heads, q_token=heads * d, q_head=d)
         plain = lib.hmm_paged_attention_workspace_size(n_seq, n_tokens, heads, hk, d)
         need = lib.hmm_paged_quant_attention_workspace_size(n_seq, n_tokens, heads, hk, d, 4 * 64, max_new)
         assert plain > 0 and need >= plain
-        wide = n_tokens * heads // hk >= 512 and max_new == 0       # rows whose keys may be widened into the workspace
+        wide = n_tokens * heads // hk // 256 * hk * 2 >= 4096 and max_new == 0      # keys may be widened into the workspace
         assert wide == (need > plain + 4 * 256 * hk * d)
         for n in (0, need - 1):
             refused(attend(c, b, max_new=max_new, nbytes=n, **kw), "workspace too small", HMM_ERR_OOM)
