@@ -22,6 +22,15 @@ inline int box_rows_of(int64_t page_tokens, int64_t most) {
     return (int)(r < most ? r : most);
 }
 
+// 1 in one lane of the warp.  (What that lane alone does needs no loop over lanes, as an instruction
+// with uniform operands does where several might run it.)
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(one));
+    return one;
+}
+
 // One box of a page array: values from x on of rows y... of a head (z) and page (w).
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
                                               int z, int w) {

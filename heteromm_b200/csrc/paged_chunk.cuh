@@ -52,6 +52,7 @@
 
 #include "paged_attn.cuh"
 #include "paged_attn_tc.cuh"
+#include "paged_code_tile.cuh"
 
 namespace hmm {
 namespace serve {
@@ -182,14 +183,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, ns));
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // One box of the queries: values [x, x + 64) of heads y... of tokens z....
 __device__ __forceinline__ void tma_load_q(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
     asm volatile(
@@ -233,13 +226,6 @@ __device__ __forceinline__ void commit_one(uint32_t one, uint64_t* bar) {
         "r"(one)
         : "memory");
 }
-__device__ __forceinline__ uint32_t elect_one() {
-    uint32_t one;
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(one));
-    return one;
-}
-
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "

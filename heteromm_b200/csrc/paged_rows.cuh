@@ -28,6 +28,7 @@
 
 #include "paged_attn.cuh"
 #include "paged_attn_tc.cuh"
+#include "paged_code_tile.cuh"
 
 namespace hmm {
 namespace serve {
@@ -141,26 +142,6 @@ __device__ __forceinline__ int64_t scan_incl(int64_t v, int64_t* wt, int64_t* to
     return v + add;
 }
 
-// In 8 bits: the first of the four codes that step k of a key's product takes in lane c of four.
-template <int DP>
-__device__ __forceinline__ int code_of_step(int k, int c) {
-    return DP == 64 ? 16 * c + 4 * k : (k >> 3) * 128 + 32 * c + 4 * (k & 7);
-}
-// Byte of 16-byte piece c of row r of a tile of codes.
-template <int DP, int BLOCK>
-__device__ __forceinline__ int code_piece(int r, int c) {
-    return DP == 64 ? r * 64 + ((c ^ (r >> 1 & 3)) * 16) : (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) * 16);
-}
-
-// Scale bytes of four groups of a token from its `per`, the 4 b-th on; behind the last the last.
-__device__ __forceinline__ uint32_t four_scales(const unsigned char* p, int b, int per) {
-    if ((per & 3) == 0) return *reinterpret_cast<const uint32_t*>(p + 4 * b);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= (uint32_t)p[min(4 * b + i, per - 1)] << (8 * i);
-    return w;
-}
-
 // (apart from the kernel's code, which streams)
 template <typename T, int C>
 __device__ __noinline__ void rows_exact(const AttnArgs& a, const Seq& q, int kvh, int row0, unsigned rows) {
@@ -184,12 +165,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     constexpr int ROW = QUANT && DP == 64 ? 64 : 128, HALVES = QUANT ? (DP + 127) / 128 : DP / 64;
     constexpr int BLOCK = KEYS * ROW;
     constexpr int STAGE = rows_stage<DP, C>(), SCALES = rows_scales<DP, C>();
-    static_assert(STAGE == 2 * HALVES * BLOCK, "K, then V");
     constexpr int MR = DP + 4;                         // joining rows: 4 banks apart
+    using M = std::conditional_t<QUANT, __half, T>;    // the products' type
     // log2 of what weights are held by: the largest is 2^14 in fp16, whose range ends at 2^-25
     // (a key 18 nats below the largest had no weight at all, and a long tail of them a share
     // of the result).  It cancels against the sum, and lse takes it back with the maximum.
-    constexpr float UP = std::is_same<T, __half>::value ? 14.0f : 0.0f;
+    constexpr float UP = std::is_same<M, __half>::value ? 14.0f : 0.0f;
     const AttnArgs& a = r.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -240,9 +221,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t ring = smem_u32(ring_p);
     unsigned char* scales_p = smem + RW_WARPS * RW_STAGES * STAGE + warp * RW_STAGES * SCALES;
     const int per = QUANT ? a.quant.per_token : 0;     // scale bytes of a token
-    // lane: box rows [sub * box_rows, +box_rows) of the warp's keys, and of the boxes there (and
-    // the scale bytes, which come as two boxes more) every (32 / subs)-th
-    const int subs = KEYS / r.box_rows, sub = lane % subs, box0 = lane / subs, box_step = 32 / subs;
+    // boxes of the warp's keys, one after the other: lane: [sub * box_rows, +box_rows)
+    const int subs = KEYS / r.box_rows, sub = lane % subs;
     uint32_t done = 0;                                 // tiles that the ring has seen
     bool dead = false;                                 // a wait gave up: no more copies
     while (cur < end) {
@@ -267,51 +247,54 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const int t = t0 + i;
             return (t < sink_tiles ? t : first + t - sink_tiles) * TILE + warp * KEYS;
         };
-        int page = a.n_pages, row = 0;                 // this lane's box rows of the next tile
+        // This lane's box rows of the next tile: the table's entry, looked at when it is used (a check
+        // here would wait for it, 1,000 clocks a tile), and the row in its page; -1: none are seen.
+        int entry = 0, row = -1;
         auto lookup = [&](int i) {
-            page = a.n_pages;                          // out of range: zeros
+            row = -1;
             if (i < n) {
                 const int k0 = key0_of(i) + sub * r.box_rows;
                 if (k0 < sp.sink || (k0 + r.box_rows > sp.lo && k0 < sp.hi)) {
                     const int lp = a.by_page(k0);
-                    const int e = page_of(a, q.row, lp);
-                    if (e >= 0) {
-                        page = e;
-                        row = k0 - lp * a.page_tokens;
-                    }
+                    entry = __ldg(a.b.table + (int64_t)q.row * a.b.pages_per_seq + lp);
+                    row = k0 - lp * a.page_tokens;
                 }
             }
+        };
+        auto page_now = [&] {                          // out of range: zeros
+            if (row < 0) return a.n_pages;
+            if (entry >= 0 && entry < a.n_pages) return entry;
+            atomicOr(a.status, HMM_STATUS_PAGE_BOUNDS);
+            return a.n_pages;
         };
         auto issue = [&](int i) {                      // copies of tile i, whose lookup is in page / row
             if (i < n && !dead) {
+                const int page = page_now();
                 const uint32_t st = (done + i) % RW_STAGES;
-                uint32_t bytes = STAGE;
-                if (QUANT)   // (scale bytes of pages out of range are not asked for)
-                    bytes += 2 * r.box_rows * per * __popc(__ballot_sync(0xffffffffu, box0 == 0 && page < a.n_pages));
-                if (lane == 0) mbar_expect_tx(&full[warp][st], bytes);
+                if (lane == 0) mbar_expect_tx(&full[warp][st], STAGE);
                 __syncwarp();
-                const uint32_t d = ring + st * STAGE + sub * r.box_rows * ROW;
-#pragma unroll 2
-                for (int b = box0; b < 2 * HALVES + (QUANT ? 2 : 0); b += box_step) {
-                    if (QUANT && b >= 2 * HALVES) {
-                        const bool of_v = b > 2 * HALVES;
-                        const Pages& p = of_v ? a.v : a.k;
-                        if (page < a.n_pages)
-                            bulk_load(smem_u32(scales_p + st * SCALES + (of_v ? SCALES / 2 : 0) + sub * r.box_rows * per),
-                                      p.base + page * p.page + kvh * p.head + a.quant.scales + (int64_t)row * per,
-                                      r.box_rows * per, &full[warp][st]);
-                    } else {
-                        tma_load_page(d + b * BLOCK, b < HALVES ? &tmK : &tmV, &full[warp][st],
-                                      (QUANT ? 128 : 64) * (b < HALVES ? b : b - HALVES), row, kvh, page);
+                uint32_t d = ring + st * STAGE;
+                const uint32_t one = elect_one();
+                for (int x = 0; x < subs; ++x, d += r.box_rows * ROW) {
+                    const int pg = __shfl_sync(0xffffffffu, page, x), rw = max(0, __shfl_sync(0xffffffffu, row, x));
+                    if (one) {
+#pragma unroll
+                        for (int b = 0; b < HALVES; ++b) {
+                            tma_load_page(d + b * BLOCK, &tmK, &full[warp][st], b * (QUANT ? 128 : 64), rw, kvh, pg);
+                            tma_load_page(d + (HALVES + b) * BLOCK, &tmV, &full[warp][st], b * (QUANT ? 128 : 64), rw, kvh, pg);
+                        }
                     }
                 }
+                if (QUANT)
+                    code_copy_scales(a, kvh, r.box_rows, page, row, smem_u32(scales_p + st * SCALES), SCALES / 2);
             }
+            if (QUANT) cp_commit();                    // (a tile that is not there is an empty group)
         };
 
-        // q fragments: rows lane / 4 and lane / 4 + 8.  (In 8 bits a lane takes the MMA's values in
-        // the order of its codes, 32 of a key in a row: four codes a step, the even ones and the odd.)
+        // q fragments: rows lane / 4 and lane / 4 + 8
         uint32_t qf[DP / 16][4];
         int pos[2];
+        float factor[2] = {a.scale_log2, a.scale_log2};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int row = lane / 4 + 8 * h;
@@ -320,20 +303,16 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             pos[h] = real ? row_pos(a, q, at) : -1;
             const unsigned char* src = a.q + (int64_t)(q.begin + at / a.group) * a.q_token +
                                        (int64_t)(kvh * a.group + at % a.group) * a.q_head;
+            if constexpr (QUANT) {
+                factor[h] *= code_queries<T, DP>(real ? src : nullptr, a.D, h, qf);
+            } else {
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                if constexpr (QUANT) {
-                    const int d = code_of_step<DP>(k, lane & 3);
-                    const uint2 x = real && d < a.D ? __ldg(reinterpret_cast<const uint2*>(src + 2 * d)) : make_uint2(0u, 0u);
-                    qf[k][h] = __byte_perm(x.x, x.y, 0x5410);
-                    qf[k][h + 2] = __byte_perm(x.x, x.y, 0x7632);
-                } else {
+                for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int d = k * 16 + j * 8 + (lane & 3) * 2;
                         qf[k][h + 2 * j] = real && d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(src + 2 * d)) : 0u;
                     }
-                }
             }
         }
 #pragma unroll
@@ -351,6 +330,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
         for (int i = 0; i < n; ++i) {
+            if (QUANT) cp_wait<RW_STAGES - 2>();       // (the scale bytes; the wait below is the warp's)
             if (!dead) {
                 const uint32_t at = done + i;
                 dead = !__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][at % RW_STAGES],
@@ -367,9 +347,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             issue(i + RW_STAGES - 1);                  // into the stage that tile i - 1 left
             lookup(i + RW_STAGES);
             const uint32_t so = ((done + i) % RW_STAGES) * STAGE;
-            const uint32_t kt = ring + so, vt = kt + HALVES * BLOCK;
-            const unsigned char* ks = scales_p + ((done + i) % RW_STAGES) * SCALES;
-            unsigned char* vs = scales_p + ((done + i) % RW_STAGES) * SCALES + SCALES / 2;
             const int key0 = key0_of(i);
             if (!(key0 >= sp.lo && key0 + KEYS <= sp.hi) && key0 + KEYS > sp.sink) {
                 // V rows that no row of the unit sees, beside some that are seen, become
@@ -379,8 +356,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     for (int c = 0; c < HALVES * (ROW / 16); ++c)
                         *reinterpret_cast<uint4*>(ring_p + so + (HALVES + c / (ROW / 16)) * BLOCK + lane * ROW +
                                                   c % (ROW / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    if (QUANT)   // (a page that was not read leaves what was there; 255 would make NaN of a zero)
-                        for (int g = 0; g < per; ++g) vs[lane * per + g] = 127;
+                    // (scale bytes of rows that were not read are anything, and 255 would make NaN of a zero)
+                    for (int g = 0; g < per; ++g) scales_p[so / STAGE * SCALES + SCALES / 2 + lane * per + g] = 127;
                 }
                 fence_proxy_async_smem();              // before the stage's next copies
                 __syncwarp();
@@ -388,29 +365,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             constexpr int NB = KEYS / 8;               // blocks of 8 keys
             float sc[NB][4] = {};
             const int mi = lane >> 3, ml = lane & 7;
+            const uint32_t kt = ring + so, vt = kt + STAGE / 2;
+            const unsigned char* scales = scales_p + so / STAGE * SCALES;
             if constexpr (QUANT) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const int row = nb * 8 + (lane >> 2), c = lane & 3;
-                    constexpr int PIECES = DP == 64 ? 1 : 2;
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) {
-                        const uint32_t s = ks[row * per + min(DP == 64 ? c >> 1 : 4 * h + c, per - 1)];
-                        const uint32_t m = multiplier<T, C>(s | s << 16);
-#pragma unroll
-                        for (int x = 0; x < PIECES; ++x) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(
-                                ring_p + so + code_piece<DP, BLOCK>(row, DP == 64 ? c : 8 * h + 2 * c + x));
-                            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                uint32_t even, odd;
-                                widen<T, C>(u[y], even, odd);
-                                mma16816<T>(sc[nb], qf[(h * PIECES + x) * 4 + y], mul_pair<T>(even, m), mul_pair<T>(odd, m));
-                            }
-                        }
-                    }
-                }
+                code_scores<DP, C>(ring_p + so, scales, per, qf, sc);
             } else {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
@@ -428,7 +386,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float x = sc[nb][j] * a.scale_log2;
+                    float x = sc[nb][j] * factor[j >> 1];
                     if (!all && !sees(a, q, pos[j >> 1], key0 + nb * 8 + (lane & 3) * 2 + (j & 1)))
                         x = -INFINITY;
                     sc[nb][j] = x;
@@ -459,40 +417,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 for (int h = 0; h < 2; ++h) {
                     const float e0 = ex2(sc[nb][2 * h] - mx[h]), e1 = ex2(sc[nb][2 * h + 1] - mx[h]);
                     l[h] += e0 + e1;
-                    // weights in the cache's type (of 8 bits: q's) for the product: off by half a step,
+                    // weights in the cache's type (in 8 bits fp16) for the product: off by half a step,
                     // 2^-8 of a weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
-                    p[2 * nb + h] = pack2<T>(e0, e1);
+                    p[2 * nb + h] = pack2<M>(e0, e1);
                 }
             if constexpr (QUANT) {
-                // The transposed load moves pairs of codes, two columns of a key: of the words of keys
-                // 2 c, 2 c + 1 the even codes are one column's pair and the odd ones its neighbour's.
-#pragma unroll
-                for (int x = 0; x < KEYS / 16; ++x) {
-                    const unsigned char* s = vs + (16 * x + 2 * (lane & 3)) * per;
-#pragma unroll
-                    for (int g4 = 0; g4 < (DP + 127) / 128; ++g4) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = four_scales(s + ((y & 1) + 8 * (y >> 1)) * per, g4, per);
-#pragma unroll
-                        for (int g = 0; g < (DP == 64 ? 2 : 4); ++g) {
-                            const int dd = 4 * g4 + g;
-                            uint32_t b[4], m[2], even, odd;
-#pragma unroll
-                            for (int y = 0; y < 2; ++y)
-                                m[y] = multiplier<T, C>(__byte_perm(w[2 * y], w[2 * y + 1], g | (4 + g) << 8) & 0x00ff00ffu);
-                            ldm4t(b, vt + code_piece<DP, BLOCK>(16 * x + ml + (mi & 1) * 8, 2 * dd + (mi >> 1)));
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                uint32_t even1, odd1;
-                                widen<T, C>(b[2 * y], even, odd);
-                                widen<T, C>(b[2 * y + 1], even1, odd1);
-                                mma16816<T>(o[4 * dd + 2 * y], p + 4 * x, mul_pair<T>(even, m[0]), mul_pair<T>(even1, m[1]));
-                                mma16816<T>(o[4 * dd + 2 * y + 1], p + 4 * x, mul_pair<T>(odd, m[0]), mul_pair<T>(odd1, m[1]));
-                            }
-                        }
-                    }
-                }
+                code_product<DP, C>(ring_p + so + STAGE / 2, scales + SCALES / 2, per, p, o);
             } else {
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
@@ -519,14 +449,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int row = lane / 4 + 8 * h;
+            float* dst = jm + (warp * RW_ROWS + row) * MR;
             if constexpr (QUANT) {
-                float* dst = jm + (warp * RW_ROWS + row) * MR + (lane & 3) * 4;
-#pragma unroll
-                for (int d = 0; d < DP / 8; d += 2)
-                    *reinterpret_cast<float4*>(dst + 8 * d) =
-                        make_float4(o[d][2 * h], o[d + 1][2 * h], o[d][2 * h + 1], o[d + 1][2 * h + 1]);
+                code_row<DP>(o, h, dst);
             } else {
-                float* dst = jm + (warp * RW_ROWS + row) * MR + (lane & 3) * 2;
+                dst += (lane & 3) * 2;
 #pragma unroll
                 for (int d = 0; d < DP / 8; ++d) {
                     dst[8 * d] = o[d][2 * h];
