@@ -110,24 +110,29 @@ __device__ __forceinline__ float code_queries(const unsigned char* src, int D, i
 }
 
 // Copies of a tile's scale bytes, K's by the lower lanes of a warp and V's by the upper ones, 16 bytes
-// each: lane s < 32 / box holds (page, row) of its boxes s, s + 32 / box ...; a page of n_pages is out
-// of range.
-__device__ __forceinline__ void code_copy_scales(const AttnArgs& a, int kvh, int box, int page, int row, uint32_t dst,
-                                                 int v_scales) {
-    const int lane = threadIdx.x & 31, per = a.quant.per_token, at = 16 * (lane & 15), box_log2 = 31 - __clz(box);
-    const int s = at / per >> box_log2;                          // (a box's bytes are a multiple of 16)
-    const int pg = __shfl_sync(0xffffffffu, page, s & 31), rw = __shfl_sync(0xffffffffu, row, s & 31);
-    if (at < CT_KEYS * per && pg < a.n_pages) {
-        const Pages& x = lane < 16 ? a.k : a.v;
-        cp16(dst + (lane < 16 ? 0 : v_scales) + at,
-             x.base + pg * x.page + kvh * x.head + a.quant.scales + (int64_t)rw * per + (at - (s << box_log2) * per), true);
-    }
+// each.  A lane's are always of the same box, so that it holds where in a page they begin.
+struct ScaleCopy {
+    const unsigned char* base;
+    int64_t page;
+    int box, dst;        // (box < 0: none for this lane)
+};
+__device__ __forceinline__ ScaleCopy scale_copy(const AttnArgs& a, int kvh, int box_rows, int v_scales) {
+    const int lane = threadIdx.x & 31, per = a.quant.per_token, at = 16 * (lane & 15), bytes = box_rows * per;
+    const Pages& x = lane < 16 ? a.k : a.v;
+    const int box = at / bytes;                                  // (a box's bytes are a multiple of 16)
+    return ScaleCopy{x.base + kvh * x.head + a.quant.scales + at - box * bytes, x.page, at < CT_KEYS * per ? box : -1,
+                     (lane < 16 ? 0 : v_scales) + at};
+}
+// Lane s holds (page, row) of box s; a page of n_pages is out of range.
+__device__ __forceinline__ void code_copy_scales(const AttnArgs& a, const ScaleCopy& c, int page, int row, uint32_t dst) {
+    const int pg = __shfl_sync(0xffffffffu, page, c.box & 31), rw = __shfl_sync(0xffffffffu, row, c.box & 31);
+    if (c.box >= 0 && pg < a.n_pages) cp16(dst + c.dst, c.base + pg * c.page + rw * a.quant.per_token, true);
 }
 
 // Scores of 16 rows and 32 keys.  (Four sums at a time: an MMA waits for the one before it in its own.)
 template <int DP, int C>
 __device__ __forceinline__ void code_scores(const unsigned char* k, const unsigned char* scales, int per,
-                                            const uint32_t (*qf)[4], float (*sc)[4]) {
+                                            const uint4* qs, float (*sc)[4]) {
     constexpr int PIECES = DP == 64 ? 1 : 2;
     const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -145,14 +150,17 @@ __device__ __forceinline__ void code_scores(const unsigned char* k, const unsign
             for (int nb = 0; nb < 4; ++nb)
                 w[nb] = *reinterpret_cast<const uint4*>(k + code_at<DP>(8 * nb + n, DP == 64 ? c : 8 * h + 2 * c + y));
 #pragma unroll
-            for (int z = 0; z < 4; ++z)
+            for (int z = 0; z < 4; ++z) {
+                const uint4 qv = qs[((h * PIECES + y) * 4 + z) * 32 + lane];
+                const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
                 for (int nb = 0; nb < 4; ++nb) {
                     const uint32_t u = z == 0 ? w[nb].x : z == 1 ? w[nb].y : z == 2 ? w[nb].z : w[nb].w;
                     uint32_t b0, b1;
                     code_pairs<C>(u, b0, b1);
-                    mma_half(sc[nb], qf[(h * PIECES + y) * 4 + z], mul_pair<__half>(b0, m[nb]), mul_pair<__half>(b1, m[nb]));
+                    mma_half(sc[nb], qa, mul_pair<__half>(b0, m[nb]), mul_pair<__half>(b1, m[nb]));
                 }
+            }
         }
     }
 }

@@ -37,7 +37,6 @@ using namespace sm100;
 constexpr int RW_WARPS = 4;
 constexpr int RW_THREADS = 32 * RW_WARPS;
 constexpr int RW_ROWS = 16;
-constexpr int RW_STAGES = 3;
 // Keys of a warp's tile, and of a CTA's: as many bytes of either cache, so that what a tile costs
 // beside them is the same.
 template <int C>
@@ -59,8 +58,13 @@ struct RowsArgs {
     uint64_t wait_ns; // limit of every bounded wait
 };
 
-template <int DP>
-constexpr int rows_ctas_per_sm() { return DP == 64 ? 4 : DP == 128 ? 2 : 1; }
+// Stages of a warp's ring, CTAs of an SM.  In 8 bits the instructions' latency counts, not the bytes
+// in flight: three CTAs with two stages take 247 us for the decode batch, two with three 293
+// (16-bit values 343 and 350, but one token 13.9 and 12.8).
+template <int DP, int C>
+__host__ __device__ constexpr int rows_stages() { return C != CODEC_NONE && DP == 128 ? 2 : 3; }
+template <int DP, int C>
+__host__ __device__ constexpr int rows_ctas_per_sm() { return DP == 64 ? 4 : DP == 128 ? (C == CODEC_NONE ? 2 : 3) : 1; }
 
 // A stage of a warp: K, then V; in 8 bits their scale bytes lie behind all warps' rings.
 template <int DP, int C>
@@ -69,7 +73,7 @@ template <int DP, int C>
 __host__ __device__ constexpr int rows_scales() { return C == CODEC_NONE ? 0 : 2 * rows_keys<C>() * DP / Q_GROUP; }
 template <int DP, int C>
 constexpr size_t rows_smem() {
-    return 1024 + (size_t)RW_WARPS * RW_STAGES * (rows_stage<DP, C>() + rows_scales<DP, C>());
+    return 1024 + (size_t)RW_WARPS * rows_stages<DP, C>() * (rows_stage<DP, C>() + rows_scales<DP, C>());
 }
 
 __device__ __forceinline__ void ldm4(uint32_t* r, uint32_t addr) {
@@ -149,15 +153,17 @@ __device__ __noinline__ void rows_exact(const AttnArgs& a, const Seq& q, int kvh
 }
 
 template <typename T, int DP, int C>
-__global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP>())
+__global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP, C>())
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ RowsArgs r) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    constexpr int RW_STAGES = rows_stages<DP, C>();
     __shared__ uint64_t full[RW_WARPS][RW_STAGES];
     __shared__ int64_t wt[RW_WARPS];
     __shared__ int64_t sh_pre;
     __shared__ int sh_seq, again, any_again, abort;
+    __shared__ uint4 qs[C != CODEC_NONE ? DP * 2 : 1];   // in 8 bits: the unit's queries [step][lane]
     constexpr bool QUANT = C != CODEC_NONE;
     constexpr int KEYS = rows_keys<C>(), TILE = rows_tile<C>();
     // A box is 128 bytes of a row (64 values, or 128 codes; 64 codes at D = 64), swizzled over as
@@ -247,6 +253,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const int t = t0 + i;
             return (t < sink_tiles ? t : first + t - sink_tiles) * TILE + warp * KEYS;
         };
+        const ScaleCopy scale_from = QUANT ? scale_copy(a, kvh, r.box_rows, SCALES / 2) : ScaleCopy{};
         // This lane's box rows of the next tile: the table's entry, looked at when it is used (a check
         // here would wait for it, 1,000 clocks a tile), and the row in its page; -1: none are seen.
         int entry = 0, row = -1;
@@ -286,7 +293,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     }
                 }
                 if (QUANT)
-                    code_copy_scales(a, kvh, r.box_rows, page, row, smem_u32(scales_p + st * SCALES), SCALES / 2);
+                    code_copy_scales(a, scale_from, page, row, smem_u32(scales_p + st * SCALES));
             }
             if (QUANT) cp_commit();                    // (a tile that is not there is an empty group)
         };
@@ -314,6 +321,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         qf[k][h + 2 * j] = real && d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(src + 2 * d)) : 0u;
                     }
             }
+        }
+        if constexpr (QUANT) {
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+                if (k % RW_WARPS == warp) qs[k * 32 + lane] = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
+            __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < RW_STAGES - 1; ++i) {
@@ -368,7 +381,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const uint32_t kt = ring + so, vt = kt + STAGE / 2;
             const unsigned char* scales = scales_p + so / STAGE * SCALES;
             if constexpr (QUANT) {
-                code_scores<DP, C>(ring_p + so, scales, per, qf, sc);
+                code_scores<DP, C>(ring_p + so, scales, per, qs, sc);
             } else {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
@@ -576,12 +589,16 @@ __global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_con
 
 inline int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-inline int64_t rows_ctas(int dp) {
-    return (int64_t)device_sm_count() * (dp == 64 ? rows_ctas_per_sm<64>() : dp == 128 ? rows_ctas_per_sm<128>() : 1);
+template <int C>
+int64_t rows_ctas(int dp) {
+    return (int64_t)device_sm_count() * (dp == 64    ? rows_ctas_per_sm<64, C>()
+                                         : dp == 128 ? rows_ctas_per_sm<128, C>()
+                                                     : rows_ctas_per_sm<256, C>());
 }
 
-inline size_t rows_workspace(int dp) {
-    const size_t g = (size_t)rows_ctas(dp);
+template <int C>
+size_t rows_workspace(int dp) {
+    const size_t g = (size_t)rows_ctas<C>(dp);
     return 2 * g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
 }
 
@@ -591,7 +608,7 @@ hmm_status_t launch_rows(const RowsArgs& r, const CUtensorMap& k, const CUtensor
     constexpr size_t smem = rows_smem<DP, C>();
     const hmm_status_t s = allow_smem(paged_rows_kernel<T, DP, C>, smem, &done);
     if (s != HMM_OK) return s;
-    return launch(paged_rows_kernel<T, DP, C>, dim3((unsigned)rows_ctas(DP)), RW_THREADS, smem, false, st,
+    return launch(paged_rows_kernel<T, DP, C>, dim3((unsigned)rows_ctas<C>(DP)), RW_THREADS, smem, false, st,
                   "paged_rows_kernel", k, v, r);
 }
 
@@ -621,7 +638,7 @@ hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cuda
     const bool with_rows = few || !chunk || (a.b.n_seq > 1 && a.min_rows <= RW_ROWS);
     const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel
     const int dp = rows_dp(a.D);
-    const int64_t ctas = rows_ctas(dp);
+    const int64_t ctas = rows_ctas<C>(dp);
     JoinArgs j{a, {(int4*)ws, (float*)(ws + 2 * (size_t)ctas * sizeof(int4))}, 0, dp, {}};
     hmm_status_t s;
     if (with_rows) {
@@ -631,7 +648,7 @@ hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cuda
     }
     if (chunk && !few) {
         s = run_chunk<C>(a, std::is_same<T, __nv_bfloat16>::value, with_rows ? most + 1 : 1, with_rows,
-                      ws + up256(rows_workspace(dp)), st, &j.chunk);
+                      ws + up256(rows_workspace<C>(dp)), st, &j.chunk);
         if (s != HMM_OK) return s;
     }
     const int64_t blocks = j.rows_ctas + (int64_t)j.chunk.ctas * j.chunk.groups;
