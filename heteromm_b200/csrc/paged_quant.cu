@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "paged_append.cuh"
+#include "paged_attn.cuh"
 
 namespace hmm {
 namespace serve {
@@ -52,6 +53,7 @@ struct ReadArgs {
     QuantRows rows;
     int64_t max_kv;
     int n_pages, hk, D, page_tokens;
+    FastDiv by_head;           // vectors of a head
     int32_t* status;
 };
 
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(RD_THREADS) paged_quant_read_kernel(const __gr
                 for (int d = 0; d < RD_DEPTH; ++d) {
                     const int i = i0 + 32 * d;
                     if (i >= 2 * per_row) continue;
-                    const int kv = i >= per_row, x = i - (kv ? per_row : 0), h = x / per_head, c = x - h * per_head;
+                    const int kv = i >= per_row, x = i - (kv ? per_row : 0), h = a.by_head(x), c = x - h * per_head;
                     const Pages& p = a.pages[kv];
                     const unsigned char* block = p.base + page * p.page + h * p.head;
                     w[d] = __ldg(reinterpret_cast<const uint4*>(block + (int64_t)in * a.D) + c);
@@ -199,6 +201,7 @@ extern "C" hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, con
     a.hk = (int)cache->n_kv_heads;
     a.D = (int)cache->D;
     a.page_tokens = (int)cache->page_tokens;
+    a.by_head = FastDiv::of(a.D / 16);
     a.status = device_status;
     const bool e4m3 = cache->codes == HMM_DTYPE_E4M3;
     const cudaStream_t st = (cudaStream_t)stream;

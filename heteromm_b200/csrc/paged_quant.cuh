@@ -162,8 +162,14 @@ __device__ __forceinline__ void store16(O* dst, const uint4& w, uint32_t s) {
             r[2 * i] = in_order_lo(even, odd);
             r[2 * i + 1] = in_order_hi(even, odd);
         }
-        reinterpret_cast<uint4*>(dst)[0] = make_uint4(r[0], r[1], r[2], r[3]);
-        reinterpret_cast<uint4*>(dst)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+        if ((reinterpret_cast<uintptr_t>(dst) & 31) == 0) {   // a sector at once
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                         "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                         : "memory");
+        } else {
+            reinterpret_cast<uint4*>(dst)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+            reinterpret_cast<uint4*>(dst)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+        }
     }
 }
 
