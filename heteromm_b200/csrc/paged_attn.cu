@@ -70,7 +70,7 @@ hmm_status_t plan_attention(const AttnCall& c, const hmm_paged_cache_t& dims, co
 
 size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared) {
     // (the rows kernel over a cache in 8 bits has as many CTAs at least)
-    return up256(rows_workspace<CODEC_E4M3>(rows_dp(D))) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared);
+    return up256(rows_workspace<CODEC_E4M3>(rows_dp(D), shared)) + chunk_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared);
 }
 
 template <>

@@ -58,22 +58,30 @@ struct RowsArgs {
     uint64_t wait_ns; // limit of every bounded wait
 };
 
-// Stages of a warp's ring, CTAs of an SM.  In 8 bits the instructions' latency counts, not the bytes
-// in flight: three CTAs with two stages take 247 us for the decode batch, two with three 293
-// (16-bit values 343 and 350, but one token 13.9 and 12.8).
+// Rows of a sequence that are this kernel's where the chunk kernel takes its caches too (one row
+// tile or two; at run_kernels).
+template <int C>
+__host__ __device__ constexpr int rows_most() { return C == CODEC_NONE ? RW_ROWS : 2 * RW_ROWS; }
+
+// CTAs of an SM at D <= 128 (64: four; 256: one): two with three stages a warp keep the bytes in flight
+// that HBM wants and start soonest; with three of two stages more instructions are in flight, and
+// more units' starts and ends.  In 8 bits the decode batch takes 247 us with three and 293 with two,
+// 16-bit sequences of 1,000 behind a shared prefix 111 and 123; one token over 777 13.9 and 12.8.
 template <int DP, int C>
-__host__ __device__ constexpr int rows_stages() { return C != CODEC_NONE && DP == 128 ? 2 : 3; }
-template <int DP, int C>
-__host__ __device__ constexpr int rows_ctas_per_sm() { return DP == 64 ? 4 : DP == 128 ? (C == CODEC_NONE ? 2 : 3) : 1; }
+__host__ __device__ constexpr int rows_ctas_per_sm(bool shared) {
+    return DP == 64 ? 4 : DP == 128 ? (C == CODEC_NONE && !shared ? 2 : 3) : 1;
+}
+template <int DP>
+__host__ __device__ constexpr int rows_stages(int ctas) { return DP == 128 && ctas == 3 ? 2 : 3; }
 
 // A stage of a warp: K, then V; in 8 bits their scale bytes lie behind all warps' rings.
 template <int DP, int C>
 __host__ __device__ constexpr int rows_stage() { return 2 * rows_keys<C>() * DP * (C == CODEC_NONE ? 2 : 1); }
 template <int DP, int C>
 __host__ __device__ constexpr int rows_scales() { return C == CODEC_NONE ? 0 : 2 * rows_keys<C>() * DP / Q_GROUP; }
-template <int DP, int C>
+template <int DP, int C, int CTAS>
 constexpr size_t rows_smem() {
-    return 1024 + (size_t)RW_WARPS * rows_stages<DP, C>() * (rows_stage<DP, C>() + rows_scales<DP, C>());
+    return 1024 + (size_t)RW_WARPS * rows_stages<DP>(CTAS) * (rows_stage<DP, C>() + rows_scales<DP, C>());
 }
 
 __device__ __forceinline__ void ldm4(uint32_t* r, uint32_t addr) {
@@ -152,13 +160,13 @@ __device__ __noinline__ void rows_exact(const AttnArgs& a, const Seq& q, int kvh
     attn_rows_exact<T, C, 1>(a, q, kvh, row0, rows);
 }
 
-template <typename T, int DP, int C>
-__global__ void __launch_bounds__(RW_THREADS, rows_ctas_per_sm<DP, C>())
+template <typename T, int DP, int C, int CTAS>
+__global__ void __launch_bounds__(RW_THREADS, CTAS)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ RowsArgs r) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    constexpr int RW_STAGES = rows_stages<DP, C>();
+    constexpr int RW_STAGES = rows_stages<DP>(CTAS);
     __shared__ uint64_t full[RW_WARPS][RW_STAGES];
     __shared__ int64_t wt[RW_WARPS];
     __shared__ int64_t sh_pre;
@@ -179,6 +187,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     constexpr float UP = std::is_same<M, __half>::value ? 14.0f : 0.0f;
     const AttnArgs& a = r.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (Parts are the kernel before's, which this one is launched ahead of; so the next may not start
+    // before either.)
+    if (a.b.shared) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (threadIdx.x == 0) {
@@ -590,26 +601,26 @@ __global__ void __launch_bounds__(RW_THREADS) paged_join_kernel(const __grid_con
 inline int rows_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 template <int C>
-int64_t rows_ctas(int dp) {
-    return (int64_t)device_sm_count() * (dp == 64    ? rows_ctas_per_sm<64, C>()
-                                         : dp == 128 ? rows_ctas_per_sm<128, C>()
-                                                     : rows_ctas_per_sm<256, C>());
+int64_t rows_ctas(int dp, bool shared) {
+    return (int64_t)device_sm_count() * (dp == 64    ? rows_ctas_per_sm<64, C>(shared)
+                                         : dp == 128 ? rows_ctas_per_sm<128, C>(shared)
+                                                     : rows_ctas_per_sm<256, C>(shared));
 }
 
 template <int C>
-size_t rows_workspace(int dp) {
-    const size_t g = (size_t)rows_ctas<C>(dp);
+size_t rows_workspace(int dp, bool shared) {
+    const size_t g = (size_t)rows_ctas<C>(dp, shared);
     return 2 * g * sizeof(int4) + g * 2 * RW_ROWS * (dp + 2) * sizeof(float);
 }
 
-template <typename T, int DP, int C>
+template <typename T, int DP, int C, int CTAS>
 hmm_status_t launch_rows(const RowsArgs& r, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t smem = rows_smem<DP, C>();
-    const hmm_status_t s = allow_smem(paged_rows_kernel<T, DP, C>, smem, &done);
+    constexpr size_t smem = rows_smem<DP, C, CTAS>();
+    const hmm_status_t s = allow_smem(paged_rows_kernel<T, DP, C, CTAS>, smem, &done);
     if (s != HMM_OK) return s;
-    return launch(paged_rows_kernel<T, DP, C>, dim3((unsigned)rows_ctas<C>(DP)), RW_THREADS, smem, false, st,
-                  "paged_rows_kernel", k, v, r);
+    return launch(paged_rows_kernel<T, DP, C, CTAS>, dim3((unsigned)(device_sm_count() * CTAS)), RW_THREADS, smem,
+                  r.a.b.shared != nullptr, st, "paged_rows_kernel", k, v, r);
 }
 
 template <typename T, int C>
@@ -620,9 +631,12 @@ hmm_status_t run_rows(const RowsArgs& r, cudaStream_t st) {
     s = make_page_map(&v, r.a, r.a.v, r.box_rows, C != CODEC_NONE);
     if (s != HMM_OK) return s;
     const int dp = rows_dp(r.a.D);
-    return dp == 64    ? launch_rows<T, 64, C>(r, k, v, st)
-           : dp == 128 ? launch_rows<T, 128, C>(r, k, v, st)
-                       : launch_rows<T, 256, C>(r, k, v, st);
+    if (dp == 64) return launch_rows<T, 64, C, 4>(r, k, v, st);
+    if (dp == 256) return launch_rows<T, 256, C, 1>(r, k, v, st);
+    if constexpr (C == CODEC_NONE) {
+        if (!r.a.b.shared) return launch_rows<T, 128, C, 2>(r, k, v, st);
+    }
+    return launch_rows<T, 128, C, 3>(r, k, v, st);
 }
 
 template <typename T, int C>
@@ -630,15 +644,19 @@ hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cuda
     // A unit of up to 16 rows (one MMA's) reads its keys once either way and the many small
     // CTAs of the rows kernel keep more reads in flight; more rows would read them again
     // there: 64 rows of 4 KV heads over 5,000, 16 sequences, D = 128, 113 us there and 69 in
-    // the chunk kernel, 32 rows 67 in both (over 777: 34 and 30, 25 and 29).  (A scale of zero is the rows kernel's, which scales before it masks: in the
-    // chunk kernel a masked score of -inf times zero would be NaN.)
+    // the chunk kernel, 32 rows 67 in both (over 777: 34 and 30, 25 and 29).  In 8 bits, where the
+    // chunk kernel has its codes widened beside the products, up to 32: 28 rows of 4 KV heads over
+    // 700, 16 sequences, D = 128, 31 us there and 39 in the chunk kernel, over 5,000 49 and 52, 32
+    // sequences over 16,000 154 and 203; 35 rows 33 and 39, 62 and 52, 211 and 203.  (A scale of zero
+    // is the rows kernel's, which scales before it masks: in the chunk kernel a masked score of -inf
+    // times zero would be NaN.)
     const bool chunk = chunk_applies(a) && a.scale_log2 != 0.0f;
     const int bound = a.b.shared ? a.b.n_tokens : max_new;       // (a group's rows are those of its sequences)
     const bool few = bound > 0 && (int64_t)std::min(bound, a.b.n_tokens) * a.group <= RW_ROWS;
-    const bool with_rows = few || !chunk || (a.b.n_seq > 1 && a.min_rows <= RW_ROWS);
-    const int most = !chunk || few ? INT32_MAX : RW_ROWS;      // rows of a sequence for the rows kernel
+    const bool with_rows = few || !chunk || (a.b.n_seq > 1 && a.min_rows <= rows_most<C>());
+    const int most = !chunk || few ? INT32_MAX : rows_most<C>();      // rows of a sequence for the rows kernel
     const int dp = rows_dp(a.D);
-    const int64_t ctas = rows_ctas<C>(dp);
+    const int64_t ctas = rows_ctas<C>(dp, a.b.shared != nullptr);
     JoinArgs j{a, {(int4*)ws, (float*)(ws + 2 * (size_t)ctas * sizeof(int4))}, 0, dp, {}};
     hmm_status_t s;
     if (with_rows) {
@@ -648,7 +666,7 @@ hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cuda
     }
     if (chunk && !few) {
         s = run_chunk<C>(a, std::is_same<T, __nv_bfloat16>::value, with_rows ? most + 1 : 1, with_rows,
-                      ws + up256(rows_workspace<C>(dp)), st, &j.chunk);
+                      ws + up256(rows_workspace<C>(dp, a.b.shared != nullptr)), st, &j.chunk);
         if (s != HMM_OK) return s;
     }
     const int64_t blocks = j.rows_ctas + (int64_t)j.chunk.ctas * j.chunk.groups;
