@@ -174,7 +174,7 @@ hmm_status_t plan_append(const AppendCall& c, const hmm_paged_cache_t& dims, con
     a.steps_k = (a.hk + n_groups - 1) / n_groups;
     // As many warps as stay on the GPU, each with a list of tokens; few tokens are shared
     // by several warps, down to a step each.
-    const int64_t slots = (int64_t)device_sm_count() * AP_MINB * (AP_THREADS / 32);
+    const int64_t slots = (int64_t)device_sm_count() * ap_minb(quant) * (AP_THREADS / 32);
     const int64_t steps = a.steps_q + 2 * (int64_t)a.steps_k;
     a.parts = (int)std::min(steps, std::max<int64_t>(1, slots / a.b.n_tokens));
     a.tokens_at_once = (int)std::min<int64_t>(a.b.n_tokens, std::max<int64_t>(1, slots / a.parts));

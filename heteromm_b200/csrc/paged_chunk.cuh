@@ -22,6 +22,9 @@
 //             with P_w from TMEM
 //   10        zeros over V rows that no row of the CTA sees (a page's end)
 //   11        the next unit (from the lengths on the device) and its queries
+//   12-15     of a cache in 8 bits: codes from a ring of their own to the stages' 16-bit tiles,
+//             zeros over V's unseen rows among them (10 rests).  8,192 tokens, int8: 735 us; what
+//             the products, which read shared memory at its full rate, leave is the bound
 // Heads of 129 to 256 values: units of one row tile, whose sums take half of TMEM, on
 // warps 0-3 and a ring of two stages (2,048 tokens, 16 query and 4 KV heads, D = 256:
 // 72 us; by the rows kernel 990).
@@ -588,7 +591,8 @@ __device__ __forceinline__ uint32_t q_at(int r, int c) {
 // neighbours' writes (16-byte pieces 0, 2, 4, 6 of a 128-byte row, swizzled by its number)
 // meet in no bank.  Rows that `seen` denies become zeros.
 // The loop is short on purpose: next to the softmax's straight code, a longer one (all rows
-// unrolled) did not stay in the instruction cache, and every role ran at a fifth of its speed.
+// unrolled) did not stay in the instruction cache, and all roles ran slower (drafted tokens 71 us, 58
+// so; a tile takes four warps 900 clocks alone and 3,000 here).
 template <typename T, int DP, int C, typename Seen>
 __device__ __forceinline__ void widen_rows(const unsigned char* codes, const AttnArgs& a, int box_log2, unsigned char* tile,
                                            int warp, int lane, bool some, Seen seen) {

@@ -2,8 +2,8 @@
 // bits: copies of its codes, scores, the product with V.
 //
 // The products are taken in fp16, whatever q is: it holds every code times its scale, and one
-// instruction makes two of two e4m3 codes (to bf16 takes six, and these conversions cost as
-// much as all else).  bf16 queries go to fp16 times a power of two per row.
+// instruction makes two of two e4m3 codes (2.2 clocks a scheduler measured; to bf16 it takes six
+// of 2).  bf16 queries go to fp16 times a power of two per row.
 //
 // Codes come as TMA boxes of a page's rows, 128 bytes (D = 64: 64) wide and swizzled over as
 // many, scale bytes by one 16-byte cp.async a lane (as bulk copies they doubled the requests;
@@ -126,7 +126,7 @@ __device__ __forceinline__ ScaleCopy scale_copy(const AttnArgs& a, int kvh, int 
 // Lane s holds (page, row) of box s; a page of n_pages is out of range.
 __device__ __forceinline__ void code_copy_scales(const AttnArgs& a, const ScaleCopy& c, int page, int row, uint32_t dst) {
     const int pg = __shfl_sync(0xffffffffu, page, c.box & 31), rw = __shfl_sync(0xffffffffu, row, c.box & 31);
-    if (c.box >= 0 && pg < a.n_pages) cp16(dst + c.dst, c.base + pg * c.page + rw * a.quant.per_token, true);
+    if (c.box >= 0 && pg < a.n_pages) cp16(dst + c.dst, c.base + pg * c.page + (int64_t)rw * a.quant.per_token, true);
 }
 
 // Scores of 16 rows and 32 keys.  (Four sums at a time: an MMA waits for the one before it in its own.)

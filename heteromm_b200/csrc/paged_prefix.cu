@@ -120,11 +120,11 @@ __global__ void __launch_bounds__(MG_THREADS) paged_merge_kernel(const __grid_co
     if (in < 0 || in >= p0.y) return;                    // a row of no sequence, left as it is
     float l2 = __ldcg(m.part_lse + row), l1 = p1.x > 0 ? __ldcg(m.part_lse + rows + row) : -INFINITY;
     const float top = fmaxf(l1, l2), ref = top == -INFINITY ? 0.0f : top;
-    float w1 = __expf(l1 - ref), w2 = __expf(l2 - ref);
+    float w1 = expf(l1 - ref), w2 = expf(l2 - ref);
     const float sum = w1 + w2;                           // (NaN if one is: so are the row and lse)
     w1 = sum == 0.0f ? 0.0f : w1 / sum;
     w2 = sum == 0.0f ? 0.0f : w2 / sum;
-    if (lane == 0 && m.lse) m.lse[row] = sum == 0.0f ? -INFINITY : ref + __logf(sum);
+    if (lane == 0 && m.lse) m.lse[row] = sum == 0.0f ? -INFINITY : ref + logf(sum);
     bool fine = true;
     for (int c = lane; c < a.D / 4; c += 32) {
         const float4 y = __ldcg(reinterpret_cast<const float4*>(m.part + row * a.D) + c);

@@ -4,7 +4,8 @@
 // paged_quant_read_kernel.  Bound by memory: 33 bytes are read and 64 written for 32 values
 // (16-bit rows).  A warp takes runs of four rows, whose places its lanes look up at once, and
 // goes through their 16-byte vectors of codes, a lane with four in flight: the codes become
-// values in a dozen integer instructions per four, without a table.
+// values in a dozen integer instructions per four, without a table.  16 sequences of up to 8,192
+// tokens, 8 heads of 128, e4m3 to fp16: 97 us, 4.6 TB/s (two rows' vectors in flight 101).
 #include <algorithm>
 
 #include "paged_append.cuh"

@@ -9,19 +9,21 @@
 //   - all units' key tiles form one list, cut into as many equal pieces as CTAs
 //     fit the GPU (ragged lengths balance by themselves); a CTA finds its piece
 //     from the lengths on the device, so no host value goes stale;
-//   - each warp owns 16 keys of a tile and its own ring of TMA stages, with no
-//     barrier between warps: a box per 64 values of a page's rows (issued by as
-//     many lanes as there are boxes, their page looked up one stage ahead), zeros
-//     for the boxes that no row of the tile sees.  The copies cost a warp about 30
-//     instructions a tile; with 16-byte cp.async (about 400) the issue slots bound
-//     the kernel, not HBM;
+//   - each warp owns 16 keys of a tile (of a cache in 8 bits 32: as many bytes) and its own ring of
+//     TMA stages, with no barrier between warps: a box per 128 bytes of a page's rows, issued by
+//     one elected lane (by as many lanes as boxes the hardware took one lane after the other: of a
+//     tile's 2,500 clocks 950, and 640 so), its page looked up one stage ahead and checked when it is
+//     used, zeros for the boxes that no row of the tile sees.  With 16-byte cp.async instead the
+//     L1 cache held the bytes in flight (478 us, 8 bits 361);
 //   - scores and the product with V on mma.sync (m16n8k16, fp32 sums), the
 //     running maximum and sum in fp32 per warp, warps joined once per piece;
 //   - a unit that several CTAs share leaves (maximum, sum, unnormalised rows) per
 //     piece in the workspace, and paged_join_kernel adds the pieces in order.
 // Measured: 64 sequences of up to 16,384 tokens, one new token each, 32 query and 8 KV
 // heads of 128: 347-351 us, 6.3 TB/s (cp.async: 478); one token over 777: 11.9 us, of
-// which 2.5 the join, over 4,000 17.6 us.
+// which 2.5 the join, over 4,000 17.6 us.  The same decode batch in e4m3: 248 us, 4.6 TB/s, where
+// HBM would allow 173: conversions, scores and softmax are 4,000 clocks of latency a tile for a
+// warp, and twelve warps an SM hide a part of them.
 #pragma once
 
 #include <algorithm>
