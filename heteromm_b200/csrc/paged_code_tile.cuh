@@ -97,7 +97,7 @@ __device__ __forceinline__ float code_queries(const unsigned char* src, int D, i
     if (std::is_same<T, __half>::value) return 1.0f;
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = min(max((int)(top >> 7), 15), 254 - 15);       // the largest's biased exponent
+    const int e = max((int)(top >> 7), 15);       // the largest's biased exponent
     const float up = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)

@@ -11,7 +11,7 @@ import torch
 import heteromm_b200 as hmm
 from heteromm_b200._abi import HMM_ERR_BOUNDS, HmmError, set_wait_limit_ns
 from heteromm_b200.paged import check_status
-from test_quant_attention_gpu import filled, raw
+from test_quant_attention_gpu import filled, long_table, raw
 from test_serve_attention_gpu import DT, check, make, reference
 
 pytestmark = pytest.mark.gpu
@@ -106,6 +106,27 @@ def test_formula_in_8_bits(cuda, batch, dtype, kind):
     kp, vp, k, v = filled(k, v, kind)
     got, lse = hmm.paged_prefix_attention(q, kp, vp, table, cu, kv_len, cg, pl, return_lse=True)
     check(got, lse, with_join(reference(q, k, v, table, new, kv)))
+
+
+@pytest.mark.parametrize("batch", [BATCHES[10], BATCHES[11], ([(1, 4, 300)], [5, 260, 20, 1, 200], [90, 600, 350, 301, 700], 8, 2, 128, 16)])
+def test_widened_parts(cuda, batch):
+    """Groups and tails of 512 rows and more, whose keys are widened first, beside others."""
+    groups, new, kv, hq, hk, d, pt = batch
+    q, k, v, table, cu, kv_len, (cg, pl) = shared(cuda, 52, groups, new, kv, hq, hk, d, pt, torch.bfloat16)
+    kp, vp, k, v = filled(k, v, "e4m3")
+    wide = long_table(table, pt, hk, hq, max(sum(new), 256))
+    got, lse = hmm.paged_prefix_attention(q, kp, vp, wide, cu, kv_len, cg, pl, return_lse=True)
+    check(got, lse, with_join(reference(q, k, v, table, new, kv)))
+
+
+def test_rows_of_nobody_before_the_first_sequence(cuda):
+    groups, new, kv = [(0, 3, 64)], [1, 2, 1, 4], [80, 90, 66, 30]
+    q, k, v, table, cu, kv_len, (cg, pl) = shared(cuda, 53, groups, new, kv, 8, 2, 128, 16, torch.bfloat16, pad=9)
+    ref = with_join(reference(q[5:], k, v, table, new, kv))
+    out = torch.full_like(q, 9.0)
+    hmm.paged_prefix_attention(q, k, v, table, cu + 5, kv_len, cg, pl, out=out)
+    check(out[5:], None, ref)
+    assert (out[:5] == 9.0).all() and (out[5 + sum(new):] == 9.0).all()
 
 
 def test_prefix_is_read_from_one_row(cuda):

@@ -35,9 +35,21 @@ def raw(pages):
     return flat[..., :t * g * 32].unflatten(-1, (t, g * 32)), flat[..., t * g * 32:].unflatten(-1, (t, g))
 
 
-def run_case(cuda, seed, new, kv, hq, hk, d, pt, dtype, kind, pad=0, max_new=0, kscale=1.0, **kw):
+def long_table(table, pt, hk, hq, tokens):
+    """The table with empty columns behind it: a call that could come to so many products of chunks and
+    long contexts that it widens the keys of those with 512 rows first."""
+    columns = -(-4096 * 128 // (max(1, tokens * (hq // hk) // 256) * hk * pt)) + 1
+    table = torch.nn.functional.pad(table, (0, columns), value=-1)
+    size = hmm.load().hmm_paged_quant_attention_workspace_size
+    assert size(table.shape[0], tokens, hq, hk, 64, table.shape[1] * pt, 0) > size(table.shape[0], tokens, hq, hk, 64, pt, 0) + (1 << 20)
+    return table
+
+
+def run_case(cuda, seed, new, kv, hq, hk, d, pt, dtype, kind, pad=0, max_new=0, kscale=1.0, wide=False, **kw):
     q, k, v, table, cu, kv_len = make(cuda, seed, new, kv, hq, hk, d, pt, DT[dtype], pad=pad, scale=kscale)
     kp, vp, k, v = filled(k, v, kind)
+    if wide:
+        table = long_table(table, pt, hk, hq, sum(new) + pad)
     out = torch.full((sum(new) + pad, hq, d), 9.0, dtype=DT[dtype], device=cuda)
     got, lse = hmm.paged_quant_attention(q, kp, vp, table, cu, kv_len, out=out, return_lse=True, max_new=max_new, **kw)
     assert got is out and (out[sum(new):] == 9.0).all()
@@ -99,12 +111,81 @@ def test_all_keys_and_scale(cuda, shape):
     ([256, 200, 260], [300, 1000, 261], 2, 1, 128, 4),            # 512 rows, 400, 520; small pages
     ([520, 40], [530, 400], 3, 3, 96, 16),
     ([128, 128, 1], [128, 700, 9], 8, 2, 256, 2),
+    ([600, 520, 3], [100, 530, 2], 4, 4, 64, 16),                 # fewer cached than new tokens
 ])
 def test_chunks_of_many_rows(cuda, shape, kind, dtype):
     """Their keys are widened into the workspace first, beside sequences that are not."""
-    run_case(cuda, 13, *shape, dtype, kind, pad=3)
-    run_case(cuda, 13, *shape, dtype, kind, max_new=max(shape[0]), window=100, sinks=5)
-    run_case(cuda, 13, *shape, dtype, kind, causal=False, scale=0.2)
+    run_case(cuda, 13, *shape, dtype, kind, pad=600, wide=True)
+    run_case(cuda, 13, *shape, dtype, kind, pad=600, max_new=max(shape[0]), wide=max(shape[0]) * shape[2] // shape[3] >= 512,
+             window=100, sinks=5)
+    run_case(cuda, 13, *shape, dtype, kind, pad=600, wide=True, causal=False, scale=0.2)
+    run_case(cuda, 13, *shape, dtype, kind, pad=3, scale=-0.1)
+
+
+def test_widened_values_that_are_not_finite(cuda):
+    """NaN groups in seen and unseen places of a chunk whose keys are widened, in a captured call."""
+    new, kv, pt = [300, 1], [420, 50], 16
+    q, k, v, table, cu, kv_len = make(cuda, 32, new, kv, 8, 2, 128, pt, torch.bfloat16)
+    kp, vp, k, v = filled(k, v, "e4m3")
+    k, v = k.contiguous(), v.contiguous()
+    wide = long_table(table, pt, 2, 8, 301)
+    for pages in (kp, vp):                       # behind the sequence's end
+        codes, scales = raw(pages)
+        codes[table[0, 419 // pt].item(), :, 420 % pt:] = 255
+        scales[table[0, 419 // pt].item(), :, 420 % pt:] = 255
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    hmm.paged_quant_attention(q, kp, vp, wide, cu, kv_len, status=status)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = hmm.paged_quant_attention(q, kp, vp, wide, cu, kv_len, return_lse=True, status=status)
+    g.replay()
+    check(out, lse, reference(q, k, v, table, new, kv))
+    for p in (380, 130):                         # seen by some rows, and by all
+        page = table[0, p // pt].item()
+        codes, scales = raw(vp)
+        codes[page, 1, p % pt, 64:96], scales[page, 1, p % pt, 2] = 0, 255
+        v[page, 1, p % pt, 64:96] = NAN
+        g.replay()
+        check(out, lse, reference(q, k, v, table, new, kv))
+    check_status(status)
+    wide[0, 3] = k.shape[0]
+    g.replay()
+    with pytest.raises(HmmError):
+        check_status(status)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_queries_at_the_ends_of_bf16(cuda, kind):
+    """Rows of 2^120 and of 2^-120, one large value beside small ones, rows of zeros: scores are
+    those of the values."""
+    new, kv = [1, 3, 20], [200, 90, 333]
+    q, k, v, table, cu, kv_len = make(cuda, 33, new, kv, 4, 2, 64, 16, torch.bfloat16)
+    q[0, 0] *= 2.0 ** -120
+    q[1, 1] = 0
+    q[2, 2, 7] = 2.0 ** 14
+    q[5] *= 2.0 ** -30
+    kp, vp, k, v = filled(k, v, kind)
+    k = k.contiguous()
+    out, lse = hmm.paged_quant_attention(q, kp, vp, table, cu, kv_len, return_lse=True)
+    check(out, lse, reference(q, k, v, table, new, kv))
+    big = q * 2.0 ** 110
+    out, lse = hmm.paged_quant_attention(big, kp, vp, table, cu, kv_len, scale=2.0 ** -113, return_lse=True)
+    check(out, lse, reference(big, k, v, table, new, kv, scale=2.0 ** -113))
+
+
+def test_rows_of_nobody_before_the_first_sequence(cuda):
+    new, kv = [2, 30, 1], [50, 400, 33]
+    q, k, v, table, cu, kv_len = make(cuda, 34, new, kv, 8, 2, 128, 16, torch.float16, pad=7)
+    kp, vp, k, v = filled(k, v, "int8")
+    ref = reference(q[4:], k, v, table, new, kv)
+    out = torch.full_like(q, 9.0)
+    hmm.paged_quant_attention(q, kp, vp, table, cu + 4, kv_len, out=out)
+    check(out[4:], None, ref)
+    assert (out[:4] == 9.0).all() and (out[4 + sum(new):] == 9.0).all()
+    k2, v2 = (torch.full((sum(new) + 7, 2, 128), 9.0, dtype=torch.float16, device=cuda) for _ in range(2))
+    hmm.paged_quant_read(kp, vp, table, cu + 4, kv_len, sum(new) + 7, dtype=torch.float16, out=(k2, v2))
+    assert (k2[:4] == 9.0).all() and (v2[4 + sum(new):] == 9.0).all()
+    assert torch.equal(k2[4], k[table[0, 3].item(), :, 0]) and torch.equal(v2[36], v[table[2, 2].item(), :, 0])
 
 
 def test_what_the_workspace_has_no_room_for(cuda):
