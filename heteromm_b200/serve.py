@@ -8,6 +8,10 @@ or [n_pages, page_tokens, D] for one head.  Any page / head / token strides that
 multiples of 8 elements do, with the last dimension contiguous: token-major pages are
 `pages.transpose(1, 2)`, interleaved ones `both[:, 0]` and `both[:, 1]`.
 
+Or it is held in 8 bits (quant_pages), for paged_quant_append, paged_quant_read and
+paged_quant_attention; paged_prefix_attention, which goes once through what sequences share,
+takes either.
+
 A batch is `page_table` [n_seq, pages_per_seq] int32, `cu_new` [n_seq + 1] int32 (the
 rows of each sequence's new tokens in the packed arrays) and `kv_len` [n_seq] int32
 (cached tokens, the new ones among them).  All of it is read on the device; rows that
