@@ -356,7 +356,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
         for (int i = 0; i < n; ++i) {
-            if (QUANT) cp_wait<RW_STAGES - 2>();       // (the scale bytes; the wait below is the warp's)
+            if (QUANT) {
+                cp_wait<RW_STAGES - 2>();              // a lane's own copies of scale bytes,
+                __syncwarp();                          // and the other lanes', which it reads
+            }
             if (!dead) {
                 const uint32_t at = done + i;
                 dead = !__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][at % RW_STAGES],
