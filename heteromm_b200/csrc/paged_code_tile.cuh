@@ -126,7 +126,8 @@ __device__ __forceinline__ ScaleCopy scale_copy(const AttnArgs& a, int kvh, int 
 // Lane s holds (page, row) of box s; a page of n_pages is out of range.
 __device__ __forceinline__ void code_copy_scales(const AttnArgs& a, const ScaleCopy& c, int page, int row, uint32_t dst) {
     const int pg = __shfl_sync(0xffffffffu, page, c.box & 31), rw = __shfl_sync(0xffffffffu, row, c.box & 31);
-    if (c.box >= 0 && pg < a.n_pages) cp16(dst + c.dst, c.base + pg * c.page + (int64_t)rw * a.quant.per_token, true);
+    const bool real = pg < a.n_pages;   // (else zeros, as the codes')
+    if (c.box >= 0) cp16(dst + c.dst, real ? c.base + pg * c.page + (int64_t)rw * a.quant.per_token : c.base, real);
 }
 
 // Scores of 16 rows and 32 keys.  (Four sums at a time: an MMA waits for the one before it in its own.)

@@ -385,7 +385,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     for (int c = 0; c < HALVES * (ROW / 16); ++c)
                         *reinterpret_cast<uint4*>(ring_p + so + (HALVES + c / (ROW / 16)) * BLOCK + lane * ROW +
                                                   c % (ROW / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    // (scale bytes of rows that were not read are anything, and 255 would make NaN of a zero)
+                    // (a slot of nobody may have a scale byte of 255, which would make NaN of a zero)
                     for (int g = 0; g < per; ++g) scales_p[so / STAGE * SCALES + SCALES / 2 + lane * per + g] = 127;
                 }
                 fence_proxy_async_smem();              // before the stage's next copies
