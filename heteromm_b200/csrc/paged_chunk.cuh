@@ -743,7 +743,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (!(ok = take(k)) || u.s < 0) break;
                 const int mine = lane / subs, sub = lane % subs;
                 auto lookup = [&](int j, int* page, int* row) {   // lane: box `sub` of tile j + mine
-                    *page = a.n_pages;                            // out of range: zeros
+                    *page = a.n_pages;                            // out of range: zeros (-1: of a seen box)
                     *row = 0;
                     if (j + mine < u.n) {
                         const int k0 = u.key0(j + mine) + sub * br;
@@ -752,6 +752,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                             if (e >= 0) {
                                 *page = e;
                                 *row = k0 - lp * a.page_tokens;
+                            } else if (QUANT) {
+                                *page = -1;
                             }
                         }
                     }
@@ -764,21 +766,30 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     const int n = min(ahead, u.n - j0);
                     for (int j = 0; ok && j < n; ++j) {
                         if constexpr (QUANT) {
-                            // (a box of a page out of range is not asked for: nothing of it is seen)
+                            // A box that no row sees is not asked for (K's scores there are masked, V's rows
+                            // become zeros); one that is seen, but whose page is out of range, is zeros.
                             const int per = a.quant.per_token, box_bytes = br * (a.D + per);
                             const int64_t in_page = (int64_t)row * a.D, scale_at = a.quant.scales + (int64_t)row * per;
 #pragma unroll 1
                             for (int x = 0; x < 2 * PARTS; ++x, ++i) {
                                 const uint32_t st = i % CST;
-                                const bool in = mine == j && page < a.n_pages && (PARTS == 1 || sub * br / CKEYS == x % PARTS);
+                                const bool here = mine == j && (PARTS == 1 || sub * br / CKEYS == x % PARTS);
+                                const bool in = here && (uint32_t)page < (uint32_t)a.n_pages;
                                 const Pages& p = x < PARTS ? a.k : a.v;
                                 const unsigned char* src = p.base + page * p.page + u.kvh * p.head;
-                                const uint32_t dst = smem_u32(Cs + st * CODES) + (PARTS == 1 ? sub : sub & (CKEYS / br - 1)) * box_bytes;
+                                unsigned char* to = Cs + st * CODES + (PARTS == 1 ? sub : sub & (CKEYS / br - 1)) * box_bytes;
                                 const uint32_t bytes = box_bytes * __popc(__ballot_sync(0xffffffffu, in));
                                 if (!(ok = wait_warp(&ctl->c_empty[st], ((i / CST) & 1) ^ 1, abort, t.wait_ns))) break;
+                                if (here && page < 0) {
+                                    for (int z = 0; z < box_bytes; z += 16)
+                                        *reinterpret_cast<uint4*>(to + z) = make_uint4(0u, 0u, 0u, 0u);
+                                    fence_proxy_async_smem();   // before the stage's next copies
+                                }
+                                __syncwarp();
                                 if (lane == 0) mbar_expect_tx(&ctl->c_full[st], bytes);
                                 __syncwarp();
                                 if (!in) continue;
+                                const uint32_t dst = smem_u32(to);
                                 if (br == a.page_tokens) {   // all of a page and head: one block
                                     bulk_load(dst, src, box_bytes, &ctl->c_full[st]);
                                 } else {

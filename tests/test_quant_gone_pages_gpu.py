@@ -1,6 +1,6 @@
 """A page-table entry out of its bounds: the call is flagged, and the rows of the sequence that
-names it are those over a page of zeros there, for both caches: nothing of them
-comes from what a CTA's shared memory held before."""
+names it are those over a page of zeros there, from both kernels and for both caches - nothing
+of them comes from what a CTA's shared memory held before."""
 import pytest
 import torch
 
@@ -48,6 +48,12 @@ SHAPES = [  # new, kv, hq, hk, d, pt, entries that are gone
     ([1] * 12, [300] * 12, 8, 2, 64, 32, [(0, 3), (1, 0), (2, 9)]),
     ([1] * 12, [300] * 12, 2, 1, 256, 16, [(0, 3), (4, 18)]),
     ([2] * 5, [90] * 5, 6, 2, 128, 4, [(0, 3), (1, 21), (2, 22), (2, 0)]),
+    ([40] * 6, [500] * 6, 8, 2, 128, 16, [(0, 3), (1, 0), (2, 31), (3, 29), (3, 30)]),         # chunk kernel
+    ([40] * 6, [500] * 6, 8, 2, 64, 16, [(0, 3), (1, 0), (2, 31), (3, 29)]),
+    ([40] * 6, [500] * 6, 4, 2, 256, 32, [(0, 3), (1, 0), (2, 15), (4, 13)]),
+    ([130] * 3, [400] * 3, 4, 1, 96, 48, [(0, 0), (1, 8), (2, 3)]),
+    ([200] * 2, [640] * 2, 4, 2, 128, 128, [(0, 0), (1, 4)]),
+    ([50] * 4, [333] * 4, 8, 2, 128, 8, [(i, j) for i in range(2) for j in range(42)]),        # every page
 ]
 
 
@@ -94,7 +100,7 @@ def test_of_a_widened_sequence(cuda, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("n_seq,new", [(6, 1)])
+@pytest.mark.parametrize("n_seq,new", [(6, 1), (12, 8)])
 def test_of_a_shared_prefix(cuda, kind, n_seq, new):
     """The pages of the prefix are those of the group's first row, for all its sequences; a
     tail's are its own."""
