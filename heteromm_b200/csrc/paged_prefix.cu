@@ -79,29 +79,33 @@ __global__ void __launch_bounds__(SH_THREADS) paged_shared_kernel(const __grid_c
         atomicAdd(a.of_group + 3 * g + 2, 1);
     }
     __syncthreads();
-    // (one sequence alone has nothing to share)
-    auto common = [&](int g) { return __ldcg(a.of_group + 3 * g + 2) > 1 ? __ldcg(a.of_group + 3 * g) : 0; };
     for (int g = threadIdx.x; g < a.n_groups; g += SH_THREADS) {
-        const int n = common(g);
-        int begin = 0, rows = 0;
+        // (one sequence alone has nothing to share)
+        int n = __ldcg(a.of_group + 3 * g + 2) > 1 ? __ldcg(a.of_group + 3 * g) : 0, begin = 0, rows = 0;
         if (n > 0) {
             begin = __ldg(a.b.cu + __ldg(a.cu_group + g));
             rows = __ldg(a.b.cu + __ldg(a.cu_group + g + 1)) - begin;
             if (begin < 0 || rows < 0 || begin + (int64_t)rows > a.b.n_tokens) {
                 atomicOr(a.status, HMM_STATUS_BATCH_BOUNDS);
-                begin = rows = 0;
+                begin = rows = n = 0;
             }
         }
         // (positions behind every key: all of them are seen)
-        a.parts[2 * g] = make_int4(begin, rows, rows > 0 ? n : 0, INT32_MAX - 1 - rows);
-        a.parts[2 * g + 1] = make_int4(0, rows > 0 ? __ldcg(a.of_group + 3 * g + 1) : 0, a.b.n_tokens + begin, 0);
+        a.parts[2 * g] = make_int4(begin, rows, n, INT32_MAX - 1 - rows);
+        a.parts[2 * g + 1] = make_int4(0, n > 0 ? __ldcg(a.of_group + 3 * g + 1) : 0, a.b.n_tokens + begin, 0);
     }
+    __syncthreads();
     for (int s = threadIdx.x; s < a.b.n_seq; s += SH_THREADS) {
         const Seq q = load_seq(a.b, a.max_kv, s, a.status);
         const int g = group_of(a, s);
+        int n = 0;
+        if (g >= 0 && q.n_new > 0) {   // (where cu_new descends its rows may not be the group's)
+            const int4 all = __ldcg(a.parts + 2 * g);
+            if (q.begin >= all.x && q.begin + q.n_new <= all.x + all.y) n = all.z;
+        }
         int4* p = a.parts + 2 * ((int64_t)a.n_groups + s);
         p[0] = make_int4(q.begin, q.n_new, q.kv, q.pos0);
-        p[1] = make_int4(g >= 0 && q.n_new > 0 ? common(g) : 0, s, q.begin, 0);
+        p[1] = make_int4(n, s, q.begin, 0);
     }
 }
 
