@@ -118,10 +118,22 @@ __global__ void __launch_bounds__(MG_THREADS) paged_merge_kernel(const __grid_co
     const int64_t row = (int64_t)blockIdx.x * (MG_THREADS / 32) + (threadIdx.x >> 5), rows = (int64_t)a.b.n_tokens * a.hq;
     if (row >= rows) return;
     const int tok = (int)(row / a.hq), head = (int)(row - (int64_t)tok * a.hq);
-    const int s = warp_find_seq(a.b, tok);
+    int s = warp_find_seq(a.b, tok);
+    auto owns = [&](const int4& p) { return tok >= p.x && tok - p.x < p.y; };
+    if (!owns(__ldcg(m.parts + 2 * (int64_t)s))) {
+        // a row of no sequence, left as it is; or one that the search missed, which takes a cu_new
+        // that ascends (another is flagged)
+        if (!(__ldcg(a.status) & HMM_STATUS_BATCH_BOUNDS)) return;
+        unsigned at = 0;
+        for (int s0 = 0; at == 0 && s0 < a.b.n_seq; s0 += 32) {
+            s = s0 + lane;
+            at = __ballot_sync(0xffffffffu, s < a.b.n_seq && owns(__ldcg(m.parts + 2 * (int64_t)s)));
+        }
+        if (at == 0) return;
+        s = __shfl_sync(0xffffffffu, s, __ffs(at) - 1);
+    }
     const int4 p0 = __ldcg(m.parts + 2 * (int64_t)s), p1 = __ldcg(m.parts + 2 * (int64_t)s + 1);
     const int in = tok - p0.x;
-    if (in < 0 || in >= p0.y) return;                    // a row of no sequence, left as it is
     float l2 = __ldcg(m.part_lse + row), l1 = p1.x > 0 ? __ldcg(m.part_lse + rows + row) : -INFINITY;
     const float top = fmaxf(l1, l2), ref = top == -INFINITY ? 0.0f : top;
     float w1 = expf(l1 - ref), w2 = expf(l2 - ref);
