@@ -289,18 +289,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Weights exp2(sc (s - m) + tc_up) of 64 of a row's scores v, packed in pairs, to TMEM, and their
 // sum (two pairs of partial sums), AT of 32 registers at a time (the warps that widen leave
-// fewer); with TOP also the largest of the 128 scores from v on.
+// fewer; 0: they stay in p, for the caller to store); with TOP also the largest of the 128
+// scores from v on.
 // m = -inf (no key seen yet) gives exp2(sc s).  The maximum (ALU) and what follows a weight (FMA
 // and ALU) stand between the exponentials, which keep the special-function unit for 8
 // clocks each: apart, the two would take their times in turn.
 template <typename T, bool TOP, int AT>
 __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float m, float sc, uint32_t to,
-                                         uint64_t* sum) {
+                                         uint32_t* p, uint64_t* sum) {
     constexpr int LAG = 2;   // pairs between a weight's exponential and its use
     const float neg = m == -INFINITY ? 0.0f : fmaf(-m, sc, tc_up<T>());
     const uint64_t neg2 = pack_f2(neg, neg);
     sum[0] = sum[1] = pack_f2(0.0f, 0.0f);
-    uint32_t p[AT];
     float x[32], y[32], mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 32 + LAG; ++i) {
@@ -319,7 +319,7 @@ __device__ __forceinline__ float weights(const uint32_t* v, uint64_t sc2, float 
             sum[u & 1] = add_f2(sum[u & 1], pack_f2(x[u], y[u]));
             // weights in the cache's type for the product: off by half a step, 2^-8 of a
             // weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
-            p[u % AT] = pack2<T>(x[u], y[u]);
+            p[u % (AT == 0 ? 32 : AT)] = pack2<T>(x[u], y[u]);
             if (AT == 16 && u % 16 == 15) tmem_st_x16(to + u - 15, p);
         }
     }
@@ -362,13 +362,12 @@ __device__ __forceinline__ int block_length(const TcArgs& t, const Seq& q, int r
     return TC_UNIT_COST + tiles_of(t.a, q, rb << t.rows_log2, last_row(t, q, rb)).n;
 }
 
-// Lane `src`'s sequence, for the warp.
-__device__ __forceinline__ Seq shared_seq(const Seq& q, int src) {
-    Seq x;
-    x.begin = __shfl_sync(0xffffffffu, q.begin, src);
-    x.n_new = __shfl_sync(0xffffffffu, q.n_new, src);
-    x.kv = __shfl_sync(0xffffffffu, q.kv, src);
-    x.ok = true;
+// Lane `src`'s sequence, for the warp; lane 0's is sequence s0.
+template <bool SHARED>
+__device__ __forceinline__ Seq shared_seq(const Seq& q, int s0, int src) {
+    Seq x = seq_of(s0 + src, __shfl_sync(0xffffffffu, q.begin, src), __shfl_sync(0xffffffffu, q.n_new, src),
+                   __shfl_sync(0xffffffffu, q.kv, src));
+    if (!SHARED) return x;
     x.pos0 = __shfl_sync(0xffffffffu, q.pos0, src);
     x.lo = __shfl_sync(0xffffffffu, q.lo, src);
     x.row = __shfl_sync(0xffffffffu, q.row, src);
@@ -392,14 +391,15 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
 }
 
 // One warp.
+template <bool SHARED>
 __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     const AttnArgs& a = t.a;
     const int lane = threadIdx.x & 31;
     if (!t.split) return Plan{0, 0};
     int64_t units = 0;
-    each_seq(a.b, a.max_kv, lane, 32, a.status, [&](const Seq& q) { units += (int64_t)row_blocks(t, q) * a.hk; });
+    each_seq<SHARED>(a.b, a.max_kv, lane, 32, a.status, [&](const Seq& q) { units += (int64_t)row_blocks(t, q) * a.hk; });
     // (A shared prefix is a long unit beside many short ones.)
-    if (!a.b.shared && warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
+    if (!(SHARED && a.b.shared) && warp_sum(units) >= (int64_t)gridDim.x) return Plan{0, 0};
     int64_t tiles = 0;   // (a few row blocks per CTA at most)
     int longest = 0;
     auto add = [&](const Seq& q, int rb) {
@@ -410,14 +410,14 @@ __device__ __forceinline__ Plan make_plan(const TcArgs& t) {
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 32) {
         const int s = s0 + lane;
         Seq q{};
-        if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
+        if (s < a.b.n_seq) q = load_seq<SHARED>(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
         if (rb > 0) add(q, 0);
         unsigned busy = __ballot_sync(0xffffffffu, rb > 1);
         while (busy) {
             const int src = __ffs(busy) - 1;
             busy &= busy - 1;
-            const Seq x = shared_seq(q, src);
+            const Seq x = shared_seq<SHARED>(q, s0, src);
             const int n = __shfl_sync(0xffffffffu, rb, src);
             for (int i = 1 + lane; i < n; i += 32) add(x, i);
         }
@@ -439,6 +439,7 @@ struct Cursor {
 
 // The k-th unit (whole units) or, from c->pos on, the next piece of this CTA's share, into
 // *u (s = -1: there is none); moves *c on.  One warp.
+template <bool SHARED>
 __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int64_t k, Cursor* c, Unit* u) {
     const AttnArgs& a = t.a;
     const int lane = threadIdx.x & 31;
@@ -455,7 +456,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
         c->units = unit_run;
         const int s = s0 + lane;
         Seq q{};
-        if (s < a.b.n_seq) q = load_seq(a.b, a.max_kv, s, a.status);
+        if (s < a.b.n_seq) q = load_seq<SHARED>(a.b, a.max_kv, s, a.status);
         const int rb = row_blocks(t, q);
         unsigned busy = __ballot_sync(0xffffffffu, rb > 0);
         if (!cut) {   // past 32 sequences at once
@@ -479,7 +480,7 @@ __device__ __forceinline__ void describe(const TcArgs& t, const Plan& plan, int6
         while (busy) {
             const int src = __ffs(busy) - 1;
             busy &= busy - 1;
-            const Seq x = shared_seq(q, src);
+            const Seq x = shared_seq<SHARED>(q, s0, src);
             const int n_rb = __shfl_sync(0xffffffffu, rb, src);
             // a sequence's last rows see the most keys: they go first, so that the short
             // blocks fill the end
@@ -638,7 +639,10 @@ __device__ __forceinline__ void widen_rows(const unsigned char* codes, const Att
     }
 }
 
-template <typename T, int DP, int C>
+// SHARED: the batch may be one of parts (Batch::shared), whose keys begin at Seq::lo and whose rows may go
+// to AttnArgs::part.  What that adds to the softmax warps' code is felt where their issue is the bound, so
+// a plain batch over 16 bits has a kernel without it.
+template <typename T, int DP, int C, bool SHARED>
 __global__ void __launch_bounds__(tc_threads<C>(), 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ TcArgs t) {
@@ -1044,7 +1048,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         } else {
             // -------------------------------------- the units, and their queries
             if (t.split && lane == 0) t.join.joint[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-            const Plan plan = make_plan(t);
+            const Plan plan = make_plan<SHARED>(t);
             if (lane == 0) ctl->plan = plan;
             Cursor at{(int64_t)blockIdx.x * plan.per, 0, 0, 0};
             int loads = 0;                       // units' queries so far
@@ -1052,7 +1056,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             for (int k = 0; ok; ++k) {
                 if (!(ok = wait_warp(&ctl->u_empty[k & 1], ((k >> 1) & 1) ^ 1, abort, t.unit_ns))) break;
                 Unit* u = &ctl->unit[k & 1];
-                describe(t, plan, k, &at, u);
+                describe<SHARED>(t, plan, k, &at, u);
                 const int s = u->s, n = u->n, row0 = u->row0, rows = u->rows, kvh = u->kvh, begin = u->q.begin;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->u_full[k & 1]);
@@ -1128,9 +1132,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 const int key0 = u.key0(u.alone ? 2 * j + w : j), kv = u.q.kv;
                 const int pos_first = __shfl_sync(0xffffffffu, pos, 0), pos_last = __shfl_sync(0xffffffffu, pos, 31);
                 if (!(key0 + TC_KEYS <= kv && (!a.causal || key0 + TC_KEYS - 1 <= pos_first) &&
-                      (a.window > 0 ? key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks : key0 >= u.q.lo))) {
+                      (a.window > 0 ? key0 > pos_last - a.window || key0 + TC_KEYS <= a.sinks : !SHARED || key0 >= u.q.lo))) {
                     const int hi = (a.causal ? min(kv, pos + 1) : kv) - key0;
-                    const int lo = (a.window > 0 ? max(0, pos - a.window + 1) : u.q.lo) - key0;
+                    const int lo = (a.window > 0 ? max(0, pos - a.window + 1) : SHARED ? u.q.lo : 0) - key0;
                     const int sink = a.window > 0 ? a.sinks - key0 : 0;
 #pragma unroll
                     for (int c0 = 0; c0 < TC_KEYS; c0 += 32) {
@@ -1144,10 +1148,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 // that is right unless the row grew by more than TC_GROWTH, which is rare.
                 // NaN and +inf show in the maximum: such a row is NaN.
                 // (They go over the scores, which are in registers, and are written again if it was not.)
+                // Stored before the vote below the weights are in TMEM sooner (32/8 heads of 128, 2,048 tokens:
+                // 59.2 -> 57.9 us); at D = 64, where these warps' issue is the bound, behind it (8,192 tokens:
+                // 429 -> 422 us).
+                constexpr int AT = QUANT ? 16 : DP == 64 ? 0 : 32;
                 uint64_t sum[2];
+                uint32_t p[AT == 0 ? 32 : AT];
 #pragma unroll 1
                 while (true) {
-                    const float top = weights<T, true, QUANT ? 16 : 32>(v, sc2, m, sc, ts, sum);
+                    const float top = weights<T, true, AT>(v, sc2, m, sc, ts, p, sum);
                     fine = fine && top < INFINITY;
                     const bool grow = (top - m) * sc > TC_GROWTH && top < INFINITY;
                     if (!__any_sync(0xffffffffu, grow)) break;
@@ -1172,11 +1181,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 // the first half's product starts while the second half is in the exponentials
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
+                if (AT == 0) tmem_st_x32(ts, p);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->p_full[w][0]);
-                weights<T, false, QUANT ? 16 : 32>(v + 64, sc2, m, sc, ts + 32, sum);
+                weights<T, false, AT>(v + 64, sc2, m, sc, ts + 32, p, sum);
+                if (AT == 0) tmem_st_x32(ts + 32, p);
                 l2[0] = add_f2(l2[0], sum[0]);
                 l2[1] = add_f2(l2[1], sum[1]);
                 tmem_wait_st();
@@ -1220,7 +1231,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 s0 = l = NAN;
             }
             const int x = u.row0 + (live ? r : 0), tok = a.by_group(x), head = x - tok * a.group;
-            const int64_t orow = (int64_t)(u.q.out + tok) * a.hq + u.kvh * a.group + head;
+            const int64_t orow = (int64_t)((SHARED ? u.q.out : u.q.begin) + tok) * a.hq + u.kvh * a.group + head;
             float* pt = t.join.part + (int64_t)u.slot * UNIT * (DP + 2);   // (pieces)
             if (whole_unit && l != 0.0f) {
                 const float inv = 1.0f / l;
@@ -1260,7 +1271,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                             make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
                     continue;
                 }
-                if (a.part) {
+                if (SHARED && a.part) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 8)
                         if (c0 + c < a.D) store32(a.part + orow * a.D + c0 + c, o + c, false);
@@ -1293,7 +1304,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     a.lse[orow] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
                 }
             }
-            const unsigned again = __ballot_sync(0xffffffffu, live && fine && !a.part && most >= 0x7f800000u);
+            const unsigned again = __ballot_sync(0xffffffffu, live && fine && !(SHARED && a.part) && most >= 0x7f800000u);
             if (lane == 0 && whole_unit && (uint32_t)u.id < (uint32_t)t.units) {
                 t.again[(int64_t)u.id * TC_SOFTMAX_WARPS + warp] = again;
                 if (again) ctl->any_again = 1;
@@ -1314,7 +1325,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const Plan plan = ctl->plan;
     Cursor at{(int64_t)blockIdx.x * plan.per, 0, 0, 0};
     for (int64_t k = 0;; ++k) {
-        describe(t, plan, k, &at, u);
+        describe<SHARED>(t, plan, k, &at, u);
         const int s = u->s, kvh = u->kvh, row0 = u->row0 + 32 * warp, slot = u->slot;
         const int id = u->id;
         const Seq q = u->q;
@@ -1328,14 +1339,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 
 inline int unit_rows(int64_t D) { return D <= 128 ? tc_rows<128>() : tc_rows<256>(); }
 
-template <typename T, int DP, int C>
+template <typename T, int DP, int C, bool SHARED>
 hmm_status_t launch_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q,
                           bool behind, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
-    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP, C>, tc_smem<DP, C>(), &done);
+    const hmm_status_t s = allow_smem(paged_chunk_kernel<T, DP, C, SHARED>, tc_smem<DP, C>(), &done);
     if (s != HMM_OK) return s;
-    return launch(paged_chunk_kernel<T, DP, C>, dim3((unsigned)device_sm_count()), tc_threads<C>(), tc_smem<DP, C>(), behind, st,
+    return launch(paged_chunk_kernel<T, DP, C, SHARED>, dim3((unsigned)device_sm_count()), tc_threads<C>(), tc_smem<DP, C>(), behind, st,
                   "paged_chunk_kernel", k, v, q, t);
+}
+
+template <typename T, int DP, int C>
+hmm_status_t choose_chunk(const TcArgs& t, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, bool behind,
+                          cudaStream_t st) {
+    if constexpr (C == CODEC_NONE) {
+        if (!t.a.b.shared) return launch_chunk<T, DP, C, false>(t, k, v, q, behind, st);
+    }
+    return launch_chunk<T, DP, C, true>(t, k, v, q, behind, st);
 }
 
 template <int C>
@@ -1378,13 +1398,13 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
         if (s != HMM_OK) return s;
     }
     if (a.D <= 64)
-        return bf16 ? launch_chunk<__nv_bfloat16, 64, C>(t, k, v, q, behind, st)
-                    : launch_chunk<__half, 64, C>(t, k, v, q, behind, st);
+        return bf16 ? choose_chunk<__nv_bfloat16, 64, C>(t, k, v, q, behind, st)
+                    : choose_chunk<__half, 64, C>(t, k, v, q, behind, st);
     if (a.D <= 128)
-        return bf16 ? launch_chunk<__nv_bfloat16, 128, C>(t, k, v, q, behind, st)
-                    : launch_chunk<__half, 128, C>(t, k, v, q, behind, st);
-    return bf16 ? launch_chunk<__nv_bfloat16, 256, C>(t, k, v, q, behind, st)
-                : launch_chunk<__half, 256, C>(t, k, v, q, behind, st);
+        return bf16 ? choose_chunk<__nv_bfloat16, 128, C>(t, k, v, q, behind, st)
+                    : choose_chunk<__half, 128, C>(t, k, v, q, behind, st);
+    return bf16 ? choose_chunk<__nv_bfloat16, 256, C>(t, k, v, q, behind, st)
+                : choose_chunk<__half, 256, C>(t, k, v, q, behind, st);
 }
 
 }  // namespace serve

@@ -68,15 +68,17 @@ __device__ __forceinline__ Seq shared_part(const Batch& b, int s) {
     return Seq{x.x, x.y, x.z, true, x.w, y.x, y.y, y.z};
 }
 
+// (SHARED: the batch may be one of parts)
+template <bool SHARED = true>
 __device__ __forceinline__ Seq load_seq(const Batch& b, int64_t max_kv, int s, int32_t* status) {
-    if (b.shared) return shared_part(b, s);
+    if (SHARED && b.shared) return shared_part(b, s);
     return check_seq(b, max_kv, s, __ldg(b.cu + s), __ldg(b.cu + s + 1), __ldg(b.kv_len + s), status);
 }
 
 // f(sequence) of every step-th sequence from s on, four sequences' loads in flight.
-template <typename F>
+template <bool SHARED = true, typename F>
 __device__ __forceinline__ void each_seq(const Batch& b, int64_t max_kv, int s, int step, int32_t* status, F&& f) {
-    if (b.shared) {
+    if (SHARED && b.shared) {
         for (; s < b.n_seq; s += step) f(shared_part(b, s));
         return;
     }
