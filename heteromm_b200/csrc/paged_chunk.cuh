@@ -736,7 +736,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // A lane looks up one box's page: of 32 boxes, that is of `ahead` key tiles, at once,
             // and of the next 32 while these are asked for.
             const int br = t.box_rows, subs = TC_KEYS / br, ahead = 32 / subs;
-            if (lane == 0) {
+            if (!QUANT && lane == 0) {
                 prefetch_tmap(&tmK);
                 prefetch_tmap(&tmV);
             }
@@ -1388,11 +1388,13 @@ hmm_status_t run_chunk(const AttnArgs& a, bool bf16, int min_rows, bool behind, 
                            device_sm_count(), (int)((most + 15) / 16), (int)rows};
     }
     *join = t.join;
-    CUtensorMap k, v, q{};
-    hmm_status_t s = make_page_map(&k, a, a.k, t.box_rows, C != CODEC_NONE);
-    if (s != HMM_OK) return s;
-    s = make_page_map(&v, a, a.v, t.box_rows, C != CODEC_NONE);
-    if (s != HMM_OK) return s;
+    CUtensorMap k{}, v{}, q{};
+    hmm_status_t s = HMM_OK;
+    if (C == CODEC_NONE) {   // (blocks of codes are copied without a map)
+        s = make_page_map(&k, a, a.k, t.box_rows, false);
+        if (s == HMM_OK) s = make_page_map(&v, a, a.v, t.box_rows, false);
+        if (s != HMM_OK) return s;
+    }
     if (boxes) {
         s = make_query_map(&q, a, a.group, TC_ROWS / a.group);
         if (s != HMM_OK) return s;
