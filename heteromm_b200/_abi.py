@@ -97,6 +97,7 @@ SIGNATURES = {
                                          C.c_int, _F, _P, _I, _I, C.c_int, _P, _P, _I, _I, _P, _P]),
     "hmm_paged_quant_read": (C.c_int, [_P, _P, C.c_int, _P, _P, _P, _P]),
     "hmm_paged_quant_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
+    "hmm_paged_quant_window_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "hmm_paged_quant_attention": (C.c_int, [_P, _P, C.c_int, _P, _I, _I, _I, _F, C.c_int, _I, _I, _I, _P, _P, _P,
                                             _P, _S, _P]),
     "hmm_paged_prefix_attention_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),

@@ -83,7 +83,7 @@ template <> hmm_status_t run_attention<__half, CODEC_I8>(const AttnArgs&, int, u
 size_t attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared);
 // (over a cache in 8 bits; max_kv: the tokens that a row of the page table can hold)
 size_t quant_attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D,
-                                 int64_t max_kv, int64_t max_new, bool shared);
+                                 int64_t max_kv, int64_t max_new, int64_t window, bool shared);
 
 // A row of a unit (sequence, KV head): row r is new token r / group, head r % group.
 struct Span {                    // keys [0, sink) and [lo, hi) hold all that some row of a tile sees

@@ -168,7 +168,7 @@ struct PrefixSpace {
 PrefixSpace prefix_space(int64_t n_seq, int64_t n_tokens, int64_t n_groups, int64_t n_heads, int64_t n_kv_heads, int64_t D,
                          bool quant, int64_t max_kv) {
     PrefixSpace w;
-    w.attention = up256(quant ? quant_attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, max_kv, 0, true)
+    w.attention = up256(quant ? quant_attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, max_kv, 0, 0, true)
                               : attention_workspace(n_seq + n_groups, n_tokens, n_heads, n_kv_heads, D, true));
     w.parts = up256(2 * sizeof(int4) * (size_t)(n_seq + n_groups));
     w.of_group = up256(3 * sizeof(int32_t) * (size_t)n_groups);

@@ -223,9 +223,10 @@ hmm_status_t run_attention<__half, CODEC_I8>(const AttnArgs& a, int max_new, uns
 }
 
 size_t quant_attention_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D,
-                                 int64_t max_kv, int64_t max_new, bool shared) {
-    // (a window may need less)
-    const size_t wide = wide_plan(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, 0, max_new, shared).bytes();
+                                 int64_t max_kv, int64_t max_new, int64_t window, bool shared) {
+    // (a window over everything is none)
+    const size_t wide = wide_plan(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, window < max_kv ? window : 0, max_new,
+                                  shared).bytes();
     return std::max(wide, attention_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, shared));
 }
 
@@ -238,8 +239,16 @@ using namespace hmm::serve;
 extern "C" size_t hmm_paged_quant_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
                                                            int64_t n_kv_heads, int64_t D, int64_t max_kv,
                                                            int64_t max_new) {
-    if (n_seq < 0 || n_tokens < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256 || max_kv < 0 || max_new < 0) return 0;
-    return quant_attention_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, max_new, false);
+    return hmm_paged_quant_window_attention_workspace_size(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, max_new, 0);
+}
+
+extern "C" size_t hmm_paged_quant_window_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
+                                                                  int64_t n_kv_heads, int64_t D, int64_t max_kv,
+                                                                  int64_t max_new, int64_t window) {
+    if (n_seq < 0 || n_tokens < 0 || n_heads < 1 || n_kv_heads < 1 || D < 1 || D > 256 || max_kv < 0 || max_new < 0 ||
+        window < 0)
+        return 0;
+    return quant_attention_workspace(n_seq, n_tokens, n_heads, n_kv_heads, D, max_kv, max_new, window, false);
 }
 
 extern "C" hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
@@ -252,9 +261,9 @@ extern "C" hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache
     if (s != HMM_OK) return s;
     HMM_REQUIRE(dtype == HMM_DTYPE_BF16 || dtype == HMM_DTYPE_F16,
                 "dtype must be HMM_DTYPE_BF16 or HMM_DTYPE_F16, got %d", dtype);
-    const size_t need = hmm_paged_quant_attention_workspace_size(batch->n_seq, batch->n_tokens, n_heads, cache->n_kv_heads,
-                                                                 cache->D, batch->pages_per_seq * cache->page_tokens,
-                                                                 max_new);
+    const size_t need = hmm_paged_quant_window_attention_workspace_size(
+        batch->n_seq, batch->n_tokens, n_heads, cache->n_kv_heads, cache->D, batch->pages_per_seq * cache->page_tokens,
+        max_new, window);
     bool nothing;
     s = plan_attention({q, q_token, q_head, n_heads, scale, causal, window, sinks, max_new, out, lse, device_status,
                         workspace, workspace_bytes, need}, quant_dims(*cache), batch, true, &a, &nothing);

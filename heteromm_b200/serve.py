@@ -39,7 +39,7 @@ from ._abi import HmmError, last_error, load
 _ENTRIES = ("hmm_paged_kv_append", "hmm_paged_attention", "hmm_paged_attention_workspace_size",
             "hmm_paged_state_workspace_size", "hmm_paged_copy_pages", "hmm_paged_free", "hmm_paged_fork",
             "hmm_paged_grow", "hmm_paged_compact", "hmm_status_read", "hmm_paged_quant_append",
-            "hmm_paged_quant_read", "hmm_paged_quant_attention", "hmm_paged_quant_attention_workspace_size",
+            "hmm_paged_quant_read", "hmm_paged_quant_attention", "hmm_paged_quant_window_attention_workspace_size",
             "hmm_paged_prefix_attention", "hmm_paged_prefix_attention_workspace_size",
             "hmm_paged_quant_prefix_attention", "hmm_paged_quant_prefix_attention_workspace_size")
 _CALLS = ("attention", "append", "copy_pages", "free", "fork", "grow", "compact", "quant_append", "quant_read",

@@ -49,7 +49,7 @@ struct Entry {
     decltype(&hmm_paged_quant_append) quant_append;
     decltype(&hmm_paged_quant_read) quant_read;
     decltype(&hmm_paged_quant_attention) quant_attention;
-    decltype(&hmm_paged_quant_attention_workspace_size) quant_attention_workspace;
+    decltype(&hmm_paged_quant_window_attention_workspace_size) quant_attention_workspace;
     decltype(&hmm_paged_prefix_attention) prefix_attention;
     decltype(&hmm_paged_prefix_attention_workspace_size) prefix_attention_workspace;
     decltype(&hmm_paged_quant_prefix_attention) quant_prefix_attention;
@@ -362,7 +362,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (with_lse) lse = empty({n_tokens, heads}, at::kFloat, c.dev);
     const Status status = status_word(a[13], c.dev, at.stream);
     const size_t bytes = QUANT ? hmm_fn.quant_attention_workspace(b.n_seq, n_tokens, heads, c.c.n_kv_heads, d,
-                                                                  b.pages_per_seq * qc.c.page_tokens, max_new)
+                                                                  b.pages_per_seq * qc.c.page_tokens, max_new, window)
                                : hmm_fn.attention_workspace(b.n_seq, n_tokens, heads, c.c.n_kv_heads, d);
     const c10::DataPtr ws = scratch(bytes);
     finish(unlocked([&] {

@@ -463,6 +463,11 @@ hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, const hmm_page
  * and more have their keys widened into it, up to 1 GiB of them). */
 size_t hmm_paged_quant_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
                                                 int64_t n_kv_heads, int64_t D, int64_t max_kv, int64_t max_new);
+/* What a call with this window needs: that, or less where the window leaves too few
+ * keys for them to be widened. */
+size_t hmm_paged_quant_window_attention_workspace_size(int64_t n_seq, int64_t n_tokens, int64_t n_heads,
+                                                       int64_t n_kv_heads, int64_t D, int64_t max_kv,
+                                                       int64_t max_new, int64_t window);
 hmm_status_t hmm_paged_quant_attention(const hmm_paged_quant_t* cache, const hmm_paged_batch_t* batch, int dtype,
                                        const void* q, int64_t q_token, int64_t q_head, int64_t n_heads,
                                        float scale, int causal, int64_t window, int64_t sinks, int64_t max_new,
