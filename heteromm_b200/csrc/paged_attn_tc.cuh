@@ -62,7 +62,7 @@ struct ChunkJoin {
 
 // Whether the kernel takes this page size: boxes of 8 rows and more.  Its producer's 32 lanes
 // look up a tile's boxes, which boxes of 4 rows would just fit (not tried) and smaller ones
-// not (2,048 tokens, 32/8 heads of 128: pages of 8 58 us here, of 4 837 in the rows kernel).
+// not (2,048 tokens, 32/8 heads of 128: pages of 8 58 us here, of 4 739 in the rows kernel).
 bool chunk_applies(const AttnArgs& a);
 // (shared: the parts of a batch of shared prefixes, in which a token counts twice)
 size_t chunk_workspace(int64_t n_seq, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t D, bool shared);

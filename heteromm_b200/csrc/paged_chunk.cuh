@@ -43,10 +43,10 @@
 // tiles and a key tile at D = 128, and as many for their exponentials on the
 // special-function units, 16 a clock.  Measured, 32 query and 8 KV heads, 8,192
 // tokens, causal: D = 128 455-478 us (1,150-1,210 TFLOP/s, about 4,000 clocks a
-// tile); without the exponentials it is no faster, with the products and loads
+// tile; 500-530 in a loop of calls, at the clocks that the power limit leaves); without the exponentials it is no faster, with the products and loads
 // alone 418: reading K and V into shared memory, 64 KB a tile and CTA, and their
 // reading by both row tiles' products bound it (bytes, not boxes: pages of 128 take 459
-// where pages of 16 take 456).  D = 64 424 us (650 TFLOP/s): the
+// where pages of 16 take 456).  D = 64 422 us (650 TFLOP/s): the
 // softmax warps' instructions do; exponentials moved to the FMA pipe only add (1 of
 // 8: 437).
 #pragma once

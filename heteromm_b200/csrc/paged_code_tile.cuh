@@ -76,7 +76,7 @@ __device__ __forceinline__ void mma_half(float* d, const uint32_t* a, uint32_t b
 
 // A row of q (null: zeros), half h of the fragments.  bf16 values go to fp16 times the power of two that
 // brings the row's largest finite one to 2^14 ... 2^15: exact down to 2^-28 of it, and off by
-// 2^-40 of it below.  Returns what the row's scores are times then.  Lanes of a row: 4 n + c.
+// 2^-39 of it below (half a step of fp16's subnormal numbers, 2^-25, beside 2^14).  Returns what the row's scores are times then.  Lanes of a row: 4 n + c.
 template <typename T, int DP>
 __device__ __forceinline__ float code_queries(const unsigned char* src, int D, int h, uint32_t (*qf)[4]) {
     const int c = threadIdx.x & 3;

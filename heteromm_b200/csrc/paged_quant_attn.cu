@@ -6,12 +6,15 @@
 // takes it 6,200 clocks and one of 16-bit values 4,000.  So keys of sequences with LONG_ROWS rows and
 // more are widened once, into a cache of the workspace, and attended to there
 // (8,192 tokens, 32/8 heads of 128, int8: 735 us within the chunk kernel, 494 so, 470 over a 16-bit
-// cache; a key costs 6 KB of memory traffic once, about 1 ns, and 60 ps per head and 256 rows more
+// cache, each by itself; in a loop of calls, at the clocks that the power limit leaves, 490-540 and
+// 500-530; a key costs 6 KB of memory traffic once, about 1 ns, and 60 ps per head and 256 rows more
 // within the kernel: as much at two blocks of eight heads, 512 rows).  The kernels for it cost 25 us
 // beside, so a call that cannot come to LONG_TILES products of 256 rows and 128 keys (1.1 us more
 // each on one of the SMs, 31 us in all) has none (8 sequences, a chunk of 1,001 tokens among them, a
-// window of 1,024: 62 us, 117 widened first).  What the workspace has no room for stays with the
-// kernels that widen.
+// window of 1,024: 62 us, 117 widened first).  How long sequences may be is taken from the page table's
+// width, so a wide table can bring the launches where nothing is long: 16 sequences' drafted tokens
+// over 5,000, 58 us, take 77 with a table for 131,072 tokens and without max_new.  What the workspace
+// has no room for stays with the kernels that widen.
 #include "paged_rows.cuh"
 
 namespace hmm {

@@ -20,8 +20,8 @@
 //   - a unit that several CTAs share leaves (maximum, sum, unnormalised rows) per
 //     piece in the workspace, and paged_join_kernel adds the pieces in order.
 // Measured: 64 sequences of up to 16,384 tokens, one new token each, 32 query and 8 KV
-// heads of 128: 347-351 us, 6.3 TB/s (cp.async: 478); one token over 777: 11.9 us, of
-// which 2.5 the join, over 4,000 17.6 us.  The same decode batch in e4m3: 248 us, 4.6 TB/s, where
+// heads of 128: 347-351 us, 6.3 TB/s (cp.async: 478); one token over 777: 12.5 us, of
+// which 2.5 the join, over 4,000 18.8 us.  The same decode batch in e4m3: 248 us, 4.6 TB/s, where
 // HBM would allow 173: conversions, scores and softmax are 4,000 clocks of latency a tile for a
 // warp, and twelve warps an SM hide a part of them.
 #pragma once
@@ -648,8 +648,8 @@ template <typename T, int C>
 hmm_status_t run_kernels(const AttnArgs& a, int max_new, unsigned char* ws, cudaStream_t st) {
     // A unit of up to 16 rows (one MMA's) reads its keys once either way and the many small
     // CTAs of the rows kernel keep more reads in flight; more rows would read them again
-    // there: 64 rows of 4 KV heads over 5,000, 16 sequences, D = 128, 113 us there and 69 in
-    // the chunk kernel, 32 rows 67 in both (over 777: 34 and 30, 25 and 29).  In 8 bits, where the
+    // there: 64 rows of 4 KV heads over 5,000, 16 sequences, D = 128, 114 us there and 70 in
+    // the chunk kernel, 32 rows 71 and 68 (over 777: 37 and 31, 31 in both).  In 8 bits, where the
     // chunk kernel has its codes widened beside the products, up to 32: 28 rows of 4 KV heads over
     // 700, 16 sequences, D = 128, 31 us there and 39 in the chunk kernel, over 5,000 49 and 52, 32
     // sequences over 16,000 154 and 203; 35 rows 33 and 39, 62 and 52, 211 and 203.  (A scale of zero

@@ -133,8 +133,8 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
     Every row of page_table lists all of its sequence's pages.  A prefix may end within a
     page, and reaches no further than what its sequences held before their new tokens.
-    The result is paged_attention's up to the order of its sums; max_new is taken as there
-    and not needed."""
+    The result is paged_attention's up to the order of its sums; max_new is taken as there,
+    checked, and has no effect."""
     return _calls.prefix_attention(q, k_pages, v_pages, page_table, cu_new, kv_len, cu_group, prefix_len, scale, max_new,
                                    return_lse, out, status)
 

@@ -387,7 +387,9 @@ hmm_status_t hmm_paged_kv_append(
  * every score is -inf; a seen score of NaN or +inf gives NaN in out and lse.
  * Keys and values that a token does not see never reach
  * its result, NaN and infinities included; page-table entries are read only
- * for pages that hold a seen key, so pages behind a window may be gone.
+ * for pages that hold a seen key, so pages behind a window may be gone.  A
+ * seen page that is out of bounds is flagged, and is zeros to the rows that see
+ * it (nothing to those that are computed again, as below).
  * (Rows beside one that sees a NaN or infinite value, which they do not see,
  * up to 256 of them, are computed again key by key: 16 ms over 4,096 cached
  * tokens, 32/8 heads of 128.)
