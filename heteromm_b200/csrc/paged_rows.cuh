@@ -447,7 +447,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     const float e0 = ex2(sc[nb][2 * h] - mx[h]), e1 = ex2(sc[nb][2 * h + 1] - mx[h]);
                     l[h] += e0 + e1;
                     // weights in the cache's type (in 8 bits fp16) for the product: off by half a step,
-                    // 2^-8 of a weight (bf16) or 2^-11, as the output's own rounding; the sum keeps fp32
+                    // 2^-8 of a weight (bf16) or 2^-11, as the output's own rounding (fp16: at least
+                    // 2^-25, 2^-39 of the largest weight); the sum keeps fp32
                     p[2 * nb + h] = pack2<M>(e0, e1);
                 }
             if constexpr (QUANT) {

@@ -460,6 +460,8 @@ hmm_status_t hmm_paged_quant_read(const hmm_paged_quant_t* cache, const hmm_page
 /* hmm_paged_attention over a cache held in 8 bits: q and out of `dtype`
  * (HMM_DTYPE_BF16 or HMM_DTYPE_F16), all else as there.  The result is that of a
  * cache that holds the values in `dtype`; a seen group with s = 255 gives NaN.
+ * (Where a sequence's rows are few, weights are rounded to fp16 whatever `dtype`:
+ * by half a step, and those below 2^-28 of the row's largest by 2^-39 of it.)
  * Workspace: with max_kv = pages_per_seq * page_tokens and the call's max_new (a
  * bound keeps it small: chunks of 512 rows (new tokens * query heads of a group)
  * and more have their keys widened into it, up to 1 GiB of them). */
