@@ -642,7 +642,7 @@ __device__ __forceinline__ void widen_rows(const unsigned char* codes, const Att
 // SHARED: the batch may be one of parts (Batch::shared), whose keys begin at Seq::lo and whose rows may go
 // to AttnArgs::part.  What that adds to the softmax warps' code is felt where their issue is the bound, so
 // a plain batch over 16 bits has a kernel without it (86 bytes of spills for 130; 8,192 tokens, heads of
-// 64: 424.5 -> 422 us, drafted tokens of 16 sequences 56.3 -> 55.0).
+// 64: 424.5 -> 422 us, heads of 128 as before).
 template <typename T, int DP, int C, bool SHARED>
 __global__ void __launch_bounds__(tc_threads<C>(), 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
